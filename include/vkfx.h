@@ -346,6 +346,125 @@ int vkfx_execute_chain(vkfx_plan *const *plans, uint32_t count, const void *d_in
 int vkfx_execute_chain_host(vkfx_plan *const *plans, uint32_t count, const void *h_in, uint64_t in_bytes,
                             void *h_out, uint64_t out_bytes);
 
+/* ----------------------------------------------------- sequence operators */
+
+/* No counterpart in vkfft-rs: what a layer that mixes a sequence needs next
+ * to a long convolution. A convolution plan mixes with a fixed filter; linear
+ * attention mixes with a filter that the data chooses and that can also run
+ * token by token, and layer norm scales the rows that enter either. Plans
+ * belong to a context like FFT plans do: destroy them before it.
+ *
+ * Calls are asynchronous on `stream` (a hipStream_t; NULL = the context's
+ * stream; hipStreamLegacy, (void *)1, = the null stream itself). They neither
+ * allocate nor synchronise nor copy from the host, so a HIP graph can capture
+ * them. A plan's own workspace serves one call at a time: calls of one plan
+ * that overlap on the GPU pass d_work each. */
+
+/* Type of the tensors' elements. Sums, statistics and states are 32 bits. */
+enum vkfx_element { VKFX_ELEMENT_F32 = 0, VKFX_ELEMENT_F16 = 1, VKFX_ELEMENT_BF16 = 2 };
+
+/* Layer norm of rows of `width` elements:
+ *   y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(variance + epsilon). */
+typedef struct {
+    uint64_t width;         /* 1 .. 2^30 */
+    int32_t element;        /* vkfx_element of x, y and their gradients */
+    int32_t weight_element; /* vkfx_element of weight, bias and their gradients */
+    double epsilon;         /* > 0 */
+} vkfx_layer_norm_desc;
+typedef struct vkfx_layer_norm vkfx_layer_norm;
+
+int vkfx_layer_norm_create(vkfx_context *ctx, const vkfx_layer_norm_desc *desc, vkfx_layer_norm **out);
+int vkfx_layer_norm_destroy(vkfx_layer_norm *plan);
+/* Bytes of the scratch a caller may pass to vkfx_layer_norm_backward, for any
+ * number of rows. */
+int vkfx_layer_norm_workspace_bytes(const vkfx_layer_norm *plan, uint64_t *out);
+/* `rows` rows, each `*_row_stride` elements after the one before (at least the
+ * width; x and dy may be broadcast with stride 0). weight and bias may be NULL
+ * (1 and 0). stats: [rows][2] floats, mean and rstd, or NULL. y may be x. */
+int vkfx_layer_norm_forward(vkfx_layer_norm *plan, uint64_t rows, const void *x, int64_t x_row_stride,
+                            const void *weight, const void *bias, void *y, int64_t y_row_stride, float *stats,
+                            void *stream);
+/* Gradients for dy, with the forward call's x and stats: dx, and dweight and
+ * dbias summed over the rows in a fixed order. Any of the three may be NULL
+ * (not computed); dx may be dy. */
+int vkfx_layer_norm_backward(vkfx_layer_norm *plan, uint64_t rows, const void *x, int64_t x_row_stride,
+                             const void *weight, const float *stats, const void *dy, int64_t dy_row_stride, void *dx,
+                             int64_t dx_row_stride, void *dweight, void *dbias, void *d_work, void *stream);
+
+/* Linear attention with a decay for each head. Head h of a sequence, keys of
+ * key_dim and values of value_dim elements, state S (key_dim x value_dim):
+ *   S[t] = decay[h] S[t-1] + k[t] v[t]^T,   out[t] = scale q[t] S[t].
+ * Query head h reads key and value head h / (heads / kv_heads) and has a state
+ * of its own. */
+typedef struct {
+    uint32_t heads;         /* query heads: 1 .. 65535 */
+    uint32_t kv_heads;      /* divides heads */
+    uint32_t key_dim;       /* 1 .. 256 */
+    uint32_t value_dim;     /* 1 .. 256 */
+    int32_t element;        /* vkfx_element of q, k, v, out and their gradients */
+    int32_t gradient;       /* 1: the plan's workspace also serves the backward pass */
+    double scale;           /* finite */
+    const double *decay;    /* [heads], each in [0, 1]; copied */
+    uint64_t max_batch;     /* most sequences (up to 65535) and tokens of one call */
+    uint64_t max_tokens;    /* up to 2^31 - 4096 */
+} vkfx_linear_attention_desc;
+typedef struct vkfx_linear_attention vkfx_linear_attention;
+
+/* A [batch][token][head][dim] tensor: element strides of the first three; the
+ * last is contiguous. Inputs may be broadcast (stride 0), outputs may not
+ * overlap themselves. */
+typedef struct {
+    const void *data;
+    int64_t batch_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+} vkfx_sequence;
+
+int vkfx_linear_attention_create(vkfx_context *ctx, const vkfx_linear_attention_desc *desc,
+                                 vkfx_linear_attention **out);
+int vkfx_linear_attention_destroy(vkfx_linear_attention *plan);
+/* Bytes of the scratch a caller may pass for calls of up to max_batch
+ * sequences of up to max_tokens tokens. */
+int vkfx_linear_attention_workspace_bytes(const vkfx_linear_attention *plan, uint64_t *out);
+
+/* `tokens` may be 1 (the next token of each sequence: the state is read and
+ * written once), as many as a prompt has, or 0. lengths: [batch] or NULL; rows
+ * of sequence b from lengths[b] on (clamped to 0 .. tokens) are not read, give
+ * zeros and leave its state alone. state_in (NULL: zeros) and state_out (NULL:
+ * not wanted), [batch][heads][key_dim][value_dim] floats, may be one buffer;
+ * out overlaps no input. */
+typedef struct {
+    uint64_t batch;
+    uint64_t tokens;
+    vkfx_sequence q; /* [batch][tokens][heads][key_dim] */
+    vkfx_sequence k; /* [batch][tokens][kv_heads][key_dim] */
+    vkfx_sequence v; /* [batch][tokens][kv_heads][value_dim] */
+    vkfx_sequence out; /* [batch][tokens][heads][value_dim], written */
+    const int32_t *lengths;
+    const float *state_in;
+    float *state_out;
+} vkfx_linear_attention_forward_args;
+int vkfx_linear_attention_forward(vkfx_linear_attention *plan, const vkfx_linear_attention_forward_args *args,
+                                  void *d_work, void *stream);
+
+/* Gradients of q, k, v and of state_in for dout and dstate_out (NULL: zeros),
+ * with the forward call's inputs. Rows past a sequence's length get zeros.
+ * dstate_in may be NULL (not wanted). The gradients of shared key and value
+ * heads are summed over their query heads in a fixed order. No output overlaps
+ * an input. */
+typedef struct {
+    uint64_t batch;
+    uint64_t tokens;
+    vkfx_sequence q, k, v, dout;
+    vkfx_sequence dq, dk, dv; /* written */
+    const int32_t *lengths;
+    const float *state_in;
+    const float *dstate_out;
+    float *dstate_in;
+} vkfx_linear_attention_backward_args;
+int vkfx_linear_attention_backward(vkfx_linear_attention *plan, const vkfx_linear_attention_backward_args *args,
+                                   void *d_work, void *stream);
+
 /* Thread-local message of the last failing call on this thread. */
 const char *vkfx_last_error(void);
 

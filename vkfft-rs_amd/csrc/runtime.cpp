@@ -20,6 +20,7 @@
 #include <string>
 #include <vector>
 
+#include "context.hpp"
 #include "kernels.hpp"
 #include "planner.hpp"
 #include "roots.hpp"
@@ -29,56 +30,8 @@ using namespace vkfx;
 
 namespace {
 
-thread_local std::string g_err;
-
-int fail(int code, const std::string& msg) {
-    g_err = msg;
-    return code;
-}
-
-int hip_fail(hipError_t e, const char* what) {
-    return fail(VKFX_ERR_NATIVE_RUNTIME, std::string(what) + ": " + hipGetErrorString(e));
-}
-
-struct DevBuf {
-    void* p = nullptr;
-    size_t bytes = 0;
-    DevBuf() = default;
-    DevBuf(const DevBuf&) = delete;
-    DevBuf& operator=(const DevBuf&) = delete;
-    ~DevBuf() {
-        if (p) (void)hipFree(p);
-    }
-};
-
 typedef long double ld;
 const ld kPi = kPiL;
-
-}  // namespace
-
-// Pooled device / pinned host buffer. `ready` (optional) is recorded on the
-// stream of its last user; the next user's stream waits on it, so reuse is
-// stream-ordered.
-struct PoolBuf {
-    void* p = nullptr;
-    size_t bytes = 0;
-    hipEvent_t ready = nullptr;
-};
-
-struct vkfx_context {
-    int device = 0;
-    hipStream_t stream = nullptr;
-    vkfx_device_profile profile{};
-    std::vector<PoolBuf> dev_pool, host_pool;  // free buffers
-    std::vector<hipStream_t> stream_pool;      // free streams for tickets
-    void* scratch = nullptr;                   // this device's static scratch (vkfx_execute_noalloc)
-    hipError_t scratch_err = hipSuccess;       // why `scratch` is null, if it is
-    std::mutex mu;                             // guards the pools, `active` and `plans`
-    int active = 0;                            // tickets submitted and not yet destroyed
-    int plans = 0;                             // plans created and not yet destroyed
-};
-
-namespace {
 
 // Buffers a launch reads or writes: the caller's input and output, the
 // plan's workspace (per stream lane) and, for mixed storage/compute
@@ -2650,9 +2603,14 @@ int plan_c2r(Ctx& c, size_t n, size_t batch, bool normalize) {
 
 // ============================================================== C ABI
 
+std::string& vkfx::last_error() {
+    thread_local std::string text;
+    return text;
+}
+
 extern "C" {
 
-const char* vkfx_last_error(void) { return g_err.c_str(); }
+const char* vkfx_last_error(void) { return last_error().c_str(); }
 
 #ifdef VKFX_INDEX_TEST
 const char* vkfx_version(void) { return "vkfx-mi355x 0.1.0 (gfx950, index-map test build)"; }

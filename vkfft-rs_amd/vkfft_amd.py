@@ -200,6 +200,48 @@ class _Profile(ctypes.Structure):
     ]
 
 
+class _LayerNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("width", ctypes.c_uint64),
+        ("element", ctypes.c_int32),
+        ("weight_element", ctypes.c_int32),
+        ("epsilon", ctypes.c_double),
+    ]
+
+
+class _LinearAttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("heads", ctypes.c_uint32),
+        ("kv_heads", ctypes.c_uint32),
+        ("key_dim", ctypes.c_uint32),
+        ("value_dim", ctypes.c_uint32),
+        ("element", ctypes.c_int32),
+        ("gradient", ctypes.c_int32),
+        ("scale", ctypes.c_double),
+        ("decay", ctypes.POINTER(ctypes.c_double)),
+        ("max_batch", ctypes.c_uint64),
+        ("max_tokens", ctypes.c_uint64),
+    ]
+
+
+def _sequence_fields(names):
+    """The four fields of a vkfx_sequence for each name, in line: a call sets
+    them all in one constructor."""
+    return [(n + f, t) for n in names for f, t in (("", ctypes.c_void_p), ("_batch", ctypes.c_int64),
+                                                   ("_token", ctypes.c_int64), ("_head", ctypes.c_int64))]
+
+
+class _ForwardArgs(ctypes.Structure):
+    _fields_ = ([("batch", ctypes.c_uint64), ("tokens", ctypes.c_uint64)] + _sequence_fields(["q", "k", "v", "out"])
+                + [(n, ctypes.c_void_p) for n in ("lengths", "state_in", "state_out")])
+
+
+class _BackwardArgs(ctypes.Structure):
+    _fields_ = ([("batch", ctypes.c_uint64), ("tokens", ctypes.c_uint64)]
+                + _sequence_fields(["q", "k", "v", "dout", "dq", "dk", "dv"])
+                + [(n, ctypes.c_void_p) for n in ("lengths", "state_in", "dstate_out", "dstate_in")])
+
+
 def lib(path: Optional[str] = None):
     """Loads libvkfft_mi355x.so (or the library at `path`, e.g. the index-map
     test build INDEX_LIB_PATH); raises if it has not been built."""
@@ -242,6 +284,17 @@ def lib(path: Optional[str] = None):
         L.vkfx_plan_timing_start.argtypes = [vp, ctypes.c_uint32]
         L.vkfx_plan_timing_stop.argtypes = [vp, ctypes.POINTER(_PassTiming), ctypes.c_uint32,
                                             ctypes.POINTER(ctypes.c_uint32)]
+        L.vkfx_layer_norm_create.argtypes = [vp, ctypes.POINTER(_LayerNormDesc), ctypes.POINTER(vp)]
+        L.vkfx_layer_norm_destroy.argtypes = [vp]
+        L.vkfx_layer_norm_workspace_bytes.argtypes = [vp, ctypes.POINTER(u64)]
+        L.vkfx_layer_norm_forward.argtypes = [vp, u64, vp, ctypes.c_int64, vp, vp, vp, ctypes.c_int64, vp, vp]
+        L.vkfx_layer_norm_backward.argtypes = [vp, u64, vp, ctypes.c_int64, vp, vp, vp, ctypes.c_int64, vp,
+                                               ctypes.c_int64, vp, vp, vp, vp]
+        L.vkfx_linear_attention_create.argtypes = [vp, ctypes.POINTER(_LinearAttentionDesc), ctypes.POINTER(vp)]
+        L.vkfx_linear_attention_destroy.argtypes = [vp]
+        L.vkfx_linear_attention_workspace_bytes.argtypes = [vp, ctypes.POINTER(u64)]
+        L.vkfx_linear_attention_forward.argtypes = [vp, ctypes.POINTER(_ForwardArgs), vp, vp]
+        L.vkfx_linear_attention_backward.argtypes = [vp, ctypes.POINTER(_BackwardArgs), vp, vp]
         L.vkfx_execute_chain.argtypes = [ctypes.POINTER(vp), ctypes.c_uint32, vp, vp, vp]
         L.vkfx_execute_chain_host.argtypes = [ctypes.POINTER(vp), ctypes.c_uint32, vp, u64, vp, u64]
         _libs[path] = L
@@ -1309,6 +1362,285 @@ class IrTicket:
             self.close()
         except Exception:
             pass
+
+
+# ------------------------------------------------------- sequence operators
+
+class Element(enum.IntEnum):
+    """Type of a sequence operator's tensors; its sums and states are 32 bits."""
+    F32 = 0
+    F16 = 1
+    BF16 = 2
+
+
+def _torch_type(element: Element):
+    import torch
+    return {Element.F32: torch.float32, Element.F16: torch.float16, Element.BF16: torch.bfloat16}[element]
+
+
+def _raw_stream(stream, device):
+    """The stream of a call on torch tensors: `stream`, or torch's current one
+    on their device. Its default stream is the null stream, which the C ABI
+    knows by hipStreamLegacy (1)."""
+    import torch
+    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream or 1
+
+
+@dataclass
+class LayerNormConfig:
+    """Layer norm of rows of `width` elements: (x - mean) rstd weight + bias."""
+    width: int
+    element: Element = Element.F32
+    weight_element: Optional[Element] = None  # of weight and bias: the rows', or F32
+    epsilon: float = 1e-5
+
+    @staticmethod
+    def new(width: int) -> "LayerNormConfig":
+        return LayerNormConfig(int(width))
+
+    def with_element(self, element: Element) -> "LayerNormConfig":
+        self.element = Element(element)
+        return self
+
+    def with_weight_element(self, element: Element) -> "LayerNormConfig":
+        self.weight_element = Element(element)
+        return self
+
+    def with_epsilon(self, epsilon: float) -> "LayerNormConfig":
+        self.epsilon = float(epsilon)
+        return self
+
+    def desc(self) -> _LayerNormDesc:
+        if not 0 <= self.width < 1 << 63:
+            raise VkFftError(-7, "width must be 1 .. 2^30")
+        weight = self.element if self.weight_element is None else self.weight_element
+        return _LayerNormDesc(self.width, int(self.element), int(weight), self.epsilon)
+
+
+class _SequencePlan:
+    """What both operators' plans share: the handle and the checks of tensors."""
+    _kind = ""
+
+    def __init__(self, ctx: "HipExecutionContext", config, desc):
+        self.ctx = ctx
+        self._L = ctx._L
+        self.config = config
+        self.handle = ctypes.c_void_p()
+        _check(getattr(self._L, f"vkfx_{self._kind}_create")(ctx.handle, ctypes.byref(desc), ctypes.byref(self.handle)),
+               self._L)
+        ctx._live_plans.add(self)
+        self._destroy = getattr(self._L, f"vkfx_{self._kind}_destroy")
+        w = ctypes.c_uint64()
+        _check(getattr(self._L, f"vkfx_{self._kind}_workspace_bytes")(self.handle, ctypes.byref(w)), self._L)
+        self.workspace_bytes = int(w.value)
+        self._type = _torch_type(config.element)
+
+    def _place(self, x):
+        """The device of a call, which is the context's."""
+        if not x.is_cuda:
+            raise VkFftError(-7, "tensors must be device tensors")
+        return x.device
+
+    def _tensor(self, name, x, shape, dtype, device):
+        if tuple(x.shape) != shape:
+            raise VkFftError(-5, f"{name}: expected shape {shape}, got {tuple(x.shape)}")
+        if x.dtype != dtype:
+            raise VkFftError(-4, f"{name}: expected {dtype}, got {x.dtype}")
+        if x.device != device:
+            raise VkFftError(-7, f"{name} must be on {device}")
+
+    def _dense(self, name, x, shape, dtype, device):
+        """Address of a contiguous tensor, or None."""
+        if x is None:
+            return None
+        self._tensor(name, x, shape, dtype, device)
+        if not x.is_contiguous():
+            raise VkFftError(-7, f"{name} must be contiguous")
+        return x.data_ptr()
+
+    def _work(self, work, device):
+        if work is None:
+            return None
+        if work.device != device or not work.is_contiguous() or work.numel() * work.element_size() < self.workspace_bytes:
+            raise VkFftError(-5, f"work must be {self.workspace_bytes} contiguous bytes on {device}")
+        return work.data_ptr()
+
+    def close(self):
+        # as with Plan: a plan outliving its context only drops its handle
+        if self.handle and self.ctx.handle:
+            _check(self._destroy(self.handle), self._L)
+        self.handle = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class LayerNormPlan(_SequencePlan):
+    """Layer norm on device-resident torch tensors. Rows are the leading
+    dimension of a 2-D tensor whose last dimension is contiguous."""
+    _kind = "layer_norm"
+
+    def __init__(self, ctx: "HipExecutionContext", config: LayerNormConfig):
+        super().__init__(ctx, config, config.desc())
+        self._weight_type = _torch_type(config.element if config.weight_element is None else config.weight_element)
+
+    def _rows(self, name, x, rows, device):
+        self._tensor(name, x, (rows, self.config.width), self._type, device)
+        row, column = x.stride()
+        if column != 1 and self.config.width > 1:
+            raise VkFftError(-7, f"{name}: the last dimension must be contiguous")
+        return x.data_ptr(), row
+
+    def forward_tensors(self, x, weight, bias, y, stats=None, stream=None):
+        """y (may be x) and, if wanted, stats [rows][2]: mean and rstd."""
+        device, w = self._place(x), (self.config.width,)
+        rows = x.shape[0]
+        xp, xs = self._rows("x", x, rows, device)
+        yp, ys = self._rows("y", y, rows, device)
+        _check(self._L.vkfx_layer_norm_forward(
+            self.handle, rows, xp, xs, self._dense("weight", weight, w, self._weight_type, device),
+            self._dense("bias", bias, w, self._weight_type, device), yp, ys,
+            self._dense("stats", stats, (rows, 2), _torch_type(Element.F32), device), _raw_stream(stream, device)), self._L)
+
+    def backward_tensors(self, x, weight, stats, dy, dx=None, dweight=None, dbias=None, work=None, stream=None):
+        """Gradients for dy; any of the three may be None (not wanted)."""
+        device, w = self._place(x), (self.config.width,)
+        rows = x.shape[0]
+        xp, xs = self._rows("x", x, rows, device)
+        gp, gs = self._rows("dy", dy, rows, device)
+        dp, ds = (None, 0) if dx is None else self._rows("dx", dx, rows, device)
+        _check(self._L.vkfx_layer_norm_backward(
+            self.handle, rows, xp, xs, self._dense("weight", weight, w, self._weight_type, device),
+            self._dense("stats", stats, (rows, 2), _torch_type(Element.F32), device), gp, gs, dp, ds,
+            self._dense("dweight", dweight, w, self._weight_type, device),
+            self._dense("dbias", dbias, w, self._weight_type, device), self._work(work, device),
+            _raw_stream(stream, device)), self._L)
+
+
+@dataclass
+class LinearAttentionConfig:
+    """Linear attention with a decay for each head:
+    S[t] = decay S[t-1] + k[t] v[t]^T, out[t] = scale q[t] S[t]."""
+    heads: int
+    key_dim: int
+    value_dim: int
+    kv_heads: Optional[int] = None  # default: heads
+    element: Element = Element.F32
+    decay: Optional[List[float]] = None  # one in [0, 1] for each head; default: 1
+    scale: Optional[float] = None  # default: 1 / sqrt(key_dim)
+    max_batch: int = 1
+    max_tokens: int = 1
+    gradient: bool = False
+
+    @staticmethod
+    def new(heads: int, key_dim: int, value_dim: int) -> "LinearAttentionConfig":
+        return LinearAttentionConfig(int(heads), int(key_dim), int(value_dim))
+
+    def with_kv_heads(self, kv_heads: int) -> "LinearAttentionConfig":
+        self.kv_heads = int(kv_heads)
+        return self
+
+    def with_element(self, element: Element) -> "LinearAttentionConfig":
+        self.element = Element(element)
+        return self
+
+    def with_decay(self, decay: Sequence[float]) -> "LinearAttentionConfig":
+        self.decay = [float(d) for d in decay]
+        return self
+
+    def with_scale(self, scale: float) -> "LinearAttentionConfig":
+        self.scale = float(scale)
+        return self
+
+    def with_capacity(self, batch: int, tokens: int) -> "LinearAttentionConfig":
+        """The most sequences and tokens of one call."""
+        self.max_batch, self.max_tokens = int(batch), int(tokens)
+        return self
+
+    def with_gradient(self, gradient: bool = True) -> "LinearAttentionConfig":
+        """Plans made with it also run the backward pass."""
+        self.gradient = bool(gradient)
+        return self
+
+    def desc(self) -> _LinearAttentionDesc:
+        kv = self.heads if self.kv_heads is None else self.kv_heads
+        decay = [1.0] * self.heads if self.decay is None else self.decay
+        if len(decay) != self.heads:
+            raise VkFftError(-5, f"{self.heads} heads need {self.heads} decays, got {len(decay)}")
+        for name, n in (("heads", self.heads), ("kv_heads", kv), ("key_dim", self.key_dim), ("value_dim", self.value_dim),
+                        ("max_batch", self.max_batch), ("max_tokens", self.max_tokens)):
+            if not 1 <= n < 1 << 31:
+                raise VkFftError(-7, f"{name} must be positive and under 2^31")
+        scale = self.key_dim ** -0.5 if self.scale is None else self.scale
+        return _LinearAttentionDesc(self.heads, kv, self.key_dim, self.value_dim, int(self.element), int(self.gradient), scale,
+                                    (ctypes.c_double * len(decay))(*decay), self.max_batch, self.max_tokens)
+
+
+class LinearAttentionPlan(_SequencePlan):
+    """Linear attention on device-resident torch tensors [batch][token][head][dim]
+    (any strides, the last dimension contiguous) and states
+    [batch][heads][key_dim][value_dim] (float32, contiguous). `lengths`: int32
+    for each sequence, or None for all tokens."""
+    _kind = "linear_attention"
+
+    def __init__(self, ctx: "HipExecutionContext", config: LinearAttentionConfig):
+        super().__init__(ctx, config, config.desc())
+        self._kv = config.heads if config.kv_heads is None else config.kv_heads
+
+    def _sequence(self, name, x, shape, device):
+        self._tensor(name, x, shape, self._type, device)
+        b, t, h, d = x.stride()
+        if d != 1 and shape[3] > 1:
+            raise VkFftError(-7, f"{name}: the last dimension must be contiguous")
+        return x.data_ptr(), b, t, h
+
+    def _states(self, shape, device, **states):
+        f32 = _torch_type(Element.F32)
+        return [self._dense(n, x, shape, f32, device) for n, x in states.items()]
+
+    def _lengths(self, lengths, batch, device):
+        if lengths is None:
+            return None
+        import torch
+        return self._dense("lengths", lengths, (batch,), torch.int32, device)
+
+    def forward_tensors(self, q, k, v, out, state_in=None, state_out=None, lengths=None, work=None, stream=None):
+        """Outputs of a prompt, or of the next token where there is one: from
+        state_in (None: zeros) to state_out (None: not wanted; may be state_in)."""
+        c, device = self.config, self._place(q)
+        if q.dim() != 4:
+            raise VkFftError(-5, "q must be [batch][token][head][key_dim]")
+        b, t = q.shape[:2]
+        args = _ForwardArgs(b, t, *self._sequence("q", q, (b, t, c.heads, c.key_dim), device),
+                            *self._sequence("k", k, (b, t, self._kv, c.key_dim), device),
+                            *self._sequence("v", v, (b, t, self._kv, c.value_dim), device),
+                            *self._sequence("out", out, (b, t, c.heads, c.value_dim), device),
+                            self._lengths(lengths, b, device),
+                            *self._states((b, c.heads, c.key_dim, c.value_dim), device, state_in=state_in, state_out=state_out))
+        _check(self._L.vkfx_linear_attention_forward(self.handle, ctypes.byref(args), self._work(work, device),
+                                                     _raw_stream(stream, device)), self._L)
+
+    def backward_tensors(self, q, k, v, dout, dq, dk, dv, state_in=None, dstate_out=None, dstate_in=None, lengths=None,
+                         work=None, stream=None):
+        """Gradients of q, k, v and (dstate_in, None: not wanted) of state_in,
+        for dout and dstate_out (None: zeros)."""
+        c, device = self.config, self._place(q)
+        if q.dim() != 4:
+            raise VkFftError(-5, "q must be [batch][token][head][key_dim]")
+        b, t = q.shape[:2]
+        key, value = (b, t, c.heads, c.key_dim), (b, t, c.heads, c.value_dim)
+        shared_key, shared_value = (b, t, self._kv, c.key_dim), (b, t, self._kv, c.value_dim)
+        args = _BackwardArgs(b, t, *self._sequence("q", q, key, device), *self._sequence("k", k, shared_key, device),
+                             *self._sequence("v", v, shared_value, device), *self._sequence("dout", dout, value, device),
+                             *self._sequence("dq", dq, key, device), *self._sequence("dk", dk, shared_key, device),
+                             *self._sequence("dv", dv, shared_value, device), self._lengths(lengths, b, device),
+                             *self._states((b, c.heads, c.key_dim, c.value_dim), device, state_in=state_in,
+                                           dstate_out=dstate_out, dstate_in=dstate_in))
+        _check(self._L.vkfx_linear_attention_backward(self.handle, ctypes.byref(args), self._work(work, device),
+                                                      _raw_stream(stream, device)), self._L)
 
 
 class HipExecutionContext:
