@@ -1,0 +1,8 @@
+// linear_f16.hip -- chunk kernels of linear attention for f16 elements.
+#include "linear_chunk.hpp"
+
+namespace vkfx {
+
+const ChunkKernel* chunk_kernel_f16(int dk, int dv) { return pick_chunk_kernel<_Float16, 32>(dk, dv); }
+
+}  // namespace vkfx

@@ -1,0 +1,8 @@
+// linear_f32.hip -- chunk kernels of linear attention for f32 elements.
+#include "linear_chunk.hpp"
+
+namespace vkfx {
+
+const ChunkKernel* chunk_kernel_f32(int dk, int dv) { return pick_chunk_kernel<float, 32>(dk, dv); }
+
+}  // namespace vkfx

@@ -80,35 +80,7 @@ __global__ __launch_bounds__(256) void k_scan_recurrent(const ScanArgs s, const 
         }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_group_sum(const float* __restrict__ from, const ScanSide to, long long batch,
-                                                   long long tokens, int kv_heads, int group, int dim) {
-    const long long total = batch * tokens * kv_heads * dim;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int c = (int)(i % dim);
-        const long long row = i / dim;  // batch, token, shared head
-        const int h = (int)(row % kv_heads);
-        const long long t = row / kv_heads % tokens, b = row / kv_heads / tokens;
-        float sum = 0.f;
-        for (int g = 0; g < group; ++g) sum += from[(row * group + g) * dim + c];
-        ((T*)to.p)[b * to.batch + t * to.token + h * to.head + c] = (T)sum;
-    }
-}
-
 }  // namespace
-
-int launch_group_sum(int element, const float* from, const ScanSide& to, long long batch, long long tokens, int kv_heads,
-                     int group, int dim, hipStream_t s) {
-    const long long blocks = (batch * tokens * kv_heads * dim + 255) / 256;
-    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
-    if (element == VKFX_ELEMENT_F32)
-        hipLaunchKernelGGL(k_group_sum<float>, grid, dim3(256), 0, s, from, to, batch, tokens, kv_heads, group, dim);
-    else if (element == VKFX_ELEMENT_F16)
-        hipLaunchKernelGGL(k_group_sum<_Float16>, grid, dim3(256), 0, s, from, to, batch, tokens, kv_heads, group, dim);
-    else
-        hipLaunchKernelGGL(k_group_sum<__bf16>, grid, dim3(256), 0, s, from, to, batch, tokens, kv_heads, group, dim);
-    return (int)hipGetLastError();
-}
 
 int launch_scan_recurrent(int element, const ScanArgs* scans, int count, const float* powers, hipStream_t s) {
     for (int i = 0; i < count; ++i) {

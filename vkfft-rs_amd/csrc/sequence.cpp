@@ -25,7 +25,8 @@ struct vkfx_linear_attention {
     vkfx_context* ctx = nullptr;
     vkfx_linear_attention_desc desc{};
     DevBuf powers;  // [heads][kDecayPowers] floats
-    DevBuf work;
+    DevBuf work;  // states between segments, then a shared head's gradients for each query head
+    uint64_t state_floats = 0;
 };
 
 namespace {
@@ -107,6 +108,17 @@ int check_sequence(const char* name, const vkfx_sequence& s, uint64_t batch, uin
 
 ScanSide side(const vkfx_sequence& s, int group) {
     return ScanSide{s.data, s.batch_stride, s.token_stride, s.head_stride, group};
+}
+
+// Floats that calls of the scans need for states between segments.
+uint64_t state_floats(const vkfx_linear_attention_desc& d) {
+    const int dk = (int)d.key_dim, dv = (int)d.value_dim, h = (int)d.heads;
+    const long long b = (long long)d.max_batch, t = (long long)d.max_tokens;
+    const uint64_t forward = scan_work_floats(d.element, dk, dv, h, 1, b, t);
+    if (!d.gradient) return forward;
+    // dq, dk over dv x dk; dv over dk x dv; all together where the widths are equal
+    if (dk == dv) return std::max<uint64_t>(forward, scan_work_floats(d.element, dk, dv, h, 3, b, t));
+    return std::max<uint64_t>(forward, scan_work_floats(d.element, dv, dk, h, 2, b, t) + forward);
 }
 
 // Floats of the gradients of k and v for each query head, summed over a shared
@@ -257,7 +269,8 @@ int vkfx_linear_attention_create(vkfx_context* ctx, const vkfx_linear_attention_
         if (int rc = allocate(p->powers, powers.size() * sizeof(float))) return rc;
         const hipError_t e = hipMemcpy(p->powers.p, powers.data(), powers.size() * sizeof(float), hipMemcpyHostToDevice);
         if (e != hipSuccess) return hip_fail(e, "hipMemcpy decays");
-        if (int rc = allocate(p->work, floats * sizeof(float))) return rc;
+        p->state_floats = state_floats(d);
+        if (int rc = allocate(p->work, (p->state_floats + floats) * sizeof(float))) return rc;
         retain(ctx);
         *out = p.release();
         return VKFX_OK;
@@ -310,7 +323,8 @@ int vkfx_linear_attention_forward(vkfx_linear_attention* plan, const vkfx_linear
         s.scale_in = (float)d.scale;
         s.scale_update = 1.f;
         (void)hipSetDevice(plan->ctx->device);
-        const int e = launch_scan_recurrent(d.element, &s, 1, (const float*)plan->powers.p, stream_of(plan->ctx, stream));
+        float* work = (float*)(d_work ? d_work : plan->work.p);
+        const int e = launch_scans(d.element, &s, 1, (const float*)plan->powers.p, work, stream_of(plan->ctx, stream));
         return e == hipSuccess ? VKFX_OK : hip_fail((hipError_t)e, "launch linear attention");
     });
 }
@@ -359,9 +373,9 @@ int vkfx_linear_attention_backward(vkfx_linear_attention* plan, const vkfx_linea
             return s;
         };
         // dq: the forward scan of (dout, v, k) from the state's transpose
-        ScanArgs scans[3] = {scan(args->dout, 1, args->v, group, args->k, group), scan(args->k, group, args->q, 1, args->dout, 1),
-                             scan(args->v, group, args->dout, 1, args->q, 1)};
-        ScanArgs &q = scans[0], &v = scans[1], &k = scans[2];
+        ScanArgs scans[3] = {scan(args->dout, 1, args->v, group, args->k, group), scan(args->v, group, args->dout, 1, args->q, 1),
+                             scan(args->k, group, args->q, 1, args->dout, 1)};
+        ScanArgs &q = scans[0], &k = scans[1], &v = scans[2];
         q.dk = dv, q.dv = dk, q.state_row = 1, q.state_col = dv, q.state_in = args->state_in;
         q.scale_in = (float)d.scale, q.scale_update = 1.f;
         v.dk = dk, v.dv = dv, v.state_row = dv, v.state_col = 1, v.state_in = args->dstate_out, v.state_out = args->dstate_in;
@@ -374,7 +388,7 @@ int vkfx_linear_attention_backward(vkfx_linear_attention* plan, const vkfx_linea
             s.out_batch = o.batch_stride, s.out_token = o.token_stride, s.out_head = o.head_stride;
         };
         to(q, args->dq);
-        float *wk = work, *wv = work + b * t * d.heads * d.key_dim;
+        float *wk = work + plan->state_floats, *wv = wk + b * t * d.heads * d.key_dim;
         if (group > 1) {  // floats of every query head, [batch][token][head][dim]
             to(k, vkfx_sequence{wk, (int64_t)(t * d.heads * dk), (int64_t)d.heads * dk, dk});
             to(v, vkfx_sequence{wv, (int64_t)(t * d.heads * dv), (int64_t)d.heads * dv, dv});
@@ -385,7 +399,7 @@ int vkfx_linear_attention_backward(vkfx_linear_attention* plan, const vkfx_linea
         }
         (void)hipSetDevice(plan->ctx->device);
         hipStream_t st = stream_of(plan->ctx, stream);
-        int e = launch_scan_recurrent(d.element, scans, 3, (const float*)plan->powers.p, st);
+        int e = launch_scans(d.element, scans, 3, (const float*)plan->powers.p, work, st);
         if (e == hipSuccess && group > 1 && t) {
             e = launch_group_sum(d.element, wk, side(args->dk, 1), (long long)b, (long long)t, (int)d.kv_heads, group, dk, st);
             if (e == hipSuccess)
