@@ -1,7 +1,22 @@
 // layer_norm.hip -- layer norm of rows and its gradients.
+//
+// Both passes are bound by memory: a row of any width that fits the registers
+// of a block is read once. Vectors of 16 bytes go to consecutive lanes; a row
+// belongs to 8 .. 64 lanes of a wave, so that short rows fill it, or to a whole
+// block. The variance is the mean of squared distances from the mean, both from
+// registers, so a mean far from zero costs no digits. Rows may start at any
+// alignment of their elements.
+//
+// Backward, with n = (x - mean) rstd and g = dy weight:
+//   dx = rstd (g - mean(g) - n mean(g n)),  dweight = sum dy n,  dbias = sum dy
+// over the rows. The lane that holds a column in one row holds it in the
+// block's every row, so the sums over rows stay in registers; each block then
+// writes one row of sums and a second launch adds those in their order.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "sequence.hpp"
 #include "vkfx.h"
@@ -10,74 +25,357 @@ namespace vkfx {
 
 namespace {
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
-__device__ __forceinline__ float to_f32(__bf16 v) { return (float)v; }
-
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
-}
-
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void k_norm_forward(const NormArgs a) {
-    __shared__ float lds[4];
-    const long long r = blockIdx.x;
-    const T* x = (const T*)a.x + r * a.x_stride;
-    T* y = (T*)a.y + r * a.y_stride;
-    float s = 0.f;
-    for (int i = threadIdx.x; i < a.width; i += 256) s += to_f32(x[i]);
-    const float mean = block_sum(s, lds) / (float)a.width;
-    s = 0.f;
-    for (int i = threadIdx.x; i < a.width; i += 256) {
-        const float d = to_f32(x[i]) - mean;
-        s += d * d;
-    }
-    const float rstd = 1.0f / sqrtf(block_sum(s, lds) / (float)a.width + a.epsilon);
-    for (int i = threadIdx.x; i < a.width; i += 256) {
-        const float w = a.weight ? to_f32(((const W*)a.weight)[i]) : 1.f;
-        const float b = a.bias ? to_f32(((const W*)a.bias)[i]) : 0.f;
-        y[i] = (T)((to_f32(x[i]) - mean) * rstd * w + b);
-    }
-    if (a.stats_out && threadIdx.x == 0) {
-        a.stats_out[2 * r] = mean;
-        a.stats_out[2 * r + 1] = rstd;
-    }
-}
-
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void k_norm_backward_x(const NormArgs a) {
-    __shared__ float lds[4];
-    const long long r = blockIdx.x;
-    const T* x = (const T*)a.x + r * a.x_stride;
-    const T* dy = (const T*)a.dy + r * a.dy_stride;
-    T* dx = (T*)a.y + r * a.y_stride;
-    const float mean = a.stats_in[2 * r], rstd = a.stats_in[2 * r + 1];
-    float s1 = 0.f, s2 = 0.f;
-    for (int i = threadIdx.x; i < a.width; i += 256) {
-        const float g = to_f32(dy[i]) * (a.weight ? to_f32(((const W*)a.weight)[i]) : 1.f);
-        s1 += g;
-        s2 += g * ((to_f32(x[i]) - mean) * rstd);
-    }
-    s1 = block_sum(s1, lds) / (float)a.width;
-    s2 = block_sum(s2, lds) / (float)a.width;
-    for (int i = threadIdx.x; i < a.width; i += 256) {
-        const float g = to_f32(dy[i]) * (a.weight ? to_f32(((const W*)a.weight)[i]) : 1.f);
-        dx[i] = (T)((g - s1 - (to_f32(x[i]) - mean) * rstd * s2) * rstd);
-    }
-}
+template <typename T, int N>
+using Some = T __attribute__((ext_vector_type(N)));
+// The same in memory, at any alignment of its elements.
+template <typename T, int N>
+struct Packed {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_norm_backward_rows(const NormArgs a) {
+constexpr int kVector = 16 / (int)sizeof(T);
+
+// Elements c .. c + N - 1 of a row of `width`, zeros past its end.
+template <typename T, int N>
+__device__ __forceinline__ Some<T, N> load_some(const T* row, int c, int width) {
+    Some<T, N> r;
+    if (c + N <= width) {
+        r = *(const typename Packed<T, N>::type*)(row + c);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) r[e] = c + e < width ? row[c + e] : (T)0.f;
+    }
+    return r;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_some(T* row, int c, int width, const Some<T, N>& r) {
+    if (c + N <= width) {
+        *(typename Packed<T, N>::type*)(row + c) = r;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (c + e < width) row[c + e] = r[e];
+}
+
+// Sum over the LPR threads of a row, the same on each. Rows wider than a wave
+// meet in `lds`, of which every call takes the other half: one barrier each.
+template <int LPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* lds, int& half) {
+#pragma unroll
+    for (int o = 1; o < (LPR < 64 ? LPR : 64); o <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    if constexpr (LPR > 64) {
+        constexpr int waves = LPR / 64;
+        const int wave = threadIdx.x >> 6, all = blockDim.x >> 6;
+        float* at = lds + half * all * N;
+        half ^= 1;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) at[wave * N + i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < waves; ++w) v[i] += at[(wave / waves * waves + w) * N + i];
+        }
+    }
+}
+
+// LPR threads a row, NV vectors each, NT threads a block.
+template <typename T, typename W, int LPR, int NV, int NT>
+__global__ __launch_bounds__(NT) void k_norm_forward(const NormArgs a) {
+    constexpr int V = kVector<T>, R = NT / LPR;
+    __shared__ float lds[2 * (NT / 64)];
+    int half = 0;
+    const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
+    Some<W, V> w[NV], b[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * LPR + lane) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[j][e] = (W)1.f, b[j][e] = (W)0.f;
+        if (a.weight) w[j] = load_some<W, V>((const W*)a.weight, c, a.width);
+        if (a.bias) b[j] = load_some<W, V>((const W*)a.bias, c, a.width);
+    }
+    Some<T, V> next[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) next[j] = (T)0.f;
+    const auto fetch = [&](long long r) {
+        if (r < a.rows)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                next[j] = load_some<T, V>((const T*)a.x + r * a.x_stride, (j * LPR + lane) * V, a.width);
+    };
+    const float over = 1.f / (float)a.width;
+    const long long stride = (long long)gridDim.x * R;
+    constexpr bool kAhead = NT < 1024 || NV == 1;  // the next row on its way, where the registers hold it
+    if constexpr (kAhead) fetch((long long)blockIdx.x * R + group);
+    for (long long r0 = (long long)blockIdx.x * R; r0 < a.rows; r0 += stride) {
+        const long long r = r0 + group;
+        const bool live = r < a.rows;  // where not, the group still meets the block's barriers
+        if constexpr (!kAhead) fetch(r);
+        Some<T, V> x[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) x[j] = next[j];
+        if constexpr (kAhead) fetch(r + stride);
+        float s[1] = {0.f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[0] += (float)x[j][e];
+        row_sum<LPR>(s, lds, half);
+        const float mean = s[0] * over;
+        s[0] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int left = a.width - (j * LPR + lane) * V;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = e < left ? (float)x[j][e] - mean : 0.f;
+                s[0] = fmaf(d, d, s[0]);
+            }
+        }
+        row_sum<LPR>(s, lds, half);
+        const float rstd = 1.f / sqrtf(fmaf(s[0], over, a.epsilon));
+        if (!live) continue;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            Some<T, V> y;
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] = (T)fmaf(((float)x[j][e] - mean) * rstd, (float)w[j][e], (float)b[j][e]);
+            store_some<T, V>((T*)a.y + r * a.y_stride, (j * LPR + lane) * V, a.width, y);
+        }
+        if (a.stats_out && lane == 0) {
+            a.stats_out[2 * r] = mean;
+            a.stats_out[2 * r + 1] = rstd;
+        }
+    }
+}
+
+template <typename T, typename W, int LPR, int NV, int NT>
+__global__ __launch_bounds__(NT) void k_norm_backward(const NormArgs a) {
+    constexpr int V = kVector<T>, R = NT / LPR;
+    constexpr bool kAhead = NT < 1024 || NV == 1;  // the next row on its way, where the registers hold it
+    extern __shared__ float sums[];  // R > 1: [2][LPR * NV * V]
+    __shared__ float lds[4 * (NT / 64)];
+    int half = 0;
+    const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
+    Some<W, V> w[NV];
+    float dw[NV][V], db[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[j][e] = (W)1.f, dw[j][e] = db[j][e] = 0.f;
+        if (kAhead && a.weight) w[j] = load_some<W, V>((const W*)a.weight, (j * LPR + lane) * V, a.width);
+    }
+    // the weights, from registers or, where the sums take those, from the cache
+    const auto weight = [&](int j) {
+        if constexpr (kAhead) return w[j];
+        if (a.weight) return load_some<W, V>((const W*)a.weight, (j * LPR + lane) * V, a.width);
+        return Some<W, V>((W)1.f);
+    };
+    Some<T, V> nx[NV], ng[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) nx[j] = ng[j] = (T)0.f;
+    float nmean = 0.f, nrstd = 0.f;
+    const auto fetch = [&](long long r) {
+        if (r >= a.rows) return;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            nx[j] = load_some<T, V>((const T*)a.x + r * a.x_stride, (j * LPR + lane) * V, a.width);
+            ng[j] = load_some<T, V>((const T*)a.dy + r * a.dy_stride, (j * LPR + lane) * V, a.width);
+        }
+        nmean = a.stats_in[2 * r];
+        nrstd = a.stats_in[2 * r + 1];
+    };
+    const float over = 1.f / (float)a.width;
+    const long long stride = (long long)gridDim.x * R;
+    if constexpr (kAhead) fetch((long long)blockIdx.x * R + group);
+    for (long long r0 = (long long)blockIdx.x * R; r0 < a.rows; r0 += stride) {
+        const long long r = r0 + group;
+        const bool live = r < a.rows;
+        if constexpr (!kAhead) fetch(r);
+        Some<T, V> x[NV], dy[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) x[j] = nx[j], dy[j] = ng[j];
+        const float mean = nmean, rstd = nrstd;
+        if constexpr (kAhead) fetch(r + stride);
+        float s[2] = {0.f, 0.f};
+        if (live)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const Some<W, V> wj = weight(j);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {  // past the row's end dy is zero
+                    const float n = ((float)x[j][e] - mean) * rstd, d = (float)dy[j][e], g = d * (float)wj[e];
+                    dw[j][e] = fmaf(d, n, dw[j][e]);
+                    db[j][e] += d;
+                    s[0] += g;
+                    s[1] = fmaf(g, n, s[1]);
+                }
+            }
+        if (!a.y) continue;
+        row_sum<LPR>(s, lds, half);
+        if (!live) continue;
+        const float m1 = s[0] * over, m2 = s[1] * over;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            Some<T, V> dx;
+            const Some<W, V> wj = weight(j);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float n = ((float)x[j][e] - mean) * rstd, g = (float)dy[j][e] * (float)wj[e];
+                dx[e] = (T)((g - m1 - n * m2) * rstd);
+            }
+            store_some<T, V>((T*)a.y + r * a.y_stride, (j * LPR + lane) * V, a.width, dx);
+        }
+    }
+    if (!a.dweight && !a.dbias) return;
+    // the block's rows side by side: lanes of a wave, then its waves one after the other
+    if constexpr (LPR < 64)
+#pragma unroll
+        for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    dw[j][e] += __shfl_xor(dw[j][e], o);
+                    db[j][e] += __shfl_xor(db[j][e], o);
+                }
+    if constexpr (R > 1) {
+        constexpr int turns = LPR < 64 ? NT / 64 : R, D = LPR * NV * V;
+        const int turn = LPR < 64 ? (int)(threadIdx.x >> 6) : group;
+        const bool mine = LPR >= 64 || (threadIdx.x & 63) < LPR;
+        for (int t = 0; t < turns; ++t) {
+            if (t == turn && mine)
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const int c = (j * LPR + lane) * V + e;
+                        if (t) dw[j][e] += sums[c], db[j][e] += sums[D + c];
+                        if (t + 1 < turns) sums[c] = dw[j][e], sums[D + c] = db[j][e];
+                    }
+            __syncthreads();
+        }
+        if (turn != turns - 1 || !mine) return;
+    }
+    // one block: its sums are the gradients
+    const bool last = gridDim.x == 1;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * LPR + lane) * V;
+        if (last) {
+            Some<W, V> p, q;
+#pragma unroll
+            for (int e = 0; e < V; ++e) p[e] = (W)dw[j][e], q[e] = (W)db[j][e];
+            if (a.dweight) store_some<W, V>((W*)a.dweight, c, a.width, p);
+            if (a.dbias) store_some<W, V>((W*)a.dbias, c, a.width, q);
+        } else {
+            Some<float, V> p, q;
+#pragma unroll
+            for (int e = 0; e < V; ++e) p[e] = dw[j][e], q[e] = db[j][e];
+            store_some<float, V>(a.partial + (long long)blockIdx.x * 2 * a.width, c, a.width, p);
+            store_some<float, V>(a.partial + ((long long)blockIdx.x * 2 + 1) * a.width, c, a.width, q);
+        }
+    }
+}
+
+// Adds the blocks' sums: 64 columns a block, its 16 waves each an equal share
+// of the blocks in their order. blockIdx.y: weight or bias.
+template <typename W>
+__global__ __launch_bounds__(1024) void k_norm_backward_sum(const NormArgs a, int parts) {
+    __shared__ float lds[16][64];
+    W* const to = (W*)(blockIdx.y ? a.dbias : a.dweight);
+    if (!to) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + lane;
+    const int first = (int)((long long)parts * wave / 16), end = (int)((long long)parts * (wave + 1) / 16);
+    float s = 0.f;
+    if (c < a.width) {
+        const float* p = a.partial + (long long)blockIdx.y * a.width + c;
+#pragma unroll 8
+        for (int i = first; i < end; ++i) s += p[(long long)i * 2 * a.width];
+    }
+    lds[wave][lane] = s;
+    __syncthreads();
+    if (wave || c >= a.width) return;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += lds[i][lane];
+    to[c] = (W)s;
+}
+
+// ---- rows too wide for a block's registers: read once for each sum
+
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void k_norm_forward_wide(const NormArgs a) {
+    __shared__ float lds[2 * 16];
+    int half = 0;
+    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = (const T*)a.x + r * a.x_stride;
+        T* y = (T*)a.y + r * a.y_stride;
+        float s[1] = {0.f};
+        for (int i = threadIdx.x; i < a.width; i += 1024) s[0] += (float)x[i];
+        row_sum<1024>(s, lds, half);
+        const float mean = s[0] / (float)a.width;
+        s[0] = 0.f;
+        for (int i = threadIdx.x; i < a.width; i += 1024) {
+            const float d = (float)x[i] - mean;
+            s[0] = fmaf(d, d, s[0]);
+        }
+        row_sum<1024>(s, lds, half);
+        const float rstd = 1.0f / sqrtf(s[0] / (float)a.width + a.epsilon);
+        for (int i = threadIdx.x; i < a.width; i += 1024) {
+            const float w = a.weight ? (float)((const W*)a.weight)[i] : 1.f;
+            const float b = a.bias ? (float)((const W*)a.bias)[i] : 0.f;
+            y[i] = (T)fmaf(((float)x[i] - mean) * rstd, w, b);
+        }
+        if (a.stats_out && threadIdx.x == 0) {
+            a.stats_out[2 * r] = mean;
+            a.stats_out[2 * r + 1] = rstd;
+        }
+    }
+}
+
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void k_norm_backward_wide(const NormArgs a) {
+    __shared__ float lds[4 * 16];
+    int half = 0;
+    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = (const T*)a.x + r * a.x_stride;
+        const T* dy = (const T*)a.dy + r * a.dy_stride;
+        T* dx = (T*)a.y + r * a.y_stride;
+        const float mean = a.stats_in[2 * r], rstd = a.stats_in[2 * r + 1];
+        float s[2] = {0.f, 0.f};
+        for (int i = threadIdx.x; i < a.width; i += 1024) {
+            const float g = (float)dy[i] * (a.weight ? (float)((const W*)a.weight)[i] : 1.f);
+            s[0] += g;
+            s[1] = fmaf(g, ((float)x[i] - mean) * rstd, s[1]);
+        }
+        row_sum<1024>(s, lds, half);
+        const float m1 = s[0] / (float)a.width, m2 = s[1] / (float)a.width;
+        for (int i = threadIdx.x; i < a.width; i += 1024) {
+            const float g = (float)dy[i] * (a.weight ? (float)((const W*)a.weight)[i] : 1.f);
+            dx[i] = (T)((g - m1 - ((float)x[i] - mean) * rstd * m2) * rstd);
+        }
+    }
+}
+
+// Sums over every gridDim.y-th row, a thread a column.
+template <typename T>
+__global__ __launch_bounds__(256) void k_norm_backward_wide_rows(const NormArgs a) {
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= a.width) return;
     float dw = 0.f, db = 0.f;
     for (long long r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const float g = to_f32(((const T*)a.dy)[r * a.dy_stride + c]);
-        dw += g * (to_f32(((const T*)a.x)[r * a.x_stride + c]) - a.stats_in[2 * r]) * a.stats_in[2 * r + 1];
+        const float g = (float)((const T*)a.dy)[r * a.dy_stride + c];
+        dw = fmaf(g, ((float)((const T*)a.x)[r * a.x_stride + c] - a.stats_in[2 * r]) * a.stats_in[2 * r + 1], dw);
         db += g;
     }
     a.partial[(long long)blockIdx.y * 2 * a.width + c] = dw;
@@ -85,36 +383,74 @@ __global__ __launch_bounds__(256) void k_norm_backward_rows(const NormArgs a) {
 }
 
 template <typename W>
-__global__ __launch_bounds__(256) void k_norm_backward_sum(const NormArgs a, int parts) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= a.width) return;
-    float dw = 0.f, db = 0.f;
-    for (int p = 0; p < parts; ++p) {
-        dw += a.partial[(long long)p * 2 * a.width + c];
-        db += a.partial[((long long)p * 2 + 1) * a.width + c];
-    }
-    if (a.dweight) ((W*)a.dweight)[c] = (W)dw;
-    if (a.dbias) ((W*)a.dbias)[c] = (W)db;
+void launch_sum(const NormArgs& a, int parts, hipStream_t s) {
+    hipLaunchKernelGGL((k_norm_backward_sum<W>), dim3((unsigned)((a.width + 63) / 64), 2), dim3(1024), 0, s, a, parts);
 }
 
-constexpr int kParts = 64;
+template <typename T, typename W, int LPR, int NV, int NT>
+int forward_with(const NormArgs& a, hipStream_t s) {
+    constexpr int R = NT / LPR;
+    // blocks that fill the CUs; further rows in their loop, which reads a row ahead
+    const long long blocks = std::min((a.rows + R - 1) / R, (long long)a.cus * (2048 / NT));
+    hipLaunchKernelGGL((k_norm_forward<T, W, LPR, NV, NT>), dim3((unsigned)blocks), dim3(NT), 0, s, a);
+    return (int)hipGetLastError();
+}
 
+template <typename T, typename W, int LPR, int NV, int NT>
+int backward_with(const NormArgs& a, hipStream_t s) {
+    constexpr int R = NT / LPR;
+    // one block a CU: every block costs a row of sums to write and to add
+    const long long blocks = std::min((a.rows + R - 1) / R, (long long)a.cus);
+    const size_t lds = R > 1 ? sizeof(float) * 2 * LPR * NV * kVector<T> : 0;
+    hipLaunchKernelGGL((k_norm_backward<T, W, LPR, NV, NT>), dim3((unsigned)blocks), dim3(NT), lds, s, a);
+    if (blocks > 1 && (a.dweight || a.dbias)) launch_sum<W>(a, (int)blocks, s);
+    return (int)hipGetLastError();
+}
+
+// By vectors in a row: lanes of a wave as long as a lane's vectors fit its
+// registers well, then a block.
 template <typename T, typename W>
 int forward_as(const NormArgs& a, hipStream_t s) {
-    if (a.rows) hipLaunchKernelGGL((k_norm_forward<T, W>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    const int n = (a.width + kVector<T> - 1) / kVector<T>;
+    if (n <= 8) return forward_with<T, W, 8, 1, 256>(a, s);
+    if (n <= 16) return forward_with<T, W, 16, 1, 256>(a, s);
+    if (n <= 32) return forward_with<T, W, 32, 1, 256>(a, s);
+    if (n <= 64) return forward_with<T, W, 64, 1, 256>(a, s);
+    if (n <= 128) return forward_with<T, W, 64, 2, 256>(a, s);
+    if (n <= 256) return forward_with<T, W, 64, 4, 256>(a, s);
+    if (n <= 512) return forward_with<T, W, 128, 4, 256>(a, s);
+    if (n <= 1024) return forward_with<T, W, 256, 4, 256>(a, s);
+    if (n <= 2048) return forward_with<T, W, 512, 4, 512>(a, s);
+    if (n <= 4096) return forward_with<T, W, 1024, 4, 1024>(a, s);
+    hipLaunchKernelGGL((k_norm_forward_wide<T, W>), dim3((unsigned)std::min(a.rows, (long long)a.cus * 2)), dim3(1024), 0, s, a);
     return (int)hipGetLastError();
 }
 
 template <typename T, typename W>
 int backward_as(const NormArgs& a, hipStream_t s) {
+    if (!a.rows) {
+        if (a.dweight || a.dbias) launch_sum<W>(a, 0, s);
+        return (int)hipGetLastError();
+    }
+    const int n = (a.width + kVector<T> - 1) / kVector<T>;
+    if (n <= 8) return backward_with<T, W, 8, 1, 1024>(a, s);
+    if (n <= 16) return backward_with<T, W, 16, 1, 1024>(a, s);
+    if (n <= 32) return backward_with<T, W, 32, 1, 1024>(a, s);
+    if (n <= 64) return backward_with<T, W, 64, 1, 1024>(a, s);
+    if (n <= 128) return backward_with<T, W, 64, 2, 512>(a, s);
+    if (n <= 256) return backward_with<T, W, 64, 4, 512>(a, s);
+    if (n <= 512) return backward_with<T, W, 128, 4, 512>(a, s);
+    if (n <= 1024) return backward_with<T, W, 256, 4, 512>(a, s);
+    if (n <= 2048) return backward_with<T, W, 512, 4, 512>(a, s);
+    if (n <= 4096) return backward_with<T, W, 1024, 4, 1024>(a, s);
     // dx may overwrite dy: the sums over the rows go first
     if (a.dweight || a.dbias) {
-        const unsigned cols = (unsigned)((a.width + 255) / 256);
-        const int parts = (int)(a.rows < kParts ? a.rows : kParts);
-        if (parts) hipLaunchKernelGGL((k_norm_backward_rows<T>), dim3(cols, parts), dim3(256), 0, s, a);
-        hipLaunchKernelGGL((k_norm_backward_sum<W>), dim3(cols), dim3(256), 0, s, a, parts);
+        const int parts = (int)std::min(a.rows, 64ll);
+        hipLaunchKernelGGL((k_norm_backward_wide_rows<T>), dim3((unsigned)((a.width + 255) / 256), parts), dim3(256), 0, s, a);
+        launch_sum<W>(a, parts, s);
     }
-    if (a.y && a.rows) hipLaunchKernelGGL((k_norm_backward_x<T, W>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    if (a.y)
+        hipLaunchKernelGGL((k_norm_backward_wide<T, W>), dim3((unsigned)std::min(a.rows, (long long)a.cus * 2)), dim3(1024), 0, s, a);
     return (int)hipGetLastError();
 }
 
@@ -134,6 +470,8 @@ int pick_element(const NormArgs& a, hipStream_t s, bool forward) {
 
 int launch_norm_forward(const NormArgs& a, hipStream_t s) { return pick_element(a, s, true); }
 int launch_norm_backward(const NormArgs& a, hipStream_t s) { return pick_element(a, s, false); }
-size_t norm_workspace_bytes(int width, int cus) { return (size_t)kParts * 2 * (size_t)width * sizeof(float); }
+size_t norm_workspace_bytes(int width, int cus) {
+    return (size_t)std::max(cus, 64) * 2 * (size_t)width * sizeof(float);
+}
 
 }  // namespace vkfx
