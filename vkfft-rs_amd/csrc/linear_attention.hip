@@ -127,9 +127,9 @@ size_t scan_work_floats(int element, int dk, int dv, int heads, int count, long 
     return most > 1 ? (size_t)states * dk * dv : 0;
 }
 
-int launch_scans(int element, const ScanArgs* scans, int count, const float* powers, float* work, hipStream_t s) {
+int launch_scans(int element, const ScanArgs* scans, int count, const float* powers, float* work, int cus, hipStream_t s) {
     // the recurrence itself while a chunk would be mostly empty
-    if (scans[0].tokens <= 8) return launch_scan_recurrent(element, scans, count, powers, s);
+    if (scans[0].tokens <= kStepTokens) return launch_steps(element, scans, count, powers, cus, s);
     // scans of one shape run side by side
     for (int i = 0; i < count;) {
         int j = i + 1;

@@ -1,4 +1,11 @@
-// linear_step.hip -- linear attention token by token: the recurrence itself.
+// linear_step.hip -- linear attention of one token of each sequence, or a few:
+// the recurrence itself.
+//
+// Bound by memory: the state is read and written once, 8 dk dv bytes a head
+// against 4 dk dv operations a token. A block holds CS columns of one head's
+// state in its registers, four neighbours a lane and rows a fixed distance
+// apart, and asks for all of them before it waits for any. Sums over the rows
+// go through the lanes of a wave, then through LDS.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -10,85 +17,135 @@ namespace vkfx {
 
 namespace {
 
-constexpr int kColumns = 16;             // state columns of a block
-constexpr int kRowGroups = 16;           // threads along the rows of a column
-constexpr int kRowsMost = 256 / kRowGroups;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-// A block holds kColumns columns of one sequence's and head's state, a thread
-// one column of every kRowGroups-th row, and walks the tokens.
-template <typename T>
-__global__ __launch_bounds__(256) void k_scan_recurrent(const ScanArgs s, const float* __restrict__ powers) {
-    __shared__ float part[kRowGroups][kColumns];
-    const int h = blockIdx.y, b = blockIdx.z;
-    const int col = threadIdx.x % kColumns, row0 = threadIdx.x / kColumns;
-    const int c = blockIdx.x * kColumns + col;
-    const bool live = c < s.dv;
-    long long n = s.tokens;
-    if (s.lengths) {
-        const long long l = s.lengths[b];
-        n = l < 0 ? 0 : l < n ? l : n;
-    }
-    // the decay in two parts: its rounding to 32 bits would grow with the
-    // tokens that a long memory spans
-    const float decay = powers[(long long)h * kDecayPowers + 1];
-    const float decay_low = powers[(long long)h * kDecayPowers + kDecayPowers - 1];
+// CS columns a block, up to NR rows a thread. PACKED: a state's columns are
+// neighbours in memory (they are not where a gradient reads its transpose).
+template <typename T, int CS, int NR, bool PACKED>
+__global__ __launch_bounds__(256) void k_step(const ScanArgs s, const float* __restrict__ powers) {
+    constexpr int LX = CS / 4, RY = 256 / LX, RW = 64 / LX;  // lanes along a row, rows of the block and of a wave
+    __shared__ float la[kStepTokens][256], lb[kStepTokens][256], lc[kStepTokens][CS];
+    __shared__ float part[kStepTokens][4][CS];
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const int row0 = tid / LX, x0 = tid % LX * 4;
+    const int col0 = blockIdx.x * CS, col = col0 + x0;
+    int n = (int)s.tokens;
+    if (s.lengths) n = s.lengths[b] < 0 ? 0 : s.lengths[b] < n ? s.lengths[b] : n;
     const long long st = ((long long)b * s.heads + h) * s.dk * s.dv;
-    float x[kRowsMost];
+
+    // Rows past the last read the last one again and never change an output:
+    // every load is on its way before the first is waited for.
+    f32x4 X[NR];
+    const bool four = PACKED && col + 4 <= s.dv;
+    if (!s.state_in) {
 #pragma unroll
-    for (int k = 0; k < kRowsMost; ++k) {
-        const int r = row0 + k * kRowGroups;
-        x[k] = live && r < s.dk && s.state_in ? s.state_in[st + (long long)r * s.state_row + (long long)c * s.state_col] : 0.f;
+        for (int k = 0; k < NR; ++k) X[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    } else if (four) {
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+            const int r = row0 + k * RY < s.dk ? row0 + k * RY : s.dk - 1;
+            X[k] = *(const f32x4_any*)(s.state_in + st + (long long)r * s.state_row + col);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+            const int r = row0 + k * RY < s.dk ? row0 + k * RY : s.dk - 1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                X[k][e] = col + e < s.dv ? s.state_in[st + (long long)r * s.state_row + (long long)(col + e) * s.state_col] : 0.f;
+        }
     }
+    // the tokens' rows, in the order of the scan
     const T* A = (const T*)s.a.p + b * s.a.batch + (h / s.a.group) * s.a.head;
     const T* B = (const T*)s.b.p + b * s.b.batch + (h / s.b.group) * s.b.head;
     const T* C = (const T*)s.c.p + b * s.c.batch + (h / s.c.group) * s.c.head;
-    const long long ob = b * s.out_batch + h * s.out_head;
-    for (long long i = 0; i < s.tokens; ++i) {
-        const bool inside = i < n;
-        const long long t = s.reverse && inside ? n - 1 - i : i;
-        float o = 0.f;
-        if (inside) {
-            const float cv = live ? (float)C[t * s.c.token + c] * s.scale_update : 0.f;
+    for (int i = 0; i < n; ++i) {
+        const long long t = s.reverse ? n - 1 - i : i;
+        la[i][tid] = tid < s.dk ? (float)A[t * s.a.token + tid] : 0.f;
+        lb[i][tid] = tid < s.dk ? (float)B[t * s.b.token + tid] : 0.f;
+        if (tid < CS) lc[i][tid] = col0 + tid < s.dv ? (float)C[t * s.c.token + col0 + tid] * s.scale_update : 0.f;
+    }
+    // the decay in two parts, so that its rounding does not grow token by token
+    const float decay = powers[(long long)h * kDecayPowers + 1];
+    const float decay_low = powers[(long long)h * kDecayPowers + kDecayPowers - 1];
+    __syncthreads();
+    for (int i = 0; i < n; ++i) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        const f32x4 c = *(const f32x4*)&lc[i][x0];
 #pragma unroll
-            for (int k = 0; k < kRowsMost; ++k) {
-                const int r = row0 + k * kRowGroups;
-                if (r < s.dk) {
-                    if (!s.reverse) x[k] = fmaf(x[k], decay, x[k] * decay_low);
-                    x[k] = fmaf((float)B[t * s.b.token + r], cv, x[k]);
-                    o = fmaf((float)A[t * s.a.token + r], x[k], o);
-                    if (s.reverse) x[k] = fmaf(x[k], decay, x[k] * decay_low);
-                }
+        for (int k = 0; k < NR; ++k) {
+            const int r = row0 + k * RY;
+            const float av = la[i][r], bv = lb[i][r];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x = X[k][e];
+                if (!s.reverse) x = fmaf(x, decay, x * decay_low);
+                x = fmaf(bv, c[e], x);
+                o[e] = fmaf(av, x, o[e]);
+                if (s.reverse) x = fmaf(x, decay, x * decay_low);
+                X[k][e] = x;
             }
         }
-        __syncthreads();
-        part[row0][col] = o;
-        __syncthreads();
-        if (row0 == 0 && live) {
-            float sum = 0.f;
-            for (int g = 0; g < kRowGroups; ++g) sum += part[g][col];
-            sum *= s.scale_in;
-            const long long at = ob + t * s.out_token + c;
-            if (s.out_f32) ((float*)s.out)[at] = sum;
-            else ((T*)s.out)[at] = (T)sum;
-        }
-    }
-    if (s.state_out)
 #pragma unroll
-        for (int k = 0; k < kRowsMost; ++k) {
-            const int r = row0 + k * kRowGroups;
-            if (live && r < s.dk) s.state_out[st + (long long)r * s.state_row + (long long)c * s.state_col] = x[k];
-        }
+        for (int d = LX; d < 64; d <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], d);
+        if ((tid & 63) < LX) *(f32x4*)&part[i][tid >> 6][x0] = o;
+    }
+    if (s.state_out && four) {
+#pragma unroll
+        for (int k = 0; k < NR; ++k)
+            if (row0 + k * RY < s.dk) *(f32x4_any*)(s.state_out + st + (long long)(row0 + k * RY) * s.state_row + col) = X[k];
+    } else if (s.state_out) {
+#pragma unroll
+        for (int k = 0; k < NR; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (row0 + k * RY < s.dk && col + e < s.dv)
+                    s.state_out[st + (long long)(row0 + k * RY) * s.state_row + (long long)(col + e) * s.state_col] = X[k][e];
+    }
+    __syncthreads();
+    for (int j = tid; j < (int)s.tokens * CS; j += 256) {
+        const int i = j / CS, c = j % CS;
+        if (col0 + c >= s.dv) continue;
+        const float y = i < n ? ((part[i][0][c] + part[i][1][c]) + (part[i][2][c] + part[i][3][c])) * s.scale_in : 0.f;
+        const long long t = s.reverse && i < n ? n - 1 - i : i;
+        const long long at = b * s.out_batch + t * s.out_token + h * s.out_head + col0 + c;
+        if (s.out_f32) ((float*)s.out)[at] = y;
+        else ((T*)s.out)[at] = (T)y;
+    }
+}
+
+template <typename T, int CS, int NR>
+void launch_as(const ScanArgs& a, const float* powers, hipStream_t s) {
+    const dim3 grid((unsigned)((a.dv + CS - 1) / CS), (unsigned)a.heads, (unsigned)a.batch);
+    if (a.state_col == 1) hipLaunchKernelGGL((k_step<T, CS, NR, true>), grid, dim3(256), 0, s, a, powers);
+    else hipLaunchKernelGGL((k_step<T, CS, NR, false>), grid, dim3(256), 0, s, a, powers);
+}
+
+// 64 columns a block, a fourth of that while those blocks are fewer than the
+// GPU's CUs: a small batch's latency is a block's share of the state.
+template <typename T>
+void launch_element(const ScanArgs& a, const float* powers, int cus, hipStream_t s) {
+    const long long blocks = (long long)a.batch * a.heads * ((a.dv + 63) / 64);
+    if (blocks >= cus) {
+        if (a.dk <= 64) launch_as<T, 64, 4>(a, powers, s);
+        else if (a.dk <= 128) launch_as<T, 64, 8>(a, powers, s);
+        else launch_as<T, 64, 16>(a, powers, s);
+    } else {
+        if (a.dk <= 128) launch_as<T, 16, 2>(a, powers, s);
+        else launch_as<T, 16, 4>(a, powers, s);
+    }
 }
 
 }  // namespace
 
-int launch_scan_recurrent(int element, const ScanArgs* scans, int count, const float* powers, hipStream_t s) {
+int launch_steps(int element, const ScanArgs* scans, int count, const float* powers, int cus, hipStream_t s) {
     for (int i = 0; i < count; ++i) {
-        const ScanArgs& a = scans[i];
-        const dim3 grid((unsigned)((a.dv + kColumns - 1) / kColumns), (unsigned)a.heads, (unsigned)a.batch);
-        if (element == VKFX_ELEMENT_F32) hipLaunchKernelGGL(k_scan_recurrent<float>, grid, dim3(256), 0, s, a, powers);
-        else if (element == VKFX_ELEMENT_F16) hipLaunchKernelGGL(k_scan_recurrent<_Float16>, grid, dim3(256), 0, s, a, powers);
-        else hipLaunchKernelGGL(k_scan_recurrent<__bf16>, grid, dim3(256), 0, s, a, powers);
+        if (element == VKFX_ELEMENT_F32) launch_element<float>(scans[i], powers, cus, s);
+        else if (element == VKFX_ELEMENT_F16) launch_element<_Float16>(scans[i], powers, cus, s);
+        else launch_element<__bf16>(scans[i], powers, cus, s);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
     }

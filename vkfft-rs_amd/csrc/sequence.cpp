@@ -324,7 +324,8 @@ int vkfx_linear_attention_forward(vkfx_linear_attention* plan, const vkfx_linear
         s.scale_update = 1.f;
         (void)hipSetDevice(plan->ctx->device);
         float* work = (float*)(d_work ? d_work : plan->work.p);
-        const int e = launch_scans(d.element, &s, 1, (const float*)plan->powers.p, work, stream_of(plan->ctx, stream));
+        const int e = launch_scans(d.element, &s, 1, (const float*)plan->powers.p, work, (int)plan->ctx->profile.compute_units,
+                                   stream_of(plan->ctx, stream));
         return e == hipSuccess ? VKFX_OK : hip_fail((hipError_t)e, "launch linear attention");
     });
 }
@@ -399,7 +400,7 @@ int vkfx_linear_attention_backward(vkfx_linear_attention* plan, const vkfx_linea
         }
         (void)hipSetDevice(plan->ctx->device);
         hipStream_t st = stream_of(plan->ctx, stream);
-        int e = launch_scans(d.element, scans, 3, (const float*)plan->powers.p, work, st);
+        int e = launch_scans(d.element, scans, 3, (const float*)plan->powers.p, work, (int)plan->ctx->profile.compute_units, st);
         if (e == hipSuccess && group > 1 && t) {
             e = launch_group_sum(d.element, wk, side(args->dk, 1), (long long)b, (long long)t, (int)d.kv_heads, group, dk, st);
             if (e == hipSuccess)

@@ -68,13 +68,14 @@ struct ScanArgs {
 // one is what 32 bits leave of the decay itself (decay - powers[1]).
 constexpr int kDecayPowers = 72;
 
-// Token by token (linear_step.hip).
-int launch_scan_recurrent(int element, const ScanArgs* scans, int count, const float* powers, hipStream_t s);
+// Up to kStepTokens tokens one after the other (linear_step.hip).
+constexpr int kStepTokens = 8;
+int launch_steps(int element, const ScanArgs* scans, int count, const float* powers, int cus, hipStream_t s);
 
 // `count` scans (up to 3) of the same batch, tokens and heads, by the kernels
 // that suit the number of tokens (linear_attention.hip). `work` holds
 // scan_work_floats of every shape among them.
-int launch_scans(int element, const ScanArgs* scans, int count, const float* powers, float* work, hipStream_t s);
+int launch_scans(int element, const ScanArgs* scans, int count, const float* powers, float* work, int cus, hipStream_t s);
 size_t scan_work_floats(int element, int dk, int dv, int heads, int count, long long max_batch, long long max_tokens);
 
 // Sums the floats [batch][token][head][dim] of each shared head's `group`

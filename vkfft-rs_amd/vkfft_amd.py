@@ -1378,14 +1378,6 @@ def _torch_type(element: Element):
     return {Element.F32: torch.float32, Element.F16: torch.float16, Element.BF16: torch.bfloat16}[element]
 
 
-def _raw_stream(stream, device):
-    """The stream of a call on torch tensors: `stream`, or torch's current one
-    on their device. Its default stream is the null stream, which the C ABI
-    knows by hipStreamLegacy (1)."""
-    import torch
-    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream or 1
-
-
 @dataclass
 class LayerNormConfig:
     """Layer norm of rows of `width` elements: (x - mean) rstd weight + bias."""
@@ -1434,35 +1426,52 @@ class _SequencePlan:
         _check(getattr(self._L, f"vkfx_{self._kind}_workspace_bytes")(self.handle, ctypes.byref(w)), self._L)
         self.workspace_bytes = int(w.value)
         self._type = _torch_type(config.element)
+        self._f32 = _torch_type(Element.F32)
+        import torch
+        # 0.1 us where torch.cuda.current_stream takes 1.1, of a call's 5
+        self._current = getattr(torch._C, "_cuda_getCurrentRawStream", None) \
+            or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
-    def _place(self, x):
-        """The device of a call, which is the context's."""
-        if not x.is_cuda:
+    def _stream(self, stream, device: int) -> int:
+        """The stream of a call: `stream`, or torch's current one on the
+        device. Its default stream is the null stream, which the C ABI knows by
+        hipStreamLegacy (1)."""
+        return (self._current(device) if stream is None else stream.cuda_stream) or 1
+
+    # A call costs a few microseconds on the GPU, so the checks below take the
+    # cheapest of what a tensor tells: get_device() is -1 on the host.
+
+    @staticmethod
+    def _place(x) -> int:
+        """The device of a call's tensors."""
+        device = x.get_device()
+        if device < 0:
             raise VkFftError(-7, "tensors must be device tensors")
-        return x.device
+        return device
 
-    def _tensor(self, name, x, shape, dtype, device):
-        if tuple(x.shape) != shape:
-            raise VkFftError(-5, f"{name}: expected shape {shape}, got {tuple(x.shape)}")
+    @staticmethod
+    def _refuse(name, x, shape, dtype, device):
+        if x.shape != shape:
+            raise VkFftError(-5, f"{name}: expected shape {tuple(shape)}, got {tuple(x.shape)}")
         if x.dtype != dtype:
             raise VkFftError(-4, f"{name}: expected {dtype}, got {x.dtype}")
-        if x.device != device:
-            raise VkFftError(-7, f"{name} must be on {device}")
+        if x.get_device() != device:
+            raise VkFftError(-7, f"{name} must be on device {device}")
+        raise VkFftError(-7, f"{name} must be contiguous")
 
     def _dense(self, name, x, shape, dtype, device):
         """Address of a contiguous tensor, or None."""
         if x is None:
             return None
-        self._tensor(name, x, shape, dtype, device)
-        if not x.is_contiguous():
-            raise VkFftError(-7, f"{name} must be contiguous")
+        if x.shape != shape or x.dtype is not dtype or x.get_device() != device or not x.is_contiguous():
+            self._refuse(name, x, shape, dtype, device)
         return x.data_ptr()
 
     def _work(self, work, device):
         if work is None:
             return None
-        if work.device != device or not work.is_contiguous() or work.numel() * work.element_size() < self.workspace_bytes:
-            raise VkFftError(-5, f"work must be {self.workspace_bytes} contiguous bytes on {device}")
+        if work.get_device() != device or not work.is_contiguous() or work.numel() * work.element_size() < self.workspace_bytes:
+            raise VkFftError(-5, f"work must be {self.workspace_bytes} contiguous bytes on device {device}")
         return work.data_ptr()
 
     def close(self):
@@ -1488,9 +1497,11 @@ class LayerNormPlan(_SequencePlan):
         self._weight_type = _torch_type(config.element if config.weight_element is None else config.weight_element)
 
     def _rows(self, name, x, rows, device):
-        self._tensor(name, x, (rows, self.config.width), self._type, device)
+        width = self.config.width
+        if x.shape != (rows, width) or x.dtype is not self._type or x.get_device() != device:
+            self._refuse(name, x, (rows, width), self._type, device)
         row, column = x.stride()
-        if column != 1 and self.config.width > 1:
+        if column != 1 and width > 1:
             raise VkFftError(-7, f"{name}: the last dimension must be contiguous")
         return x.data_ptr(), row
 
@@ -1503,7 +1514,7 @@ class LayerNormPlan(_SequencePlan):
         _check(self._L.vkfx_layer_norm_forward(
             self.handle, rows, xp, xs, self._dense("weight", weight, w, self._weight_type, device),
             self._dense("bias", bias, w, self._weight_type, device), yp, ys,
-            self._dense("stats", stats, (rows, 2), _torch_type(Element.F32), device), _raw_stream(stream, device)), self._L)
+            self._dense("stats", stats, (rows, 2), self._f32, device), self._stream(stream, device)), self._L)
 
     def backward_tensors(self, x, weight, stats, dy, dx=None, dweight=None, dbias=None, work=None, stream=None):
         """Gradients for dy; any of the three may be None (not wanted)."""
@@ -1514,10 +1525,10 @@ class LayerNormPlan(_SequencePlan):
         dp, ds = (None, 0) if dx is None else self._rows("dx", dx, rows, device)
         _check(self._L.vkfx_layer_norm_backward(
             self.handle, rows, xp, xs, self._dense("weight", weight, w, self._weight_type, device),
-            self._dense("stats", stats, (rows, 2), _torch_type(Element.F32), device), gp, gs, dp, ds,
+            self._dense("stats", stats, (rows, 2), self._f32, device), gp, gs, dp, ds,
             self._dense("dweight", dweight, w, self._weight_type, device),
             self._dense("dbias", dbias, w, self._weight_type, device), self._work(work, device),
-            _raw_stream(stream, device)), self._L)
+            self._stream(stream, device)), self._L)
 
 
 @dataclass
@@ -1591,15 +1602,15 @@ class LinearAttentionPlan(_SequencePlan):
         self._kv = config.heads if config.kv_heads is None else config.kv_heads
 
     def _sequence(self, name, x, shape, device):
-        self._tensor(name, x, shape, self._type, device)
+        if x.shape != shape or x.dtype is not self._type or x.get_device() != device:
+            self._refuse(name, x, shape, self._type, device)
         b, t, h, d = x.stride()
         if d != 1 and shape[3] > 1:
             raise VkFftError(-7, f"{name}: the last dimension must be contiguous")
         return x.data_ptr(), b, t, h
 
     def _states(self, shape, device, **states):
-        f32 = _torch_type(Element.F32)
-        return [self._dense(n, x, shape, f32, device) for n, x in states.items()]
+        return [self._dense(n, x, shape, self._f32, device) for n, x in states.items()]
 
     def _lengths(self, lengths, batch, device):
         if lengths is None:
@@ -1621,7 +1632,7 @@ class LinearAttentionPlan(_SequencePlan):
                             self._lengths(lengths, b, device),
                             *self._states((b, c.heads, c.key_dim, c.value_dim), device, state_in=state_in, state_out=state_out))
         _check(self._L.vkfx_linear_attention_forward(self.handle, ctypes.byref(args), self._work(work, device),
-                                                     _raw_stream(stream, device)), self._L)
+                                                     self._stream(stream, device)), self._L)
 
     def backward_tensors(self, q, k, v, dout, dq, dk, dv, state_in=None, dstate_out=None, dstate_in=None, lengths=None,
                          work=None, stream=None):
@@ -1640,7 +1651,7 @@ class LinearAttentionPlan(_SequencePlan):
                              *self._states((b, c.heads, c.key_dim, c.value_dim), device, state_in=state_in,
                                            dstate_out=dstate_out, dstate_in=dstate_in))
         _check(self._L.vkfx_linear_attention_backward(self.handle, ctypes.byref(args), self._work(work, device),
-                                                      _raw_stream(stream, device)), self._L)
+                                                      self._stream(stream, device)), self._L)
 
 
 class HipExecutionContext:
