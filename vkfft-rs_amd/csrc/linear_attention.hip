@@ -19,17 +19,28 @@ __global__ __launch_bounds__(256) void k_chunk_join(const ChunkArgs args) {
         const long long l = s.lengths[b];
         n = l < 0 ? 0 : l < n ? l : n;
     }
+    // the decay of a whole segment, by squaring
     const float* p = args.powers + (long long)h * kDecayPowers;
-    const float decay = (float)pow((double)p[1] + (double)p[kDecayPowers - 1], (double)args.segment);
+    double power = 1.0, square = (double)p[1] + (double)p[kDecayPowers - 1];
+    for (long long i = args.segment; i; i >>= 1, square *= square)
+        if (i & 1) power *= square;
+    const float decay = (float)power;
     const int row = e / s.dv, col = e % s.dv;
     const long long head = (long long)b * s.heads + h;
     float x = s.state_in ? s.state_in[head * size + (long long)row * s.state_row + (long long)col * s.state_col] : 0.f;
     float* slot = args.slots + ((long long)z * s.batch * s.heads + head) * args.segments * size + e;
+    // segments before the last that has tokens; eight are read before the first is needed
+    const int last = (int)((n + args.segment - 1) / args.segment);
     slot[0] = x;
-    for (int k = 1; k < args.segments && k * args.segment < n; ++k) {
-        slot += size;
-        x = fmaf(x, decay, *slot);
-        *slot = x;
+    for (int k = 1; k < last; k += 8) {
+        float added[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) added[u] = k + u < last ? slot[(long long)(k + u) * size] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            x = fmaf(x, decay, added[u]);
+            if (k + u < last) slot[(long long)(k + u) * size] = x;
+        }
     }
 }
 
@@ -56,19 +67,21 @@ const ChunkKernel* chunk_kernel(int element, int dk, int dv) {
                                          : chunk_kernel_bf16(dk, dv);
 }
 
-// Fewest blocks that keep the GPU's 256 CUs busy, two on each.
-constexpr long long kBlocks = 512;
+// Waves that keep the GPU's 256 CUs busy: two on each SIMD. (Half as many, with
+// fewer segments to join: bf16, 8 x 2048 tokens of 16 heads of 128, 114 us
+// instead of 88; 1 x 65536 of 16 heads of 64, 188 instead of 112.)
+constexpr long long kWaves = 2048;
 
 struct Split {
     int segments;
     long long segment;
 };
 
-// Where the blocks of whole sequences are fewer than half of kBlocks, the
-// tokens are split too: every segment but the last is read once more for its
+// Where the waves of whole sequences are fewer than half of kWaves, the tokens
+// are split too: every segment but the last is read once more for its
 // share of the state. A segment has four chunks or more.
-Split split_tokens(long long blocks, long long tokens, int chunk) {
-    long long k = blocks * 2 > kBlocks ? 1 : kBlocks / std::max(1ll, blocks);
+Split split_tokens(long long waves, long long tokens, int chunk) {
+    long long k = waves * 2 > kWaves ? 1 : kWaves / std::max(1ll, waves);
     k = std::max(1ll, std::min(k, tokens / (4 * chunk)));
     const long long chunks = (tokens + chunk - 1) / chunk;
     const long long each = (chunks + k - 1) / k;
@@ -78,13 +91,14 @@ Split split_tokens(long long blocks, long long tokens, int chunk) {
     return s;
 }
 
-int launch_with(const void* fn, long long blocks, size_t lds, const ChunkArgs& a, hipStream_t s) {
+int launch_with(const void* fn, long long blocks, const ChunkKernel* k, const ChunkArgs& a, hipStream_t s) {
+    const size_t lds = k->lds;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return (int)e;
     }
     void* kargs[1] = {(void*)&a};
-    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(256), kargs, lds, s);
+    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)blocks), dim3((unsigned)k->threads), kargs, lds, s);
     return e != hipSuccess ? (int)e : (int)hipGetLastError();
 }
 
@@ -100,7 +114,7 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
     a.scans = count;
     a.slices = (first.dv + k->cols - 1) / k->cols;
     const long long whole = (long long)count * first.batch * first.heads * a.slices;
-    const Split sp = split_tokens(whole, first.tokens, k->chunk);
+    const Split sp = split_tokens(whole * (k->threads / 64), first.tokens, k->chunk);
     a.segments = sp.segments;
     a.segment = sp.segment;
     a.powers = powers;
@@ -108,12 +122,12 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
     if (whole * a.segments > 0x7fffffffll) return (int)hipErrorInvalidConfiguration;
     if (a.segments > 1) {
         work += slot_floats(first, count, a.segments);
-        if (int e = launch_with(k->state_only, whole * a.segments, k->lds, a, st)) return e;
+        if (int e = launch_with(k->state_only, whole * a.segments, k, a, st)) return e;
         const dim3 grid((unsigned)((first.dk * first.dv + 255) / 256), (unsigned)(first.batch * first.heads), (unsigned)count);
         hipLaunchKernelGGL(k_chunk_join, grid, dim3(256), 0, st, a);
         if (hipError_t e = hipGetLastError()) return (int)e;
     }
-    return launch_with(k->run, whole * a.segments, k->lds, a, st);
+    return launch_with(k->run, whole * a.segments, k, a, st);
 }
 
 }  // namespace
@@ -121,9 +135,9 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
 size_t scan_work_floats(int element, int dk, int dv, int heads, int count, long long max_batch, long long max_tokens) {
     const ChunkKernel* k = chunk_kernel(element, dk, dv);
     const int slices = (dv + k->cols - 1) / k->cols;
-    // segments > 1 only below kBlocks blocks in all, and never over tokens / (4 chunk) of them
+    // segments > 1 only below kWaves waves in all, and never over tokens / (4 chunk) of them
     const long long most = std::max(1ll, max_tokens / (4 * k->chunk));
-    const long long states = std::min((long long)count * max_batch * heads * most, kBlocks / slices);
+    const long long states = std::min((long long)count * max_batch * heads * most, kWaves / (k->threads / 64) / slices);
     return most > 1 ? (size_t)states * dk * dv : 0;
 }
 

@@ -3,8 +3,8 @@
 //
 // For a chunk of C tokens and the state X before it (sequence.hpp has the
 // scan's definition; g the head's decay, n <= C the tokens that are left):
-//   P[i][j] = scale_update g^(i-j) (A[i] . B[j])           for j <= i, else 0
-//   out[i]  = scale_in ( g^(i+1-lead) A[i] X + sum_j P[i][j] C[j] )
+//   P[i][j] = scale_in scale_update g^(i-j) (A[i] . B[j])           for j <= i, else 0
+//   out[i]  = scale_in g^(i+1-lead) A[i] X + sum_j P[i][j] C[j]
 //   X      <- g^n X + scale_update sum_j g^(n-1-j+lead) B[j] C[j]^T
 // four products of small matrices, all on mfma 16x16x32 bf16 with f32 sums.
 //
@@ -15,9 +15,9 @@
 // update takes three always, since the state is an f32 result. Products of
 // parts that lie below the kept bits are left out.
 //
-// Four waves share the chunk's A, B, C and P in LDS. Each wave owns 16 NT of
-// the block's 64 NT columns of C, X and out, so that X stays in its
-// accumulators from the first token to the last. The layout of accumulators
+// A block's waves share the chunk's A, B, C and P in LDS. Each owns 16 NT
+// columns of C, X and out, so that X stays in its accumulators from the first
+// token to the last. The layout of accumulators
 // (lane: one column, four rows) is that of an operand (lane: one row or column,
 // eight along the summed axis) when that axis is taken in the order 0-3, 16-19
 // of lane group 0, 4-7, 20-23 of group 1, ...: X enters A X without moving, and
@@ -67,98 +67,199 @@ __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Sum of the products of parts whose orders add up to less than `orders`.
-template <int N, int M>
-__device__ __forceinline__ f32x4 mma_parts(const bf16x8 (&a)[N], const bf16x8 (&b)[M], f32x4 c, int orders) {
+// c[u] += sum of the products of a[u]'s and b[u]'s parts whose orders add up to
+// less than `orders`, small ones first. One product of every u before the next:
+// a product that adds to the one before it would wait for that.
+template <int U, int N, int M>
+__device__ __forceinline__ void mma_parts(const bf16x8 (&a)[U][N], const bf16x8 (&b)[U][M], f32x4 (&c)[U], int orders) {
 #pragma unroll
-    for (int o = N + M - 2; o >= 0; --o)  // small ones first
+    for (int o = N + M - 2; o >= 0; --o)
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < M; ++j)
-                if (i + j == o && o < orders) c = mma(a[i], b[j], c);
-    return c;
+                if (i + j == o && o < orders)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) c[u] = mma(a[u][i], b[u][j], c[u]);
+}
+// The same with one first operand for all.
+template <int U, int N, int M>
+__device__ __forceinline__ void mma_parts(const bf16x8 (&a)[N], const bf16x8 (&b)[U][M], f32x4* c, int orders) {
+#pragma unroll
+    for (int o = N + M - 2; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < M; ++j)
+                if (i + j == o && o < orders)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) c[u] = mma(a[i], b[u][j], c[u]);
+}
+// And with one second operand for all.
+template <int U, int N, int M>
+__device__ __forceinline__ void mma_parts(const bf16x8 (&a)[U][N], const bf16x8 (&b)[M], f32x4* c, int orders) {
+#pragma unroll
+    for (int o = N + M - 2; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < M; ++j)
+                if (i + j == o && o < orders)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) c[u] = mma(a[u][i], b[j], c[u]);
 }
 
-template <int N>
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[N]) {
-    float r[8];
+// x as a sum of N bf16 parts, each the rounding of what the ones before leave.
+// SUMMED: elements that meet in one sum. There v_dot2_f32_bf16 takes a part off
+// in one instruction, x - 1 p[0] - 0 p[1], exactly; elsewhere an infinite
+// neighbour must not make that a NaN.
+template <bool SUMMED, int N, int E, typename V>
+__device__ __forceinline__ void split(const float (&x)[E], V (&p)[N]) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned u32s __attribute__((ext_vector_type(E / 2)));
+    // in registers: as an immediate the instruction takes (-1, 0) for another value
+    unsigned first, second;
+    asm("s_mov_b32 %0, 0xbf80" : "=s"(first));
+    asm("s_mov_b32 %0, 0xbf800000" : "=s"(second));
+    u32s q[N];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = x[e];
+    for (int e = 0; e < E / 2; ++e) {
+        float a = x[2 * e], b = x[2 * e + 1];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            p[i][e] = (__bf16)r[e];
-            if (i + 1 < N) r[e] -= (float)p[i][e];
+        for (int i = 0; i < N; ++i) {
+            const bf16x2 both = __builtin_convertvector(f32x2{a, b}, bf16x2);
+            q[i][e] = __builtin_bit_cast(unsigned, both);
+            if (i + 1 == N) continue;
+            if constexpr (SUMMED) {
+                a = __builtin_amdgcn_fdot2_f32_bf16(both, __builtin_bit_cast(bf16x2, first), a, false);
+                b = __builtin_amdgcn_fdot2_f32_bf16(both, __builtin_bit_cast(bf16x2, second), b, false);
+            } else {
+                a -= __builtin_bit_cast(float, q[i][e] << 16);
+                b -= __builtin_bit_cast(float, q[i][e] & 0xffff0000u);
+            }
         }
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = __builtin_bit_cast(V, q[i]);
 }
 
-// Eight neighbours of a row at any alignment of its elements.
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Eight {
-    T v[8];
+using Eight = T __attribute__((ext_vector_type(8)));
+// The same in memory, at any alignment of its elements.
+template <typename T>
+struct PackedEight {
+    typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
 // One thread's share of a chunk of rows [C][D] on its way to LDS: vectors of
-// eight elements, read ahead while the chunk before is worked on.
-template <typename T, int C, int D>
+// eight elements at one column of every kRows-th row, read ahead while the
+// chunk before is worked on. The reads take no branch, which would make the
+// compiler wait for them on the spot: rows past the last one read that again,
+// threads without a column read the first, and what does not belong is left
+// out on the way to LDS.
+template <typename T, int C, int D, int THREADS>
 struct Staged {
-    static constexpr int kVectors = C * D / 8;
-    static constexpr int kEach = (kVectors + 255) / 256;
+    static constexpr int kLanes = D / 8 <= 4 ? 4 : D / 8 <= 8 ? 8 : D / 8 <= 16 ? 16 : 32;  // threads along a row
+    static constexpr int kRows = THREADS / kLanes, kEach = kRows < C ? C / kRows : 1;
     Eight<T> r[kEach];
+    const char* next;  // the row of the next chunk's first token, at the block's first column
+    long long token;   // bytes from a token to the next in the order of the scan
+    unsigned step;     // the same, of the lower address to the higher
+    int row, col, at;  // this thread's first row and column, and the column where its vectors start
+    int width;         // columns that the block has
+    bool slow;         // rows of fewer than eight elements or 2^24 bytes apart: read when they are needed
+    bool plain;        // no vector starts early
 
-    // rows: tokens first .. first + n - 1 (in scan order), zeros from there on
-    __device__ __forceinline__ void load(const T* base, long long token, long long first, int n, int step, int col0, int dim) {
+    __device__ __forceinline__ void init(const ScanSide& s, int b, int h, int col0, int dim, long long first, int reverse) {
+        const long long apart = s.token * (long long)sizeof(T);
+        next = (const char*)((const T*)s.p + b * s.batch + (h / s.group) * s.head + col0) + first * apart;
+        token = reverse ? -apart : apart;
+        row = (int)threadIdx.x / kLanes;
+        col = (int)threadIdx.x % kLanes * 8;
+        width = dim - col0 < D ? dim - col0 : D;
+        slow = width < 8 || apart >= 1 << 24;
+        step = slow ? 0u : (unsigned)apart;
+        plain = !slow && width % 8 == 0;
+        // the vector over the last column starts early, on what its neighbour reads too
+        at = col >= width || slow ? 0 : col + 8 > width ? width - 8 : col;  // slow: of what is read for nothing
+    }
+
+    // Asks for the next chunk's `left` rows.
+    __device__ __forceinline__ void load(int left, int reverse, const void* elsewhere) {
+        const char* p = slow ? (const char*)elsewhere : reverse ? next - (unsigned)(left - 1) * step : next;
 #pragma unroll
         for (int u = 0; u < kEach; ++u) {
-            const int v = (int)threadIdx.x + 256 * u;
-            const int row = v / (D / 8), c = col0 + v % (D / 8) * 8;
-            if ((kVectors % 256 == 0 || v < kVectors) && row < n && c + 8 <= dim) {
-                r[u] = *(const Eight<T>*)(base + (first + (long long)step * row) * token + c);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) r[u].v[e] = (T)0.f;
-                if ((kVectors % 256 == 0 || v < kVectors) && row < n && c < dim) {
-                    const T* p = base + (first + (long long)step * row) * token + c;
-#pragma unroll
-                    for (int e = 0; e < 7; ++e)
-                        if (c + e < dim) r[u].v[e] = p[e];
-                }
-            }
+            int i = row + u * kRows;
+            i = i < left ? i : left - 1;
+            i = reverse ? left - 1 - i : i;
+            const unsigned offset = __umul24((unsigned)i, step) + (unsigned)at * (unsigned)sizeof(T);
+            r[u] = *(const typename PackedEight<T>::type*)(p + offset);
         }
     }
 
-    // to lds[part][C][pitch]
-    __device__ __forceinline__ void store(__bf16* lds, int pitch) const {
+    // Waits for what was read ahead.
+    __device__ __forceinline__ void arrive() {
 #pragma unroll
-        for (int u = 0; u < kEach; ++u) {
-            const int v = (int)threadIdx.x + 256 * u;
-            if (kVectors % 256 != 0 && v >= kVectors) continue;
-            __bf16* to = lds + v / (D / 8) * pitch + v % (D / 8) * 8;
-            if constexpr (Parts<T>::in == 1) {
-                bf16x8 p;
+        for (int u = 0; u < kEach; ++u) asm volatile("" : "+v"(r[u]));
+    }
+
+    // The chunk that was asked for to lds[part][C][pitch], rows from `left` on as zeros; then on to the next.
+    __device__ __forceinline__ void store(__bf16* lds, int pitch, int left) {
+        if (plain && left == C) {
+            if (col < width && row < C)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = r[u].v[e];
-                *(bf16x8*)to = p;
+                for (int u = 0; u < kEach; ++u) put(lds + (row + u * kRows) * pitch + col, pitch, r[u], true);
+        } else if (!slow) {
+            if (col < width && row < C)
+#pragma unroll
+                for (int u = 0; u < kEach; ++u) {
+                    const Eight<T> zero = (T)0.f;
+                    put(lds + (row + u * kRows) * pitch + at, pitch, row + u * kRows < left ? r[u] : zero, at == col);
+                }
+        } else {
+#pragma unroll 1
+            for (int j = (int)threadIdx.x; j < C * D; j += THREADS) {
+                const int i = j / D, c = j % D;
+                float f = i < left && c < width ? (float)((const T*)(next + i * token))[c] : 0.f;
+#pragma unroll
+                for (int k = 0; k < Parts<T>::in; ++k) {
+                    const __bf16 v = (__bf16)f;
+                    lds[(k * C + i) * pitch + c] = v;
+                    f -= (float)v;
+                }
+            }
+        }
+        next += C * token;
+    }
+
+    // Eight elements' parts; aligned: as vectors.
+    static __device__ __forceinline__ void put(__bf16* to, int pitch, const Eight<T>& x, bool aligned) {
+        bf16x8 p[Parts<T>::in];
+        if constexpr (Parts<T>::in == 1) {
+            p[0] = x;
+        } else {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = (float)x[e];
+            split<false>(f, p);
+        }
+#pragma unroll
+        for (int i = 0; i < Parts<T>::in; ++i) {
+            if (aligned) {
+                *(bf16x8*)(to + i * C * pitch) = p[i];
             } else {
-                float x[8];
-                bf16x8 p[Parts<T>::in];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = (float)r[u].v[e];
-                split8(x, p);
-#pragma unroll
-                for (int i = 0; i < Parts<T>::in; ++i) *(bf16x8*)(to + i * C * pitch) = p[i];
+                for (int e = 0; e < 8; ++e) to[i * C * pitch + e] = p[i][e];
             }
         }
     }
 };
 
-// Row `row` of a matrix in LDS as an operand: elements k0 + (0-3, 16-19) + 4 g.
-__device__ __forceinline__ bf16x8 row_operand(const __bf16* m, int pitch, int row, int k0, int g) {
-    const bf16x4 a = *(const bf16x4*)(m + row * pitch + k0 + 4 * g);
-    const bf16x4 b = *(const bf16x4*)(m + row * pitch + k0 + 16 + 4 * g);
+// A row of a matrix in LDS as an operand: elements k0 + (0-3, 16-19) + 4 g.
+__device__ __forceinline__ bf16x8 row_operand(const __bf16* row, int k0, int g) {
+    const bf16x4 a = *(const bf16x4*)(row + k0 + 4 * g);
+    const bf16x4 b = *(const bf16x4*)(row + k0 + 16 + 4 * g);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -172,25 +273,46 @@ __device__ __forceinline__ bf16x8 column_operand(const __bf16* m, int pitch, int
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-template <typename T, int DK, int NT, int C>
+// Four neighbours, as many as there is room for.
+template <typename T>
+__device__ __forceinline__ void store_four(T* to, f32x4 y, int room) {
+    typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (room >= 4) {
+        *(four*)to = four{(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
+    } else {
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+            if (r < room) to[r] = (T)y[r];
+    }
+}
+
+template <typename T, int DK, int WAVES, int NT, int C>
 struct ChunkShape {
     static constexpr int kIn = Parts<T>::in, kMid = Parts<T>::mid;
-    static constexpr int kCols = 64 * NT;
-    // 16 bytes more a row: a quarter wave's 8-byte reads down the rows meet different banks
+    static constexpr int kThreads = 64 * WAVES, kCols = 16 * NT * WAVES;
+        // 16 bytes more a row: a quarter wave's 8-byte reads down the rows meet different banks
     static constexpr int kPitchK = DK + 8, kPitchV = kCols + 8, kPitchP = C + 8;
+    // A, B and C, twice where a CU's LDS then still holds a second block or there is none anyway: the next chunk is
+    // written while other waves read this one
     static constexpr size_t kA = 0, kB = kA + (size_t)kIn * C * kPitchK, kC = kB + (size_t)kIn * C * kPitchK,
-                            kP = kC + (size_t)kIn * C * kPitchV, kEnd = kP + (size_t)kMid * C * kPitchP;
+                            kOne = kC + (size_t)kIn * C * kPitchV, kRest = (size_t)kMid * C * kPitchP * 2 + kDecayPowers * 4 + 16;
+    static constexpr size_t kCu = 160 * 1024;
+    static constexpr bool kTwice = 2 * (4 * kOne + kRest) <= kCu || (2 * (2 * kOne + kRest) > kCu && 4 * kOne + kRest <= kCu);
+    static constexpr size_t kP = kTwice ? 2 * kOne : kOne, kEnd = kP + (size_t)kMid * C * kPitchP;
     static constexpr size_t kLds = kEnd * 2 + kDecayPowers * 4 + 16;
+    // waves that share a SIMD's registers: two, or the one that the LDS leaves
+    static constexpr int kShare = (int)(kCu / kLds) * WAVES >= 8 ? 2 : 1;
 };
 
-template <typename T, int DK, int NT, int C, bool STATE_ONLY>
-__global__ __launch_bounds__(256, 2) void k_chunk(const ChunkArgs args) {
-    using S = ChunkShape<T, DK, NT, C>;
-    constexpr int IN = S::kIn, MID = S::kMid, TI = C / 16;
+template <typename T, int DK, int WAVES, int NT, int C, bool STATE_ONLY>
+__global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShare)) void k_chunk(const ChunkArgs args) {
+    using S = ChunkShape<T, DK, WAVES, NT, C>;
+    constexpr int IN = S::kIn, MID = S::kMid, TI = C / 16, THREADS = S::kThreads;
     extern __shared__ __align__(16) char lds[];
-    __bf16* const la = (__bf16*)lds + S::kA;
-    __bf16* const lb = (__bf16*)lds + S::kB;
-    __bf16* const lc = (__bf16*)lds + S::kC;
+    __bf16* la = (__bf16*)lds + S::kA;
+    __bf16* lb = (__bf16*)lds + S::kB;
+    __bf16* lc = (__bf16*)lds + S::kC;
+    int other = S::kTwice ? (int)S::kOne : 0;  // from this chunk's buffer to the next one's
     __bf16* const lp = (__bf16*)lds + S::kP;
     float* const pw = (float*)((__bf16*)lds + S::kEnd);
 
@@ -206,145 +328,186 @@ __global__ __launch_bounds__(256, 2) void k_chunk(const ChunkArgs args) {
     const int z = (int)(id / args.scan[0].batch);
     const ScanArgs& s = args.scan[z];
 
-    long long n = s.tokens;
-    if (s.lengths) {
-        const long long l = s.lengths[b];
-        n = l < 0 ? 0 : l < n ? l : n;
-    }
-    const long long begin = seg * args.segment;
-    const long long end = begin + args.segment < s.tokens ? begin + args.segment : s.tokens;
+    const int tokens = (int)s.tokens, segment = (int)args.segment;
+    int n = tokens;
+    if (s.lengths) n = s.lengths[b] < 0 ? 0 : s.lengths[b] < n ? s.lengths[b] : n;
+    const int begin = seg * segment, end = tokens - begin > segment ? begin + segment : tokens;
+    const int stop = end < n ? end : n;  // of what the scan reads
     // a state before the next segment is needed only where that one has tokens
-    if (STATE_ONLY && begin + args.segment >= n) return;
+    if (STATE_ONLY && n - begin <= segment) return;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int g = lane >> 4, l16 = lane & 15;
     const int col0 = slice * S::kCols, wcol = wave * 16 * NT;
     const int lead = s.reverse;
     if (tid < kDecayPowers) pw[tid] = args.powers[(long long)h * kDecayPowers + tid];
-    if (!STATE_ONLY)  // tiles of P right of the diagonal that a product of 32 tokens meets
-        for (int i = tid; i < MID * C * S::kPitchP; i += 256) lp[i] = (__bf16)0.f;
-
-    const T* const A = (const T*)s.a.p + b * s.a.batch + (h / s.a.group) * s.a.head;
-    const T* const B = (const T*)s.b.p + b * s.b.batch + (h / s.b.group) * s.b.head;
-    const T* const Cc = (const T*)s.c.p + b * s.c.batch + (h / s.c.group) * s.c.head;
-    const int step = s.reverse ? -1 : 1;
-    const auto token_of = [&](long long i) { return s.reverse ? n - 1 - i : i; };
+    // columns past the tensors', and tiles of P right of the diagonal that a product of 32 tokens meets
+    for (int i = tid; i < (int)(S::kEnd / 8); i += THREADS) ((bf16x8*)lds)[i] = (__bf16)0.f;
 
     // the state: rows 16 a + 4 g + r, columns col0 + wcol + 16 t + l16
-    f32x4 X[DK / 16][NT];
+    f32x4 X[NT][DK / 16];
+    const int col = col0 + wcol + l16;
     const long long head_state = ((long long)b * s.heads + h) * s.dk * s.dv;
     float* const slot = args.slots + ((((long long)z * s.batch + b) * s.heads + h) * args.segments + seg) * s.dk * s.dv;
     {
-        const float* from = STATE_ONLY ? nullptr : args.segments > 1 ? slot : s.state_in ? s.state_in + head_state : nullptr;
         const bool native = args.segments > 1;
+        const float* from = STATE_ONLY ? nullptr : native ? slot : s.state_in ? s.state_in + head_state : nullptr;
         const int sr = native ? s.dv : s.state_row, sc = native ? 1 : s.state_col;
 #pragma unroll
-        for (int a = 0; a < DK / 16; ++a)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int a = 0; a < DK / 16; ++a)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * a + 4 * g + r, col = col0 + wcol + 16 * t + l16;
-                    X[a][t][r] = from && row < s.dk && col < s.dv ? from[(long long)row * sr + (long long)col * sc] : 0.f;
+                    const int row = 16 * a + 4 * g + r, c = col + 16 * t;
+                    X[t][a][r] = from && row < s.dk && c < s.dv ? from[(long long)row * sr + (long long)c * sc] : 0.f;
                 }
     }
 
-    Staged<T, C, DK> sa, sb;
-    Staged<T, C, S::kCols> sc;
-    const auto fetch = [&](long long at) {
-        const int left = (int)(n - at < C ? (n - at > 0 ? n - at : 0) : C);
-        const long long first = token_of(at);
-        if (!STATE_ONLY) sa.load(A, s.a.token, first, left, step, 0, s.dk);
-        sb.load(B, s.b.token, first, left, step, 0, s.dk);
-        sc.load(Cc, s.c.token, first, left, step, col0, s.dv);
+    const int reverse = s.reverse;
+    const long long first = reverse ? (long long)n - 1 - begin : begin;
+    const float scale_update = s.scale_update, scale_in = s.scale_in;
+    Staged<T, C, DK, THREADS> sa, sb;
+    Staged<T, C, S::kCols, THREADS> sc;
+    if (!STATE_ONLY) sa.init(s.a, b, h, 0, s.dk, first, reverse);
+    sb.init(s.b, b, h, 0, s.dk, first, reverse);
+    sc.init(s.c, b, h, col0, s.dv, first, reverse);
+    const auto fetch = [&](int left) {
+        if (!STATE_ONLY) sa.load(left, reverse, args.powers);
+        sb.load(left, reverse, args.powers);
+        sc.load(left, reverse, args.powers);
+    };
+    // on every way to the loop's next turn, or the compiler waits where that asks for more
+    const auto arrive = [&]() {
+        if (!STATE_ONLY) sa.arrive();
+        sb.arrive();
+        sc.arrive();
+    };
+    const auto stage = [&](int left) {
+        if (!STATE_ONLY) sa.store(la, S::kPitchK, left);
+        sb.store(lb, S::kPitchK, left);
+        sc.store(lc, S::kPitchV, left);
     };
 
-    long long at = begin;
-    if (at < n) fetch(at);
-    for (; at < end && at < n; at += C) {
-        const int left = (int)(n - at < C ? n - at : C);
-        __syncthreads();  // the chunk before has been read
-        if (!STATE_ONLY) sa.store(la, S::kPitchK);
-        sb.store(lb, S::kPitchK);
-        sc.store(lc, S::kPitchV);
-        __syncthreads();
-        if (at + C < end && at + C < n) fetch(at + C);
+    // where this lane's token of a chunk's first 16 goes, from its first column on
+    const int out_col = col0 + wcol + 4 * g, room = s.dv - out_col, out_f32 = s.out_f32;
+    const long long out_step = (reverse ? -s.out_token : s.out_token) * (out_f32 ? 4ll : (long long)sizeof(T));
+    char* out = (char*)s.out + (b * s.out_batch + h * s.out_head + first * s.out_token + out_col) * (out_f32 ? 4ll : (long long)sizeof(T)) +
+                l16 * out_step;
 
-        f32x4 o[TI][NT];
+    // Weights, the same for every whole chunk. P: the tiles on and left of the diagonal, dealt to the waves; a wave
+    // without a tile of its own in the last turn does the last one once more.
+    constexpr int tiles = TI * (TI + 1) / 2, each = (tiles + WAVES - 1) / WAVES;
+    int pi[each], pj[each];
+    float pweight[each][4], oweight[TI], uweight[C / 32][8];
+    __syncthreads();  // pw, and the clearing
+    if constexpr (!STATE_ONLY) {
+#pragma unroll
+        for (int u = 0; u < each; ++u) {
+            const int tile = wave + u * WAVES < tiles ? wave + u * WAVES : tiles - 1;
+            const int I = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3;
+            pi[u] = 16 * I, pj[u] = 16 * (tile - I * (I + 1) / 2);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = pi[u] + l16 - (pj[u] + 4 * g + r);
+                pweight[u][r] = d < 0 ? 0.f : pw[d] * scale_update * scale_in;
+            }
+        }
+#pragma unroll
+        for (int I = 0; I < TI; ++I) oweight[I] = pw[16 * I + l16 + 1 - lead] * scale_in;
+    }
+    const auto update_weights = [&](int left) {
+#pragma unroll
+        for (int k = 0; k < C / 32; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = left - 1 - (32 * k + 8 * g + e) + lead;
+                uweight[k][e] = pw[d < 0 ? 0 : d] * scale_update;
+            }
+    };
+    update_weights(C);
+
+    // the state is here before the loop begins: a wait for it inside would be one for the chunk that is read ahead
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int a = 0; a < DK / 16; ++a) asm volatile("" : "+v"(X[t][a]));
+    if (begin < stop) fetch(stop - begin < C ? stop - begin : C);
+    arrive();
+    if (begin < stop) stage(stop - begin < C ? stop - begin : C);
+#pragma unroll 1
+    for (int at = begin; at < stop; at += C) {
+        const int left = stop - at < C ? stop - at : C;
+        const int more = stop - at - left < C ? stop - at - left : C;  // tokens of the next chunk
+        __syncthreads();
+        if (more) fetch(more);
+        if (left < C) update_weights(left);
+
+        f32x4 o[NT][TI];
         if constexpr (!STATE_ONLY) {
-            // P, transposed: rows j, columns i; the tiles on and left of the diagonal dealt to the waves
-            int tile = 0;
+            // P, transposed: rows j, columns i
+            f32x4 p[each];
 #pragma unroll
-            for (int I = 0; I < TI; ++I)
+            for (int u = 0; u < each; ++u) p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int J = 0; J <= I; ++J, ++tile) {
-                    if ((tile & 3) != wave) continue;
-                    f32x4 p = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < DK / 32; ++k) {
+                bf16x8 bj[each][IN], ai[each][IN];
 #pragma unroll
-                    for (int k = 0; k < DK / 32; ++k) {
-                        bf16x8 bj[IN], ai[IN];
+                for (int u = 0; u < each; ++u)
 #pragma unroll
-                        for (int i = 0; i < IN; ++i) {
-                            bj[i] = row_operand(lb + i * C * S::kPitchK, S::kPitchK, 16 * J + l16, 32 * k, g);
-                            ai[i] = row_operand(la + i * C * S::kPitchK, S::kPitchK, 16 * I + l16, 32 * k, g);
-                        }
-                        p = mma_parts(bj, ai, p, IN == 3 ? 3 : 2);
+                    for (int i = 0; i < IN; ++i) {
+                        bj[u][i] = row_operand(lb + (i * C + pj[u] + l16) * S::kPitchK, 32 * k, g);
+                        ai[u][i] = row_operand(la + (i * C + pi[u] + l16) * S::kPitchK, 32 * k, g);
                     }
-                    const int i = 16 * I + l16, j0 = 16 * J + 4 * g;
-                    bf16x4 q[MID];
+                mma_parts(bj, ai, p, IN == 3 ? 3 : 2);
+            }
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int d = i - (j0 + r);
-                        float x = d < 0 ? 0.f : p[r] * (pw[d < 0 ? 0 : d] * s.scale_update);
+            for (int u = 0; u < each; ++u) {
+                bf16x4 q[MID];
+                float x[4];
 #pragma unroll
-                        for (int m = 0; m < MID; ++m) {
-                            q[m][r] = (__bf16)x;
-                            x -= (float)q[m][r];
-                        }
-                    }
+                for (int r = 0; r < 4; ++r)  // not by a product: what is masked may be infinite
+                    x[r] = pi[u] + l16 < pj[u] + 4 * g + r ? 0.f : p[u][r] * pweight[u][r];
+                split<true>(x, q);
 #pragma unroll
-                    for (int m = 0; m < MID; ++m) *(bf16x4*)(lp + (m * C + i) * S::kPitchP + j0) = q[m];
-                }
+                for (int m = 0; m < MID; ++m) *(bf16x4*)(lp + (m * C + pi[u] + l16) * S::kPitchP + pj[u] + 4 * g) = q[m];
+            }
 
             // out = A X, transposed
 #pragma unroll
-            for (int I = 0; I < TI; ++I)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) o[I][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int I = 0; I < TI; ++I) o[t][I] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < DK / 32; ++k) {
-                bf16x8 x[NT][MID];
+                bf16x8 ai[TI][IN];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = X[2 * k + e / 4][t][e % 4];
-                    split8(v, x[t]);
-                }
-#pragma unroll
-                for (int I = 0; I < TI; ++I) {
-                    bf16x8 ai[IN];
+                for (int I = 0; I < TI; ++I)
 #pragma unroll
                     for (int i = 0; i < IN; ++i)
-                        ai[i] = row_operand(la + i * C * S::kPitchK, S::kPitchK, 16 * I + l16, 32 * k, g);
+                        ai[I][i] = row_operand(la + (i * C + 16 * I + l16) * S::kPitchK, 32 * k, g);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) o[I][t] = mma_parts(x[t], ai, o[I][t], MID);
+                for (int t = 0; t < NT; ++t) {
+                    bf16x8 x[MID];
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = X[t][2 * k + e / 4][e % 4];
+                    split<true>(v, x);
+                    mma_parts(x, ai, o[t], MID);
                 }
             }
 #pragma unroll
-            for (int I = 0; I < TI; ++I) {
-                const float w = pw[16 * I + l16 + 1 - lead];
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) o[I][t] *= w;
-            }
+                for (int I = 0; I < TI; ++I) o[t][I] *= oweight[I];
             __syncthreads();  // P is written
         }
 
         const float whole = pw[left];
 #pragma unroll
-        for (int a = 0; a < DK / 16; ++a)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) X[a][t] *= whole;
+            for (int a = 0; a < DK / 16; ++a) X[t][a] *= whole;
 #pragma unroll
         for (int k = 0; k < C / 32; ++k) {
             bf16x8 cv[NT][IN], cw[NT][3];
@@ -354,72 +517,63 @@ __global__ __launch_bounds__(256, 2) void k_chunk(const ChunkArgs args) {
                 for (int i = 0; i < IN; ++i)
                     cv[t][i] = column_operand(lc + i * C * S::kPitchV, S::kPitchV, 32 * k, wcol + 16 * t, lane);
             if constexpr (!STATE_ONLY) {
+                // tiles of 16 tokens from 32 k on, two at a time
 #pragma unroll
-                for (int I = 2 * k; I < TI; ++I) {
-                    bf16x8 p[MID];
+                for (int I = 2 * k; I < TI; I += 2) {
+                    bf16x8 p[2][MID];
 #pragma unroll
-                    for (int m = 0; m < MID; ++m)
-                        p[m] = *(const bf16x8*)(lp + (m * C + 16 * I + l16) * S::kPitchP + 32 * k + 8 * g);
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) o[I][t] = mma_parts(cv[t], p, o[I][t], MID);
+                        for (int m = 0; m < MID; ++m)
+                            p[u][m] = *(const bf16x8*)(lp + (m * C + 16 * (I + u) + l16) * S::kPitchP + 32 * k + 8 * g);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) mma_parts(cv[t], p, o[t] + I, MID);
                 }
-            }
-            float w[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = left - 1 - (32 * k + 8 * g + e) + lead;
-                w[e] = pw[d < 0 ? 0 : d] * s.scale_update;
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[e] = 0.f;
+                    v[e] = (float)cv[t][IN - 1][e];
 #pragma unroll
-                    for (int i = IN - 1; i >= 0; --i) v[e] += (float)cv[t][i][e];
-                    v[e] *= w[e];
+                    for (int i = IN - 2; i >= 0; --i) v[e] += (float)cv[t][i][e];
+                    v[e] *= uweight[k][e];
                 }
-                split8(v, cw[t]);
+                split<true>(v, cw[t]);
             }
 #pragma unroll
-            for (int a = 0; a < DK / 16; ++a) {
-                bf16x8 bt[IN];
+            for (int a = 0; a < DK / 16; a += 2) {
+                bf16x8 bt[2][IN];
 #pragma unroll
-                for (int i = 0; i < IN; ++i) bt[i] = column_operand(lb + i * C * S::kPitchK, S::kPitchK, 32 * k, 16 * a, lane);
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) X[a][t] = mma_parts(bt, cw[t], X[a][t], 3);
+                    for (int i = 0; i < IN; ++i)
+                        bt[u][i] = column_operand(lb + i * C * S::kPitchK, S::kPitchK, 32 * k, 16 * (a + u), lane);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma_parts(bt, cw[t], X[t] + a, 3);
             }
         }
 
+        if (!S::kTwice) __syncthreads();  // the chunk has been read
+        arrive();
+        la += other, lb += other, lc += other;
+        other = -other;
+        // before this chunk's stores: loads and stores are waited for in their order
+        if (more) stage(more);
         if constexpr (!STATE_ONLY) {
 #pragma unroll
             for (int I = 0; I < TI; ++I) {
-                const int i = 16 * I + l16;
-                if (i >= left) continue;
-                const long long row = b * s.out_batch + token_of(at + i) * s.out_token + h * s.out_head;
+                if (16 * I + l16 >= left) continue;
+                char* const to = out + 16 * I * out_step;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const int c = col0 + wcol + 16 * t + 4 * g;
-                    const f32x4 y = o[I][t] * s.scale_in;
-                    if (s.out_f32) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (c + r < s.dv) ((float*)s.out)[row + c + r] = y[r];
-                    } else if (c + 4 <= s.dv) {
-                        struct __attribute__((packed, aligned(sizeof(T)))) Four {
-                            T v[4];
-                        } f;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) f.v[r] = (T)y[r];
-                        *(Four*)((T*)s.out + row + c) = f;
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (c + r < s.dv) ((T*)s.out)[row + c + r] = (T)y[r];
-                    }
+                    const f32x4 y = o[t][I];
+                    if (out_f32) store_four((float*)to + 16 * t, y, room - 16 * t);
+                    else store_four((T*)to + 16 * t, y, room - 16 * t);
                 }
             }
+            out += C * out_step;
         }
     }
 
@@ -427,34 +581,34 @@ __global__ __launch_bounds__(256, 2) void k_chunk(const ChunkArgs args) {
         // what this segment adds goes to the next one's slot
         float* const to = slot + (long long)s.dk * s.dv;
 #pragma unroll
-        for (int a = 0; a < DK / 16; ++a)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int a = 0; a < DK / 16; ++a)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * a + 4 * g + r, col = col0 + wcol + 16 * t + l16;
-                    if (row < s.dk && col < s.dv) to[(long long)row * s.dv + col] = X[a][t][r];
+                    const int row = 16 * a + 4 * g + r, c = col + 16 * t;
+                    if (row < s.dk && c < s.dv) to[(long long)row * s.dv + c] = X[t][a][r];
                 }
         return;
     }
     // rows past the sequence's length
-    for (long long i = (begin > n ? begin : n) + wave; i < end; i += 4) {
-        const long long row = b * s.out_batch + i * s.out_token + h * s.out_head;
+    for (int i = (begin > n ? begin : n) + wave; i < end; i += WAVES) {
+        const long long row = b * s.out_batch + (long long)i * s.out_token + h * s.out_head;
         for (int c = col0 + lane; c < s.dv && c < col0 + S::kCols; c += 64) {
             if (s.out_f32) ((float*)s.out)[row + c] = 0.f;
             else ((T*)s.out)[row + c] = (T)0.f;
         }
     }
-    if (s.state_out && seg == (n > 0 ? (n - 1) / args.segment : 0)) {
+    if (s.state_out && seg == (n > 0 ? (n - 1) / segment : 0)) {
 #pragma unroll
-        for (int a = 0; a < DK / 16; ++a)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int a = 0; a < DK / 16; ++a)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * a + 4 * g + r, col = col0 + wcol + 16 * t + l16;
-                    if (row < s.dk && col < s.dv)
-                        s.state_out[head_state + (long long)row * s.state_row + (long long)col * s.state_col] = X[a][t][r];
+                    const int row = 16 * a + 4 * g + r, c = col + 16 * t;
+                    if (row < s.dk && c < s.dv)
+                        s.state_out[head_state + (long long)row * s.state_row + (long long)c * s.state_col] = X[t][a][r];
                 }
     }
 }
@@ -464,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void k_chunk(const ChunkArgs args) {
 __global__ void k_chunk_join(const ChunkArgs args);
 
 struct ChunkKernel {
-    int dk, cols, chunk;  // padded key width, columns of a block, tokens of a chunk
+    int cols, chunk, threads;  // columns and threads of a block, tokens of a chunk
     size_t lds;
     const void* run;
     const void* state_only;
@@ -474,23 +628,27 @@ const ChunkKernel* chunk_kernel_f32(int dk, int dv);
 const ChunkKernel* chunk_kernel_f16(int dk, int dv);
 const ChunkKernel* chunk_kernel_bf16(int dk, int dv);
 
-template <typename T, int DK, int NT, int C>
+template <typename T, int DK, int WAVES, int NT, int C>
 ChunkKernel chunk_kernel_of() {
-    return ChunkKernel{DK, 64 * NT, C, ChunkShape<T, DK, NT, C>::kLds, (const void*)k_chunk<T, DK, NT, C, false>,
-                       (const void*)k_chunk<T, DK, NT, C, true>};
+    using S = ChunkShape<T, DK, WAVES, NT, C>;
+    return ChunkKernel{S::kCols, C, S::kThreads, S::kLds, (const void*)k_chunk<T, DK, WAVES, NT, C, false>,
+                       (const void*)k_chunk<T, DK, WAVES, NT, C, true>};
 }
 
-// Key widths are padded to one of six. Blocks take 128 columns where there are
-// more than 64 and the state of 128 rows or fewer still fits the registers.
+// Key widths are padded to one of six. A block has 64 columns, or 128 where
+// there are more values than 64; a wave 32 of them while the state's rows leave
+// it the registers: what it reads of A, B and P then serves two products.
 template <typename T, int C>
 const ChunkKernel* pick_chunk_kernel(int dk, int dv) {
-    static const ChunkKernel narrow[6] = {chunk_kernel_of<T, 32, 1, C>(),  chunk_kernel_of<T, 64, 1, C>(),
-                                          chunk_kernel_of<T, 96, 1, C>(),  chunk_kernel_of<T, 128, 1, C>(),
-                                          chunk_kernel_of<T, 192, 1, C>(), chunk_kernel_of<T, 256, 1, C>()};
-    static const ChunkKernel wide[4] = {chunk_kernel_of<T, 32, 2, C>(), chunk_kernel_of<T, 64, 2, C>(),
-                                        chunk_kernel_of<T, 96, 2, C>(), chunk_kernel_of<T, 128, 2, C>()};
-    const int i = dk <= 32 ? 0 : dk <= 64 ? 1 : dk <= 96 ? 2 : dk <= 128 ? 3 : dk <= 192 ? 4 : 5;
-    return dv > 64 && i < 4 ? &wide[i] : &narrow[i];
+    constexpr bool f32 = Parts<T>::in == 3;  // a third part of everything
+    static const ChunkKernel kernels[6][2] = {
+        {chunk_kernel_of<T, 32, 2, 2, C>(), chunk_kernel_of<T, 32, 4, 2, C>()},
+        {chunk_kernel_of<T, 64, 2, 2, C>(), chunk_kernel_of<T, 64, 4, 2, C>()},
+        {chunk_kernel_of<T, 96, f32 ? 4 : 2, f32 ? 1 : 2, C>(), chunk_kernel_of<T, 96, 4, 2, C>()},
+        {chunk_kernel_of<T, 128, 4, 1, C>(), chunk_kernel_of<T, 128, f32 ? 8 : 4, f32 ? 1 : 2, C>()},
+        {chunk_kernel_of<T, 192, 4, 1, C>(), chunk_kernel_of<T, 192, 8, 1, C>()},
+        {chunk_kernel_of<T, 256, 4, 1, C>(), chunk_kernel_of<T, 256, 8, 1, C>()}};
+    return &kernels[dk <= 32 ? 0 : dk <= 64 ? 1 : dk <= 96 ? 2 : dk <= 128 ? 3 : dk <= 192 ? 4 : 5][dv > 64];
 }
 
 }  // namespace vkfx
