@@ -420,3 +420,18 @@ def test_plans_hold_their_context(hip_ctx):
     assert ctx._L.vkfx_context_destroy(ctx.handle) == -2
     plan.close()
     ctx.close()
+
+
+@pytest.mark.parametrize("lengths", [None, [4200, 700]])
+def test_long_prompts_update_a_state_in_place(hip_ctx, lengths):
+    """The tokens are split over blocks: none of them may read what another one has already written."""
+    import torch
+    b, t, h, d = 2, 4200, 2, 64
+    plan = _plan(hip_ctx, b, t, h, h, d, d, "bf16", decay=[0.998, 0.9])
+    q, k, v = (_tensor(i, (b, t, h, d), "bf16") for i in (1, 2, 3))
+    n = torch.tensor(lengths, device="cuda", dtype=torch.int32) if lengths else None
+    state, out, again = _state(4, b, h, d, d), torch.empty_like(v), torch.empty_like(v)
+    after = torch.empty_like(state)
+    plan.forward_tensors(q, k, v, out, state_in=state, state_out=after, lengths=n)
+    plan.forward_tensors(q, k, v, again, state_in=state, state_out=state, lengths=n)
+    assert torch.equal(out, again) and torch.equal(after, state)

@@ -7,57 +7,72 @@
 
 namespace vkfx {
 
+namespace {
+
+// Joins the segments: place k = g^segment place k-1 + what segment k-1 added.
+// A thread takes EACH elements of a state, 256 apart, and reads AHEAD segments
+// before it needs the first.
+template <int EACH, int AHEAD>
 __global__ __launch_bounds__(256) void k_chunk_join(const ChunkArgs args) {
-    const int z = blockIdx.z;
+    const int batch = args.scan[0].batch, z = blockIdx.z / batch, b = blockIdx.z % batch, h = blockIdx.y;
     const ScanArgs& s = args.scan[z];
-    const int b = blockIdx.y / s.heads, h = blockIdx.y % s.heads;
-    const int e = blockIdx.x * 256 + threadIdx.x;
-    const int size = s.dk * s.dv;
-    if (e >= size) return;
     long long n = s.tokens;
-    if (s.lengths) {
-        const long long l = s.lengths[b];
-        n = l < 0 ? 0 : l < n ? l : n;
+    if (s.lengths) n = s.lengths[b] < 0 ? 0 : s.lengths[b] < n ? s.lengths[b] : n;
+    const int last = (int)((n + args.segment - 1) / args.segment);  // segments that have tokens
+    if (last < 3) return;
+    const int size = s.dk * s.dv, e = blockIdx.x * 256 * EACH + threadIdx.x;
+    float* slot = args.slots + (((long long)z * batch + b) * s.heads + h) * args.segments * size + size;
+    int at[EACH];
+    float x[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        at[j] = e + 256 * j < size ? e + 256 * j : size - 1;
+        x[j] = slot[at[j]];
     }
-    // the decay of a whole segment, by squaring
-    const float* p = args.powers + (long long)h * kDecayPowers;
-    double power = 1.0, square = (double)p[1] + (double)p[kDecayPowers - 1];
-    for (long long i = args.segment; i; i >>= 1, square *= square)
-        if (i & 1) power *= square;
-    const float decay = (float)power;
-    const int row = e / s.dv, col = e % s.dv;
-    const long long head = (long long)b * s.heads + h;
-    float x = s.state_in ? s.state_in[head * size + (long long)row * s.state_row + (long long)col * s.state_col] : 0.f;
-    float* slot = args.slots + ((long long)z * s.batch * s.heads + head) * args.segments * size + e;
-    // segments before the last that has tokens; eight are read before the first is needed
-    const int last = (int)((n + args.segment - 1) / args.segment);
-    slot[0] = x;
-    for (int k = 1; k < last; k += 8) {
-        float added[8];
+    const float decay = whole_segment(args.powers + (long long)h * kDecayPowers, args.segment);
+    for (int k = 2; k < last; k += AHEAD) {
+        float added[AHEAD][EACH];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) added[u] = k + u < last ? slot[(long long)(k + u) * size] : 0.f;
+        for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            x = fmaf(x, decay, added[u]);
-            if (k + u < last) slot[(long long)(k + u) * size] = x;
+            for (int j = 0; j < EACH; ++j)
+                added[u][j] = slot[(long long)(k + u < last ? u + 1 : last - k) * size + at[j]];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (k + u >= last) break;
+            slot += size;
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) {
+                x[j] = fmaf(x[j], decay, added[u][j]);
+                if (e + 256 * j < size) slot[at[j]] = x[j];
+            }
         }
     }
 }
 
-namespace {
+template <int EACH, int AHEAD>
+int launch_join(const ChunkArgs& a, hipStream_t s) {
+    const ScanArgs& f = a.scan[0];
+    const dim3 grid((unsigned)((f.dk * f.dv + 256 * EACH - 1) / (256 * EACH)), (unsigned)f.heads, (unsigned)(f.batch * a.scans));
+    hipLaunchKernelGGL((k_chunk_join<EACH, AHEAD>), grid, dim3(256), 0, s, a);
+    return (int)hipGetLastError();
+}
 
+// blockIdx.y: one of the two tensors.
 template <typename T>
-__global__ __launch_bounds__(256) void k_group_sum(const float* __restrict__ from, const ScanSide to, long long batch,
-                                                   long long tokens, int kv_heads, int group, int dim) {
-    const long long total = batch * tokens * kv_heads * dim;
+__global__ __launch_bounds__(256) void k_group_sum(const GroupSum a, const GroupSum b, long long batch, long long tokens,
+                                                   int kv_heads, int group) {
+    const GroupSum& s = blockIdx.y ? b : a;
+    const long long total = batch * tokens * kv_heads * s.dim;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int c = (int)(i % dim);
-        const long long row = i / dim;  // batch, token, shared head
+        const int c = (int)(i % s.dim);
+        const long long row = i / s.dim;  // batch, token, shared head
         const int h = (int)(row % kv_heads);
-        const long long t = row / kv_heads % tokens, b = row / kv_heads / tokens;
+        const long long t = row / kv_heads % tokens, n = row / kv_heads / tokens;
+        const float* from = s.from + row * group * s.dim + c;
         float sum = 0.f;
-        for (int g = 0; g < group; ++g) sum += from[(row * group + g) * dim + c];
-        ((T*)to.p)[b * to.batch + t * to.token + h * to.head + c] = (T)sum;
+        for (int g = 0; g < group; ++g) sum += from[(long long)g * s.dim];
+        ((T*)s.to.p)[n * s.to.batch + t * s.to.token + h * s.to.head + c] = (T)sum;
     }
 }
 
@@ -119,13 +134,16 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
     a.segment = sp.segment;
     a.powers = powers;
     a.slots = work;
+    // a whole sequence's block reads its state before it writes it: only segments need the copy
+    for (int i = 0; i < count && a.segments > 1; ++i)
+        if (scans[i].state_in && scans[i].state_in == scans[i].state_out) a.in_place = 1;
     if (whole * a.segments > 0x7fffffffll) return (int)hipErrorInvalidConfiguration;
     if (a.segments > 1) {
         work += slot_floats(first, count, a.segments);
         if (int e = launch_with(k->state_only, whole * a.segments, k, a, st)) return e;
-        const dim3 grid((unsigned)((first.dk * first.dv + 255) / 256), (unsigned)(first.batch * first.heads), (unsigned)count);
-        hipLaunchKernelGGL(k_chunk_join, grid, dim3(256), 0, st, a);
-        if (hipError_t e = hipGetLastError()) return (int)e;
+        // few segments come with many states, many segments with few
+        if (a.segments > 2)
+            if (int e = a.segments <= 8 ? launch_join<4, 4>(a, st) : launch_join<1, 16>(a, st)) return e;
     }
     return launch_with(k->run, whole * a.segments, k, a, st);
 }
@@ -154,16 +172,16 @@ int launch_scans(int element, const ScanArgs* scans, int count, const float* pow
     return (int)hipSuccess;
 }
 
-int launch_group_sum(int element, const float* from, const ScanSide& to, long long batch, long long tokens, int kv_heads,
-                     int group, int dim, hipStream_t s) {
-    const long long blocks = (batch * tokens * kv_heads * dim + 255) / 256;
-    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+int launch_group_sum(int element, const GroupSum& a, const GroupSum& b, long long batch, long long tokens, int kv_heads,
+                     int group, hipStream_t s) {
+    const long long blocks = (batch * tokens * kv_heads * std::max(a.dim, b.dim) + 255) / 256;
+    const dim3 grid((unsigned)std::min(blocks, 4096ll), 2);
     if (element == VKFX_ELEMENT_F32)
-        hipLaunchKernelGGL(k_group_sum<float>, grid, dim3(256), 0, s, from, to, batch, tokens, kv_heads, group, dim);
+        hipLaunchKernelGGL(k_group_sum<float>, grid, dim3(256), 0, s, a, b, batch, tokens, kv_heads, group);
     else if (element == VKFX_ELEMENT_F16)
-        hipLaunchKernelGGL(k_group_sum<_Float16>, grid, dim3(256), 0, s, from, to, batch, tokens, kv_heads, group, dim);
+        hipLaunchKernelGGL(k_group_sum<_Float16>, grid, dim3(256), 0, s, a, b, batch, tokens, kv_heads, group);
     else
-        hipLaunchKernelGGL(k_group_sum<__bf16>, grid, dim3(256), 0, s, from, to, batch, tokens, kv_heads, group, dim);
+        hipLaunchKernelGGL(k_group_sum<__bf16>, grid, dim3(256), 0, s, a, b, batch, tokens, kv_heads, group);
     return (int)hipGetLastError();
 }
 

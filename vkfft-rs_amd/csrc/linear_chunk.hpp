@@ -38,13 +38,25 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
+// The decay of a whole segment, by squaring, from a head's table.
+__device__ __forceinline__ float whole_segment(const float* powers, long long segment) {
+    double power = 1.0, square = (double)powers[1] + (double)powers[kDecayPowers - 1];
+    for (long long i = segment; i; i >>= 1, square *= square)
+        if (i & 1) power *= square;
+    return (float)power;
+}
+
 struct ChunkArgs {
     ScanArgs scan[3];
     int scans;
     int slices;     // blocks side by side over dv
     int segments;   // parts of the tokens, each `segment` long (a multiple of the chunk)
     long long segment;
-    float* slots;   // segments > 1: [scan][batch][head][segment][dk][dv] states before each segment
+    // segments > 1: [scan][batch][head][segment][dk][dv], the state before each segment; until k_chunk_join ran, from
+    // the third on what the segment before it adds. The first is state_in itself, or with in_place (another block's
+    // state_out may then overwrite that) its copy.
+    float* slots;
+    int in_place;
     const float* powers;
 };
 
@@ -333,9 +345,6 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
     if (s.lengths) n = s.lengths[b] < 0 ? 0 : s.lengths[b] < n ? s.lengths[b] : n;
     const int begin = seg * segment, end = tokens - begin > segment ? begin + segment : tokens;
     const int stop = end < n ? end : n;  // of what the scan reads
-    // a state before the next segment is needed only where that one has tokens
-    if (STATE_ONLY && n - begin <= segment) return;
-
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int g = lane >> 4, l16 = lane & 15;
     const int col0 = slice * S::kCols, wcol = wave * 16 * NT;
@@ -349,10 +358,22 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
     const int col = col0 + wcol + l16;
     const long long head_state = ((long long)b * s.heads + h) * s.dk * s.dv;
     float* const slot = args.slots + ((((long long)z * s.batch + b) * s.heads + h) * args.segments + seg) * s.dk * s.dv;
-    {
-        const bool native = args.segments > 1;
-        const float* from = STATE_ONLY ? nullptr : native ? slot : s.state_in ? s.state_in + head_state : nullptr;
-        const int sr = native ? s.dv : s.state_row, sc = native ? 1 : s.state_col;
+    // All of a state's elements are asked for before the first is waited for: rows and columns past the last
+    // read the last one, and are left out by what they meet - zeros in A, B and C - and where X is written.
+    const auto read_state = [&](const float* from, int row_step, int col_step) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int c = col + 16 * t < s.dv ? col + 16 * t : s.dv - 1;
+#pragma unroll
+            for (int a = 0; a < DK / 16; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * a + 4 * g + r < s.dk ? 16 * a + 4 * g + r : s.dk - 1;
+                    X[t][a][r] = from[row * row_step + c * col_step];
+                }
+        }
+    };
+    const auto write_state = [&](float* to, int row_step, int col_step) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -360,8 +381,23 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int row = 16 * a + 4 * g + r, c = col + 16 * t;
-                    X[t][a][r] = from && row < s.dk && c < s.dv ? from[(long long)row * sr + (long long)c * sc] : 0.f;
+                    if (row < s.dk && c < s.dv) to[row * row_step + c * col_step] = X[t][a][r];
                 }
+    };
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int a = 0; a < DK / 16; ++a) X[t][a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int state_size = s.dk * s.dv;
+    if constexpr (STATE_ONLY) {
+        if (seg == 0 && s.state_in) read_state(s.state_in + head_state, s.state_row, s.state_col);
+        if (seg == 0 && args.in_place) write_state(slot, s.dv, 1);
+        // a state before the next segment is needed only where that one has tokens
+        if (n - begin <= segment) return;
+    } else if (seg == 0 && !args.in_place) {
+        if (s.state_in) read_state(s.state_in + head_state, s.state_row, s.state_col);
+    } else if (begin < n || seg == 0) {
+        read_state(slot, s.dv, 1);
     }
 
     const int reverse = s.reverse;
@@ -578,17 +614,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
     }
 
     if constexpr (STATE_ONLY) {
-        // what this segment adds goes to the next one's slot
-        float* const to = slot + (long long)s.dk * s.dv;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int a = 0; a < DK / 16; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * a + 4 * g + r, c = col + 16 * t;
-                    if (row < s.dk && c < s.dv) to[(long long)row * s.dv + c] = X[t][a][r];
-                }
+        write_state(slot + state_size, s.dv, 1);  // to the next segment's place
         return;
     }
     // rows past the sequence's length
@@ -599,23 +625,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
             else ((T*)s.out)[row + c] = (T)0.f;
         }
     }
-    if (s.state_out && seg == (n > 0 ? (n - 1) / segment : 0)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int a = 0; a < DK / 16; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * a + 4 * g + r, c = col + 16 * t;
-                    if (row < s.dk && c < s.dv)
-                        s.state_out[head_state + (long long)row * s.state_row + (long long)c * s.state_col] = X[t][a][r];
-                }
-    }
+    if (s.state_out && seg == (n > 0 ? (n - 1) / segment : 0)) write_state(s.state_out + head_state, s.state_row, s.state_col);
 }
-
-// Joins the segments: slot 0 = state_in, slot k+1 = g^segment slot k + what
-// segment k added (which the slot holds).
-__global__ void k_chunk_join(const ChunkArgs args);
 
 struct ChunkKernel {
     int cols, chunk, threads;  // columns and threads of a block, tokens of a chunk

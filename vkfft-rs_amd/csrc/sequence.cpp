@@ -402,9 +402,8 @@ int vkfx_linear_attention_backward(vkfx_linear_attention* plan, const vkfx_linea
         hipStream_t st = stream_of(plan->ctx, stream);
         int e = launch_scans(d.element, scans, 3, (const float*)plan->powers.p, work, (int)plan->ctx->profile.compute_units, st);
         if (e == hipSuccess && group > 1 && t) {
-            e = launch_group_sum(d.element, wk, side(args->dk, 1), (long long)b, (long long)t, (int)d.kv_heads, group, dk, st);
-            if (e == hipSuccess)
-                e = launch_group_sum(d.element, wv, side(args->dv, 1), (long long)b, (long long)t, (int)d.kv_heads, group, dv, st);
+            e = launch_group_sum(d.element, GroupSum{wk, side(args->dk, 1), dk}, GroupSum{wv, side(args->dv, 1), dv},
+                                 (long long)b, (long long)t, (int)d.kv_heads, group, st);
         }
         return e == hipSuccess ? VKFX_OK : hip_fail((hipError_t)e, "launch linear attention gradients");
     });

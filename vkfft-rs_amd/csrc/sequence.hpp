@@ -79,8 +79,13 @@ int launch_scans(int element, const ScanArgs* scans, int count, const float* pow
 size_t scan_work_floats(int element, int dk, int dv, int heads, int count, long long max_batch, long long max_tokens);
 
 // Sums the floats [batch][token][head][dim] of each shared head's `group`
-// query heads, in their order, into `to`.
-int launch_group_sum(int element, const float* from, const ScanSide& to, long long batch, long long tokens, int kv_heads,
-                     int group, int dim, hipStream_t s);
+// query heads, in their order; two tensors at once.
+struct GroupSum {
+    const float* from;
+    ScanSide to;
+    int dim;
+};
+int launch_group_sum(int element, const GroupSum& a, const GroupSum& b, long long batch, long long tokens, int kv_heads,
+                     int group, hipStream_t s);
 
 }  // namespace vkfx
