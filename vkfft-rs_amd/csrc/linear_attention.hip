@@ -93,27 +93,26 @@ struct Split {
 };
 
 // Where the waves of whole sequences are fewer than half of kWaves, the tokens
-// are split too: every segment but the last is read once more for its
-// share of the state. A segment has four chunks or more.
-Split split_tokens(long long waves, long long tokens, int chunk) {
+// are split too: every segment but the last is read once more for its share of
+// the state. A segment has two chunks or more (f32, 3 x 1001 tokens of 12 heads
+// of 80 x 96: 44 us; 49 with four or more).
+Split split_tokens(long long waves, long long tokens) {
     long long k = waves * 2 > kWaves ? 1 : kWaves / std::max(1ll, waves);
-    k = std::max(1ll, std::min(k, tokens / (4 * chunk)));
-    const long long chunks = (tokens + chunk - 1) / chunk;
-    const long long each = (chunks + k - 1) / k;
+    k = std::max(1ll, std::min(k, tokens / (2 * kChunk)));
+    const long long chunks = (tokens + kChunk - 1) / kChunk;
     Split s;
-    s.segment = std::max(1ll, each) * chunk;
+    s.segment = std::max(1ll, (chunks + k - 1) / k) * kChunk;
     s.segments = (int)std::max(1ll, (tokens + s.segment - 1) / s.segment);
     return s;
 }
 
-int launch_with(const void* fn, long long blocks, const ChunkKernel* k, const ChunkArgs& a, hipStream_t s) {
-    const size_t lds = k->lds;
+int launch_with(const void* fn, long long blocks, int threads, size_t lds, const ChunkArgs& a, hipStream_t s) {
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return (int)e;
     }
     void* kargs[1] = {(void*)&a};
-    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)blocks), dim3((unsigned)k->threads), kargs, lds, s);
+    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)blocks), dim3((unsigned)threads), kargs, lds, s);
     return e != hipSuccess ? (int)e : (int)hipGetLastError();
 }
 
@@ -129,7 +128,7 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
     a.scans = count;
     a.slices = (first.dv + k->cols - 1) / k->cols;
     const long long whole = (long long)count * first.batch * first.heads * a.slices;
-    const Split sp = split_tokens(whole * (k->threads / 64), first.tokens, k->chunk);
+    const Split sp = split_tokens(whole * (k->threads / 64), first.tokens);
     a.segments = sp.segments;
     a.segment = sp.segment;
     a.powers = powers;
@@ -140,12 +139,12 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
     if (whole * a.segments > 0x7fffffffll) return (int)hipErrorInvalidConfiguration;
     if (a.segments > 1) {
         work += slot_floats(first, count, a.segments);
-        if (int e = launch_with(k->state_only, whole * a.segments, k, a, st)) return e;
+        if (int e = launch_with(k->state_only, whole * a.segments, k->threads, k->state_lds, a, st)) return e;
         // few segments come with many states, many segments with few
         if (a.segments > 2)
             if (int e = a.segments <= 8 ? launch_join<4, 4>(a, st) : launch_join<1, 16>(a, st)) return e;
     }
-    return launch_with(k->run, whole * a.segments, k, a, st);
+    return launch_with(k->run, whole * a.segments, k->threads, k->lds, a, st);
 }
 
 }  // namespace
@@ -153,8 +152,8 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
 size_t scan_work_floats(int element, int dk, int dv, int heads, int count, long long max_batch, long long max_tokens) {
     const ChunkKernel* k = chunk_kernel(element, dk, dv);
     const int slices = (dv + k->cols - 1) / k->cols;
-    // segments > 1 only below kWaves waves in all, and never over tokens / (4 chunk) of them
-    const long long most = std::max(1ll, max_tokens / (4 * k->chunk));
+    // segments > 1 only below kWaves waves in all, and never over tokens / (2 kChunk) of them
+    const long long most = std::max(1ll, max_tokens / (2 * kChunk));
     const long long states = std::min((long long)count * max_batch * heads * most, kWaves / (k->threads / 64) / slices);
     return most > 1 ? (size_t)states * dk * dv : 0;
 }

@@ -46,6 +46,11 @@ __device__ __forceinline__ float whole_segment(const float* powers, long long se
     return (float)power;
 }
 
+// Tokens of a chunk: what one product sums over. With 64 the state is split
+// half as often, but o, the weights and what is read ahead take the registers of
+// a second wave (bf16, 8 x 2048 tokens, 16 heads of 128: 157 us, with 32 90).
+constexpr int kChunk = 32;
+
 struct ChunkArgs {
     ScanArgs scan[3];
     int scans;
@@ -298,7 +303,7 @@ __device__ __forceinline__ void store_four(T* to, f32x4 y, int room) {
     }
 }
 
-template <typename T, int DK, int WAVES, int NT, int C>
+template <typename T, int DK, int WAVES, int NT, int C, bool STATE_ONLY>
 struct ChunkShape {
     static constexpr int kIn = Parts<T>::in, kMid = Parts<T>::mid;
     static constexpr int kThreads = 64 * WAVES, kCols = 16 * NT * WAVES;
@@ -306,19 +311,19 @@ struct ChunkShape {
     static constexpr int kPitchK = DK + 8, kPitchV = kCols + 8, kPitchP = C + 8;
     // A, B and C, twice where a CU's LDS then still holds a second block or there is none anyway: the next chunk is
     // written while other waves read this one
-    static constexpr size_t kA = 0, kB = kA + (size_t)kIn * C * kPitchK, kC = kB + (size_t)kIn * C * kPitchK,
-                            kOne = kC + (size_t)kIn * C * kPitchV, kRest = (size_t)kMid * C * kPitchP * 2 + kDecayPowers * 4 + 16;
+    static constexpr size_t kA = 0, kB = STATE_ONLY ? 0 : (size_t)kIn * C * kPitchK, kC = kB + (size_t)kIn * C * kPitchK,
+                            kOne = kC + (size_t)kIn * C * kPitchV, kScores = STATE_ONLY ? 0 : (size_t)kMid * C * kPitchP, kRest = kScores * 2 + kDecayPowers * 4 + 16;
     static constexpr size_t kCu = 160 * 1024;
     static constexpr bool kTwice = 2 * (4 * kOne + kRest) <= kCu || (2 * (2 * kOne + kRest) > kCu && 4 * kOne + kRest <= kCu);
-    static constexpr size_t kP = kTwice ? 2 * kOne : kOne, kEnd = kP + (size_t)kMid * C * kPitchP;
+    static constexpr size_t kP = kTwice ? 2 * kOne : kOne, kEnd = kP + kScores;
     static constexpr size_t kLds = kEnd * 2 + kDecayPowers * 4 + 16;
     // waves that share a SIMD's registers: two, or the one that the LDS leaves
     static constexpr int kShare = (int)(kCu / kLds) * WAVES >= 8 ? 2 : 1;
 };
 
 template <typename T, int DK, int WAVES, int NT, int C, bool STATE_ONLY>
-__global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShare)) void k_chunk(const ChunkArgs args) {
-    using S = ChunkShape<T, DK, WAVES, NT, C>;
+__global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_ONLY>::kShare)) void k_chunk(const ChunkArgs args) {
+    using S = ChunkShape<T, DK, WAVES, NT, C, STATE_ONLY>;
     constexpr int IN = S::kIn, MID = S::kMid, TI = C / 16, THREADS = S::kThreads;
     extern __shared__ __align__(16) char lds[];
     __bf16* la = (__bf16*)lds + S::kA;
@@ -388,6 +393,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int a = 0; a < DK / 16; ++a) X[t][a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float factor = 1.f;  // the state is factor X
     const int state_size = s.dk * s.dv;
     if constexpr (STATE_ONLY) {
         if (seg == 0 && s.state_in) read_state(s.state_in + head_state, s.state_row, s.state_col);
@@ -535,15 +541,21 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int I = 0; I < TI; ++I) o[t][I] *= oweight[I];
+                for (int I = 0; I < TI; ++I) o[t][I] *= oweight[I] * factor;
             __syncthreads();  // P is written
         }
 
-        const float whole = pw[left];
+        // the state decays by its factor; X itself only when that gets small, so that what is added to X does not
+        // get large
+        factor *= pw[left];
+        if (factor < 0x1p-10f) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int a = 0; a < DK / 16; ++a) X[t][a] *= whole;
+                for (int a = 0; a < DK / 16; ++a) X[t][a] *= factor;
+            factor = 1.f;
+        }
+        const float added = 1.f / factor;
 #pragma unroll
         for (int k = 0; k < C / 32; ++k) {
             bf16x8 cv[NT][IN], cw[NT][3];
@@ -566,6 +578,9 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
                     for (int t = 0; t < NT; ++t) mma_parts(cv[t], p, o[t] + I, MID);
                 }
             }
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = uweight[k][e] * added;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float v[8];
@@ -574,7 +589,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
                     v[e] = (float)cv[t][IN - 1][e];
 #pragma unroll
                     for (int i = IN - 2; i >= 0; --i) v[e] += (float)cv[t][i][e];
-                    v[e] *= uweight[k][e];
+                    v[e] *= w[e];
                 }
                 split<true>(v, cw[t]);
             }
@@ -613,6 +628,10 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
         }
     }
 
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int a = 0; a < DK / 16; ++a) X[t][a] *= factor;
     if constexpr (STATE_ONLY) {
         write_state(slot + state_size, s.dv, 1);  // to the next segment's place
         return;
@@ -629,8 +648,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C>::kShar
 }
 
 struct ChunkKernel {
-    int cols, chunk, threads;  // columns and threads of a block, tokens of a chunk
-    size_t lds;
+    int cols, threads;  // of a block
+    size_t lds, state_lds;
     const void* run;
     const void* state_only;
 };
@@ -641,16 +660,21 @@ const ChunkKernel* chunk_kernel_bf16(int dk, int dv);
 
 template <typename T, int DK, int WAVES, int NT, int C>
 ChunkKernel chunk_kernel_of() {
-    using S = ChunkShape<T, DK, WAVES, NT, C>;
-    return ChunkKernel{S::kCols, C, S::kThreads, S::kLds, (const void*)k_chunk<T, DK, WAVES, NT, C, false>,
+    using S = ChunkShape<T, DK, WAVES, NT, C, false>;
+    return ChunkKernel{S::kCols,
+                       S::kThreads,
+                       S::kLds,
+                       ChunkShape<T, DK, WAVES, NT, C, true>::kLds,
+                       (const void*)k_chunk<T, DK, WAVES, NT, C, false>,
                        (const void*)k_chunk<T, DK, WAVES, NT, C, true>};
 }
 
 // Key widths are padded to one of six. A block has 64 columns, or 128 where
 // there are more values than 64; a wave 32 of them while the state's rows leave
 // it the registers: what it reads of A, B and P then serves two products.
-template <typename T, int C>
+template <typename T>
 const ChunkKernel* pick_chunk_kernel(int dk, int dv) {
+    constexpr int C = kChunk;
     constexpr bool f32 = Parts<T>::in == 3;  // a third part of everything
     static const ChunkKernel kernels[6][2] = {
         {chunk_kernel_of<T, 32, 2, 2, C>(), chunk_kernel_of<T, 32, 4, 2, C>()},
