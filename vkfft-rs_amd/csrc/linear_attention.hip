@@ -21,7 +21,7 @@ __global__ __launch_bounds__(256) void k_chunk_join(const ChunkArgs args) {
     const int last = (int)((n + args.segment - 1) / args.segment);  // segments that have tokens
     if (last < 3) return;
     const int size = s.dk * s.dv, e = blockIdx.x * 256 * EACH + threadIdx.x;
-    float* slot = args.slots + (((long long)z * batch + b) * s.heads + h) * args.segments * size + size;
+    float* slot = args.slots[z] + ((long long)b * s.heads + h) * args.segments * size + size;
     int at[EACH];
     float x[EACH];
 #pragma unroll
@@ -82,29 +82,14 @@ const ChunkKernel* chunk_kernel(int element, int dk, int dv) {
                                          : chunk_kernel_bf16(dk, dv);
 }
 
-// Waves that keep the GPU's 256 CUs busy: two on each SIMD. (Half as many, with
-// fewer segments to join: bf16, 8 x 2048 tokens of 16 heads of 128, 114 us
-// instead of 88; 1 x 65536 of 16 heads of 64, 188 instead of 112.)
-constexpr long long kWaves = 2048;
-
-struct Split {
-    int segments;
-    long long segment;
-};
-
-// Where the waves of whole sequences are fewer than half of kWaves, the tokens
-// are split too: every segment but the last is read once more for its share of
-// the state. A segment has two chunks or more (f32, 3 x 1001 tokens of 12 heads
-// of 80 x 96: 44 us; 49 with four or more).
-Split split_tokens(long long waves, long long tokens) {
-    long long k = waves * 2 > kWaves ? 1 : kWaves / std::max(1ll, waves);
-    k = std::max(1ll, std::min(k, tokens / (2 * kChunk)));
-    const long long chunks = (tokens + kChunk - 1) / kChunk;
-    Split s;
-    s.segment = std::max(1ll, (chunks + k - 1) / k) * kChunk;
-    s.segments = (int)std::max(1ll, (tokens + s.segment - 1) / s.segment);
-    return s;
+// Blocks of a kernel that the GPU holds at a time: two waves on each SIMD, as
+// far as the LDS goes.
+long long resident(const ChunkKernel* k, size_t lds, int cus) {
+    return (long long)cus * std::max(1, std::min(8 / (k->threads / 64), (int)(160 * 1024 / lds)));
 }
+
+// Most states that a call keeps between segments.
+constexpr long long kStates = 1024;
 
 int launch_with(const void* fn, long long blocks, int threads, size_t lds, const ChunkArgs& a, hipStream_t s) {
     if (lds > 65536) {
@@ -116,59 +101,115 @@ int launch_with(const void* fn, long long blocks, int threads, size_t lds, const
     return e != hipSuccess ? (int)e : (int)hipGetLastError();
 }
 
-long long slot_floats(const ScanArgs& s, int count, int segments) {
-    return segments > 1 ? (long long)count * s.batch * s.heads * segments * s.dk * s.dv : 0;
+// Scans of one shape: one launch.
+struct Part {
+    const ChunkKernel* k;
+    ChunkArgs a;
+    int members[3], states;  // scans that form a state come first
+    long long run, state;    // blocks of a segment
+};
+
+// Tokens of a segment. Where whole sequences leave part of the GPU idle, the
+// tokens are split; every segment but the last is then read once more for its
+// share of the state, at about 0.4 of the cost. The time of k segments is that
+// of the rounds of resident blocks, each 1/k of the tokens long at 3 us a chunk,
+// and of the states' bytes, written, joined and read at 4 TB/s. (bf16, 4 x 4096
+// tokens, 16 heads of 128, backward, 192 blocks: 298 us with the 5 segments that
+// this gives, two rounds; 341 with 2, 328 with 8.) A segment has two chunks or
+// more.
+long long split_tokens(const Part* parts, int count, long long states, int size, long long tokens, int cus) {
+    const long long most = std::max(1ll, std::min(tokens / (2 * kChunk), kStates / states));
+    const double whole = 3.0 * (double)std::max(1ll, tokens / kChunk), state = 16.0 * (double)states * size / 4e6 / whole;
+    const auto rounds = [](long long blocks, long long fit) { return (double)((blocks + fit - 1) / fit); };
+    long long best = 1;
+    double least = 0;
+    for (long long k = 1; k <= most; ++k) {
+        double time = state * (double)(k - 1);
+        for (int i = 0; i < count; ++i) {
+            const Part& p = parts[i];
+            time += (rounds(p.run * k, resident(p.k, p.k->lds, cus)) +
+                     0.4 * rounds(p.state * (k - 1), resident(p.k, p.k->state_lds, cus))) / (double)k;
+        }
+        if (k == 1 || time < least) best = k, least = time;
+    }
+    const long long chunks = (tokens + kChunk - 1) / kChunk;
+    return std::max(1ll, (chunks + best - 1) / best) * kChunk;
 }
 
-int launch_chunks(int element, const ScanArgs* scans, int count, const float* powers, float*& work, hipStream_t st) {
+int launch_chunks(int element, const ScanArgs* scans, int count, const float* powers, float* work, int cus, hipStream_t st) {
     const ScanArgs& first = scans[0];
-    const ChunkKernel* k = chunk_kernel(element, first.dk, first.dv);
-    ChunkArgs a{};
-    for (int i = 0; i < count; ++i) a.scan[i] = scans[i];
-    a.scans = count;
-    a.slices = (first.dv + k->cols - 1) / k->cols;
-    const long long whole = (long long)count * first.batch * first.heads * a.slices;
-    const Split sp = split_tokens(whole * (k->threads / 64), first.tokens);
-    a.segments = sp.segments;
-    a.segment = sp.segment;
-    a.powers = powers;
-    a.slots = work;
-    // a whole sequence's block reads its state before it writes it: only segments need the copy
-    for (int i = 0; i < count && a.segments > 1; ++i)
-        if (scans[i].state_in && scans[i].state_in == scans[i].state_out) a.in_place = 1;
-    if (whole * a.segments > 0x7fffffffll) return (int)hipErrorInvalidConfiguration;
-    if (a.segments > 1) {
-        work += slot_floats(first, count, a.segments);
-        if (int e = launch_with(k->state_only, whole * a.segments, k->threads, k->state_lds, a, st)) return e;
-        // few segments come with many states, many segments with few
-        if (a.segments > 2)
-            if (int e = a.segments <= 8 ? launch_join<4, 4>(a, st) : launch_join<1, 16>(a, st)) return e;
+    Part parts[3] = {};
+    int n = 0, part_of[3], place[3], states = 0;
+    for (int i = 0; i < count; ++i) {
+        int p = 0;
+        while (p < n && (scans[parts[p].members[0]].dk != scans[i].dk || scans[parts[p].members[0]].dv != scans[i].dv)) ++p;
+        if (p == n) {
+            ++n;
+            parts[p].k = chunk_kernel(element, scans[i].dk, scans[i].dv);
+            parts[p].a.slices = (scans[i].dv + parts[p].k->cols - 1) / parts[p].k->cols;
+            parts[p].a.powers = powers;
+        }
+        part_of[i] = p;
+        place[i] = parts[p].a.scans++;
+        parts[p].members[place[i]] = i;
+        parts[p].a.scan[place[i]] = scans[i];
+        const long long blocks = first.batch * (long long)first.heads * parts[p].a.slices;
+        parts[p].run += blocks;
+        if (scans[i].like < 0) {
+            ++parts[p].states;
+            ++states;
+            parts[p].state += blocks;
+        }
     }
-    return launch_with(k->run, whole * a.segments, k->threads, k->lds, a, st);
+    const long long heads = first.batch * (long long)first.heads;
+    const long long segment = split_tokens(parts, n, states * heads, first.dk * first.dv, first.tokens, cus);
+    const int segments = (int)std::max(1ll, (first.tokens + segment - 1) / segment);
+    const long long floats = heads * segments * first.dk * first.dv;
+    float* slots[3];
+    for (int i = 0; i < count; ++i) {
+        const int from = scans[i].like < 0 ? i : scans[i].like;
+        ChunkArgs& a = parts[part_of[i]].a;
+        a.segments = segments;
+        a.segment = segment;
+        if (segments == 1) continue;
+        if (from == i) {
+            slots[i] = work;
+            work += floats;
+        }
+        a.slots[place[i]] = slots[from];
+        a.slot_row[place[i]] = from == i ? scans[i].dv : 1;
+        a.slot_col[place[i]] = from == i ? 1 : scans[i].dk;
+        // a whole sequence's block reads its state before it writes it: only segments need the copy
+        if (scans[i].state_in && scans[i].state_in == scans[i].state_out) a.in_place = 1;
+    }
+    for (int p = 0; p < n; ++p)
+        if (parts[p].run * segments > 0x7fffffffll) return (int)hipErrorInvalidConfiguration;
+    for (int p = 0; p < n && segments > 1; ++p) {
+        ChunkArgs a = parts[p].a;
+        a.scans = parts[p].states;
+        if (!a.scans) continue;
+        if (int e = launch_with(parts[p].k->state_only, parts[p].state * segments, parts[p].k->threads, parts[p].k->state_lds, a, st))
+            return e;
+        // few segments come with many states, many segments with few
+        if (segments > 2)
+            if (int e = segments <= 8 ? launch_join<4, 4>(a, st) : launch_join<1, 16>(a, st)) return e;
+    }
+    for (int p = 0; p < n; ++p)
+        if (int e = launch_with(parts[p].k->run, parts[p].run * segments, parts[p].k->threads, parts[p].k->lds, parts[p].a, st)) return e;
+    return (int)hipSuccess;
 }
 
 }  // namespace
 
-size_t scan_work_floats(int element, int dk, int dv, int heads, int count, long long max_batch, long long max_tokens) {
-    const ChunkKernel* k = chunk_kernel(element, dk, dv);
-    const int slices = (dv + k->cols - 1) / k->cols;
-    // segments > 1 only below kWaves waves in all, and never over tokens / (2 kChunk) of them
-    const long long most = std::max(1ll, max_tokens / (2 * kChunk));
-    const long long states = std::min((long long)count * max_batch * heads * most, kWaves / (k->threads / 64) / slices);
-    return most > 1 ? (size_t)states * dk * dv : 0;
+size_t scan_work_floats(int dk, int dv, int heads, int states, long long max_batch, long long max_tokens) {
+    const long long most = max_tokens / (2 * kChunk);
+    return most > 1 ? (size_t)std::min(states * max_batch * heads * most, kStates) * (size_t)(dk * dv) : 0;
 }
 
 int launch_scans(int element, const ScanArgs* scans, int count, const float* powers, float* work, int cus, hipStream_t s) {
     // the recurrence itself while a chunk would be mostly empty
     if (scans[0].tokens <= kStepTokens) return launch_steps(element, scans, count, powers, cus, s);
-    // scans of one shape run side by side
-    for (int i = 0; i < count;) {
-        int j = i + 1;
-        while (j < count && scans[j].dk == scans[i].dk && scans[j].dv == scans[i].dv) ++j;
-        if (int e = launch_chunks(element, scans + i, j - i, powers, work, s)) return e;
-        i = j;
-    }
-    return (int)hipSuccess;
+    return launch_chunks(element, scans, count, powers, work, cus, s);
 }
 
 int launch_group_sum(int element, const GroupSum& a, const GroupSum& b, long long batch, long long tokens, int kv_heads,

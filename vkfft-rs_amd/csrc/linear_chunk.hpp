@@ -57,10 +57,11 @@ struct ChunkArgs {
     int slices;     // blocks side by side over dv
     int segments;   // parts of the tokens, each `segment` long (a multiple of the chunk)
     long long segment;
-    // segments > 1: [scan][batch][head][segment][dk][dv], the state before each segment; until k_chunk_join ran, from
-    // the third on what the segment before it adds. The first is state_in itself, or with in_place (another block's
-    // state_out may then overwrite that) its copy.
-    float* slots;
+    // segments > 1: each scan's [batch][head][segment][dk][dv], the state before each segment; until k_chunk_join ran,
+    // from the third on what the segment before it adds. The first is state_in itself, or with in_place (another
+    // block's state_out may then overwrite that) its copy. A scan whose state another one forms reads that transposed.
+    float* slots[3];
+    int slot_row[3], slot_col[3];
     int in_place;
     const float* powers;
 };
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
     f32x4 X[NT][DK / 16];
     const int col = col0 + wcol + l16;
     const long long head_state = ((long long)b * s.heads + h) * s.dk * s.dv;
-    float* const slot = args.slots + ((((long long)z * s.batch + b) * s.heads + h) * args.segments + seg) * s.dk * s.dv;
+    float* const slot = args.slots[z] + (((long long)b * s.heads + h) * args.segments + seg) * s.dk * s.dv;
     // All of a state's elements are asked for before the first is waited for: rows and columns past the last
     // read the last one, and are left out by what they meet - zeros in A, B and C - and where X is written.
     const auto read_state = [&](const float* from, int row_step, int col_step) {
@@ -397,13 +398,13 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
     const int state_size = s.dk * s.dv;
     if constexpr (STATE_ONLY) {
         if (seg == 0 && s.state_in) read_state(s.state_in + head_state, s.state_row, s.state_col);
-        if (seg == 0 && args.in_place) write_state(slot, s.dv, 1);
+        if (seg == 0 && args.in_place) write_state(slot, args.slot_row[z], args.slot_col[z]);
         // a state before the next segment is needed only where that one has tokens
         if (n - begin <= segment) return;
     } else if (seg == 0 && !args.in_place) {
         if (s.state_in) read_state(s.state_in + head_state, s.state_row, s.state_col);
     } else if (begin < n || seg == 0) {
-        read_state(slot, s.dv, 1);
+        read_state(slot, args.slot_row[z], args.slot_col[z]);
     }
 
     const int reverse = s.reverse;
@@ -633,7 +634,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
 #pragma unroll
         for (int a = 0; a < DK / 16; ++a) X[t][a] *= factor;
     if constexpr (STATE_ONLY) {
-        write_state(slot + state_size, s.dv, 1);  // to the next segment's place
+        write_state(slot + state_size, args.slot_row[z], args.slot_col[z]);  // to the next segment's place
         return;
     }
     // rows past the sequence's length

@@ -112,13 +112,9 @@ ScanSide side(const vkfx_sequence& s, int group) {
 
 // Floats that calls of the scans need for states between segments.
 uint64_t state_floats(const vkfx_linear_attention_desc& d) {
-    const int dk = (int)d.key_dim, dv = (int)d.value_dim, h = (int)d.heads;
-    const long long b = (long long)d.max_batch, t = (long long)d.max_tokens;
-    const uint64_t forward = scan_work_floats(d.element, dk, dv, h, 1, b, t);
-    if (!d.gradient) return forward;
-    // dq, dk over dv x dk; dv over dk x dv; all together where the widths are equal
-    if (dk == dv) return std::max<uint64_t>(forward, scan_work_floats(d.element, dk, dv, h, 3, b, t));
-    return std::max<uint64_t>(forward, scan_work_floats(d.element, dv, dk, h, 2, b, t) + forward);
+    // backward: the state for dq, its gradient for dk and dv
+    return scan_work_floats((int)d.key_dim, (int)d.value_dim, (int)d.heads, d.gradient ? 2 : 1, (long long)d.max_batch,
+                            (long long)d.max_tokens);
 }
 
 // Floats of the gradients of k and v for each query head, summed over a shared
@@ -322,6 +318,7 @@ int vkfx_linear_attention_forward(vkfx_linear_attention* plan, const vkfx_linear
         s.dv = (int)d.value_dim;
         s.scale_in = (float)d.scale;
         s.scale_update = 1.f;
+        s.like = -1;
         (void)hipSetDevice(plan->ctx->device);
         float* work = (float*)(d_work ? d_work : plan->work.p);
         const int e = launch_scans(d.element, &s, 1, (const float*)plan->powers.p, work, (int)plan->ctx->profile.compute_units,
@@ -374,9 +371,11 @@ int vkfx_linear_attention_backward(vkfx_linear_attention* plan, const vkfx_linea
             return s;
         };
         // dq: the forward scan of (dout, v, k) from the state's transpose
-        ScanArgs scans[3] = {scan(args->dout, 1, args->v, group, args->k, group), scan(args->v, group, args->dout, 1, args->q, 1),
-                             scan(args->k, group, args->q, 1, args->dout, 1)};
-        ScanArgs &q = scans[0], &k = scans[1], &v = scans[2];
+        ScanArgs scans[3] = {scan(args->dout, 1, args->v, group, args->k, group), scan(args->k, group, args->q, 1, args->dout, 1),
+                             scan(args->v, group, args->dout, 1, args->q, 1)};
+        ScanArgs &q = scans[0], &v = scans[1], &k = scans[2];
+        q.like = v.like = -1;
+        k.like = 1;
         q.dk = dv, q.dv = dk, q.state_row = 1, q.state_col = dv, q.state_in = args->state_in;
         q.scale_in = (float)d.scale, q.scale_update = 1.f;
         v.dk = dk, v.dv = dv, v.state_row = dv, v.state_col = 1, v.state_in = args->dstate_out, v.state_out = args->dstate_in;

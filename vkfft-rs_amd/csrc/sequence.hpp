@@ -62,6 +62,7 @@ struct ScanArgs {
     int batch, heads, dk, dv;
     int reverse;  // and lead
     float scale_in, scale_update;
+    int like;  // -1, or the scan whose state is this one's transpose, which then forms it for both
 };
 
 // Powers 0, 1, ... of each head's decay, kDecayPowers floats a head; the last
@@ -74,9 +75,9 @@ int launch_steps(int element, const ScanArgs* scans, int count, const float* pow
 
 // `count` scans (up to 3) of the same batch, tokens and heads, by the kernels
 // that suit the number of tokens (linear_attention.hip). `work` holds
-// scan_work_floats of every shape among them.
+// scan_work_floats, `states`: scans without a `like`.
 int launch_scans(int element, const ScanArgs* scans, int count, const float* powers, float* work, int cus, hipStream_t s);
-size_t scan_work_floats(int element, int dk, int dv, int heads, int count, long long max_batch, long long max_tokens);
+size_t scan_work_floats(int dk, int dv, int heads, int states, long long max_batch, long long max_tokens);
 
 // Sums the floats [batch][token][head][dim] of each shared head's `group`
 // query heads, in their order; two tensors at once.
