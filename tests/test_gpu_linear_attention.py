@@ -435,3 +435,36 @@ def test_long_prompts_update_a_state_in_place(hip_ctx, lengths):
     plan.forward_tensors(q, k, v, out, state_in=state, state_out=after, lengths=n)
     plan.forward_tensors(q, k, v, again, state_in=state, state_out=state, lengths=n)
     assert torch.equal(out, again) and torch.equal(after, state)
+
+
+@pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 100), (5, 6)])
+def test_bad_values_do_not_reach_the_tokens_before(hip_ctx, element, dk, dv):
+    """An infinity or a NaN in a token changes that token and later ones; backwards, keys and values of that token and earlier ones."""
+    import torch
+    t, at = 100, 43
+    plan = _plan(hip_ctx, 1, t, 2, 2, dk, dv, element, True)
+    x = [_tensor(i, (1, t, 2, d), element) for i, d in ((1, dk), (2, dk), (3, dv), (4, dv))]
+
+    def run():
+        o = [torch.full_like(x[i], 3) for i in (3, 0, 1, 2)]
+        plan.forward_tensors(*x[:3], o[0])
+        plan.backward_tensors(*x, *o[1:])
+        return o
+
+    want = run()
+    for i, value in ((0, float("nan")), (1, float("inf")), (2, float("nan")), (2, float("inf")), (3, float("-inf"))):
+        keep = x[i].clone()
+        x[i][0, at, 0, 0] = value
+        out, dq, dk_, dv_ = run()
+        x[i].copy_(keep)
+        forward, backward = i != 3, i in (0, 3)
+        assert torch.equal(out[:, :at], want[0][:, :at])
+        assert torch.equal(dq[:, :at], want[1][:, :at])
+        assert torch.equal(out[:, :, 1], want[0][:, :, 1])
+        if backward:  # q and dout enter the state's gradient from their token backwards
+            assert torch.equal(dk_[:, at + 1:], want[2][:, at + 1:]) and torch.equal(dv_[:, at + 1:], want[3][:, at + 1:])
+        if forward:
+            assert not torch.isfinite(out[:, at, 0]).all()
+        if not backward:
+            assert torch.equal(dv_ if i == 2 else dk_, want[3 if i == 2 else 2])  # dv does not depend on v, dk not on k

@@ -170,6 +170,29 @@ struct PackedEight {
     typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
+// 0, or a NaN where an element is infinite or a NaN.
+__device__ __forceinline__ float times_zero(const Eight<float>& x) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(x[e], 0.f, s);
+    return s;
+}
+__device__ __forceinline__ float times_zero(const Eight<_Float16>& x) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) s = __builtin_amdgcn_fdot2(f16x2{x[e], x[e + 1]}, f16x2{0, 0}, s, false);
+    return s;
+}
+__device__ __forceinline__ float times_zero(const Eight<__bf16>& x) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+        s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[e], x[e + 1]}, bf16x2{(__bf16)0.f, (__bf16)0.f}, s, false);
+    return s;
+}
+
 // One thread's share of a chunk of rows [C][D] on its way to LDS: vectors of
 // eight elements at one column of every kRows-th row, read ahead while the
 // chunk before is worked on. The reads take no branch, which would make the
@@ -220,6 +243,24 @@ struct Staged {
     __device__ __forceinline__ void arrive() {
 #pragma unroll
         for (int u = 0; u < kEach; ++u) asm volatile("" : "+v"(r[u]));
+    }
+
+    // Bits of the rows that hold an infinity or a NaN.
+    __device__ __forceinline__ void mark(unsigned* bad, int left) const {
+        if (slow) {
+#pragma unroll 1
+            for (int j = (int)threadIdx.x; j < left * width; j += THREADS) {
+                const float f = (float)((const T*)(next + j / width * token))[j % width];
+                if (f - f != 0.f) atomicOr(bad, 1u << (j / width));
+            }
+            return;
+        }
+        if (col >= width || row >= C) return;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const float none = times_zero(r[u]);
+            if (none != 0.f && row + u * kRows < left) atomicOr(bad, 1u << (row + u * kRows));
+        }
     }
 
     // The chunk that was asked for to lds[part][C][pitch], rows from `left` on as zeros; then on to the next.
@@ -333,6 +374,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
     int other = S::kTwice ? (int)S::kOne : 0;  // from this chunk's buffer to the next one's
     __bf16* const lp = (__bf16*)lds + S::kP;
     float* const pw = (float*)((__bf16*)lds + S::kEnd);
+    unsigned* const bad = (unsigned*)(pw + kDecayPowers);  // of this chunk and of the next, in turn
 
     // block -> (scan, sequence, head, segment, slice), slices side by side
     long long id = blockIdx.x;
@@ -355,6 +397,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
     const int g = lane >> 4, l16 = lane & 15;
     const int col0 = slice * S::kCols, wcol = wave * 16 * NT;
     const int lead = s.reverse;
+    if (tid < 2) bad[tid] = 0;
     if (tid < kDecayPowers) pw[tid] = args.powers[(long long)h * kDecayPowers + tid];
     // columns past the tensors', and tiles of P right of the diagonal that a product of 32 tokens meets
     for (int i = tid; i < (int)(S::kEnd / 8); i += THREADS) ((bf16x8*)lds)[i] = (__bf16)0.f;
@@ -426,7 +469,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
         sb.arrive();
         sc.arrive();
     };
-    const auto stage = [&](int left) {
+    const auto stage = [&](int left, unsigned* marks) {
+        if (!STATE_ONLY) sc.mark(marks, left);
         if (!STATE_ONLY) sa.store(la, S::kPitchK, left);
         sb.store(lb, S::kPitchK, left);
         sc.store(lc, S::kPitchV, left);
@@ -477,7 +521,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
         for (int a = 0; a < DK / 16; ++a) asm volatile("" : "+v"(X[t][a]));
     if (begin < stop) fetch(stop - begin < C ? stop - begin : C);
     arrive();
-    if (begin < stop) stage(stop - begin < C ? stop - begin : C);
+    if (begin < stop) stage(stop - begin < C ? stop - begin : C, bad);
+    int turn = 0;
 #pragma unroll 1
     for (int at = begin; at < stop; at += C) {
         const int left = stop - at < C ? stop - at : C;
@@ -485,6 +530,9 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
         __syncthreads();
         if (more) fetch(more);
         if (left < C) update_weights(left);
+        const unsigned unsafe = STATE_ONLY ? 0u : (unsigned)__builtin_amdgcn_readfirstlane((int)bad[turn]);
+        turn ^= 1;
+        if (tid == 0) bad[turn] = 0;  // nobody marks the next chunk's rows before P's barrier
 
         f32x4 o[NT][TI];
         if constexpr (!STATE_ONLY) {
@@ -566,6 +614,17 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
                 for (int i = 0; i < IN; ++i)
                     cv[t][i] = column_operand(lc + i * C * S::kPitchV, S::kPitchV, 32 * k, wcol + 16 * t, lane);
             if constexpr (!STATE_ONLY) {
+                static_assert(C == 32, "one word of marks, one turn of this loop");
+                // A row of C that is not finite would reach the tokens before it through their zeros in P: it is left out
+                // here and added to the others below.
+                if (unsafe)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < IN; ++i)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (unsafe >> (8 * g + e) & 1) cv[t][i][e] = (__bf16)0.f;
                 // tiles of 16 tokens from 32 k on, two at a time
 #pragma unroll
                 for (int I = 2 * k; I < TI; I += 2) {
@@ -577,6 +636,34 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
                             p[u][m] = *(const bf16x8*)(lp + (m * C + 16 * (I + u) + l16) * S::kPitchP + 32 * k + 8 * g);
 #pragma unroll
                     for (int t = 0; t < NT; ++t) mma_parts(cv[t], p, o[t] + I, MID);
+                }
+                if (unsafe) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < IN; ++i)
+                            cv[t][i] = column_operand(lc + i * C * S::kPitchV, S::kPitchV, 32 * k, wcol + 16 * t, lane);
+#pragma unroll 1
+                    for (int j = 0; j < C; ++j) {
+                        if (!(unsafe >> j & 1)) continue;
+#pragma unroll
+                        for (int I = 0; I < TI; ++I) {
+                            if (16 * I + l16 < j) continue;
+                            float p = 0.f;
+#pragma unroll
+                            for (int m = MID - 1; m >= 0; --m) p += (float)lp[(m * C + 16 * I + l16) * S::kPitchP + j];
+#pragma unroll
+                            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    float c = 0.f;
+#pragma unroll
+                                    for (int i = IN - 1; i >= 0; --i)
+                                        c += (float)lc[(i * C + j) * S::kPitchV + wcol + 16 * t + 4 * g + r];
+                                    o[t][I][r] = fmaf(p, c, o[t][I][r]);
+                                }
+                        }
+                    }
                 }
             }
             float w[8];
@@ -612,7 +699,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
         la += other, lb += other, lc += other;
         other = -other;
         // before this chunk's stores: loads and stores are waited for in their order
-        if (more) stage(more);
+        if (more) stage(more, bad + turn);
         if constexpr (!STATE_ONLY) {
 #pragma unroll
             for (int I = 0; I < TI; ++I) {
