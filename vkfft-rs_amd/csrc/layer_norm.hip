@@ -157,11 +157,20 @@ __global__ __launch_bounds__(NT) void k_norm_forward(const NormArgs a) {
     }
 }
 
+// Floats in which half of a block's row groups hand the other half their sums,
+// both kinds at a time where that stays within 48 KB.
+template <typename T, int LPR, int NV, int NT>
+constexpr int kHalf = NT > LPR ? NV * LPR * kVector<T> * (LPR < 64 ? NT / 64 : NT / LPR) / 2 : 0;
+template <typename T, int LPR, int NV, int NT>
+constexpr bool kSumsBoth = kHalf<T, LPR, NV, NT> * 8 <= 48 * 1024;
+template <typename T, int LPR, int NV, int NT>
+constexpr int kSums = kHalf<T, LPR, NV, NT> * (kSumsBoth<T, LPR, NV, NT> ? 2 : 1);
+
 template <typename T, typename W, int LPR, int NV, int NT>
 __global__ __launch_bounds__(NT) void k_norm_backward(const NormArgs a) {
     constexpr int V = kVector<T>, R = NT / LPR;
     constexpr bool kAhead = NT < 1024 || NV == 1;  // the next row on its way, where the registers hold it
-    extern __shared__ float sums[];  // R > 1: [2][LPR * NV * V]
+    extern __shared__ float sums[];  // kSums floats
     __shared__ float lds[4 * (NT / 64)];
     int half = 0;
     const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
@@ -248,22 +257,39 @@ __global__ __launch_bounds__(NT) void k_norm_backward(const NormArgs a) {
                     db[j][e] += __shfl_xor(db[j][e], o);
                 }
     if constexpr (R > 1) {
-        constexpr int turns = LPR < 64 ? NT / 64 : R, D = LPR * NV * V;
-        const int turn = LPR < 64 ? (int)(threadIdx.x >> 6) : group;
+        // by halves: the upper ones hand their sums to the lower ones
+        constexpr int parts = LPR < 64 ? NT / 64 : R;
+        const int part = LPR < 64 ? (int)(threadIdx.x >> 6) : group;
         const bool mine = LPR >= 64 || (threadIdx.x & 63) < LPR;
-        for (int t = 0; t < turns; ++t) {
-            if (t == turn && mine)
+        const auto at = [&](int p, int j, int e) { return ((p * V + e) * NV + j) * LPR + lane; };
 #pragma unroll
-                for (int j = 0; j < NV; ++j)
+        for (int h = parts / 2; h; h >>= 1) {
+            constexpr int D = parts / 2 * LPR * NV * V;
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const int c = (j * LPR + lane) * V + e;
-                        if (t) dw[j][e] += sums[c], db[j][e] += sums[D + c];
-                        if (t + 1 < turns) sums[c] = dw[j][e], sums[D + c] = db[j][e];
-                    }
-            __syncthreads();
+            for (int both = kSumsBoth<T, LPR, NV, NT> ? 1 : 2, i = 0; i < both; ++i) {
+                const bool w = both == 1 || i == 0, b = both == 1 || i == 1;
+                const int second = both == 1 ? D : 0;
+                if (part >= h && part < 2 * h && mine)
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            if (w) sums[at(part - h, j, e)] = dw[j][e];
+                            if (b) sums[at(part - h, j, e) + second] = db[j][e];
+                        }
+                __syncthreads();
+                if (part < h && mine)
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            if (w) dw[j][e] += sums[at(part, j, e)];
+                            if (b) db[j][e] += sums[at(part, j, e) + second];
+                        }
+                __syncthreads();
+            }
         }
-        if (turn != turns - 1 || !mine) return;
+        if (part || !mine) return;
     }
     // one block: its sums are the gradients
     const bool last = gridDim.x == 1;
@@ -401,7 +427,7 @@ int backward_with(const NormArgs& a, hipStream_t s) {
     constexpr int R = NT / LPR;
     // one block a CU: every block costs a row of sums to write and to add
     const long long blocks = std::min((a.rows + R - 1) / R, (long long)a.cus);
-    const size_t lds = R > 1 ? sizeof(float) * 2 * LPR * NV * kVector<T> : 0;
+    constexpr size_t lds = sizeof(float) * kSums<T, LPR, NV, NT>;
     hipLaunchKernelGGL((k_norm_backward<T, W, LPR, NV, NT>), dim3((unsigned)blocks), dim3(NT), lds, s, a);
     if (blocks > 1 && (a.dweight || a.dbias)) launch_sum<W>(a, (int)blocks, s);
     return (int)hipGetLastError();
