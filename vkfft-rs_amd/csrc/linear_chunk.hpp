@@ -170,23 +170,20 @@ struct PackedEight {
     typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
-// 0, or a NaN where an element is infinite or a NaN.
-__device__ __forceinline__ float times_zero(const Eight<float>& x) {
-    float s = 0.f;
+// s, or a NaN where an element is infinite or a NaN.
+__device__ __forceinline__ float times_zero(const Eight<float>& x, float s) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) s = fmaf(x[e], 0.f, s);
     return s;
 }
-__device__ __forceinline__ float times_zero(const Eight<_Float16>& x) {
+__device__ __forceinline__ float times_zero(const Eight<_Float16>& x, float s) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    float s = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) s = __builtin_amdgcn_fdot2(f16x2{x[e], x[e + 1]}, f16x2{0, 0}, s, false);
     return s;
 }
-__device__ __forceinline__ float times_zero(const Eight<__bf16>& x) {
+__device__ __forceinline__ float times_zero(const Eight<__bf16>& x, float s) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    float s = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; e += 2)
         s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[e], x[e + 1]}, bf16x2{(__bf16)0.f, (__bf16)0.f}, s, false);
@@ -245,26 +242,22 @@ struct Staged {
         for (int u = 0; u < kEach; ++u) asm volatile("" : "+v"(r[u]));
     }
 
-    // Bits of the rows that hold an infinity or a NaN.
-    __device__ __forceinline__ void mark(unsigned* bad, int left) const {
-        if (slow) {
-#pragma unroll 1
-            for (int j = (int)threadIdx.x; j < left * width; j += THREADS) {
-                const float f = (float)((const T*)(next + j / width * token))[j % width];
-                if (f - f != 0.f) atomicOr(bad, 1u << (j / width));
-            }
-            return;
-        }
-        if (col >= width || row >= C) return;
+    // Infinities and NaN of the chunk that was asked for become zeros, and *bad tells of them.
+    __device__ __forceinline__ void make_finite(unsigned* bad) {
+        float none = 0.f;
 #pragma unroll
-        for (int u = 0; u < kEach; ++u) {
-            const float none = times_zero(r[u]);
-            if (none != 0.f && row + u * kRows < left) atomicOr(bad, 1u << (row + u * kRows));
-        }
+        for (int u = 0; u < kEach; ++u) none = times_zero(r[u], none);
+        if (none == 0.f) return;
+        *bad = 1;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if ((float)r[u][e] * 0.f != 0.f) r[u][e] = (T)0.f;
     }
 
     // The chunk that was asked for to lds[part][C][pitch], rows from `left` on as zeros; then on to the next.
-    __device__ __forceinline__ void store(__bf16* lds, int pitch, int left) {
+    __device__ __forceinline__ void store(__bf16* lds, int pitch, int left, unsigned* bad = nullptr) {
         if (plain && left == C) {
             if (col < width && row < C)
 #pragma unroll
@@ -281,6 +274,7 @@ struct Staged {
             for (int j = (int)threadIdx.x; j < C * D; j += THREADS) {
                 const int i = j / D, c = j % D;
                 float f = i < left && c < width ? (float)((const T*)(next + i * token))[c] : 0.f;
+                if (bad && f * 0.f != 0.f) *bad = 1, f = 0.f;
 #pragma unroll
                 for (int k = 0; k < Parts<T>::in; ++k) {
                     const __bf16 v = (__bf16)f;
@@ -470,10 +464,11 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
         sc.arrive();
     };
     const auto stage = [&](int left, unsigned* marks) {
-        if (!STATE_ONLY) sc.mark(marks, left);
+        // rows of C that are not finite would reach the tokens before them through their zeros in P
+        if (!STATE_ONLY) sc.make_finite(marks);
         if (!STATE_ONLY) sa.store(la, S::kPitchK, left);
         sb.store(lb, S::kPitchK, left);
-        sc.store(lc, S::kPitchV, left);
+        sc.store(lc, S::kPitchV, left, STATE_ONLY ? nullptr : marks);
     };
 
     // where this lane's token of a chunk's first 16 goes, from its first column on
@@ -530,9 +525,9 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
         __syncthreads();
         if (more) fetch(more);
         if (left < C) update_weights(left);
-        const unsigned unsafe = STATE_ONLY ? 0u : (unsigned)__builtin_amdgcn_readfirstlane((int)bad[turn]);
+        const unsigned* const marks = bad + turn;
         turn ^= 1;
-        if (tid == 0) bad[turn] = 0;  // nobody marks the next chunk's rows before P's barrier
+        if (!STATE_ONLY && tid == 0) bad[turn] = 0;  // nobody marks the next chunk before P's barrier
 
         f32x4 o[NT][TI];
         if constexpr (!STATE_ONLY) {
@@ -614,17 +609,6 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
                 for (int i = 0; i < IN; ++i)
                     cv[t][i] = column_operand(lc + i * C * S::kPitchV, S::kPitchV, 32 * k, wcol + 16 * t, lane);
             if constexpr (!STATE_ONLY) {
-                static_assert(C == 32, "one word of marks, one turn of this loop");
-                // A row of C that is not finite would reach the tokens before it through their zeros in P: it is left out
-                // here and added to the others below.
-                if (unsafe)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int i = 0; i < IN; ++i)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (unsafe >> (8 * g + e) & 1) cv[t][i][e] = (__bf16)0.f;
                 // tiles of 16 tokens from 32 k on, two at a time
 #pragma unroll
                 for (int I = 2 * k; I < TI; I += 2) {
@@ -636,34 +620,6 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
                             p[u][m] = *(const bf16x8*)(lp + (m * C + 16 * (I + u) + l16) * S::kPitchP + 32 * k + 8 * g);
 #pragma unroll
                     for (int t = 0; t < NT; ++t) mma_parts(cv[t], p, o[t] + I, MID);
-                }
-                if (unsafe) {
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int i = 0; i < IN; ++i)
-                            cv[t][i] = column_operand(lc + i * C * S::kPitchV, S::kPitchV, 32 * k, wcol + 16 * t, lane);
-#pragma unroll 1
-                    for (int j = 0; j < C; ++j) {
-                        if (!(unsafe >> j & 1)) continue;
-#pragma unroll
-                        for (int I = 0; I < TI; ++I) {
-                            if (16 * I + l16 < j) continue;
-                            float p = 0.f;
-#pragma unroll
-                            for (int m = MID - 1; m >= 0; --m) p += (float)lp[(m * C + 16 * I + l16) * S::kPitchP + j];
-#pragma unroll
-                            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    float c = 0.f;
-#pragma unroll
-                                    for (int i = IN - 1; i >= 0; --i)
-                                        c += (float)lc[(i * C + j) * S::kPitchV + wcol + 16 * t + 4 * g + r];
-                                    o[t][I][r] = fmaf(p, c, o[t][I][r]);
-                                }
-                        }
-                    }
                 }
             }
             float w[8];
@@ -694,6 +650,42 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
             }
         }
 
+        if constexpr (!STATE_ONLY) {
+            if (*marks) {  // what was left out of C, where it belongs
+#pragma unroll 1
+                for (int j = 0; j < left; ++j) {
+                    const T* const row = (const T*)s.c.p + b * s.c.batch + (h / s.c.group) * s.c.head +
+                                         (reverse ? (long long)n - 1 - at - j : (long long)at + j) * s.c.token;
+                    const float weight = pw[left - 1 - j + lead] * scale_update * added;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float c = room > 16 * t + r ? (float)row[out_col + 16 * t + r] : 0.f;
+                            if (c * 0.f == 0.f) continue;
+#pragma unroll
+                            for (int I = 0; I < TI; ++I) {
+                                float p = 0.f;
+#pragma unroll
+                                for (int m = MID - 1; m >= 0; --m) p += (float)lp[(m * C + 16 * I + l16) * S::kPitchP + j];
+                                if (16 * I + l16 >= j) o[t][I][r] = fmaf(p, c, o[t][I][r]);
+                            }
+                        }
+                        const float c = col + 16 * t < s.dv ? (float)row[col + 16 * t] : 0.f;
+                        if (c * 0.f == 0.f) continue;
+#pragma unroll
+                        for (int a = 0; a < DK / 16; ++a)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                float k = 0.f;
+#pragma unroll
+                                for (int i = IN - 1; i >= 0; --i) k += (float)lb[(i * C + j) * S::kPitchK + 16 * a + 4 * g + r];
+                                X[t][a][r] = fmaf(k, weight * c, X[t][a][r]);
+                            }
+                    }
+                }
+            }
+        }
         if (!S::kTwice) __syncthreads();  // the chunk has been read
         arrive();
         la += other, lb += other, lc += other;
