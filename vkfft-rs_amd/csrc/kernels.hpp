@@ -250,6 +250,9 @@ const FixedKernel* kind_variant(const FixedKernel* f, KernelKind kind);
 // t_end: when both are set, HIP events bound to this dispatch
 // (hipExtLaunchKernel) that read the kernel's own begin and end. Returns a
 // hipError_t value.
+// Lets a kernel ask for `bytes` of dynamic LDS on the current device (asked of the runtime once).
+int raise_lds_limit(const void* fn, size_t bytes);
+
 int launch(KernelKind kind, int prec, int dir, const KArgs& a, unsigned grid, unsigned block,
            size_t lds_bytes, hipStream_t stream, const FixedKernel* fixed = nullptr, hipEvent_t t_begin = nullptr,
            hipEvent_t t_end = nullptr);

@@ -206,7 +206,7 @@ static KernelFn pick_kernel(KernelKind kind, int prec, int dir, int flags) {
 // Raises a kernel's dynamic-LDS limit once per (device, kernel) to the
 // largest size launched so far: the attribute persists, and setting it on
 // every launch costs host time on the launch path.
-static int raise_lds_limit(const void* fn, size_t bytes) {
+int raise_lds_limit(const void* fn, size_t bytes) {
     static std::mutex mu;
     static std::map<std::pair<int, const void*>, size_t> done;
     int dev = 0;

@@ -2,6 +2,7 @@
 // of a long sequence's segments and the sum over a shared head's query heads.
 #include <algorithm>
 
+#include "kernels.hpp"
 #include "linear_chunk.hpp"
 #include "vkfx.h"
 
@@ -92,10 +93,8 @@ long long resident(const ChunkKernel* k, size_t lds, int cus) {
 constexpr long long kStates = 1024;
 
 int launch_with(const void* fn, long long blocks, int threads, size_t lds, const ChunkArgs& a, hipStream_t s) {
-    if (lds > 65536) {
-        const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return (int)e;
-    }
+    if (lds > 65536)
+        if (int e = raise_lds_limit(fn, lds)) return e;
     void* kargs[1] = {(void*)&a};
     const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)blocks), dim3((unsigned)threads), kargs, lds, s);
     return e != hipSuccess ? (int)e : (int)hipGetLastError();

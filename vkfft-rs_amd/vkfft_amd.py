@@ -1599,7 +1599,8 @@ class LinearAttentionPlan(_SequencePlan):
 
     def __init__(self, ctx: "HipExecutionContext", config: LinearAttentionConfig):
         super().__init__(ctx, config, config.desc())
-        self._kv = config.heads if config.kv_heads is None else config.kv_heads
+        kv = config.heads if config.kv_heads is None else config.kv_heads
+        self._dims = config.heads, kv, config.key_dim, config.value_dim
 
     def _sequence(self, name, x, shape, device):
         if x.shape != shape or x.dtype is not self._type or x.get_device() != device:
@@ -1608,9 +1609,6 @@ class LinearAttentionPlan(_SequencePlan):
         if d != 1 and shape[3] > 1:
             raise VkFftError(-7, f"{name}: the last dimension must be contiguous")
         return x.data_ptr(), b, t, h
-
-    def _states(self, shape, device, **states):
-        return [self._dense(n, x, shape, self._f32, device) for n, x in states.items()]
 
     def _lengths(self, lengths, batch, device):
         if lengths is None:
@@ -1621,16 +1619,15 @@ class LinearAttentionPlan(_SequencePlan):
     def forward_tensors(self, q, k, v, out, state_in=None, state_out=None, lengths=None, work=None, stream=None):
         """Outputs of a prompt, or of the next token where there is one: from
         state_in (None: zeros) to state_out (None: not wanted; may be state_in)."""
-        c, device = self.config, self._place(q)
+        device, (h, kv, dk, dv) = self._place(q), self._dims
         if q.dim() != 4:
             raise VkFftError(-5, "q must be [batch][token][head][key_dim]")
-        b, t = q.shape[:2]
-        args = _ForwardArgs(b, t, *self._sequence("q", q, (b, t, c.heads, c.key_dim), device),
-                            *self._sequence("k", k, (b, t, self._kv, c.key_dim), device),
-                            *self._sequence("v", v, (b, t, self._kv, c.value_dim), device),
-                            *self._sequence("out", out, (b, t, c.heads, c.value_dim), device),
-                            self._lengths(lengths, b, device),
-                            *self._states((b, c.heads, c.key_dim, c.value_dim), device, state_in=state_in, state_out=state_out))
+        b, t = q.size(0), q.size(1)
+        f, state = self._sequence, (b, h, dk, dv)
+        args = _ForwardArgs(b, t, *f("q", q, (b, t, h, dk), device), *f("k", k, (b, t, kv, dk), device),
+                            *f("v", v, (b, t, kv, dv), device), *f("out", out, (b, t, h, dv), device),
+                            self._lengths(lengths, b, device), self._dense("state_in", state_in, state, self._f32, device),
+                            self._dense("state_out", state_out, state, self._f32, device))
         _check(self._L.vkfx_linear_attention_forward(self.handle, ctypes.byref(args), self._work(work, device),
                                                      self._stream(stream, device)), self._L)
 
@@ -1638,18 +1635,18 @@ class LinearAttentionPlan(_SequencePlan):
                          work=None, stream=None):
         """Gradients of q, k, v and (dstate_in, None: not wanted) of state_in,
         for dout and dstate_out (None: zeros)."""
-        c, device = self.config, self._place(q)
+        device, (h, kv, dk_, dv_) = self._place(q), self._dims
         if q.dim() != 4:
             raise VkFftError(-5, "q must be [batch][token][head][key_dim]")
-        b, t = q.shape[:2]
-        key, value = (b, t, c.heads, c.key_dim), (b, t, c.heads, c.value_dim)
-        shared_key, shared_value = (b, t, self._kv, c.key_dim), (b, t, self._kv, c.value_dim)
-        args = _BackwardArgs(b, t, *self._sequence("q", q, key, device), *self._sequence("k", k, shared_key, device),
-                             *self._sequence("v", v, shared_value, device), *self._sequence("dout", dout, value, device),
-                             *self._sequence("dq", dq, key, device), *self._sequence("dk", dk, shared_key, device),
-                             *self._sequence("dv", dv, shared_value, device), self._lengths(lengths, b, device),
-                             *self._states((b, c.heads, c.key_dim, c.value_dim), device, state_in=state_in,
-                                           dstate_out=dstate_out, dstate_in=dstate_in))
+        b, t = q.size(0), q.size(1)
+        f, state = self._sequence, (b, h, dk_, dv_)
+        key, value, shared_key, shared_value = (b, t, h, dk_), (b, t, h, dv_), (b, t, kv, dk_), (b, t, kv, dv_)
+        args = _BackwardArgs(b, t, *f("q", q, key, device), *f("k", k, shared_key, device), *f("v", v, shared_value, device),
+                             *f("dout", dout, value, device), *f("dq", dq, key, device), *f("dk", dk, shared_key, device),
+                             *f("dv", dv, shared_value, device), self._lengths(lengths, b, device),
+                             self._dense("state_in", state_in, state, self._f32, device),
+                             self._dense("dstate_out", dstate_out, state, self._f32, device),
+                             self._dense("dstate_in", dstate_in, state, self._f32, device))
         _check(self._L.vkfx_linear_attention_backward(self.handle, ctypes.byref(args), self._work(work, device),
                                                       self._stream(stream, device)), self._L)
 
