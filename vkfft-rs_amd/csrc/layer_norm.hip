@@ -60,6 +60,16 @@ __device__ __forceinline__ void store_some(T* row, int c, int width, const Some<
         if (c + e < width) row[c + e] = r[e];
 }
 
+// Makes the compiler take `r` for new: where it is used again it is converted
+// once more, rather than kept in 32 bits from the first time.
+template <typename T, int N>
+__device__ __forceinline__ void again(Some<T, N>& r) {
+    typedef unsigned words __attribute__((ext_vector_type(sizeof(r) / 4)));
+    words w = __builtin_bit_cast(words, r);
+    asm volatile("" : "+v"(w));
+    r = __builtin_bit_cast(Some<T, N>, w);
+}
+
 // Sum over the LPR threads of a row, the same on each. Rows wider than a wave
 // meet in `lds`, of which every call takes the other half: one barrier each.
 template <int LPR, int N>
@@ -166,7 +176,8 @@ constexpr bool kSumsBoth = kHalf<T, LPR, NV, NT> * 8 <= 48 * 1024;
 template <typename T, int LPR, int NV, int NT>
 constexpr int kSums = kHalf<T, LPR, NV, NT> * (kSumsBoth<T, LPR, NV, NT> ? 2 : 1);
 
-template <typename T, typename W, int LPR, int NV, int NT>
+// SUMS: with the gradients of weight and bias.
+template <typename T, typename W, int LPR, int NV, int NT, bool SUMS>
 __global__ __launch_bounds__(NT) void k_norm_backward(const NormArgs a) {
     constexpr int V = kVector<T>, R = NT / LPR;
     constexpr bool kAhead = NT < 1024 || NV == 1;  // the next row on its way, where the registers hold it
@@ -222,8 +233,10 @@ __global__ __launch_bounds__(NT) void k_norm_backward(const NormArgs a) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {  // past the row's end dy is zero
                     const float n = ((float)x[j][e] - mean) * rstd, d = (float)dy[j][e], g = d * (float)wj[e];
-                    dw[j][e] = fmaf(d, n, dw[j][e]);
-                    db[j][e] += d;
+                    if constexpr (SUMS) {
+                        dw[j][e] = fmaf(d, n, dw[j][e]);
+                        db[j][e] += d;
+                    }
                     s[0] += g;
                     s[1] = fmaf(g, n, s[1]);
                 }
@@ -235,6 +248,7 @@ __global__ __launch_bounds__(NT) void k_norm_backward(const NormArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             Some<T, V> dx;
+            if constexpr (!SUMS) again<T, V>(x[j]), again<T, V>(dy[j]);
             const Some<W, V> wj = weight(j);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -244,7 +258,7 @@ __global__ __launch_bounds__(NT) void k_norm_backward(const NormArgs a) {
             store_some<T, V>((T*)a.y + r * a.y_stride, (j * LPR + lane) * V, a.width, dx);
         }
     }
-    if (!a.dweight && !a.dbias) return;
+    if (!SUMS || (!a.dweight && !a.dbias)) return;
     // the block's rows side by side: lanes of a wave, then its waves one after the other
     if constexpr (LPR < 64)
 #pragma unroll
@@ -393,19 +407,24 @@ __global__ __launch_bounds__(1024) void k_norm_backward_wide(const NormArgs a) {
     }
 }
 
-// Sums over every gridDim.y-th row, a thread a column.
+// Sums over every gridDim.y-th row, a thread four columns.
 template <typename T>
 __global__ __launch_bounds__(256) void k_norm_backward_wide_rows(const NormArgs a) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
     if (c >= a.width) return;
-    float dw = 0.f, db = 0.f;
+    Some<float, 4> dw = 0.f, db = 0.f;
     for (long long r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const float g = (float)((const T*)a.dy)[r * a.dy_stride + c];
-        dw = fmaf(g, ((float)((const T*)a.x)[r * a.x_stride + c] - a.stats_in[2 * r]) * a.stats_in[2 * r + 1], dw);
-        db += g;
+        const Some<T, 4> dy = load_some<T, 4>((const T*)a.dy + r * a.dy_stride, c, a.width);
+        const Some<T, 4> x = load_some<T, 4>((const T*)a.x + r * a.x_stride, c, a.width);
+        const float mean = a.stats_in[2 * r], rstd = a.stats_in[2 * r + 1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            dw[e] = fmaf((float)dy[e], ((float)x[e] - mean) * rstd, dw[e]);
+            db[e] += (float)dy[e];
+        }
     }
-    a.partial[(long long)blockIdx.y * 2 * a.width + c] = dw;
-    a.partial[((long long)blockIdx.y * 2 + 1) * a.width + c] = db;
+    store_some<float, 4>(a.partial + (long long)blockIdx.y * 2 * a.width, c, a.width, dw);
+    store_some<float, 4>(a.partial + ((long long)blockIdx.y * 2 + 1) * a.width, c, a.width, db);
 }
 
 template <typename W>
@@ -422,14 +441,14 @@ int forward_with(const NormArgs& a, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-template <typename T, typename W, int LPR, int NV, int NT>
+template <typename T, typename W, int LPR, int NV, int NT, bool SUMS = true>
 int backward_with(const NormArgs& a, hipStream_t s) {
     constexpr int R = NT / LPR;
     // one block a CU: every block costs a row of sums to write and to add
     const long long blocks = std::min((a.rows + R - 1) / R, (long long)a.cus);
     constexpr size_t lds = sizeof(float) * kSums<T, LPR, NV, NT>;
-    hipLaunchKernelGGL((k_norm_backward<T, W, LPR, NV, NT>), dim3((unsigned)blocks), dim3(NT), lds, s, a);
-    if (blocks > 1 && (a.dweight || a.dbias)) launch_sum<W>(a, (int)blocks, s);
+    hipLaunchKernelGGL((k_norm_backward<T, W, LPR, NV, NT, SUMS>), dim3((unsigned)blocks), dim3(NT), lds, s, a);
+    if (SUMS && blocks > 1 && (a.dweight || a.dbias)) launch_sum<W>(a, (int)blocks, s);
     return (int)hipGetLastError();
 }
 
@@ -442,10 +461,10 @@ int forward_as(const NormArgs& a, hipStream_t s) {
     if (n <= 16) return forward_with<T, W, 16, 1, 256>(a, s);
     if (n <= 32) return forward_with<T, W, 32, 1, 256>(a, s);
     if (n <= 64) return forward_with<T, W, 64, 1, 256>(a, s);
-    if (n <= 128) return forward_with<T, W, 64, 2, 256>(a, s);
-    if (n <= 256) return forward_with<T, W, 64, 4, 256>(a, s);
-    if (n <= 512) return forward_with<T, W, 128, 4, 256>(a, s);
-    if (n <= 1024) return forward_with<T, W, 256, 4, 256>(a, s);
+    if (n <= 128) return forward_with<T, W, 128, 1, 256>(a, s);
+    if (n <= 256) return forward_with<T, W, 256, 1, 256>(a, s);
+    if (n <= 512) return forward_with<T, W, 512, 1, 512>(a, s);
+    if (n <= 1024) return forward_with<T, W, 512, 2, 512>(a, s);
     if (n <= 2048) return forward_with<T, W, 512, 4, 512>(a, s);
     if (n <= 4096) return forward_with<T, W, 1024, 4, 1024>(a, s);
     hipLaunchKernelGGL((k_norm_forward_wide<T, W>), dim3((unsigned)std::min(a.rows, (long long)a.cus * 2)), dim3(1024), 0, s, a);
@@ -464,19 +483,22 @@ int backward_as(const NormArgs& a, hipStream_t s) {
     if (n <= 32) return backward_with<T, W, 32, 1, 1024>(a, s);
     if (n <= 64) return backward_with<T, W, 64, 1, 1024>(a, s);
     if (n <= 128) return backward_with<T, W, 64, 2, 512>(a, s);
-    if (n <= 256) return backward_with<T, W, 64, 4, 512>(a, s);
-    if (n <= 512) return backward_with<T, W, 128, 4, 512>(a, s);
+    if (n <= 256) return backward_with<T, W, 256, 1, 1024>(a, s);
+    if (n <= 512) return backward_with<T, W, 512, 1, 1024>(a, s);
     if (n <= 1024) return backward_with<T, W, 256, 4, 512>(a, s);
     if (n <= 2048) return backward_with<T, W, 512, 4, 512>(a, s);
-    if (n <= 4096) return backward_with<T, W, 1024, 4, 1024>(a, s);
+    if constexpr (sizeof(T) == 4)
+        if (n <= 4096) return backward_with<T, W, 1024, 4, 1024>(a, s);
     // dx may overwrite dy: the sums over the rows go first
     if (a.dweight || a.dbias) {
         const int parts = (int)std::min(a.rows, 64ll);
-        hipLaunchKernelGGL((k_norm_backward_wide_rows<T>), dim3((unsigned)((a.width + 255) / 256), parts), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_norm_backward_wide_rows<T>), dim3((unsigned)((a.width + 1023) / 1024), parts), dim3(256), 0, s, a);
         launch_sum<W>(a, parts, s);
     }
-    if (a.y)
-        hipLaunchKernelGGL((k_norm_backward_wide<T, W>), dim3((unsigned)std::min(a.rows, (long long)a.cus * 2)), dim3(1024), 0, s, a);
+    if (!a.y) return (int)hipGetLastError();
+    if constexpr (sizeof(T) < 4)
+        if (n <= 4096) return backward_with<T, W, 1024, 4, 1024, false>(a, s);
+    hipLaunchKernelGGL((k_norm_backward_wide<T, W>), dim3((unsigned)std::min(a.rows, (long long)a.cus * 2)), dim3(1024), 0, s, a);
     return (int)hipGetLastError();
 }
 
