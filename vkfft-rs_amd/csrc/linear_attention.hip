@@ -77,10 +77,10 @@ __global__ __launch_bounds__(256) void k_group_sum(const GroupSum a, const Group
     }
 }
 
-const ChunkKernel* chunk_kernel(int element, int dk, int dv) {
-    return element == VKFX_ELEMENT_F32   ? chunk_kernel_f32(dk, dv)
-           : element == VKFX_ELEMENT_F16 ? chunk_kernel_f16(dk, dv)
-                                         : chunk_kernel_bf16(dk, dv);
+const ChunkKernel* chunk_kernel(int element, int dk, int dv, bool gradient) {
+    return element == VKFX_ELEMENT_F32   ? chunk_kernel_f32(dk, dv, gradient)
+           : element == VKFX_ELEMENT_F16 ? chunk_kernel_f16(dk, dv, gradient)
+                                         : chunk_kernel_bf16(dk, dv, gradient);
 }
 
 // Blocks of a kernel that the GPU holds at a time: two waves on each SIMD, as
@@ -89,7 +89,9 @@ long long resident(const ChunkKernel* k, size_t lds, int cus) {
     return (long long)cus * std::max(1, std::min(8 / (k->threads / 64), (int)(160 * 1024 / lds)));
 }
 
-// Most states that a call keeps between segments.
+// Most states that a call keeps between segments: with a block for each there
+// are four a CU, twice what is resident (16 heads of 64 over 65536 tokens, 64
+// segments: 162 us; 264 with 32).
 constexpr long long kStates = 1024;
 
 int launch_with(const void* fn, long long blocks, int threads, size_t lds, const ChunkArgs& a, hipStream_t s) {
@@ -113,9 +115,11 @@ struct Part {
 // share of the state, at about 0.4 of the cost. The time of k segments is that
 // of the rounds of resident blocks, each 1/k of the tokens long at 3 us a chunk,
 // and of the states' bytes, written, joined and read at 4 TB/s. (bf16, 4 x 4096
-// tokens, 16 heads of 128, backward, 192 blocks: 298 us with the 5 segments that
-// this gives, two rounds; 341 with 2, 328 with 8.) A segment has two chunks or
-// more.
+// tokens, 16 heads of 128, backward, 192 blocks: 303 us with the 5 segments that
+// this gives, two rounds; 390 with 1, 343 with 2, 328 with 8. 8 x 2048 forward:
+// 124 with its 4, 197 with 1, 150 with 2, 155 with 8. 32 x 1024, whole: 151, 208
+// with 2.) A segment has two chunks or more (f32, 3 x 1001 tokens, 12 heads of
+// 80 x 96: 44 us, 49 with four or more).
 long long split_tokens(const Part* parts, int count, long long states, int size, long long tokens, int cus) {
     const long long most = std::max(1ll, std::min(tokens / (2 * kChunk), kStates / states));
     const double whole = 3.0 * (double)std::max(1ll, tokens / kChunk), state = 16.0 * (double)states * size / 4e6 / whole;
@@ -144,7 +148,7 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
         while (p < n && (scans[parts[p].members[0]].dk != scans[i].dk || scans[parts[p].members[0]].dv != scans[i].dv)) ++p;
         if (p == n) {
             ++n;
-            parts[p].k = chunk_kernel(element, scans[i].dk, scans[i].dv);
+            parts[p].k = chunk_kernel(element, scans[i].dk, scans[i].dv, count > 1);
             parts[p].a.slices = (scans[i].dv + parts[p].k->cols - 1) / parts[p].k->cols;
             parts[p].a.powers = powers;
         }
@@ -189,7 +193,9 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
         if (!a.scans) continue;
         if (int e = launch_with(parts[p].k->state_only, parts[p].state * segments, parts[p].k->threads, parts[p].k->state_lds, a, st))
             return e;
-        // few segments come with many states, many segments with few
+        // Few segments come with many states and are joined four elements a thread, many segments with few states one
+        // element a thread (bf16 prompts: 8 x 2048 tokens of 16 heads of 128, 4 segments, 124 us, 133 the other way;
+        // 1 x 16384 of 4 heads of 64, 64 segments, 52 and 72; 16 segments the same either way)
         if (segments > 2)
             if (int e = segments <= 8 ? launch_join<4, 4>(a, st) : launch_join<1, 16>(a, st)) return e;
     }
@@ -206,7 +212,9 @@ size_t scan_work_floats(int dk, int dv, int heads, int states, long long max_bat
 }
 
 int launch_scans(int element, const ScanArgs* scans, int count, const float* powers, float* work, int cus, hipStream_t s) {
-    // the recurrence itself while a chunk would be mostly empty
+    // The recurrence itself while a chunk would be mostly empty: for one sequence of 16 heads of 128 x 128 a step of 8
+    // tokens takes 10.4 us and a chunk 12.6, of 2 tokens 4.7 and 12.6; 8 sequences 15.4 and 15.1 at 8 tokens, 10.2 and
+    // 15.1 at 4. Only large batches turn sooner (64 sequences: 52 and 43 at 8, 35 and 41 at 4).
     if (scans[0].tokens <= kStepTokens) return launch_steps(element, scans, count, powers, cus, s);
     return launch_chunks(element, scans, count, powers, work, cus, s);
 }

@@ -3,6 +3,6 @@
 
 namespace vkfx {
 
-const ChunkKernel* chunk_kernel_bf16(int dk, int dv) { return pick_chunk_kernel<__bf16>(dk, dv); }
+const ChunkKernel* chunk_kernel_bf16(int dk, int dv, bool gradient) { return pick_chunk_kernel<__bf16>(dk, dv, gradient); }
 
 }  // namespace vkfx

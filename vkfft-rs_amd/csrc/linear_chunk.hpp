@@ -343,7 +343,7 @@ template <typename T, int DK, int WAVES, int NT, int C, bool STATE_ONLY>
 struct ChunkShape {
     static constexpr int kIn = Parts<T>::in, kMid = Parts<T>::mid;
     static constexpr int kThreads = 64 * WAVES, kCols = 16 * NT * WAVES;
-        // 16 bytes more a row: a quarter wave's 8-byte reads down the rows meet different banks
+    // 16 bytes more a row: a quarter wave's 8-byte reads down the rows meet different banks
     static constexpr int kPitchK = DK + 8, kPitchV = kCols + 8, kPitchP = C + 8;
     // A, B and C, twice where a CU's LDS then still holds a second block or there is none anyway: the next chunk is
     // written while other waves read this one
@@ -733,10 +733,10 @@ struct ChunkKernel {
     const void* run;
     const void* state_only;
 };
-// The element's kernel for a scan of dk x dv.
-const ChunkKernel* chunk_kernel_f32(int dk, int dv);
-const ChunkKernel* chunk_kernel_f16(int dk, int dv);
-const ChunkKernel* chunk_kernel_bf16(int dk, int dv);
+// The element's kernel for a scan of dk x dv, on its own or of a gradient's three.
+const ChunkKernel* chunk_kernel_f32(int dk, int dv, bool gradient);
+const ChunkKernel* chunk_kernel_f16(int dk, int dv, bool gradient);
+const ChunkKernel* chunk_kernel_bf16(int dk, int dv, bool gradient);
 
 template <typename T, int DK, int WAVES, int NT, int C>
 ChunkKernel chunk_kernel_of() {
@@ -749,20 +749,38 @@ ChunkKernel chunk_kernel_of() {
                        (const void*)k_chunk<T, DK, WAVES, NT, C, true>};
 }
 
-// Key widths are padded to one of six. A block has 64 columns, or 128 where
-// there are more values than 64; a wave 32 of them while the state's rows leave
-// it the registers: what it reads of A, B and P then serves two products.
+// Key widths are padded to one of six. Up to 64 values a block has their 64
+// columns, above that 128, so that what it reads of A and B serves more of them
+// (bf16, 8 x 2048 tokens, 16 heads of 128 x 128: 127 us, with 64 columns 141;
+// 64 x 128: 91 and 97), except where keys are wider than 128 and the CU holds
+// two blocks of 64 columns but one of 128 (8 heads of 256 x 256, bf16 201 us and
+// 213; where the LDS has no room for the second, f16 gradients 600 and 462).
+//
+// A wave has 32 columns where that leaves enough waves: what it reads of A, B
+// and P then serves two products (bf16, 64 x 128: 95 us, with 16 columns 112;
+// 96 x 96: 105 and 128). Not where it leaves two waves a block and these have
+// much to do between them: operands of two or three parts, 96 keys or the scans
+// of a gradient (16 heads of 64 x 64, with 16 columns and with 32: f16 86 us and
+// 119, f32 109 and 188, bf16 gradients 133 and 153; 96 x 64 bf16 79 and 114), nor
+// where a state of more than 96 rows, for f32 128, takes the registers. Two parts
+// and 32 keys run as fast either way (73 and 76); bf16 forward is slower with 16
+// columns where the sequence is long (1 x 65536, 64 x 64: 182 and 170).
 template <typename T>
-const ChunkKernel* pick_chunk_kernel(int dk, int dv) {
+const ChunkKernel* pick_chunk_kernel(int dk, int dv, bool gradient) {
     constexpr int C = kChunk;
-    constexpr bool f32 = Parts<T>::in == 3;  // a third part of everything
+    constexpr int parts = Parts<T>::in;
+    constexpr int wide192 = 2 * ChunkShape<T, 192, 4, 1, C, false>::kLds <= ChunkShape<T, 192, 4, 1, C, false>::kCu ? 4 : 8;
+    constexpr int wide256 = 2 * ChunkShape<T, 256, 4, 1, C, false>::kLds <= ChunkShape<T, 256, 4, 1, C, false>::kCu ? 4 : 8;
+    constexpr int few32 = parts == 3 ? 4 : 2, few64 = parts > 1 ? 4 : 2, many128 = parts == 3 ? 8 : 4;
     static const ChunkKernel kernels[6][2] = {
-        {chunk_kernel_of<T, 32, 2, 2, C>(), chunk_kernel_of<T, 32, 4, 2, C>()},
-        {chunk_kernel_of<T, 64, 2, 2, C>(), chunk_kernel_of<T, 64, 4, 2, C>()},
-        {chunk_kernel_of<T, 96, f32 ? 4 : 2, f32 ? 1 : 2, C>(), chunk_kernel_of<T, 96, 4, 2, C>()},
-        {chunk_kernel_of<T, 128, 4, 1, C>(), chunk_kernel_of<T, 128, f32 ? 8 : 4, f32 ? 1 : 2, C>()},
-        {chunk_kernel_of<T, 192, 4, 1, C>(), chunk_kernel_of<T, 192, 8, 1, C>()},
-        {chunk_kernel_of<T, 256, 4, 1, C>(), chunk_kernel_of<T, 256, 8, 1, C>()}};
+        {chunk_kernel_of<T, 32, few32, 4 / few32, C>(), chunk_kernel_of<T, 32, 4, 2, C>()},
+        {chunk_kernel_of<T, 64, few64, 4 / few64, C>(), chunk_kernel_of<T, 64, 4, 2, C>()},
+        {chunk_kernel_of<T, 96, 4, 1, C>(), chunk_kernel_of<T, 96, 4, 2, C>()},
+        {chunk_kernel_of<T, 128, 4, 1, C>(), chunk_kernel_of<T, 128, many128, 8 / many128, C>()},
+        {chunk_kernel_of<T, 192, 4, 1, C>(), chunk_kernel_of<T, 192, wide192, 1, C>()},
+        {chunk_kernel_of<T, 256, 4, 1, C>(), chunk_kernel_of<T, 256, wide256, 1, C>()}};
+    static const ChunkKernel gradient64 = chunk_kernel_of<T, 64, 4, 1, C>();
+    if (gradient && dk > 32 && dk <= 64 && dv <= 64) return &gradient64;
     return &kernels[dk <= 32 ? 0 : dk <= 64 ? 1 : dk <= 96 ? 2 : dk <= 128 ? 3 : dk <= 192 ? 4 : 5][dv > 64];
 }
 

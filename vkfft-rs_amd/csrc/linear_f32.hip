@@ -3,6 +3,6 @@
 
 namespace vkfx {
 
-const ChunkKernel* chunk_kernel_f32(int dk, int dv) { return pick_chunk_kernel<float>(dk, dv); }
+const ChunkKernel* chunk_kernel_f32(int dk, int dv, bool gradient) { return pick_chunk_kernel<float>(dk, dv, gradient); }
 
 }  // namespace vkfx

@@ -124,12 +124,15 @@ void launch_as(const ScanArgs& a, const float* powers, hipStream_t s) {
     else hipLaunchKernelGGL((k_step<T, CS, NR, false>), grid, dim3(256), 0, s, a, powers);
 }
 
-// 64 columns a block, a fourth of that while those blocks are fewer than the
-// GPU's CUs: a small batch's latency is a block's share of the state.
+// 64 columns a block; a fourth of that while those blocks would use less than an
+// eighth of the CUs, where latency is a block's share of the state (4 heads of
+// 256 x 256, 16 blocks of 64: 5.0 us, 4.2 with 16 columns; 32 blocks: 5.1 and 5.2;
+// 16 heads of 128 x 128, 2 sequences, 64 blocks: 4.2 and 5.0, 32 sequences: 13.4
+// and 23.6).
 template <typename T>
 void launch_element(const ScanArgs& a, const float* powers, int cus, hipStream_t s) {
     const long long blocks = (long long)a.batch * a.heads * ((a.dv + 63) / 64);
-    if (blocks >= cus) {
+    if (blocks >= cus / 8) {
         if (a.dk <= 64) launch_as<T, 64, 4>(a, powers, s);
         else if (a.dk <= 128) launch_as<T, 64, 8>(a, powers, s);
         else launch_as<T, 64, 16>(a, powers, s);
