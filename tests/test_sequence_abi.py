@@ -50,3 +50,17 @@ def test_defaults():
     assert d.kv_heads == 3 and d.scale == 0.125 and [d.decay[i] for i in range(3)] == [1.0] * 3 and not d.gradient
     n = vk.LayerNormConfig.new(8).with_element(vk.Element.BF16).desc()
     assert n.element == n.weight_element == 2
+
+
+@pytest.mark.parametrize("cls", [vk.LayerNormPlan, vk.LinearAttentionPlan])
+@pytest.mark.parametrize("device", [-1, 0, 2])
+def test_tensors_of_another_device_are_refused(cls, device):
+    class Tensor:
+        def get_device(self):
+            return device
+
+    plan = cls.__new__(cls)  # a plan of device 1: its place alone, no GPU
+    plan.handle, plan._device = None, 1
+    with pytest.raises(vk.VkFftError) as e:
+        plan._place(Tensor())
+    assert e.value.kind == "InvalidArgument"

@@ -1417,6 +1417,7 @@ class _SequencePlan:
         self.ctx = ctx
         self._L = ctx._L
         self.config = config
+        self._device = ctx.device_index
         self.handle = ctypes.c_void_p()
         _check(getattr(self._L, f"vkfx_{self._kind}_create")(ctx.handle, ctypes.byref(desc), ctypes.byref(self.handle)),
                self._L)
@@ -1441,12 +1442,12 @@ class _SequencePlan:
     # A call costs a few microseconds on the GPU, so the checks below take the
     # cheapest of what a tensor tells: get_device() is -1 on the host.
 
-    @staticmethod
-    def _place(x) -> int:
-        """The device of a call's tensors."""
+    def _place(self, x) -> int:
+        """The device of a call's tensors: the context's."""
         device = x.get_device()
-        if device < 0:
-            raise VkFftError(-7, "tensors must be device tensors")
+        if device != self._device:
+            raise VkFftError(-7, f"tensors must be on the context's device {self._device}" if device >= 0
+                             else "tensors must be device tensors")
         return device
 
     @staticmethod
@@ -1660,6 +1661,7 @@ class HipExecutionContext:
         self._L = lib(library)
         self.handle = ctypes.c_void_p()
         _check(self._L.vkfx_context_create(device_index, ctypes.byref(self.handle)), self._L)
+        self.device_index = int(device_index)
         self._plans = {}
         self._live_plans = weakref.WeakSet()  # every Plan built on this context
         self._live_tickets = weakref.WeakSet()  # every TransformTicket submitted on it
