@@ -118,6 +118,12 @@ def test_shared_heads(hip_ctx, element, h, kv):
 
 
 @pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("dk,dv", [(1, 3), (5, 6), (30, 129), (254, 255)])
+def test_shared_heads_of_any_width(hip_ctx, element, dk, dv):
+    _run(hip_ctx, element, 2, 37, 6, 2, dk, dv, pad=3, offset=1)
+
+
+@pytest.mark.parametrize("element", ELEMENTS)
 @pytest.mark.parametrize("t,lengths", [(5, [0, 1, 5, 3]), (1, [0, 1, 1, 0]), (130, [130, 0, 64, 65]), (200, [1, 63, 199, 200]),
                                        (70, [-3, 71, 2 ** 31 - 1, 7])])
 def test_uneven_lengths(hip_ctx, element, t, lengths):
