@@ -119,7 +119,7 @@ long long resident(const ChunkKernel* k, size_t lds, int cus) {
 
 // Most states that a call keeps between segments: with a block for each there
 // are four a CU, twice what is resident (16 heads of 64 over 65536 tokens, 64
-// segments: 162 us; 264 with 32).
+// segments: 166 us; 267 with 32).
 constexpr long long kStates = 1024;
 
 int launch_with(const void* fn, long long blocks, int threads, size_t lds, const ChunkArgs& a, hipStream_t s) {
@@ -143,11 +143,11 @@ struct Part {
 // share of the state, at about 0.4 of the cost. The time of k segments is that
 // of the rounds of resident blocks, each 1/k of the tokens long at 3 us a chunk,
 // and of the states' bytes, written, joined and read at 4 TB/s. (bf16, 4 x 4096
-// tokens, 16 heads of 128, backward, 192 blocks: 303 us with the 5 segments that
-// this gives, two rounds; 390 with 1, 343 with 2, 328 with 8. 8 x 2048 forward:
-// 124 with its 4, 197 with 1, 150 with 2, 155 with 8. 32 x 1024, whole: 151, 208
+// tokens, 16 heads of 128, backward, 192 blocks: 308 us with the 5 segments that
+// this gives, two rounds; 397 with 1, 358 with 2, 335 with 8. 8 x 2048 forward:
+// 124 with its 4, 205 with 1, 156 with 2, 164 with 8. 32 x 1024, whole: 165, 232
 // with 2.) A segment has two chunks or more (f32, 3 x 1001 tokens, 12 heads of
-// 80 x 96: 44 us, 49 with four or more).
+// 80 x 96: 54 us, 63 with three or more).
 long long split_tokens(const Part* parts, int count, long long states, int size, long long tokens, int cus) {
     const long long most = std::max(1ll, std::min(tokens / (2 * kChunk), kStates / states));
     const double whole = 3.0 * (double)std::max(1ll, tokens / kChunk), state = 16.0 * (double)states * size / 4e6 / whole;
