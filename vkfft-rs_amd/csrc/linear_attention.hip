@@ -147,7 +147,7 @@ struct Part {
 // this gives, two rounds; 397 with 1, 358 with 2, 335 with 8. 8 x 2048 forward:
 // 124 with its 4, 205 with 1, 156 with 2, 164 with 8. 32 x 1024, whole: 165, 232
 // with 2.) A segment has two chunks or more (f32, 3 x 1001 tokens, 12 heads of
-// 80 x 96: 54 us, 63 with three or more).
+// 80 x 96: 54 us with the three that this gives, 63 with four).
 long long split_tokens(const Part* parts, int count, long long states, int size, long long tokens, int cus) {
     const long long most = std::max(1ll, std::min(tokens / (2 * kChunk), kStates / states));
     const double whole = 3.0 * (double)std::max(1ll, tokens / kChunk), state = 16.0 * (double)states * size / 4e6 / whole;
