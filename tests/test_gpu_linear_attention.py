@@ -474,3 +474,21 @@ def test_bad_values_do_not_reach_the_tokens_before(hip_ctx, element, dk, dv):
             assert not torch.isfinite(out[:, at, 0]).all()
         if not backward:
             assert torch.equal(dv_ if i == 2 else dk_, want[3 if i == 2 else 2])  # dv does not depend on v, dk not on k
+
+
+def test_more_blocks_than_32_bits_count_threads(hip_ctx):
+    """65535 heads of 300 sequences: more than 2^32 threads, one block a state."""
+    import torch
+    b, t, h = 300, 9, 65535
+    plan = _plan(hip_ctx, b, t, h, 1, 1, 1, "f32", decay=[0.5] * h, scale=1.0)
+    q, k, v = (_tensor(i, (b, t, 1, 1), "f32") for i in (1, 2, 3))
+    out = torch.full((b, t, h, 1), float("nan"), device="cuda")
+    state = torch.full((b, h, 1, 1), float("nan"), device="cuda")
+    plan.forward_tensors(q.expand(b, t, h, 1), k, v, out, state_out=state)
+    assert torch.equal(out, out[:, :, :1].expand_as(out)) and torch.equal(state, state[:, :1].expand_as(state))
+    qn, kn, vn = _np(q, k, v)
+    args = ([0.5], 1.0, np.full(b, t))
+    zero = np.zeros((b, 1, 1, 1))
+    want, total = ref.attention(qn, kn, vn, zero, *args), ref.attention(*map(np.abs, (qn, kn, vn, zero)), *args)
+    ref.check("out", out[:, :, :1], want[0], total[0], "f32", ref.TERM["f32"])
+    ref.check("state", state[:, :1], want[1], total[1], "f32", ref.STATE_TERM)

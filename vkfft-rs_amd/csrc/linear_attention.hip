@@ -122,11 +122,16 @@ long long resident(const ChunkKernel* k, size_t lds, int cus) {
 // segments: 166 us; 267 with 32).
 constexpr long long kStates = 1024;
 
-int launch_with(const void* fn, long long blocks, int threads, size_t lds, const ChunkArgs& a, hipStream_t s) {
+// Blocks along x: their threads have to stay under 2^32 (a launch of more starts the remainder only).
+constexpr long long kGridX = 1 << 22;
+
+int launch_with(const void* fn, long long blocks, int threads, size_t lds, ChunkArgs a, hipStream_t s) {
     if (lds > 65536)
         if (int e = raise_lds_limit(fn, lds)) return e;
+    a.blocks = blocks;
     void* kargs[1] = {(void*)&a};
-    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)blocks), dim3((unsigned)threads), kargs, lds, s);
+    const dim3 grid((unsigned)std::min(blocks, kGridX), (unsigned)((blocks + kGridX - 1) / kGridX));
+    const hipError_t e = hipLaunchKernel(fn, grid, dim3((unsigned)threads), kargs, lds, s);
     return e != hipSuccess ? (int)e : (int)hipGetLastError();
 }
 
@@ -213,8 +218,6 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
         // a whole sequence's block reads its state before it writes it: only segments need the copy
         if (scans[i].state_in && scans[i].state_in == scans[i].state_out) a.in_place = 1;
     }
-    for (int p = 0; p < n; ++p)
-        if (parts[p].run * segments > 0x7fffffffll) return (int)hipErrorInvalidConfiguration;
     for (int p = 0; p < n && segments > 1; ++p) {
         ChunkArgs a = parts[p].a;
         a.scans = parts[p].states;

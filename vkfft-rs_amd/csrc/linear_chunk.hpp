@@ -54,6 +54,7 @@ constexpr int kChunk = 32;
 struct ChunkArgs {
     ScanArgs scan[3];
     int scans;
+    long long blocks;  // of the launch: more than 2^32 threads take a second dimension of the grid
     int slices;     // blocks side by side over dv
     int segments;   // parts of the tokens, each `segment` long (a multiple of the chunk)
     long long segment;
@@ -371,7 +372,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
     unsigned* const bad = (unsigned*)(pw + kDecayPowers);  // of this chunk and of the next, in turn
 
     // block -> (scan, sequence, head, segment, slice), slices side by side
-    long long id = blockIdx.x;
+    long long id = blockIdx.x + (long long)blockIdx.y * gridDim.x;
+    if (id >= args.blocks) return;
     const int slice = (int)(id % args.slices);
     id /= args.slices;
     const int seg = (int)(id % args.segments);
