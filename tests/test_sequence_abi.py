@@ -64,3 +64,77 @@ def test_tensors_of_another_device_are_refused(cls, device):
     with pytest.raises(vk.VkFftError) as e:
         plan._place(Tensor())
     assert e.value.kind == "InvalidArgument"
+
+
+class _Tensor:
+    """What the plans ask of a tensor, without a GPU."""
+    def __init__(self, *shape, dtype=None, device=0, address=4096, stride=None):
+        import torch
+        self.shape, self.dtype, self._device, self._address = torch.Size(shape), dtype or torch.float32, device, address
+        self._stride = stride or tuple(int(n) for n in torch.empty(shape, device="meta").stride())
+
+    def get_device(self):
+        return self._device
+
+    def stride(self):
+        return self._stride
+
+    def data_ptr(self):
+        return self._address
+
+    def is_contiguous(self):
+        return True
+
+    def dim(self):
+        return len(self.shape)
+
+    def size(self, i):
+        return self.shape[i]
+
+
+class _Context:
+    """A context whose library takes every call and remembers it."""
+    def __init__(self):
+        import types
+        self.handle, self.device_index, self._live_plans, self.calls = 1, 0, set(), []
+
+        def entry(name):
+            return lambda *a: self.calls.append((name, a)) or 0
+
+        names = [f"vkfx_{k}_{f}" for k in ("layer_norm", "linear_attention")
+                 for f in ("create", "destroy", "workspace_bytes", "forward", "backward")]
+        self._L = types.SimpleNamespace(**{n: entry(n) for n in names})
+
+    def plan(self, config):
+        p = (vk.LayerNormPlan if isinstance(config, vk.LayerNormConfig) else vk.LinearAttentionPlan)(self, config)
+        p._current = lambda device: 0
+        del self.calls[:]
+        return p
+
+
+def test_a_plan_keeps_the_sizes_it_was_made_with():
+    """The caller's configuration may change afterwards; the plan's kernels do not."""
+    ctx = _Context()
+    config = vk.LayerNormConfig.new(16)
+    plan = ctx.plan(config)
+    config.width = 8
+    config.with_element(vk.Element.BF16)
+    w = _Tensor(8)
+    for f in (lambda: plan.forward_tensors(_Tensor(4, 8), w, w, _Tensor(4, 8)),
+              lambda: plan.backward_tensors(_Tensor(4, 8), w, _Tensor(4, 2), _Tensor(4, 8), _Tensor(4, 8), w, w)):
+        with pytest.raises(vk.VkFftError) as e:
+            f()
+        assert e.value.kind == "InputLengthMismatch"
+    assert not ctx.calls
+    w = _Tensor(16)
+    plan.forward_tensors(_Tensor(4, 16), w, w, _Tensor(4, 16))
+    assert ctx.calls
+
+    config = vk.LinearAttentionConfig.new(4, 16, 24).with_kv_heads(2)
+    plan = ctx.plan(config)
+    config.heads, config.kv_heads, config.key_dim, config.value_dim = 2, 1, 8, 12
+    with pytest.raises(vk.VkFftError) as e:
+        plan.forward_tensors(_Tensor(1, 1, 2, 8), _Tensor(1, 1, 1, 8), _Tensor(1, 1, 1, 12), _Tensor(1, 1, 2, 12))
+    assert e.value.kind == "InputLengthMismatch" and not ctx.calls
+    plan.forward_tensors(_Tensor(1, 1, 4, 16), _Tensor(1, 1, 2, 16), _Tensor(1, 1, 2, 24), _Tensor(1, 1, 4, 24))
+    assert ctx.calls

@@ -1495,10 +1495,11 @@ class LayerNormPlan(_SequencePlan):
 
     def __init__(self, ctx: "HipExecutionContext", config: LayerNormConfig):
         super().__init__(ctx, config, config.desc())
+        self._width = config.width  # the caller may change the configuration afterwards
         self._weight_type = _torch_type(config.element if config.weight_element is None else config.weight_element)
 
     def _rows(self, name, x, rows, device):
-        width = self.config.width
+        width = self._width
         if x.shape != (rows, width) or x.dtype is not self._type or x.get_device() != device:
             self._refuse(name, x, (rows, width), self._type, device)
         row, column = x.stride()
@@ -1508,7 +1509,7 @@ class LayerNormPlan(_SequencePlan):
 
     def forward_tensors(self, x, weight, bias, y, stats=None, stream=None):
         """y (may be x) and, if wanted, stats [rows][2]: mean and rstd."""
-        device, w = self._place(x), (self.config.width,)
+        device, w = self._place(x), (self._width,)
         rows = x.shape[0]
         xp, xs = self._rows("x", x, rows, device)
         yp, ys = self._rows("y", y, rows, device)
@@ -1519,7 +1520,7 @@ class LayerNormPlan(_SequencePlan):
 
     def backward_tensors(self, x, weight, stats, dy, dx=None, dweight=None, dbias=None, work=None, stream=None):
         """Gradients for dy; any of the three may be None (not wanted)."""
-        device, w = self._place(x), (self.config.width,)
+        device, w = self._place(x), (self._width,)
         rows = x.shape[0]
         xp, xs = self._rows("x", x, rows, device)
         gp, gs = self._rows("dy", dy, rows, device)
