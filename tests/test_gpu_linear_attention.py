@@ -492,3 +492,37 @@ def test_more_blocks_than_32_bits_count_threads(hip_ctx):
     want, total = ref.attention(qn, kn, vn, zero, *args), ref.attention(*map(np.abs, (qn, kn, vn, zero)), *args)
     ref.check("out", out[:, :, :1], want[0], total[0], "f32", ref.TERM["f32"])
     ref.check("state", state[:, :1], want[1], total[1], "f32", ref.STATE_TERM)
+
+
+@pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("decay", [0.99995, 0.999997])
+def test_slow_decays_over_many_chunks(hip_ctx, element, decay):
+    """With nothing added the states are powers of the decay alone, in the order of the tokens and backwards; enough
+    heads that no sequence is split over its tokens."""
+    import torch
+    t, h, d = 16384, 520, 8
+    plan = _plan(hip_ctx, 1, t, h, 1, d, d, element, True, decay=[decay] * h)
+    one = lambda heads: torch.ones(1, 1, 1, d, device="cuda", dtype=_types()[element]).expand(1, t, heads, d)  # noqa: E731
+    none = lambda heads: torch.zeros(1, 1, 1, d, device="cuda", dtype=_types()[element]).expand(1, t, heads, d)  # noqa: E731
+    state = _state(1, 1, h, d, d).abs_()
+    after = torch.empty_like(state)
+    out = torch.empty(1, t, h, d, device="cuda", dtype=_types()[element])
+    plan.forward_tensors(one(h), one(1), none(1), out, state_in=state, state_out=after)
+    sn, = _np(state)
+    want = decay ** t * sn
+    ref.check("state", after, want, want, "f32", ref.STATE_TERM)
+    for i in (0, 31, 32, t // 2, t - 1):
+        want = np.float64(np.float32(d ** -0.5)) * decay ** (i + 1) * sn[0].sum(1)
+        ref.check(f"out {i}", out[0, i], want, want, element, ref.TERM[element])
+    back = torch.empty_like(state)
+    dq = torch.empty_like(out)
+    dk, dv = torch.empty(1, t, 1, d, device="cuda", dtype=out.dtype), torch.empty(1, t, 1, d, device="cuda", dtype=out.dtype)
+    plan.backward_tensors(none(h), one(1), one(1), none(h), dq, dk, dv, state_in=state, dstate_out=state, dstate_in=back)
+    want = decay ** t * sn
+    ref.check("dstate_in", back, want, want, "f32", ref.STATE_TERM)
+    for i in (0, 1, t // 2, t - 32, t - 1):
+        power = decay ** (t - 1 - i)
+        # dk sums 520 heads of 8 terms in 32 bits
+        for name, got, axes in (("dk", dk, (0, 1, 3)), ("dv", dv, (0, 1, 2))):
+            want = power * sn.sum(axes)
+            ref.check(f"{name} {i}", got[0, i, 0], want, want, element, ref.TERM[element])

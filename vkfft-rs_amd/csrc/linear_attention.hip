@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void k_chunk_join(const ChunkArgs args) {
         at[j] = e + 256 * j < size ? e + 256 * j : size - 1;
         x[j] = slot[at[j]];
     }
-    const float decay = whole_segment(args.powers + (long long)h * kDecayPowers, args.segment);
+    const float decay = (float)decay_of(args.powers + (long long)h * kDecayPowers, args.segment);
     for (int k = 2; k < last; k += AHEAD) {
         float added[AHEAD][EACH];
 #pragma unroll

@@ -38,12 +38,19 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// The decay of a whole segment, by squaring, from a head's table.
-__device__ __forceinline__ float whole_segment(const float* powers, long long segment) {
+// The decay of n tokens, by squaring, from a head's table.
+__device__ __forceinline__ double decay_of(const float* powers, long long n) {
     double power = 1.0, square = (double)powers[1] + (double)powers[kDecayPowers - 1];
-    for (long long i = segment; i; i >>= 1, square *= square)
+    for (long long i = n; i; i >>= 1, square *= square)
         if (i & 1) power *= square;
-    return (float)power;
+    return power;
+}
+
+// A number that is the same in every lane, held in scalar registers.
+__device__ __forceinline__ double same_in_all(double x) {
+    typedef int two __attribute__((ext_vector_type(2)));
+    const two w = __builtin_bit_cast(two, x);
+    return __builtin_bit_cast(double, two{__builtin_amdgcn_readfirstlane(w[0]), __builtin_amdgcn_readfirstlane(w[1])});
 }
 
 // Tokens of a chunk: what one product sums over. With 64 the state is split
@@ -433,7 +440,9 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int a = 0; a < DK / 16; ++a) X[t][a] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float factor = 1.f;  // the state is factor X
+    // The state is factor X. In 64 bits: in 32 the decay of a chunk, rounded once, would round every chunk's state to the
+    // same side (after 512 chunks a state would be off by 1.4e-5 at a decay of 0.999997).
+    double factor = 1.0;
     const int state_size = s.dk * s.dv;
     if constexpr (STATE_ONLY) {
         if (seg == 0 && s.state_in) read_state(s.state_in + head_state, s.state_row, s.state_col);
@@ -510,6 +519,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
             }
     };
     update_weights(C);
+    const double whole = same_in_all(decay_of(pw, C));
 
     // the state is here before the loop begins: a wait for it inside would be one for the chunk that is read ahead
 #pragma unroll
@@ -587,21 +597,21 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int I = 0; I < TI; ++I) o[t][I] *= oweight[I] * factor;
+                for (int I = 0; I < TI; ++I) o[t][I] *= oweight[I] * (float)factor;
             __syncthreads();  // P is written
         }
 
         // the state decays by its factor; X itself only when that gets small, so that what is added to X does not
         // get large
-        factor *= pw[left];
-        if (factor < 0x1p-10f) {
+        factor = same_in_all(factor * (left < C ? (double)pw[left] : whole));
+        if (factor < 0x1p-10) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int a = 0; a < DK / 16; ++a) X[t][a] *= factor;
-            factor = 1.f;
+                for (int a = 0; a < DK / 16; ++a) X[t][a] *= (float)factor;
+            factor = 1.0;
         }
-        const float added = 1.f / factor;
+        const float added = 1.f / (float)factor;
 #pragma unroll
         for (int k = 0; k < C / 32; ++k) {
             bf16x8 cv[NT][IN], cw[NT][3];
@@ -713,7 +723,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int a = 0; a < DK / 16; ++a) X[t][a] *= factor;
+        for (int a = 0; a < DK / 16; ++a) X[t][a] *= (float)factor;
     if constexpr (STATE_ONLY) {
         write_state(slot + state_size, args.slot_row[z], args.slot_col[z]);  // to the next segment's place
         return;
