@@ -526,3 +526,28 @@ def test_slow_decays_over_many_chunks(hip_ctx, element, decay):
         for name, got, axes in (("dk", dk, (0, 1, 3)), ("dv", dv, (0, 1, 2))):
             want = power * sn.sum(axes)
             ref.check(f"{name} {i}", got[0, i, 0], want, want, element, ref.TERM[element])
+
+
+@pytest.mark.parametrize("element", ["f32", "bf16"])
+def test_states_near_the_largest_number(hip_ctx, element):
+    """States of 1e37 and their gradients, which 32 bits hold, over a prompt's chunks."""
+    import torch
+    b, t, h, d = 1, 96, 2, 32
+    plan = _plan(hip_ctx, b, t, h, h, d, d, element, True, decay=[0.9, 0.99], scale=1.0)
+    q, k, v, dout = (_tensor(i, (b, t, h, d), element).abs_() for i in range(4))
+    k, v = (k * 1e18).to(q.dtype), (v * 1e18).to(q.dtype)
+    q, dout = (q * 1e-2).to(q.dtype), (dout * 1e-2).to(q.dtype)
+    out, state = torch.empty_like(v), torch.empty(b, h, d, d, device="cuda")
+    plan.forward_tensors(q, k, v, out, state_out=state)
+    qn, kn, vn, dn = _np(q, k, v, dout)
+    zero = np.zeros((b, h, d, d))
+    args = ([0.9, 0.99], 1.0, np.array([t]))
+    want, want_state = ref.attention(qn, kn, vn, zero, *args)
+    assert 1e36 < np.abs(want_state).max() < 3e38 and want.max() < 3e38
+    ref.check("state", state, want_state, want_state, "f32", ref.STATE_TERM)
+    ref.check("out", out, want, want, element, ref.TERM[element])
+    dq, dk, dv = (torch.empty_like(x) for x in (q, k, v))
+    plan.backward_tensors(q, k, v, dout, dq, dk, dv)
+    wants = ref.attention_gradients(qn, kn, vn, zero, dn, zero, *args)
+    for name, got, w in zip(("dq", "dk", "dv"), (dq, dk, dv), wants):
+        ref.check(name, got, w, w, element, ref.TERM[element])

@@ -541,6 +541,16 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
         turn ^= 1;
         if (!STATE_ONLY && tid == 0) bad[turn] = 0;  // nobody marks the next chunk before P's barrier
 
+        // The state decays by its factor, which runs from 2^7 down to 1: X is never larger than the state, which may come
+        // near the largest number, and at most 2^7 times smaller, where the parts of small numbers vanish. X itself decays
+        // in every second chunk at most, or in each one where a chunk leaves so little that this saves nothing.
+        const float before = (float)factor;
+        factor = same_in_all(factor * (left < C ? (double)pw[left] : whole));
+        const bool fast = whole < 0x1p-7, decays = factor < 1.0;
+        const float shrink = (float)factor * (fast ? 1.f : 0x1p-7f);
+        if (decays) factor = fast ? 1.0 : 0x1p7;
+        const float added = 1.f / (float)factor;
+
         f32x4 o[NT][TI];
         if constexpr (!STATE_ONLY) {
             // P, transposed: rows j, columns i
@@ -597,21 +607,16 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int I = 0; I < TI; ++I) o[t][I] *= oweight[I] * (float)factor;
+                for (int I = 0; I < TI; ++I) o[t][I] *= oweight[I] * before;
             __syncthreads();  // P is written
         }
 
-        // the state decays by its factor; X itself only when that gets small, so that what is added to X does not
-        // get large
-        factor = same_in_all(factor * (left < C ? (double)pw[left] : whole));
-        if (factor < 0x1p-10) {
+        if (decays) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int a = 0; a < DK / 16; ++a) X[t][a] *= (float)factor;
-            factor = 1.0;
+                for (int a = 0; a < DK / 16; ++a) X[t][a] *= shrink;
         }
-        const float added = 1.f / (float)factor;
 #pragma unroll
         for (int k = 0; k < C / 32; ++k) {
             bf16x8 cv[NT][IN], cw[NT][3];
