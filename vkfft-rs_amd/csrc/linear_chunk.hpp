@@ -607,7 +607,12 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int I = 0; I < TI; ++I) o[t][I] *= oweight[I] * before;
+                for (int I = 0; I < TI; ++I) {
+                    o[t][I] *= oweight[I] * before;
+                    // Here, and not after the branch below: the compiler counts the wait for a matrix product's result
+                    // along one way to a place that two lead to, which may be the longer one.
+                    asm volatile("" : "+v"(o[t][I]));
+                }
             __syncthreads();  // P is written
         }
 
