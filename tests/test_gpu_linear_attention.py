@@ -551,3 +551,39 @@ def test_states_near_the_largest_number(hip_ctx, element):
     wants = ref.attention_gradients(qn, kn, vn, zero, dn, zero, *args)
     for name, got, w in zip(("dq", "dk", "dv"), (dq, dk, dv), wants):
         ref.check(name, got, w, w, element, ref.TERM[element])
+
+
+@pytest.mark.parametrize("dk", [5, 33, 64, 100, 128, 200])
+@pytest.mark.parametrize("batch", [1, 40])
+def test_an_infinite_state_row_gives_infinite_outputs_of_a_token(hip_ctx, dk, batch):
+    """The state's last row, which the rows that pad a block must not meet with zeros."""
+    import torch
+    h, dv = 4, 24
+    q, k, v = (_tensor(i, (batch, 1, h, d), "f32").abs_() + 0.1 for i, d in ((1, dk), (2, dk), (3, dv)))
+    state = _state(4, batch, h, dk, dv)
+    state[:, :, dk - 1, 3] = float("inf")
+    state[:, 3, dk - 1, 5] = float("-inf")
+    plan = _plan(hip_ctx, batch, 1, h, h, dk, dv, "f32", decay=[0.5, 0.9375, 0.998, 1.0])
+    out = torch.empty(batch, 1, h, dv, device="cuda")
+    plan.forward_tensors(q, k, v, out, state_in=state, state_out=state)
+    assert torch.isposinf(out[:, 0, :, 3]).all() and torch.isneginf(out[:, 0, 3, 5]).all()
+    out[:, :, :, 3] = 0
+    out[:, :, 3, 5] = 0
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dk", [5, 33, 64, 100, 200])
+@pytest.mark.parametrize("batch", [1, 40])
+def test_an_infinite_value_of_a_token_gives_an_infinite_output(hip_ctx, dk, batch):
+    """The same for the token itself: an infinity in v enters every row of the state's column, and no other column."""
+    import torch
+    h, dv = 4, 24
+    q, k, v = (_tensor(i, (batch, 3, h, d), "f32").abs_() + 0.1 for i, d in ((1, dk), (2, dk), (3, dv)))
+    v[:, 1, :, 3] = float("inf")
+    plan = _plan(hip_ctx, batch, 3, h, h, dk, dv, "f32", decay=[0.5, 0.9375, 0.998, 1.0])
+    out, state = torch.empty(batch, 3, h, dv, device="cuda"), torch.empty(batch, h, dk, dv, device="cuda")
+    plan.forward_tensors(q, k, v, out, state_out=state)
+    assert torch.isposinf(out[:, 1:, :, 3]).all() and torch.isposinf(state[:, :, :, 3]).all()
+    out[:, 1:, :, 3] = 0
+    state[:, :, :, 3] = 0
+    assert torch.isfinite(out).all() and torch.isfinite(state).all()

@@ -40,7 +40,7 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 // The decay of n tokens, by squaring, from a head's table.
 __device__ __forceinline__ double decay_of(const float* powers, long long n) {
-    double power = 1.0, square = (double)powers[1] + (double)powers[kDecayPowers - 1];
+    double power = 1.0, square = (double)powers[kDecayHigh] + (double)powers[kDecayLow];
     for (long long i = n; i; i >>= 1, square *= square)
         if (i & 1) power *= square;
     return power;

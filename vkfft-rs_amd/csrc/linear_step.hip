@@ -10,6 +10,8 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "sequence.hpp"
 #include "vkfx.h"
 
@@ -22,9 +24,10 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // CS columns a block, up to NR rows a thread. PACKED: a state's columns are
 // neighbours in memory (they are not where a gradient reads its transpose).
-template <typename T, int CS, int NR, bool PACKED>
+// WHOLE: each thread has its NR rows.
+template <typename T, int CS, int NR, bool PACKED, bool WHOLE>
 __global__ __launch_bounds__(256) void k_step(const ScanArgs s, const float* __restrict__ powers) {
-    constexpr int LX = CS / 4, RY = 256 / LX, RW = 64 / LX;  // lanes along a row, rows of the block and of a wave
+    constexpr int LX = CS / 4, RY = 256 / LX;  // lanes along a row, rows of the block
     __shared__ float la[kStepTokens][256], lb[kStepTokens][256], lc[kStepTokens][CS];
     __shared__ float part[kStepTokens][4][CS];
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
@@ -34,8 +37,8 @@ __global__ __launch_bounds__(256) void k_step(const ScanArgs s, const float* __r
     if (s.lengths) n = s.lengths[b] < 0 ? 0 : s.lengths[b] < n ? s.lengths[b] : n;
     const long long st = ((long long)b * s.heads + h) * s.dk * s.dv;
 
-    // Rows past the last read the last one again and never change an output:
-    // every load is on its way before the first is waited for.
+    // Rows past the last read the last one again, for nothing: every load is on
+    // its way before the first is waited for. Then they are zeros.
     f32x4 X[NR];
     const bool four = PACKED && col + 4 <= s.dv;
     if (!s.state_in) {
@@ -66,13 +69,16 @@ __global__ __launch_bounds__(256) void k_step(const ScanArgs s, const float* __r
         lb[i][tid] = tid < s.dk ? (float)B[t * s.b.token + tid] : 0.f;
         if (tid < CS) lc[i][tid] = col0 + tid < s.dv ? (float)C[t * s.c.token + col0 + tid] * s.scale_update : 0.f;
     }
+    if constexpr (!WHOLE)
+#pragma unroll
+        for (int k = 0; k < NR; ++k)
+            if (row0 + k * RY >= s.dk) X[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     // the decay in two parts, so that its rounding does not grow token by token
-    const float decay = powers[(long long)h * kDecayPowers + 1];
-    const float decay_low = powers[(long long)h * kDecayPowers + kDecayPowers - 1];
+    const float decay = powers[(long long)h * kDecayPowers + kDecayHigh];
+    const float decay_low = powers[(long long)h * kDecayPowers + kDecayLow];
     __syncthreads();
-    for (int i = 0; i < n; ++i) {
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        const f32x4 c = *(const f32x4*)&lc[i][x0];
+    // MASKED: rows past the last are left out; otherwise they meet zeros, which a value that is infinite would not survive.
+    const auto advance = [&](int i, f32x4 c, f32x4& o, auto masked) {
 #pragma unroll
         for (int k = 0; k < NR; ++k) {
             const int r = row0 + k * RY;
@@ -82,11 +88,17 @@ __global__ __launch_bounds__(256) void k_step(const ScanArgs s, const float* __r
                 float x = X[k][e];
                 if (!s.reverse) x = fmaf(x, decay, x * decay_low);
                 x = fmaf(bv, c[e], x);
-                o[e] = fmaf(av, x, o[e]);
+                o[e] = !decltype(masked)::value || r < s.dk ? fmaf(av, x, o[e]) : o[e];
                 if (s.reverse) x = fmaf(x, decay, x * decay_low);
-                X[k][e] = x;
+                X[k][e] = decltype(masked)::value && r >= s.dk ? 0.f : x;
             }
         }
+    };
+    for (int i = 0; i < n; ++i) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        const f32x4 c = *(const f32x4*)&lc[i][x0];
+        if (WHOLE || (c[0] * 0.f + c[1] * 0.f) + (c[2] * 0.f + c[3] * 0.f) == 0.f) advance(i, c, o, std::false_type{});
+        else advance(i, c, o, std::true_type{});
 #pragma unroll
         for (int d = LX; d < 64; d <<= 1)
 #pragma unroll
@@ -120,8 +132,10 @@ __global__ __launch_bounds__(256) void k_step(const ScanArgs s, const float* __r
 template <typename T, int CS, int NR>
 void launch_as(const ScanArgs& a, const float* powers, hipStream_t s) {
     const dim3 grid((unsigned)((a.dv + CS - 1) / CS), (unsigned)a.heads, (unsigned)a.batch);
-    if (a.state_col == 1) hipLaunchKernelGGL((k_step<T, CS, NR, true>), grid, dim3(256), 0, s, a, powers);
-    else hipLaunchKernelGGL((k_step<T, CS, NR, false>), grid, dim3(256), 0, s, a, powers);
+    const bool packed = a.state_col == 1, whole = a.dk == 256 * 4 / CS * NR;
+    const auto kernel = packed ? (whole ? k_step<T, CS, NR, true, true> : k_step<T, CS, NR, true, false>)
+                               : (whole ? k_step<T, CS, NR, false, true> : k_step<T, CS, NR, false, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, powers);
 }
 
 // 64 columns a block; a fourth of that while those blocks would use less than an

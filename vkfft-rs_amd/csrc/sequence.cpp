@@ -2,6 +2,7 @@
 // linear attention. Arguments are checked here, before anything is launched;
 // the kernels rely on it.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <exception>
 #include <memory>
@@ -251,8 +252,12 @@ int vkfx_linear_attention_create(vkfx_context* ctx, const vkfx_linear_attention_
         for (uint32_t h = 0; h < d.heads; ++h) {
             if (!(d.decay[h] >= 0 && d.decay[h] <= 1)) return bad("decay must be in [0, 1]: head " + std::to_string(h));
             float* row = powers.data() + (size_t)h * kDecayPowers;
-            for (int n = 0; n < kDecayPowers - 1; ++n) row[n] = (float)std::pow(d.decay[h], n);
-            row[kDecayPowers - 1] = (float)(d.decay[h] - (double)row[1]);
+            for (int n = 0; n < kDecayHigh; ++n) row[n] = (float)std::pow(d.decay[h], n);
+            float high = (float)d.decay[h];
+            if ((double)high > d.decay[h]) high = std::nextafter(high, 0.f);
+            row[kDecayHigh] = high;
+            row[kDecayLow] = (float)(d.decay[h] - (double)high);
+            if (d.decay[h] > 0 && row[kDecayLow] == 0.f) row[kDecayLow] = std::max(high * 0x1p-60f, FLT_TRUE_MIN);
         }
         uint64_t floats = 0;
         if (d.gradient && !group_floats(d, d.max_batch, d.max_tokens, &floats))

@@ -66,8 +66,10 @@ struct ScanArgs {
 };
 
 // Powers 0, 1, ... of each head's decay, kDecayPowers floats a head; the last
-// one is what 32 bits leave of the decay itself (decay - powers[1]).
-constexpr int kDecayPowers = 72;
+// two are the decay itself as a sum: its 24 bits towards zero and the rest. The
+// rest is never negative, nor zero unless the decay is, so that a state times
+// both parts stays infinite where it is.
+constexpr int kDecayPowers = 72, kDecayHigh = kDecayPowers - 2, kDecayLow = kDecayPowers - 1;
 
 // Up to kStepTokens tokens one after the other (linear_step.hip).
 constexpr int kStepTokens = 8;
