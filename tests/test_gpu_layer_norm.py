@@ -289,3 +289,10 @@ def test_refusals(hip_ctx):
     refused("InvalidArgument", plan.backward_tensors, x, w, None, y, y, w, w)
     refused("InvalidArgument", plan.backward_tensors, x, w, st, y, x, w, w)
     refused("InputLengthMismatch", plan.backward_tensors, x, w, st, y, y, w, w, work=torch.zeros(4, device="cuda"))
+
+
+def test_an_epsilon_past_32_bits_is_refused(hip_ctx):
+    """Its square root would make every row the bias."""
+    with pytest.raises(vk.VkFftError) as e:
+        vk.LayerNormPlan(hip_ctx, vk.LayerNormConfig.new(8).with_epsilon(1e39))
+    assert e.value.kind == "InvalidArgument"

@@ -139,7 +139,7 @@ int vkfx_layer_norm_create(vkfx_context* ctx, const vkfx_layer_norm_desc* desc, 
         if (!known_element(desc->element)) return fail(VKFX_ERR_UNSUPPORTED_PRECISION, "element must be F32, F16 or BF16");
         if (desc->weight_element != desc->element && desc->weight_element != VKFX_ELEMENT_F32)
             return fail(VKFX_ERR_UNSUPPORTED_PRECISION, "weights must be F32 or of the rows' element");
-        if (!(desc->epsilon > 0) || !std::isfinite(desc->epsilon) || (float)desc->epsilon == 0.f)
+        if (!(desc->epsilon > 0) || !std::isfinite((float)desc->epsilon) || (float)desc->epsilon == 0.f)
             return bad("epsilon must be positive and finite in 32 bits");
         auto p = std::make_unique<vkfx_layer_norm>();
         p->ctx = ctx;
