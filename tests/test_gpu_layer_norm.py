@@ -296,3 +296,27 @@ def test_an_epsilon_past_32_bits_is_refused(hip_ctx):
     with pytest.raises(vk.VkFftError) as e:
         vk.LayerNormPlan(hip_ctx, vk.LayerNormConfig.new(8).with_epsilon(1e39))
     assert e.value.kind == "InvalidArgument"
+
+
+@pytest.mark.parametrize("width", [1 << 20, (1 << 20) + 77])
+def test_long_rows_of_one_value_keep_their_sums(hip_ctx, width):
+    """Equal elements round to the same side at every addition: a thread's long sums would drift."""
+    import torch
+    plan = _plan(hip_ctx, width, "f32")
+    x = torch.full((2, width), 0.1, device="cuda")
+    w, b = _normal(2, (width,), "f32", 0.2, 1.0), _normal(3, (width,), "f32", 0.2)
+    y, stats = torch.empty_like(x), torch.empty(2, 2, device="cuda")
+    plan.forward_tensors(x, w, b, y, stats)
+    xn, wn, bn = _np(x, w, b)
+    want, want_stats = ref.norm(xn, wn, bn, 1e-5)
+    ref.check("mean", stats[:, :1], want_stats[:, :1], np.abs(want_stats[:, :1]), "f32", ref.NORM_TERM)
+    ref.check("y", y, want, ref.norm_bound(xn, wn, bn, want_stats), "f32", ref.NORM_TERM)
+    # gradients: the rows of a usual input, dy weight the same everywhere
+    x = _normal(4, (2, width), "f32", 1.5, 0.4)
+    xn, = _np(x)
+    stats = torch.from_numpy(ref.norm(xn, 1.0, 0.0, 1e-5)[1]).float().cuda()
+    dy = torch.full((2, width), 0.1, device="cuda")
+    dx = torch.empty_like(x)
+    plan.backward_tensors(x, None, stats, dy, dx)
+    one, (sn, dyn) = np.ones(width), _np(stats, dy)
+    ref.check("dx", dx, ref.norm_gradients(xn, one, sn, dyn)[0], ref.norm_gradients_bound(xn, one, sn, dyn)[0], "f32", ref.NORM_TERM)

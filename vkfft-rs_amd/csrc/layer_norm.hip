@@ -351,7 +351,10 @@ __global__ __launch_bounds__(1024) void k_norm_backward_sum(const NormArgs a, in
     to[c] = (W)s;
 }
 
-// ---- rows too wide for a block's registers: read once for each sum
+// ---- rows too wide for a block's registers: read once for each sum. A thread's
+// own sums are long (a row of 2^20 elements gives it 1024 terms, which are added
+// one by one), so they are in 64 bits: equal elements would round to one side
+// each time.
 
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void k_norm_forward_wide(const NormArgs a) {
@@ -360,15 +363,17 @@ __global__ __launch_bounds__(1024) void k_norm_forward_wide(const NormArgs a) {
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = (const T*)a.x + r * a.x_stride;
         T* y = (T*)a.y + r * a.y_stride;
-        float s[1] = {0.f};
-        for (int i = threadIdx.x; i < a.width; i += 1024) s[0] += (float)x[i];
+        double sum = 0.0;
+        for (int i = threadIdx.x; i < a.width; i += 1024) sum += (double)(float)x[i];
+        float s[1] = {(float)sum};
         row_sum<1024>(s, lds, half);
         const float mean = s[0] / (float)a.width;
-        s[0] = 0.f;
+        sum = 0.0;
         for (int i = threadIdx.x; i < a.width; i += 1024) {
             const float d = (float)x[i] - mean;
-            s[0] = fmaf(d, d, s[0]);
+            sum += (double)(d * d);
         }
+        s[0] = (float)sum;
         row_sum<1024>(s, lds, half);
         const float rstd = 1.0f / sqrtf(s[0] / (float)a.width + a.epsilon);
         for (int i = threadIdx.x; i < a.width; i += 1024) {
@@ -392,12 +397,13 @@ __global__ __launch_bounds__(1024) void k_norm_backward_wide(const NormArgs a) {
         const T* dy = (const T*)a.dy + r * a.dy_stride;
         T* dx = (T*)a.y + r * a.y_stride;
         const float mean = a.stats_in[2 * r], rstd = a.stats_in[2 * r + 1];
-        float s[2] = {0.f, 0.f};
+        double sum = 0.0, product = 0.0;
         for (int i = threadIdx.x; i < a.width; i += 1024) {
             const float g = (float)dy[i] * (a.weight ? (float)((const W*)a.weight)[i] : 1.f);
-            s[0] += g;
-            s[1] = fmaf(g, ((float)x[i] - mean) * rstd, s[1]);
+            sum += (double)g;
+            product += (double)(g * (((float)x[i] - mean) * rstd));
         }
+        float s[2] = {(float)sum, (float)product};
         row_sum<1024>(s, lds, half);
         const float m1 = s[0] / (float)a.width, m2 = s[1] / (float)a.width;
         for (int i = threadIdx.x; i < a.width; i += 1024) {
