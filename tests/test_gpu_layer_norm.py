@@ -320,3 +320,32 @@ def test_long_rows_of_one_value_keep_their_sums(hip_ctx, width):
     plan.backward_tensors(x, None, stats, dy, dx)
     one, (sn, dyn) = np.ones(width), _np(stats, dy)
     ref.check("dx", dx, ref.norm_gradients(xn, one, sn, dyn)[0], ref.norm_gradients_bound(xn, one, sn, dyn)[0], "f32", ref.NORM_TERM)
+
+
+def test_plans_of_every_width_that_is_promised(hip_ctx):
+    """The workspace follows what a width's kernels write, so that the widest plan fits beside its rows."""
+    import torch
+    for width in (32769, 1 << 17, 1 << 20, 1 << 27):
+        plan = _plan(hip_ctx, width, "f16")
+        assert plan.workspace_bytes <= max(1 << 26, 8 * width)
+        plan.close()
+    width = 1 << 30
+    plan = _plan(hip_ctx, width, "f16")
+    x = torch.zeros(1, width, device="cuda", dtype=torch.float16)
+    x[:, ::2] = 1
+    y, stats = torch.full_like(x, 7), torch.empty(1, 2, device="cuda")
+    plan.forward_tensors(x, None, None, y, stats)
+    # a mean of 1/2, and 1 in 16 bits as what lies around it
+    assert stats[0, 0].item() == 0.5 and (y[:, 1::2] == -1).all() and (y[:, ::2] == 1).all()
+    dw, db = torch.full_like(x[0], 7), torch.full_like(x[0], 7)
+    plan.backward_tensors(x, None, stats, x, y, dw, db)
+    assert torch.equal(db, x[0]) and torch.equal(dw, x[0])
+    # dx = rstd (g - mean g - n mean(g n)) with g = x: 4 epsilon, and a few roundings of 1/2
+    assert y.abs().max().item() <= 4.2e-5
+    plan.close()
+
+
+@pytest.mark.parametrize("element", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,width", [(70, 65536), (9, 300001), (5, 1 << 22), (3, (1 << 22) + 1)])
+def test_rows_split_over_fewer_sums_where_they_are_wide(hip_ctx, element, rows, width):
+    _run(hip_ctx, rows, width, element)

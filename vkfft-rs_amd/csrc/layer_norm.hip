@@ -327,14 +327,15 @@ __global__ __launch_bounds__(NT) void k_norm_backward(const NormArgs a) {
 }
 
 // Adds the blocks' sums: 64 columns a block, its 16 waves each an equal share
-// of the blocks in their order. blockIdx.y: weight or bias.
+// of the blocks in their order. blockIdx.y: weight or bias; blockIdx.z: columns
+// past what a launch's threads along x can count.
 template <typename W>
 __global__ __launch_bounds__(1024) void k_norm_backward_sum(const NormArgs a, int parts) {
     __shared__ float lds[16][64];
     W* const to = (W*)(blockIdx.y ? a.dbias : a.dweight);
     if (!to) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane;
+    const long long c = ((long long)blockIdx.z * gridDim.x + blockIdx.x) * 64 + lane;
     const int first = (int)((long long)parts * wave / 16), end = (int)((long long)parts * (wave + 1) / 16);
     float s = 0.f;
     if (c < a.width) {
@@ -435,8 +436,19 @@ __global__ __launch_bounds__(256) void k_norm_backward_wide_rows(const NormArgs 
 
 template <typename W>
 void launch_sum(const NormArgs& a, int parts, hipStream_t s) {
-    hipLaunchKernelGGL((k_norm_backward_sum<W>), dim3((unsigned)((a.width + 63) / 64), 2), dim3(1024), 0, s, a, parts);
+    const unsigned blocks = (unsigned)((a.width + 63) / 64), x = std::min(blocks, 1u << 21);
+    hipLaunchKernelGGL((k_norm_backward_sum<W>), dim3(x, 2, (blocks + x - 1) / x), dim3(1024), 0, s, a, parts);
 }
+
+// Whether a row's sums over the rows stay in a block's registers.
+bool sums_in_registers(int element, int width) {
+    return element == VKFX_ELEMENT_F32 ? width <= 4096 * kVector<float> : width <= 2048 * kVector<_Float16>;
+}
+
+// Rows of sums that the rows of a wider one are split over: 64, and fewer where
+// the columns alone fill the GPU (gradients of 64 rows of 2^20 f32: 1336 us with the
+// 4 that this gives, 1542 with 64).
+int wide_parts(int width) { return std::max(1, std::min(64, (1 << 22) / width)); }
 
 template <typename T, typename W, int LPR, int NV, int NT>
 int forward_with(const NormArgs& a, hipStream_t s) {
@@ -494,10 +506,10 @@ int backward_as(const NormArgs& a, hipStream_t s) {
     if (n <= 1024) return backward_with<T, W, 256, 4, 512>(a, s);
     if (n <= 2048) return backward_with<T, W, 512, 4, 512>(a, s);
     if constexpr (sizeof(T) == 4)
-        if (n <= 4096) return backward_with<T, W, 1024, 4, 1024>(a, s);
+        if (sums_in_registers(a.element, a.width)) return backward_with<T, W, 1024, 4, 1024>(a, s);
     // dx may overwrite dy: the sums over the rows go first
     if (a.dweight || a.dbias) {
-        const int parts = (int)std::min(a.rows, 64ll);
+        const int parts = (int)std::min(a.rows, (long long)wide_parts(a.width));
         hipLaunchKernelGGL((k_norm_backward_wide_rows<T>), dim3((unsigned)((a.width + 1023) / 1024), parts), dim3(256), 0, s, a);
         launch_sum<W>(a, parts, s);
     }
@@ -524,8 +536,8 @@ int pick_element(const NormArgs& a, hipStream_t s, bool forward) {
 
 int launch_norm_forward(const NormArgs& a, hipStream_t s) { return pick_element(a, s, true); }
 int launch_norm_backward(const NormArgs& a, hipStream_t s) { return pick_element(a, s, false); }
-size_t norm_workspace_bytes(int width, int cus) {
-    return (size_t)std::max(cus, 64) * 2 * (size_t)width * sizeof(float);
+size_t norm_workspace_bytes(int element, int width, int cus) {
+    return (size_t)(sums_in_registers(element, width) ? cus : wide_parts(width)) * 2 * (size_t)width * sizeof(float);
 }
 
 }  // namespace vkfx

@@ -145,7 +145,7 @@ int vkfx_layer_norm_create(vkfx_context* ctx, const vkfx_layer_norm_desc* desc, 
         p->ctx = ctx;
         p->desc = *desc;
         (void)hipSetDevice(ctx->device);
-        if (int rc = allocate(p->work, norm_workspace_bytes((int)desc->width, (int)ctx->profile.compute_units))) return rc;
+        if (int rc = allocate(p->work, norm_workspace_bytes(desc->element, (int)desc->width, (int)ctx->profile.compute_units))) return rc;
         retain(ctx);
         *out = p.release();
         return VKFX_OK;

@@ -20,7 +20,7 @@ struct NormArgs {
     float* stats_out;
     void* dweight;
     void* dbias;
-    float* partial;  // backward: [blocks][2][width] sums of a block's rows
+    float* partial;  // backward: [blocks][2][width] sums of a block's rows, norm_workspace_bytes
     long long rows, x_stride, dy_stride, y_stride;
     int width;
     int element, weight_element;  // vkfx_element
@@ -30,7 +30,7 @@ struct NormArgs {
 
 int launch_norm_forward(const NormArgs& a, hipStream_t s);
 int launch_norm_backward(const NormArgs& a, hipStream_t s);
-size_t norm_workspace_bytes(int width, int cus);
+size_t norm_workspace_bytes(int element, int width, int cus);
 
 // ------------------------------------------------------- linear attention
 
