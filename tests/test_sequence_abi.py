@@ -138,3 +138,47 @@ def test_a_plan_keeps_the_sizes_it_was_made_with():
     assert e.value.kind == "InputLengthMismatch" and not ctx.calls
     plan.forward_tensors(_Tensor(1, 1, 4, 16), _Tensor(1, 1, 2, 16), _Tensor(1, 1, 2, 24), _Tensor(1, 1, 4, 24))
     assert ctx.calls
+
+
+def _refused(kind, f, *a, **kw):
+    with pytest.raises(vk.VkFftError) as e:
+        f(*a, **kw)
+    assert e.value.kind == kind, e.value
+
+
+@pytest.mark.parametrize("missing", [None, [1.0], 3])
+def test_what_is_no_tensor_is_refused_as_an_argument(missing):
+    ctx = _Context()
+    norm = ctx.plan(vk.LayerNormConfig.new(8))
+    w, x, st = _Tensor(8), _Tensor(4, 8), _Tensor(4, 2)
+    _refused("InvalidArgument", norm.forward_tensors, missing, w, w, x)
+    _refused("InvalidArgument", norm.forward_tensors, x, w, w, missing)
+    _refused("InvalidArgument", norm.backward_tensors, missing, w, st, x, x, w, w)
+    _refused("InvalidArgument", norm.backward_tensors, x, w, st, missing, x, w, w)
+    mix = ctx.plan(vk.LinearAttentionConfig.new(2, 8, 8).with_capacity(1, 4).with_gradient())
+    t = [_Tensor(1, 4, 2, 8) for _ in range(7)]
+    for i in range(4):
+        _refused("InvalidArgument", mix.forward_tensors, *[missing if j == i else x for j, x in enumerate(t[:4])])
+    for i in range(7):
+        _refused("InvalidArgument", mix.backward_tensors, *[missing if j == i else x for j, x in enumerate(t)])
+    if missing is not None:  # None is the way to leave these out
+        _refused("InvalidArgument", norm.forward_tensors, x, missing, w, x)
+        _refused("InvalidArgument", norm.backward_tensors, x, w, st, x, x, missing, w)
+        _refused("InvalidArgument", norm.backward_tensors, x, w, st, x, missing, w, w)
+        _refused("InvalidArgument", mix.forward_tensors, *t[:4], state_in=missing)
+        _refused("InvalidArgument", mix.forward_tensors, *t[:4], lengths=missing)
+        _refused("InvalidArgument", mix.forward_tensors, *t[:4], work=missing)
+    assert not ctx.calls
+
+
+def test_a_tensor_without_dimensions_is_refused():
+    ctx = _Context()
+    norm = ctx.plan(vk.LayerNormConfig.new(8))
+    w, x = _Tensor(8), _Tensor(4, 8)
+    for y in (_Tensor(), _Tensor(8), _Tensor(1, 4, 8)):
+        _refused("InputLengthMismatch", norm.forward_tensors, y, w, w, x)
+        _refused("InputLengthMismatch", norm.backward_tensors, y, w, _Tensor(4, 2), x, x, w, w)
+    mix = ctx.plan(vk.LinearAttentionConfig.new(2, 8, 8).with_capacity(1, 4))
+    t = [_Tensor(1, 4, 2, 8) for _ in range(4)]
+    _refused("InputLengthMismatch", mix.forward_tensors, _Tensor(), *t[1:])
+    assert not ctx.calls

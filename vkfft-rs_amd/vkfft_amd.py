@@ -1444,7 +1444,10 @@ class _SequencePlan:
 
     def _place(self, x) -> int:
         """The device of a call's tensors: the context's."""
-        device = x.get_device()
+        try:
+            device = x.get_device()
+        except AttributeError:
+            device = -1
         if device != self._device:
             raise VkFftError(-7, f"tensors must be on the context's device {self._device}" if device >= 0
                              else "tensors must be device tensors")
@@ -1452,6 +1455,8 @@ class _SequencePlan:
 
     @staticmethod
     def _refuse(name, x, shape, dtype, device):
+        if not hasattr(x, "get_device"):
+            raise VkFftError(-7, f"{name} must be a device tensor")
         if x.shape != shape:
             raise VkFftError(-5, f"{name}: expected shape {tuple(shape)}, got {tuple(x.shape)}")
         if x.dtype != dtype:
@@ -1464,13 +1469,15 @@ class _SequencePlan:
         """Address of a contiguous tensor, or None."""
         if x is None:
             return None
-        if x.shape != shape or x.dtype is not dtype or x.get_device() != device or not x.is_contiguous():
+        if getattr(x, "shape", None) != shape or x.dtype is not dtype or x.get_device() != device or not x.is_contiguous():
             self._refuse(name, x, shape, dtype, device)
         return x.data_ptr()
 
     def _work(self, work, device):
         if work is None:
             return None
+        if not hasattr(work, "get_device"):
+            raise VkFftError(-7, "work must be a device tensor")
         if work.get_device() != device or not work.is_contiguous() or work.numel() * work.element_size() < self.workspace_bytes:
             raise VkFftError(-5, f"work must be {self.workspace_bytes} contiguous bytes on device {device}")
         return work.data_ptr()
@@ -1500,7 +1507,7 @@ class LayerNormPlan(_SequencePlan):
 
     def _rows(self, name, x, rows, device):
         width = self._width
-        if x.shape != (rows, width) or x.dtype is not self._type or x.get_device() != device:
+        if getattr(x, "shape", None) != (rows, width) or x.dtype is not self._type or x.get_device() != device:
             self._refuse(name, x, (rows, width), self._type, device)
         row, column = x.stride()
         if column != 1 and width > 1:
@@ -1510,7 +1517,7 @@ class LayerNormPlan(_SequencePlan):
     def forward_tensors(self, x, weight, bias, y, stats=None, stream=None):
         """y (may be x) and, if wanted, stats [rows][2]: mean and rstd."""
         device, w = self._place(x), (self._width,)
-        rows = x.shape[0]
+        rows = x.shape[0] if x.shape else 0
         xp, xs = self._rows("x", x, rows, device)
         yp, ys = self._rows("y", y, rows, device)
         _check(self._L.vkfx_layer_norm_forward(
@@ -1521,7 +1528,7 @@ class LayerNormPlan(_SequencePlan):
     def backward_tensors(self, x, weight, stats, dy, dx=None, dweight=None, dbias=None, work=None, stream=None):
         """Gradients for dy; any of the three may be None (not wanted)."""
         device, w = self._place(x), (self._width,)
-        rows = x.shape[0]
+        rows = x.shape[0] if x.shape else 0
         xp, xs = self._rows("x", x, rows, device)
         gp, gs = self._rows("dy", dy, rows, device)
         dp, ds = (None, 0) if dx is None else self._rows("dx", dx, rows, device)
@@ -1605,7 +1612,7 @@ class LinearAttentionPlan(_SequencePlan):
         self._dims = config.heads, kv, config.key_dim, config.value_dim
 
     def _sequence(self, name, x, shape, device):
-        if x.shape != shape or x.dtype is not self._type or x.get_device() != device:
+        if getattr(x, "shape", None) != shape or x.dtype is not self._type or x.get_device() != device:
             self._refuse(name, x, shape, self._type, device)
         b, t, h, d = x.stride()
         if d != 1 and shape[3] > 1:
