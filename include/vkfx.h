@@ -357,7 +357,9 @@ int vkfx_execute_chain_host(vkfx_plan *const *plans, uint32_t count, const void 
  * Calls are asynchronous on `stream` (a hipStream_t; NULL = the context's
  * stream; hipStreamLegacy, (void *)1, = the null stream itself). They neither
  * allocate nor synchronise nor copy from the host, so a HIP graph can capture
- * them. A plan's own workspace serves one call at a time: calls of one plan
+ * them. Outputs share no memory with inputs or each other, except in place where
+ * that is said; it is refused where it shows without going through the elements
+ * (a tensor without gaps, or two views of one layout). A plan's own workspace serves one call at a time: calls of one plan
  * that overlap on the GPU pass d_work each. */
 
 /* Type of the tensors' elements. Sums, statistics and states are 32 bits. */

@@ -349,3 +349,43 @@ def test_plans_of_every_width_that_is_promised(hip_ctx):
 @pytest.mark.parametrize("rows,width", [(70, 65536), (9, 300001), (5, 1 << 22), (3, (1 << 22) + 1)])
 def test_rows_split_over_fewer_sums_where_they_are_wide(hip_ctx, element, rows, width):
     _run(hip_ctx, rows, width, element)
+
+
+def test_partial_overlaps_are_refused_and_interleaved_rows_are_not(hip_ctx):
+    import torch
+    plan = _plan(hip_ctx, 64, "f32")
+    buf = torch.zeros(40, 128, device="cuda")
+    w, b, st = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda"), torch.zeros(8, 2, device="cuda")
+    flat = buf.view(-1)
+    x = flat[:512].view(8, 64)
+
+    def refused(f, *a, **kw):
+        with pytest.raises(vk.VkFftError) as e:
+            f(*a, **kw)
+        assert e.value.kind == "InvalidArgument" and "overlap" in str(e.value)
+
+    for at in (1, 64, 511):
+        refused(plan.forward_tensors, x, w, b, flat[at:at + 512].view(8, 64))
+    refused(plan.forward_tensors, x, w, b, buf[:8, 64:])  # rows of another pitch
+    refused(plan.forward_tensors, buf[:8, :64], w, b, buf[2:10, 32:96])
+    refused(plan.forward_tensors, x, w, b, buf[20:28, :64], flat[500:516].view(8, 2))
+    refused(plan.forward_tensors, buf[20:28, :64], flat[:64], b, x)
+    refused(plan.forward_tensors, buf[20:28, :64], w, flat[448:512], x)
+    dy, dx, dw, db = buf[10:18, :64], buf[20:28, :64], torch.zeros_like(w), torch.zeros_like(w)
+    refused(plan.backward_tensors, x, w, st, dy, flat[64:576].view(8, 64), dw, db)
+    refused(plan.backward_tensors, x, w, st, dy, buf[11:19, :64], dw, db)
+    refused(plan.backward_tensors, x, w, st, dy, dx, dw, dw)
+    refused(plan.backward_tensors, x, w, st, dy, dx, buf[20, :64], db)
+    refused(plan.backward_tensors, x, w, st, dy, dx, dw, x[3])
+    work = torch.zeros(plan.workspace_bytes // 4 + 64, device="cuda")
+    refused(plan.backward_tensors, x, w, st, dy, dx, dw, work[-128:-64], work=work[:-64])
+
+    # the two halves of every row of one buffer, and the same rows
+    buf.copy_(_normal(1, (40, 128), "f32"))
+    want = torch.empty(8, 64, device="cuda")
+    plan.forward_tensors(buf[:8, :64], w, b, want, st)
+    plan.forward_tensors(buf[:8, :64], w, b, buf[:8, 64:], st)
+    assert torch.equal(buf[:8, 64:], want)
+    plan.backward_tensors(buf[:8, :64], w, st, buf[10:18, :64], buf[10:18, 64:], dw, db)
+    plan.backward_tensors(buf[:8, :64], w, st, buf[10:18, :64], buf[10:18, :64], dw, db)
+    assert torch.equal(buf[10:18, :64], buf[10:18, 64:])

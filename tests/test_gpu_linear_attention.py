@@ -587,3 +587,54 @@ def test_an_infinite_value_of_a_token_gives_an_infinite_output(hip_ctx, dk, batc
     out[:, 1:, :, 3] = 0
     state[:, :, :, 3] = 0
     assert torch.isfinite(out).all() and torch.isfinite(state).all()
+
+
+def test_partial_overlaps_are_refused_and_packed_tensors_are_not(hip_ctx):
+    import torch
+    b, t, h, d = 2, 40, 4, 16
+    plan = _plan(hip_ctx, b, t, h, h, d, d, "f32", True)
+    n = b * t * h * d
+
+    def at(flat, i):
+        return flat[i:i + n].view(b, t, h, d)
+
+    def refused(f, *a, **kw):
+        with pytest.raises(vk.VkFftError) as e:
+            f(*a, **kw)
+        assert e.value.kind == "InvalidArgument" and "overlap" in str(e.value)
+
+    flat = torch.zeros(9 * n, device="cuda")
+    q, k, v, out = (at(flat, i * n) for i in range(4))
+    states = torch.zeros(2 * b * h * d * d, device="cuda")
+    size = b * h * d * d
+    s, s2 = states[:size].view(b, h, d, d), states[d:size + d].view(b, h, d, d)
+    f, g = plan.forward_tensors, plan.backward_tensors
+    for i in range(3):
+        refused(f, q, k, v, at(flat, i * n + 1 if i < 2 else 3 * n - 5))
+    refused(f, q, k, v, at(flat, n // 2))
+    refused(f, q, k, v, out, state_in=s, state_out=s2)
+    refused(f, q, k, v, out, state_out=flat[4 * n - size:4 * n].view(b, h, d, d))
+    refused(f, q, k, v, out, state_out=s, lengths=states[:b].view(torch.int32))
+    dq, dk, dv = (at(flat, i * n) for i in (4, 5, 6))
+    for i, name in enumerate((dq, dk, dv)):
+        for j in (0, 1, 2, 3):
+            moved = [dq, dk, dv]
+            moved[i] = at(flat, j * n + 3)
+            refused(g, q, k, v, out, *moved)
+    refused(g, q, k, v, out, dq, at(flat, 5 * n - 1), dv)
+    refused(g, q, k, v, out, dq, dk, dv, state_in=s, dstate_in=s2)
+    refused(g, q, k, v, out, dq, dk, dv, dstate_out=s, dstate_in=s2)
+    # views of one projection, and of one buffer for its gradients
+    packed, grads = (torch.zeros(b, t, 3, h, d, device="cuda") for _ in range(2))
+    packed.copy_(_tensor(1, (b, t, 3 * h, d), "f32").view(b, t, 3, h, d))
+    dout = _tensor(2, (b, t, h, d), "f32")
+    wide = torch.zeros(b, t, 2, h, d, device="cuda")  # out beside dout
+    wide[:, :, 1] = dout
+    f(*packed.unbind(2), wide[:, :, 0])
+    g(*packed.unbind(2), wide[:, :, 1], *grads.unbind(2))
+    want = [torch.empty(b, t, h, d, device="cuda") for _ in range(4)]
+    apart = [x.contiguous() for x in packed.unbind(2)]
+    f(*apart, want[0])
+    g(*apart, dout, *want[1:])
+    assert torch.equal(wide[:, :, 0], want[0])
+    assert all(torch.equal(x, y) for x, y in zip(grads.unbind(2), want[1:]))

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "context.hpp"
+#include "overlap.hpp"
 #include "sequence.hpp"
 #include "vkfx.h"
 
@@ -83,8 +84,52 @@ int destroy(P* plan) {
     return VKFX_OK;
 }
 
-// a * b in *out; false on overflow.
-bool mul(uint64_t a, uint64_t b, uint64_t* out) { return !__builtin_mul_overflow(a, b, out) && *out < (1ull << 62); }
+// a * b in *out; false past 2^60, from where on a count of bytes could overflow.
+bool mul(uint64_t a, uint64_t b, uint64_t* out) { return !__builtin_mul_overflow(a, b, out) && *out < (1ull << 60); }
+
+uint64_t bytes_of(int32_t element) { return element == VKFX_ELEMENT_F32 ? 4 : 2; }
+
+// A tensor of a call, for the check that outputs share no memory with inputs
+// nor with each other. No data: nothing.
+struct Tensor {
+    const char* name;
+    Region region;
+    bool written;
+};
+
+Tensor flat(const char* name, const void* p, uint64_t bytes, bool written) {
+    Tensor t{name, {}, written};
+    t.region.at = (uintptr_t)p;
+    t.region.run = p ? bytes : 0;
+    return t;
+}
+
+Tensor rows_of(const char* name, const void* p, uint64_t rows, int64_t stride, uint64_t width, int32_t element, bool written) {
+    Tensor t = flat(name, p, width * bytes_of(element), written);
+    t.region.axis(0, (uint64_t)stride * bytes_of(element), rows);
+    return t;
+}
+
+Tensor sequence_of(const char* name, const vkfx_sequence& s, uint64_t batch, uint64_t tokens, uint64_t heads, uint64_t dim,
+                   int32_t element, bool written) {
+    const uint64_t size = bytes_of(element);
+    Tensor t = flat(name, s.data, dim * size, written);
+    t.region.axis(0, (uint64_t)s.batch_stride * size, batch).axis(1, (uint64_t)s.token_stride * size, tokens);
+    t.region.axis(2, (uint64_t)s.head_stride * size, heads);
+    return t;
+}
+
+// `out` and `in`: the names of an output that stands in its input's place.
+template <size_t N>
+int check_apart(const Tensor (&tensors)[N], const char* out = nullptr, const char* in = nullptr) {
+    for (size_t i = 0; i < N; ++i)
+        for (size_t j = 0; j < N; ++j) {
+            const Tensor &w = tensors[i], &t = tensors[j];
+            if (!w.written || i == j || (t.written && j < i) || (w.name == out && t.name == in)) continue;
+            if (overlap(w.region, t.region)) return bad(std::string(w.name) + " overlaps " + t.name);
+        }
+    return VKFX_OK;
+}
 
 // Strides of one [batch][token][head][dim] tensor: none negative, every offset
 // within 62 bits, and for an output no two elements at one place.
@@ -173,7 +218,15 @@ int vkfx_layer_norm_forward(vkfx_layer_norm* plan, uint64_t rows, const void* x,
         if (y_row_stride < w && rows > 1) return bad("y: rows overlap");
         if (x == y && x_row_stride != y_row_stride && rows > 1) return bad("y may be x only with x's stride");
         if (!mul((uint64_t)x_row_stride, rows, &reach) || (rows > 1 && !mul((uint64_t)y_row_stride, rows, &reach)))
-            return fail(VKFX_ERR_ARITHMETIC_OVERFLOW, "row strides reach past 2^62 elements");
+            return fail(VKFX_ERR_ARITHMETIC_OVERFLOW, "row strides reach past 2^60 elements");
+        const int32_t element = plan->desc.element;
+        const uint64_t weights = (uint64_t)w * bytes_of(plan->desc.weight_element);
+        const char *nx = "x", *ny = "y";
+        if (int rc = check_apart({rows_of(ny, y, rows, y_row_stride, w, element, true), flat("stats", stats, rows * 8, true),
+                                  rows_of(nx, x, rows, x_row_stride, w, element, false), flat("weight", weight, weights, false),
+                                  flat("bias", bias, weights, false)},
+                                 x == y ? ny : nullptr, nx))
+            return rc;
         NormArgs a{};
         a.x = x;
         a.weight = weight;
@@ -207,10 +260,19 @@ int vkfx_layer_norm_backward(vkfx_layer_norm* plan, uint64_t rows, const void* x
         if (dy_row_stride < 0 || (dy_row_stride && dy_row_stride < w && rows > 1)) return bad("dy: rows overlap");
         if (dx && dx_row_stride < w && rows > 1) return bad("dx: rows overlap");
         if (dx && dx == dy && dx_row_stride != dy_row_stride && rows > 1) return bad("dx may be dy only with dy's stride");
-        if (dx && dx == x && rows) return bad("dx may not be x");
         if (!mul((uint64_t)x_row_stride, rows, &reach) || !mul((uint64_t)dy_row_stride, rows, &reach) ||
             (dx && rows > 1 && !mul((uint64_t)dx_row_stride, rows, &reach)))
-            return fail(VKFX_ERR_ARITHMETIC_OVERFLOW, "row strides reach past 2^62 elements");
+            return fail(VKFX_ERR_ARITHMETIC_OVERFLOW, "row strides reach past 2^60 elements");
+        const int32_t element = plan->desc.element;
+        const uint64_t weights = (uint64_t)w * bytes_of(plan->desc.weight_element);
+        const char *nx = "dx", *ny = "dy";
+        if (int rc = check_apart({rows_of(nx, dx, rows, dx_row_stride, w, element, true), flat("dweight", dweight, weights, true),
+                                  flat("dbias", dbias, weights, true), flat("work", d_work, plan->work.bytes, true),
+                                  rows_of(ny, dy, rows, dy_row_stride, w, element, false),
+                                  rows_of("x", x, rows, x_row_stride, w, element, false), flat("weight", weight, weights, false),
+                                  flat("stats", stats, rows * 8, false)},
+                                 dx == dy ? nx : nullptr, ny))
+            return rc;
         NormArgs a{};
         a.x = x;
         a.weight = weight;
@@ -299,9 +361,17 @@ int vkfx_linear_attention_forward(vkfx_linear_attention* plan, const vkfx_linear
             if (int rc = check_sequence("k", args->k, args->batch, args->tokens, d.kv_heads, d.key_dim, false)) return rc;
             if (int rc = check_sequence("v", args->v, args->batch, args->tokens, d.kv_heads, d.value_dim, false)) return rc;
             if (int rc = check_sequence("out", args->out, args->batch, args->tokens, d.heads, d.value_dim, true)) return rc;
-            if (args->out.data == args->q.data || args->out.data == args->k.data || args->out.data == args->v.data)
-                return bad("out overlaps an input");
         }
+        const uint64_t b = args->batch, t = args->tokens, states = b * d.heads * d.key_dim * d.value_dim * 4;
+        const char *in = "state_in", *after = "state_out";
+        if (int rc = check_apart({sequence_of("out", args->out, b, t, d.heads, d.value_dim, d.element, true),
+                                  flat(after, args->state_out, states, true), flat("work", d_work, plan->work.bytes, true),
+                                  flat(in, args->state_in, states, false), flat("lengths", args->lengths, b * 4, false),
+                                  sequence_of("q", args->q, b, t, d.heads, d.key_dim, d.element, false),
+                                  sequence_of("k", args->k, b, t, d.kv_heads, d.key_dim, d.element, false),
+                                  sequence_of("v", args->v, b, t, d.kv_heads, d.value_dim, d.element, false)},
+                                 args->state_in == args->state_out ? after : nullptr, in))
+            return rc;
         const int group = (int)(d.heads / d.kv_heads);
         ScanArgs s{};
         s.a = side(args->q, 1);
@@ -350,16 +420,19 @@ int vkfx_linear_attention_backward(vkfx_linear_attention* plan, const vkfx_linea
             if (int rc = check_sequence("dq", args->dq, b, t, d.heads, d.key_dim, true)) return rc;
             if (int rc = check_sequence("dk", args->dk, b, t, d.kv_heads, d.key_dim, true)) return rc;
             if (int rc = check_sequence("dv", args->dv, b, t, d.kv_heads, d.value_dim, true)) return rc;
-            const void* in[4] = {args->q.data, args->k.data, args->v.data, args->dout.data};
-            const void* wr[3] = {args->dq.data, args->dk.data, args->dv.data};
-            for (int i = 0; i < 3; ++i) {
-                for (const void* p : in)
-                    if (wr[i] == p) return bad("a gradient overlaps an input");
-                if (wr[i] == wr[(i + 1) % 3]) return bad("two gradients overlap");
-            }
         }
-        if (args->dstate_in && (args->dstate_in == args->dstate_out || args->dstate_in == args->state_in))
-            return bad("dstate_in overlaps an input");
+        const uint64_t states = b * d.heads * d.key_dim * d.value_dim * 4;
+        if (int rc = check_apart({sequence_of("dq", args->dq, b, t, d.heads, d.key_dim, d.element, true),
+                                  sequence_of("dk", args->dk, b, t, d.kv_heads, d.key_dim, d.element, true),
+                                  sequence_of("dv", args->dv, b, t, d.kv_heads, d.value_dim, d.element, true),
+                                  flat("dstate_in", args->dstate_in, states, true), flat("work", d_work, plan->work.bytes, true),
+                                  flat("state_in", args->state_in, states, false),
+                                  flat("dstate_out", args->dstate_out, states, false), flat("lengths", args->lengths, b * 4, false),
+                                  sequence_of("q", args->q, b, t, d.heads, d.key_dim, d.element, false),
+                                  sequence_of("k", args->k, b, t, d.kv_heads, d.key_dim, d.element, false),
+                                  sequence_of("v", args->v, b, t, d.kv_heads, d.value_dim, d.element, false),
+                                  sequence_of("dout", args->dout, b, t, d.heads, d.value_dim, d.element, false)}))
+            return rc;
         const int group = (int)(d.heads / d.kv_heads);
         const int dk = (int)d.key_dim, dv = (int)d.value_dim;
         float* work = (float*)(d_work ? d_work : plan->work.p);
