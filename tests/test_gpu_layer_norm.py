@@ -389,3 +389,27 @@ def test_partial_overlaps_are_refused_and_interleaved_rows_are_not(hip_ctx):
     plan.backward_tensors(buf[:8, :64], w, st, buf[10:18, :64], buf[10:18, 64:], dw, db)
     plan.backward_tensors(buf[:8, :64], w, st, buf[10:18, :64], buf[10:18, :64], dw, db)
     assert torch.equal(buf[10:18, :64], buf[10:18, 64:])
+
+
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,width", [(20011, 40), (40009, 100), (9001, 512), (2500, 1001), (2100, 2049), (1100, 4100), (600, 8200), (600, 20011),
+                                        (520, 33000), (517, 70003)])
+def test_blocks_that_take_several_rows(hip_ctx, element, rows, width):
+    """More rows than the blocks that a launch has, in no multiple of them: rows read ahead, a last turn in which only
+    some of a block's groups have a row, and sums carried from row to row."""
+    _run(hip_ctx, rows, width, element)
+
+
+@pytest.mark.parametrize("element", ["f16", "bf16"])
+@pytest.mark.parametrize("width", [200, 16385, 20011, 33000])
+def test_gradients_in_place_of_their_input_in_16_bits(hip_ctx, element, width):
+    import torch
+    plan = _plan(hip_ctx, width, element)
+    x, w, dy = _normal(1, (300, width), element), _normal(2, (width,), element), _normal(3, (300, width), element)
+    y, stats = torch.empty_like(x), torch.empty(300, 2, device="cuda")
+    plan.forward_tensors(x, w, w, y, stats)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
+    plan.backward_tensors(x, w, stats, dy, dx, dw, db)
+    dw2, db2 = torch.empty_like(w), torch.empty_like(w)
+    plan.backward_tensors(x, w, stats, dy, dy, dw2, db2)
+    assert torch.equal(dx, dy) and torch.equal(dw, dw2) and torch.equal(db, db2)
