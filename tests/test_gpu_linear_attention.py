@@ -638,3 +638,11 @@ def test_partial_overlaps_are_refused_and_packed_tensors_are_not(hip_ctx):
     g(*apart, dout, *want[1:])
     assert torch.equal(wide[:, :, 0], want[0])
     assert all(torch.equal(x, y) for x, y in zip(grads.unbind(2), want[1:]))
+
+
+@pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("dk,dv", [(64, 64), (100, 130), (130, 61), (200, 256), (256, 33)])
+@pytest.mark.parametrize("t", [1, 5, 8])
+def test_few_tokens_of_many_states(hip_ctx, element, dk, dv, t):
+    """Enough states for blocks of 64 columns, whose gradients read their states transposed."""
+    _run(hip_ctx, element, 8, t, 8, 8, dk, dv, lengths=[t, 0, 1, t, t // 2, t, t - 1, t])
