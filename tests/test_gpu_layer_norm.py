@@ -413,3 +413,30 @@ def test_gradients_in_place_of_their_input_in_16_bits(hip_ctx, element, width):
     dw2, db2 = torch.empty_like(w), torch.empty_like(w)
     plan.backward_tensors(x, w, stats, dy, dy, dw2, db2)
     assert torch.equal(dx, dy) and torch.equal(dw, dw2) and torch.equal(db, db2)
+
+
+def test_a_transform_and_a_norm_are_ordered_by_default(hip_ctx):
+    """The context's stream, where transforms run by default, and torch's default stream, where norms then run, wait for
+    each other."""
+    import torch
+    n, batch = 4096, 4096
+    fft = hip_ctx.plan(vk.TransformIr.build(vk.FftConfig.new([n]).with_batch_count(batch), vk.Direction.Forward))
+    plan = _plan(hip_ctx, 2 * n, "f32")
+    x = _normal(1, (batch, 2 * n), "f32")
+
+    def run(wait):
+        a, b, c = (torch.full_like(x, float("nan")) for _ in range(3))
+        wait()
+        for _ in range(4):  # transforms take longer than the norm that reads the last one
+            fft.execute_tensors(x, a)
+        wait()
+        plan.forward_tensors(a, None, None, b)
+        wait()
+        fft.execute_tensors(b, c)
+        wait()
+        torch.cuda.synchronize()
+        return a, b, c
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(want, run(lambda: None)))

@@ -646,3 +646,46 @@ def test_partial_overlaps_are_refused_and_packed_tensors_are_not(hip_ctx):
 def test_few_tokens_of_many_states(hip_ctx, element, dk, dv, t):
     """Enough states for blocks of 64 columns, whose gradients read their states transposed."""
     _run(hip_ctx, element, 8, t, 8, 8, dk, dv, lengths=[t, 0, 1, t, t // 2, t, t - 1, t])
+
+
+@pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_bad_values_in_a_split_sequence(hip_ctx, element, value):
+    """A token of a middle segment: what comes before it, the other heads and the other sequence stay as they are; the
+    state after the last token, and backwards the gradient of the first state, do not."""
+    import torch
+    b, t, h, dk, dv, at = 2, 4200, 2, 64, 48, 2049
+    plan = _plan(hip_ctx, b, t, h, h, dk, dv, element, True, decay=[0.998, 0.99])
+    x = [_tensor(i, (b, t, h, d), element) for i, d in ((1, dk), (2, dk), (3, dv), (4, dv))]
+    s, ds = _state(5, b, h, dk, dv), _state(6, b, h, dk, dv)
+
+    def run():
+        o = [torch.full_like(x[i], 3) for i in (3, 0, 1, 2)] + [torch.empty_like(s), torch.empty_like(s)]
+        plan.forward_tensors(*x[:3], o[0], state_in=s, state_out=o[4])
+        plan.backward_tensors(*x, *o[1:4], state_in=s, dstate_out=ds, dstate_in=o[5])
+        return o
+
+    want = run()
+    assert all(torch.isfinite(o).all() for o in want)
+    for i in range(4):
+        keep = x[i].clone()
+        x[i][0, at, 0, 7] = value
+        out, dq, dk_, dv_, after, back = run()
+        x[i].copy_(keep)
+        for got, w in zip((out, dq, dk_, dv_, after, back), want):
+            assert torch.equal(got[1], w[1])
+        for got, w in zip((out, dq, dk_, dv_), want):
+            assert torch.equal(got[0, :, 1], w[0, :, 1])
+        for got, w in zip((after, back), want[4:]):
+            assert torch.equal(got[0, 1], w[0, 1])
+        assert torch.equal(out[0, :at], want[0][0, :at]) and torch.equal(dq[0, :at], want[1][0, :at])
+        if i in (0, 3):  # q and dout reach the state's gradient alone
+            assert torch.equal(dk_[0, at + 1:], want[2][0, at + 1:]) and torch.equal(dv_[0, at + 1:], want[3][0, at + 1:])
+            assert torch.equal(after, want[4]) and not torch.isfinite(back[0, 0]).all()
+        else:  # k and v reach the state alone, and the other one's gradient at their own token
+            assert torch.equal(back, want[5]) and not torch.isfinite(after[0, 0]).all()
+            same, other = ((dk_, want[2]), (dv_, want[3]))[::1 if i == 1 else -1]
+            assert torch.equal(*same)
+            rest = torch.arange(t, device="cuda") != at
+            assert torch.equal(other[0][:, rest], other[1][:, rest])
+            assert not torch.isfinite(other[0][0, at, 0]).all()
