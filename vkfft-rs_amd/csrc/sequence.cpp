@@ -122,10 +122,12 @@ Tensor sequence_of(const char* name, const vkfx_sequence& s, uint64_t batch, uin
 // `out` and `in`: the names of an output that stands in its input's place.
 template <size_t N>
 int check_apart(const Tensor (&tensors)[N], const char* out = nullptr, const char* in = nullptr) {
-    for (size_t i = 0; i < N; ++i)
-        for (size_t j = 0; j < N; ++j) {
+    uintptr_t end[N];
+    for (size_t i = 0; i < N; ++i) end[i] = tensors[i].region.run ? tensors[i].region.at + tensors[i].region.span() : 0;
+    for (size_t i = 0; i < N && tensors[i].written; ++i)  // outputs come first
+        for (size_t j = i + 1; j < N; ++j) {
             const Tensor &w = tensors[i], &t = tensors[j];
-            if (!w.written || i == j || (t.written && j < i) || (w.name == out && t.name == in)) continue;
+            if (w.region.at >= end[j] || t.region.at >= end[i] || (w.name == out && t.name == in)) continue;
             if (overlap(w.region, t.region)) return bad(std::string(w.name) + " overlaps " + t.name);
         }
     return VKFX_OK;
