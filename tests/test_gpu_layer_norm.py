@@ -440,3 +440,22 @@ def test_a_transform_and_a_norm_are_ordered_by_default(hip_ctx):
     want = run(torch.cuda.synchronize)
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(want, run(lambda: None)))
+
+
+@pytest.mark.parametrize("element,rows,width", [("f32", 262147, 2100), ("bf16", 1 << 24, 16), ("bf16", 1 << 22, 1001), ("f16", 1 << 19, 5000),
+                                                ("bf16", 65537, 20000), ("f32", 65537, 16385)])
+def test_sums_over_many_rows_of_one_value(hip_ctx, element, rows, width):
+    """The gradient of a mean is the same in every row: weight and bias gradients add equal numbers, which round to one
+    side where they are added one by one."""
+    import torch
+    plan = _plan(hip_ctx, width, element, "f32")
+    x, dy = _normal(1, (1, width), element), torch.full((1, width), 0.1, device="cuda", dtype=_types()[element])
+    xn, dyn = _np(x, dy)
+    st = ref.norm(xn, 1.0, 0.0, 1e-5)[1].astype(np.float32)
+    stats = torch.from_numpy(st).cuda().expand(rows, 2).contiguous()
+    dw, db = torch.empty(width, device="cuda"), torch.empty(width, device="cuda")
+    plan.backward_tensors(x.expand(rows, width), None, stats, dy.expand(rows, width), None, dw, db)
+    one, sn = np.ones(width), st.astype(np.float64)
+    wants, totals = ref.norm_gradients(xn, one, sn, dyn), ref.norm_gradients_bound(xn, one, sn, dyn)
+    for name, got, i in (("dw", dw, 1), ("db", db, 2)):
+        ref.check(name, got, rows * wants[i], rows * totals[i], "f32", ref.NORM_TERM)

@@ -22,6 +22,7 @@ struct NormArgs {
     void* dbias;
     float* partial;  // backward: [blocks][2][width] sums of a block's rows, norm_workspace_bytes
     long long rows, x_stride, dy_stride, y_stride;
+    int parts;  // backward: rows of sums
     int width;
     int element, weight_element;  // vkfx_element
     float epsilon;
