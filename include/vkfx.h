@@ -359,10 +359,13 @@ int vkfx_execute_chain_host(vkfx_plan *const *plans, uint32_t count, const void 
  * allocate nor synchronise nor copy from the host, so a HIP graph can capture
  * them. Outputs share no memory with inputs or each other, except in place where
  * that is said; it is refused where it shows without going through the elements
- * (a tensor without gaps, or two views of one layout). A plan's own workspace serves one call at a time: calls of one plan
- * that overlap on the GPU pass d_work each. */
+ * (a tensor without gaps, or two views of one layout). A plan's own workspace
+ * serves one call at a time: calls of one plan that overlap on the GPU pass
+ * d_work each. */
 
-/* Type of the tensors' elements. Sums, statistics and states are 32 bits. */
+/* Type of the tensors' elements. Sums, statistics and states are 32 bits. On
+ * their way into an output of 16 bits, scores and states count with their first
+ * 16 bits; into a state or an output of 32 bits with all of theirs. */
 enum vkfx_element { VKFX_ELEMENT_F32 = 0, VKFX_ELEMENT_F16 = 1, VKFX_ELEMENT_BF16 = 2 };
 
 /* Layer norm of rows of `width` elements:
@@ -378,7 +381,8 @@ typedef struct vkfx_layer_norm vkfx_layer_norm;
 int vkfx_layer_norm_create(vkfx_context *ctx, const vkfx_layer_norm_desc *desc, vkfx_layer_norm **out);
 int vkfx_layer_norm_destroy(vkfx_layer_norm *plan);
 /* Bytes of the scratch a caller may pass to vkfx_layer_norm_backward, for any
- * number of rows. */
+ * number of rows: with 256 CUs 2 KB an element of a row up to widths of 16384,
+ * up to 34 MB to 2^22, then 8 bytes an element. A plan holds as much itself. */
 int vkfx_layer_norm_workspace_bytes(const vkfx_layer_norm *plan, uint64_t *out);
 /* `rows` rows, each `*_row_stride` elements after the one before (at least the
  * width; x and dy may be broadcast with stride 0). weight and bias may be NULL
@@ -433,8 +437,10 @@ int vkfx_linear_attention_workspace_bytes(const vkfx_linear_attention *plan, uin
  * written once), as many as a prompt has, or 0. lengths: [batch] or NULL; rows
  * of sequence b from lengths[b] on (clamped to 0 .. tokens) are not read, give
  * zeros and leave its state alone. state_in (NULL: zeros) and state_out (NULL:
- * not wanted), [batch][heads][key_dim][value_dim] floats, may be one buffer;
- * out overlaps no input. */
+ * not wanted), [batch][heads][key_dim][value_dim] floats, may be one buffer.
+ * What is not finite reaches its own token and later ones of its head only; a
+ * result that is infinite by the formulas may be a NaN where there are more than
+ * 8 tokens. */
 typedef struct {
     uint64_t batch;
     uint64_t tokens;

@@ -244,15 +244,15 @@ const FixedKernel* fixed_variant(const FixedKernel* f, bool nti, bool nto);
 // null if there is none.
 const FixedKernel* kind_variant(const FixedKernel* f, KernelKind kind);
 
+// Lets a kernel ask for `bytes` of dynamic LDS on the current device (asked of the runtime once).
+int raise_lds_limit(const void* fn, size_t bytes);
+
 // Launches one kernel. prec: 0 = f32, 1 = f64. dir: -1 forward, +1 inverse
 // (direction of the first FFT the kernel runs). fixed: the fixed-shape
 // instantiation to run, or nullptr for the runtime-shape kernel. t_begin /
 // t_end: when both are set, HIP events bound to this dispatch
 // (hipExtLaunchKernel) that read the kernel's own begin and end. Returns a
 // hipError_t value.
-// Lets a kernel ask for `bytes` of dynamic LDS on the current device (asked of the runtime once).
-int raise_lds_limit(const void* fn, size_t bytes);
-
 int launch(KernelKind kind, int prec, int dir, const KArgs& a, unsigned grid, unsigned block,
            size_t lds_bytes, hipStream_t stream, const FixedKernel* fixed = nullptr, hipEvent_t t_begin = nullptr,
            hipEvent_t t_end = nullptr);

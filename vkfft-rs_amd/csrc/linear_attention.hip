@@ -112,14 +112,16 @@ const ChunkKernel* chunk_kernel(int element, int dk, int dv, bool gradient) {
 }
 
 // Blocks of a kernel that the GPU holds at a time: two waves on each SIMD, as
-// far as the LDS goes.
+// far as the LDS goes. That is what the outputs' kernels have; the states' ones
+// would fit three to five by their registers and are counted as two as well.
 long long resident(const ChunkKernel* k, size_t lds, int cus) {
     return (long long)cus * std::max(1, std::min(8 / (k->threads / 64), (int)(160 * 1024 / lds)));
 }
 
 // Most states that a call keeps between segments: with a block for each there
-// are four a CU, twice what is resident (16 heads of 64 over 65536 tokens, 64
-// segments: 166 us; 267 with 32).
+// are four a CU, which is what a CU holds of blocks of two waves (16 heads of 64
+// over 65536 tokens, 64 segments: 165 us; 264 with 32) and twice what it holds of
+// blocks of four.
 constexpr long long kStates = 1024;
 
 // Blocks along x: their threads have to stay under 2^32 (a launch of more starts the remainder only).
@@ -148,11 +150,17 @@ struct Part {
 // share of the state, at about 0.4 of the cost. The time of k segments is that
 // of the rounds of resident blocks, each 1/k of the tokens long at 3 us a chunk,
 // and of the states' bytes, written, joined and read at 4 TB/s. (bf16, 4 x 4096
-// tokens, 16 heads of 128, backward, 192 blocks: 308 us with the 5 segments that
-// this gives, two rounds; 397 with 1, 358 with 2, 335 with 8. 8 x 2048 forward:
-// 124 with its 4, 205 with 1, 156 with 2, 164 with 8. 32 x 1024, whole: 165, 232
+// tokens, 16 heads of 128, backward, 192 blocks: 309 us with the 5 segments that
+// this gives, two rounds; 397 with 1, 355 with 2, 337 with 8. 8 x 2048 forward:
+// 128 with its 4, 203 with 1, 155 with 2, 169 with 8. 32 x 1024, whole: 165, 232
 // with 2.) A segment has two chunks or more (f32, 3 x 1001 tokens, 12 heads of
-// 80 x 96: 54 us with the three that this gives, 63 with four).
+// 80 x 96: 55 us with the 11 segments that this gives, 81 with 4). The join's
+// steps from segment to segment are not counted: one head of 64 over 65536 tokens
+// gets 683 segments and takes 95 us, with 256 it would take 65.
+//
+// Times in this file and in linear_chunk.hpp are of calls on the same inputs one
+// after the other, part of which the Infinity Cache keeps; on new inputs the same
+// calls take up to 6% longer.
 long long split_tokens(const Part* parts, int count, long long states, int size, long long tokens, int cus) {
     const long long most = std::max(1ll, std::min(tokens / (2 * kChunk), kStates / states));
     const double whole = 3.0 * (double)std::max(1ll, tokens / kChunk), state = 16.0 * (double)states * size / 4e6 / whole;
@@ -225,8 +233,8 @@ int launch_chunks(int element, const ScanArgs* scans, int count, const float* po
         if (int e = launch_with(parts[p].k->state_only, parts[p].state * segments, parts[p].k->threads, parts[p].k->state_lds, a, st))
             return e;
         // Few segments come with many states and are joined four elements a thread, many segments with few states one
-        // element a thread (bf16 prompts: 8 x 2048 tokens of 16 heads of 128, 4 segments, 124 us, 133 the other way;
-        // 1 x 16384 of 4 heads of 64, 64 segments, 52 and 72; 16 segments the same either way)
+        // element a thread (bf16 prompts: 8 x 2048 tokens of 16 heads of 128, 4 segments, 128 us, 137 the other way;
+        // 1 x 16384 of 4 heads of 64, 171 segments, 50 and 77)
         if (segments > 2)
             if (int e = segments <= 8 ? launch_join<4, 4>(a, st) : launch_join<1, 16>(a, st)) return e;
     }

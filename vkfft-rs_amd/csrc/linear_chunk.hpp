@@ -784,7 +784,7 @@ ChunkKernel chunk_kernel_of() {
 // much to do between them: operands of two or three parts, 96 keys or the scans
 // of a gradient (16 heads of 64 x 64, with 16 columns and with 32: f16 86 us and
 // 119, f32 109 and 188, bf16 gradients 133 and 153; 96 x 64 bf16 79 and 114), nor
-// where a state of more than 96 rows, for f32 128, takes the registers. Two parts
+// where a state of more than 128 rows, for f32 96, takes the registers. Two parts
 // and 32 keys run as fast either way (73 and 76); bf16 forward is slower with 16
 // columns where the sequence is long (1 x 65536, 64 x 64: 182 and 170).
 template <typename T>
