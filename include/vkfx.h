@@ -440,7 +440,7 @@ int vkfx_linear_attention_workspace_bytes(const vkfx_linear_attention *plan, uin
  * not wanted), [batch][heads][key_dim][value_dim] floats, may be one buffer.
  * What is not finite reaches its own token and later ones of its head only; a
  * result that is infinite by the formulas may be a NaN where there are more than
- * 8 tokens. */
+ * 8 tokens, and f32 inputs past 3.396e38 may count as infinite there. */
 typedef struct {
     uint64_t batch;
     uint64_t tokens;

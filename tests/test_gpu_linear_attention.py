@@ -689,3 +689,38 @@ def test_bad_values_in_a_split_sequence(hip_ctx, element, value):
             rest = torch.arange(t, device="cuda") != at
             assert torch.equal(other[0][:, rest], other[1][:, rest])
             assert not torch.isfinite(other[0][0, at, 0]).all()
+
+
+@pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 100), (5, 6)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_the_largest_numbers_do_not_reach_the_tokens_before(hip_ctx, element, dk, dv, sign):
+    """The type's largest and lowest numbers in a token: not infinite, but near enough that a rounding makes them so."""
+    import torch
+    t, at = 100, 43
+    plan = _plan(hip_ctx, 1, t, 2, 2, dk, dv, element, True)
+    x = [_tensor(i, (1, t, 2, d), element) for i, d in ((1, dk), (2, dk), (3, dv), (4, dv))]
+    value = sign * torch.finfo(x[0].dtype).max
+
+    def run():
+        o = [torch.full_like(x[i], 3) for i in (3, 0, 1, 2)]
+        plan.forward_tensors(*x[:3], o[0])
+        plan.backward_tensors(*x, *o[1:])
+        return o
+
+    want = run()
+    for i in range(4):
+        keep = x[i].clone()
+        x[i][0, at, 0, 0] = value
+        out, dq, dk_, dv_ = run()
+        x[i].copy_(keep)
+        for got, w in zip((out, dq, dk_, dv_), want):
+            assert torch.equal(got[:, :, 1], w[:, :, 1])
+        assert torch.equal(out[:, :at], want[0][:, :at]) and torch.equal(dq[:, :at], want[1][:, :at])
+        if i in (0, 3):
+            assert torch.equal(dk_[:, at + 1:], want[2][:, at + 1:]) and torch.equal(dv_[:, at + 1:], want[3][:, at + 1:])
+        else:
+            same, other = ((dk_, want[2]), (dv_, want[3]))[::1 if i == 1 else -1]
+            assert torch.equal(*same)
+            rest = torch.arange(t, device="cuda") != at
+            assert torch.equal(other[0][:, rest], other[1][:, rest])

@@ -178,10 +178,15 @@ struct PackedEight {
     typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
-// s, or a NaN where an element is infinite or a NaN.
+// Zero, or a NaN where x or its rounding to bf16 is infinite or a NaN. In units
+// of 2^120 bf16's largest number is 255, what rounds past it begins at 255.5, and
+// kPast leads that, but not 255, past the end of 32 bits at 256.
+constexpr float kPast = 1.003f;
+__device__ __forceinline__ float times_zero(float x) { return x * kPast * 0.f; }
+// s, or a NaN where an element is such a one.
 __device__ __forceinline__ float times_zero(const Eight<float>& x, float s) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(x[e], 0.f, s);
+    for (int e = 0; e < 8; ++e) s = fmaf(x[e] * kPast, 0.f, s);
     return s;
 }
 __device__ __forceinline__ float times_zero(const Eight<_Float16>& x, float s) {
@@ -261,7 +266,7 @@ struct Staged {
         for (int u = 0; u < kEach; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if ((float)r[u][e] * 0.f != 0.f) r[u][e] = (T)0.f;
+                if (times_zero((float)r[u][e]) != 0.f) r[u][e] = (T)0.f;
     }
 
     // The chunk that was asked for to lds[part][C][pitch], rows from `left` on as zeros; then on to the next.
@@ -282,7 +287,7 @@ struct Staged {
             for (int j = (int)threadIdx.x; j < C * D; j += THREADS) {
                 const int i = j / D, c = j % D;
                 float f = i < left && c < width ? (float)((const T*)(next + i * token))[c] : 0.f;
-                if (bad && f * 0.f != 0.f) *bad = 1, f = 0.f;
+                if (bad && times_zero(f) != 0.f) *bad = 1, f = 0.f;
 #pragma unroll
                 for (int k = 0; k < Parts<T>::in; ++k) {
                     const __bf16 v = (__bf16)f;
@@ -684,7 +689,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const float c = room > 16 * t + r ? (float)row[out_col + 16 * t + r] : 0.f;
-                            if (c * 0.f == 0.f) continue;
+                            if (times_zero(c) == 0.f) continue;
 #pragma unroll
                             for (int I = 0; I < TI; ++I) {
                                 float p = 0.f;
@@ -694,7 +699,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<T, DK, WAVES, NT, C, STATE_
                             }
                         }
                         const float c = col + 16 * t < s.dv ? (float)row[col + 16 * t] : 0.f;
-                        if (c * 0.f == 0.f) continue;
+                        if (times_zero(c) == 0.f) continue;
 #pragma unroll
                         for (int a = 0; a < DK / 16; ++a)
 #pragma unroll
