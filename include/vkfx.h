@@ -473,6 +473,148 @@ typedef struct {
 int vkfx_linear_attention_backward(vkfx_linear_attention *plan, const vkfx_linear_attention_backward_args *args,
                                    void *d_work, void *stream);
 
+/* Rotary positions of queries and keys, with a norm of each head in front
+ * where it is wanted. A head is a row x of head_dim elements, at position p of
+ * its sequence:
+ *   norm:  u = x rstd weight, rstd = 1 / sqrt(mean(x^2) + epsilon); without, u = x
+ *   pair i < rotary_dim / 2 of u turns by p frequencies[i]:
+ *     y1 = amplitude (u1 cos - u2 sin),  y2 = amplitude (u1 sin + u2 cos)
+ *   elements from rotary_dim on are u.
+ * Angles are right to 2^-31 of a turn at every 32-bit position. */
+enum vkfx_rotary_layout {
+    VKFX_ROTARY_INTERLEAVED = 0, /* pair i: elements 2 i and 2 i + 1 */
+    VKFX_ROTARY_HALF = 1         /* elements i and i + rotary_dim / 2 */
+};
+typedef struct {
+    uint32_t heads;         /* of q: 1 .. 65535 */
+    uint32_t kv_heads;      /* of k: 0 (none) .. 65535 */
+    uint32_t head_dim;      /* 1 .. 256 */
+    uint32_t rotary_dim;    /* even, 0 .. head_dim */
+    int32_t layout;         /* vkfx_rotary_layout */
+    int32_t element;        /* vkfx_element of q, k, their results and gradients */
+    int32_t weight_element; /* vkfx_element of the weights and their gradients: element or F32 */
+    int32_t norm;           /* 1: with the norm */
+    double epsilon;         /* with the norm: 2^-126 .. the largest float */
+    double amplitude;       /* finite in 32 bits */
+    const double *frequencies; /* [rotary_dim / 2] radians a position, at most a turn (2 pi) either way; copied */
+} vkfx_rotary_desc;
+typedef struct vkfx_rotary vkfx_rotary;
+
+int vkfx_rotary_create(vkfx_context *ctx, const vkfx_rotary_desc *desc, vkfx_rotary **out);
+int vkfx_rotary_destroy(vkfx_rotary *plan);
+/* Bytes of the scratch a caller may pass to vkfx_rotary_backward, for any
+ * number of tokens (0 without the norm). */
+int vkfx_rotary_workspace_bytes(const vkfx_rotary *plan, uint64_t *out);
+
+/* Up to 2^31 - 1 tokens in all (batch times tokens). A token's position is
+ * positions[b][t], else starts[b] + t, else t; only one of the two may be
+ * given. lengths: [batch] or NULL; rows of sequence b from lengths[b] on
+ * (clamped to 0 .. tokens) are not read and give zeros. q or k whose data is NULL
+ * are left out (then their result is not written). q_out may be q, and k_out k, with
+ * the same strides. */
+typedef struct {
+    uint64_t batch;
+    uint64_t tokens;
+    vkfx_sequence q;     /* [batch][tokens][heads][head_dim] */
+    vkfx_sequence k;     /* [batch][tokens][kv_heads][head_dim] */
+    vkfx_sequence q_out; /* written, as k_out */
+    vkfx_sequence k_out;
+    const void *q_weight; /* [head_dim], with the norm; NULL: 1 */
+    const void *k_weight;
+    const int32_t *positions;
+    const int32_t *starts;
+    const int32_t *lengths;
+} vkfx_rotary_forward_args;
+int vkfx_rotary_forward(vkfx_rotary *plan, const vkfx_rotary_forward_args *args, void *stream);
+
+/* Gradients dq, dk for dq_out, dk_out; with the norm also of its weights, summed
+ * over all tokens and heads in a fixed order, where wanted (not NULL). q and k are the
+ * forward call's inputs, which only the norm needs. dq may be dq_out and dk dk_out, with
+ * the same strides. dq_out or dk_out whose data is NULL are left out; a weight's
+ * gradient then is zeros. */
+typedef struct {
+    uint64_t batch;
+    uint64_t tokens;
+    vkfx_sequence dq_out, dk_out, q, k;
+    vkfx_sequence dq, dk; /* written */
+    const void *q_weight, *k_weight;
+    void *dq_weight, *dk_weight;
+    const int32_t *positions;
+    const int32_t *starts;
+    const int32_t *lengths;
+} vkfx_rotary_backward_args;
+int vkfx_rotary_backward(vkfx_rotary *plan, const vkfx_rotary_backward_args *args, void *d_work, void *stream);
+
+/* Gated recurrence: every channel of a sequence has a state of its own, which a
+ * gate from the data lets decay,
+ *   a = sigmoid(gate) or exp(min(gate, 0)),  m = 1 - a (complement) or 1
+ *   h[t] = a[t] h[t-1] + m[t] x[t],  y[t] = h[t]. */
+enum vkfx_gate { VKFX_GATE_SIGMOID = 0, VKFX_GATE_EXP = 1 };
+typedef struct {
+    uint64_t channels;  /* 1 .. 2^30 */
+    int32_t element;    /* vkfx_element of x, gate, y and their gradients */
+    int32_t gate;       /* vkfx_gate */
+    int32_t complement; /* 1: m = 1 - a */
+    int32_t reserved;   /* 0 */
+} vkfx_gated_recurrence_desc;
+typedef struct vkfx_gated_recurrence vkfx_gated_recurrence;
+
+/* A [batch][token][channel] tensor: element strides of the first two; the last
+ * is contiguous. Inputs may be broadcast (stride 0), outputs may not overlap
+ * themselves. */
+typedef struct {
+    const void *data;
+    int64_t batch_stride;
+    int64_t token_stride;
+} vkfx_channels;
+
+int vkfx_gated_recurrence_create(vkfx_context *ctx, const vkfx_gated_recurrence_desc *desc,
+                                 vkfx_gated_recurrence **out);
+int vkfx_gated_recurrence_destroy(vkfx_gated_recurrence *plan);
+/* Bytes of the scratch a caller may pass, for any number of sequences and tokens. */
+int vkfx_gated_recurrence_workspace_bytes(const vkfx_gated_recurrence *plan, uint64_t *out);
+
+/* saved (NULL: not wanted), for the backward pass: the states before tokens 0, 16,
+ * 32, ..., [batch][(tokens + 15) / 16][channels] floats. */
+#define VKFX_RECURRENCE_SPAN 16
+
+/* `tokens` may be 1 (the next token of each sequence), as many as a prompt has,
+ * or 0; up to 65535 sequences and 2^31 - 65536 tokens. lengths: [batch] or NULL; rows
+ * of sequence b from lengths[b] on (clamped to 0 .. tokens) are not read, give zeros and
+ * leave its state alone. state_in (NULL: zeros) and state_out (NULL: not wanted),
+ * [batch][channels] floats, may be one buffer; y may be x with the same strides.
+ * What is not finite reaches its own token and later ones of its channel only; a
+ * result that is infinite by the formulas may be a NaN. */
+typedef struct {
+    uint64_t batch;
+    uint64_t tokens;
+    vkfx_channels x, gate;
+    vkfx_channels y; /* written */
+    const int32_t *lengths;
+    const float *state_in;
+    float *state_out;
+    float *saved;
+} vkfx_gated_recurrence_forward_args;
+int vkfx_gated_recurrence_forward(vkfx_gated_recurrence *plan, const vkfx_gated_recurrence_forward_args *args,
+                                  void *d_work, void *stream);
+
+/* Gradients of x, gate and of state_in for dy and dstate_out (NULL: zeros), with
+ * the forward call's inputs and its saved states. Rows past a sequence's length
+ * get zeros. dstate_in may be NULL (not wanted) or dstate_out; dx may be dy with the
+ * same strides. A gate past the clamp of the exponential form has no gradient. */
+typedef struct {
+    uint64_t batch;
+    uint64_t tokens;
+    vkfx_channels x, gate, dy;
+    vkfx_channels dx, dgate; /* written */
+    const int32_t *lengths;
+    const float *saved;
+    const float *dstate_out;
+    float *dstate_in;
+} vkfx_gated_recurrence_backward_args;
+int vkfx_gated_recurrence_backward(vkfx_gated_recurrence *plan, const vkfx_gated_recurrence_backward_args *args,
+                                   void *d_work, void *stream);
+
 /* Thread-local message of the last failing call on this thread. */
 const char *vkfx_last_error(void);
 

@@ -12,53 +12,15 @@
 // over the rows. The lane that holds a column in one row holds it in the
 // block's every row, so the sums over rows stay in registers; each block then
 // writes one row of sums and a second launch adds those in their order.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
-#include <hip/hip_runtime.h>
-
 #include <algorithm>
 
 #include "sequence.hpp"
+#include "sequence_device.hpp"
 #include "vkfx.h"
 
 namespace vkfx {
 
 namespace {
-
-template <typename T, int N>
-using Some = T __attribute__((ext_vector_type(N)));
-// The same in memory, at any alignment of its elements.
-template <typename T, int N>
-struct Packed {
-    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-};
-
-template <typename T>
-constexpr int kVector = 16 / (int)sizeof(T);
-
-// Elements c .. c + N - 1 of a row of `width`, zeros past its end.
-template <typename T, int N>
-__device__ __forceinline__ Some<T, N> load_some(const T* row, int c, int width) {
-    Some<T, N> r;
-    if (c + N <= width) {
-        r = *(const typename Packed<T, N>::type*)(row + c);
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) r[e] = c + e < width ? row[c + e] : (T)0.f;
-    }
-    return r;
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void store_some(T* row, int c, int width, const Some<T, N>& r) {
-    if (c + N <= width) {
-        *(typename Packed<T, N>::type*)(row + c) = r;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-        if (c + e < width) row[c + e] = r[e];
-}
 
 // Makes the compiler take `r` for new: where it is used again it is converted
 // once more, rather than kept in 32 bits from the first time.

@@ -1,5 +1,6 @@
 // sequence.hpp -- launch interface of the sequence operators' kernels
-// (layer_norm.hip, linear_attention.hip), used by sequence.cpp.
+// (layer_norm.hip, linear_attention.hip, rotary.hip, recurrence.hip), used by
+// sequence.cpp, rotary_plan.cpp and recurrence_plan.cpp.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -91,5 +92,63 @@ struct GroupSum {
 };
 int launch_group_sum(int element, const GroupSum& a, const GroupSum& b, long long batch, long long tokens, int kv_heads,
                      int group, hipStream_t s);
+
+// ----------------------------------------------------------------- rotary
+
+struct RotarySide {
+    const void* p;
+    long long batch, token, head;  // element strides
+};
+// Queries or keys. No heads: left out.
+struct RotaryRows {
+    RotarySide x;   // backward: dy
+    RotarySide in;  // backward with the norm: the forward pass's input
+    RotarySide out;
+    const void* weight;  // null: 1
+    void* dweight;       // null: not wanted
+    int heads;
+};
+struct RotaryArgs {
+    RotaryRows rows[2];
+    const uint64_t* turns;  // [turned / 2] 2^-64 turns a position
+    const int *positions, *starts, *lengths;  // null: none
+    float* partial;  // rotary_workspace_bytes
+    long long tokens, all;  // of a sequence, of the batch
+    int dim, turned, layout;
+    int element, weight_element;
+    int norm;
+    float epsilon, amplitude;
+    int cus;
+};
+int launch_rotary_forward(const RotaryArgs& a, hipStream_t s);
+int launch_rotary_backward(const RotaryArgs& a, hipStream_t s);
+size_t rotary_workspace_bytes(int dim, int cus);
+
+// ------------------------------------------------------- gated recurrence
+
+constexpr int kSpan = 16;  // tokens between saved states
+
+struct RecurrenceSide {
+    const void* p;
+    long long batch, token;  // element strides
+};
+struct RecurrenceArgs {
+    RecurrenceSide x, gate;
+    RecurrenceSide dy;      // backward
+    RecurrenceSide y;       // backward: dx
+    RecurrenceSide dgate;   // backward
+    const int* lengths;     // null: tokens
+    const float* state_in;  // null: zeros; backward: dstate_out
+    float* state_out;       // null: not wanted; backward: dstate_in
+    float* saved;           // null: not wanted; backward: read
+    float* work;            // recurrence_workspace_bytes
+    long long tokens, channels;
+    int batch;
+    int element, gate_kind, complement;
+    int cus;
+};
+int launch_recurrence_forward(const RecurrenceArgs& a, hipStream_t s);
+int launch_recurrence_backward(const RecurrenceArgs& a, hipStream_t s);
+size_t recurrence_workspace_bytes(int element, long long channels, int cus);
 
 }  // namespace vkfx

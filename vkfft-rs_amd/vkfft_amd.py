@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import enum
 import json
+import math
 import os
 import weakref
 from dataclasses import dataclass, field
@@ -242,6 +243,58 @@ class _BackwardArgs(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("lengths", "state_in", "dstate_out", "dstate_in")])
 
 
+class _RotaryDesc(ctypes.Structure):
+    _fields_ = [
+        ("heads", ctypes.c_uint32),
+        ("kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("rotary_dim", ctypes.c_uint32),
+        ("layout", ctypes.c_int32),
+        ("element", ctypes.c_int32),
+        ("weight_element", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("epsilon", ctypes.c_double),
+        ("amplitude", ctypes.c_double),
+        ("frequencies", ctypes.POINTER(ctypes.c_double)),
+    ]
+
+
+class _RotaryForwardArgs(ctypes.Structure):
+    _fields_ = ([("batch", ctypes.c_uint64), ("tokens", ctypes.c_uint64)] + _sequence_fields(["q", "k", "q_out", "k_out"])
+                + [(n, ctypes.c_void_p) for n in ("q_weight", "k_weight", "positions", "starts", "lengths")])
+
+
+class _RotaryBackwardArgs(ctypes.Structure):
+    _fields_ = ([("batch", ctypes.c_uint64), ("tokens", ctypes.c_uint64)]
+                + _sequence_fields(["dq_out", "dk_out", "q", "k", "dq", "dk"])
+                + [(n, ctypes.c_void_p) for n in ("q_weight", "k_weight", "dq_weight", "dk_weight", "positions", "starts", "lengths")])
+
+
+class _GatedRecurrenceDesc(ctypes.Structure):
+    _fields_ = [
+        ("channels", ctypes.c_uint64),
+        ("element", ctypes.c_int32),
+        ("gate", ctypes.c_int32),
+        ("complement", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+def _channels_fields(names):
+    """The three fields of a vkfx_channels for each name, in line."""
+    return [(n + f, t) for n in names for f, t in (("", ctypes.c_void_p), ("_batch", ctypes.c_int64), ("_token", ctypes.c_int64))]
+
+
+class _RecurrenceForwardArgs(ctypes.Structure):
+    _fields_ = ([("batch", ctypes.c_uint64), ("tokens", ctypes.c_uint64)] + _channels_fields(["x", "gate", "y"])
+                + [(n, ctypes.c_void_p) for n in ("lengths", "state_in", "state_out", "saved")])
+
+
+class _RecurrenceBackwardArgs(ctypes.Structure):
+    _fields_ = ([("batch", ctypes.c_uint64), ("tokens", ctypes.c_uint64)] + _channels_fields(["x", "gate", "dy", "dx", "dgate"])
+                + [(n, ctypes.c_void_p) for n in ("lengths", "saved", "dstate_out", "dstate_in")])
+
+
 def lib(path: Optional[str] = None):
     """Loads libvkfft_mi355x.so (or the library at `path`, e.g. the index-map
     test build INDEX_LIB_PATH); raises if it has not been built."""
@@ -295,6 +348,16 @@ def lib(path: Optional[str] = None):
         L.vkfx_linear_attention_workspace_bytes.argtypes = [vp, ctypes.POINTER(u64)]
         L.vkfx_linear_attention_forward.argtypes = [vp, ctypes.POINTER(_ForwardArgs), vp, vp]
         L.vkfx_linear_attention_backward.argtypes = [vp, ctypes.POINTER(_BackwardArgs), vp, vp]
+        L.vkfx_rotary_create.argtypes = [vp, ctypes.POINTER(_RotaryDesc), ctypes.POINTER(vp)]
+        L.vkfx_rotary_destroy.argtypes = [vp]
+        L.vkfx_rotary_workspace_bytes.argtypes = [vp, ctypes.POINTER(u64)]
+        L.vkfx_rotary_forward.argtypes = [vp, ctypes.POINTER(_RotaryForwardArgs), vp]
+        L.vkfx_rotary_backward.argtypes = [vp, ctypes.POINTER(_RotaryBackwardArgs), vp, vp]
+        L.vkfx_gated_recurrence_create.argtypes = [vp, ctypes.POINTER(_GatedRecurrenceDesc), ctypes.POINTER(vp)]
+        L.vkfx_gated_recurrence_destroy.argtypes = [vp]
+        L.vkfx_gated_recurrence_workspace_bytes.argtypes = [vp, ctypes.POINTER(u64)]
+        L.vkfx_gated_recurrence_forward.argtypes = [vp, ctypes.POINTER(_RecurrenceForwardArgs), vp, vp]
+        L.vkfx_gated_recurrence_backward.argtypes = [vp, ctypes.POINTER(_RecurrenceBackwardArgs), vp, vp]
         L.vkfx_execute_chain.argtypes = [ctypes.POINTER(vp), ctypes.c_uint32, vp, vp, vp]
         L.vkfx_execute_chain_host.argtypes = [ctypes.POINTER(vp), ctypes.c_uint32, vp, u64, vp, u64]
         _libs[path] = L
@@ -1410,7 +1473,7 @@ class LayerNormConfig:
 
 
 class _SequencePlan:
-    """What both operators' plans share: the handle and the checks of tensors."""
+    """What the operators' plans share: the handle and the checks of tensors."""
     _kind = ""
 
     def __init__(self, ctx: "HipExecutionContext", config, desc):
@@ -1472,6 +1535,20 @@ class _SequencePlan:
         if getattr(x, "shape", None) != shape or x.dtype is not dtype or x.get_device() != device or not x.is_contiguous():
             self._refuse(name, x, shape, dtype, device)
         return x.data_ptr()
+
+    def _sequence(self, name, x, shape, device):
+        if getattr(x, "shape", None) != shape or x.dtype is not self._type or x.get_device() != device:
+            self._refuse(name, x, shape, self._type, device)
+        b, t, h, d = x.stride()
+        if d != 1 and shape[3] > 1:
+            raise VkFftError(-7, f"{name}: the last dimension must be contiguous")
+        return x.data_ptr(), b, t, h
+
+    def _lengths(self, lengths, batch, device):
+        if lengths is None:
+            return None
+        import torch
+        return self._dense("lengths", lengths, (batch,), torch.int32, device)
 
     def _work(self, work, device):
         if work is None:
@@ -1611,20 +1688,6 @@ class LinearAttentionPlan(_SequencePlan):
         kv = config.heads if config.kv_heads is None else config.kv_heads
         self._dims = config.heads, kv, config.key_dim, config.value_dim
 
-    def _sequence(self, name, x, shape, device):
-        if getattr(x, "shape", None) != shape or x.dtype is not self._type or x.get_device() != device:
-            self._refuse(name, x, shape, self._type, device)
-        b, t, h, d = x.stride()
-        if d != 1 and shape[3] > 1:
-            raise VkFftError(-7, f"{name}: the last dimension must be contiguous")
-        return x.data_ptr(), b, t, h
-
-    def _lengths(self, lengths, batch, device):
-        if lengths is None:
-            return None
-        import torch
-        return self._dense("lengths", lengths, (batch,), torch.int32, device)
-
     def forward_tensors(self, q, k, v, out, state_in=None, state_out=None, lengths=None, work=None, stream=None):
         """Outputs of a prompt, or of the next token where there is one: from
         state_in (None: zeros) to state_out (None: not wanted; may be state_in)."""
@@ -1657,6 +1720,297 @@ class LinearAttentionPlan(_SequencePlan):
                              self._dense("dstate_out", dstate_out, state, self._f32, device),
                              self._dense("dstate_in", dstate_in, state, self._f32, device))
         _check(self._L.vkfx_linear_attention_backward(self.handle, ctypes.byref(args), self._work(work, device),
+                                                      self._stream(stream, device)), self._L)
+
+
+class RotaryLayout(enum.IntEnum):
+    """Which elements of a head form its pair i."""
+    Interleaved = 0  # 2 i and 2 i + 1
+    Half = 1  # i and i + rotary_dim / 2
+
+
+@dataclass
+class RotaryConfig:
+    """Rotary positions of queries and keys, with a norm of each head in front where it is wanted: the first rotary_dim
+    elements of a head form pairs, and pair i at position p turns by p frequencies[i],
+    (u1, u2) -> amplitude (u1 cos - u2 sin, u1 sin + u2 cos). With the norm, u = x / sqrt(mean(x^2) + epsilon) weight."""
+    heads: int
+    head_dim: int
+    kv_heads: Optional[int] = None  # default: heads; 0: queries alone
+    rotary_dim: Optional[int] = None  # default: head_dim
+    layout: RotaryLayout = RotaryLayout.Half
+    element: Element = Element.F32
+    weight_element: Optional[Element] = None  # of the norm's weights: the heads', or F32
+    epsilon: Optional[float] = None  # None: no norm
+    amplitude: float = 1.0
+    base: float = 10000.0
+    frequencies: Optional[List[float]] = None  # default: base^(-2 i / rotary_dim), scaled
+    scaling: Optional[Tuple] = None
+
+    @staticmethod
+    def new(heads: int, head_dim: int) -> "RotaryConfig":
+        return RotaryConfig(int(heads), int(head_dim))
+
+    def with_kv_heads(self, kv_heads: int) -> "RotaryConfig":
+        self.kv_heads = int(kv_heads)
+        return self
+
+    def with_rotary_dim(self, rotary_dim: int) -> "RotaryConfig":
+        """An even part of the head; the rest does not turn."""
+        self.rotary_dim = int(rotary_dim)
+        return self
+
+    def with_layout(self, layout: RotaryLayout) -> "RotaryConfig":
+        self.layout = RotaryLayout(layout)
+        return self
+
+    def with_element(self, element: Element) -> "RotaryConfig":
+        self.element = Element(element)
+        return self
+
+    def with_weight_element(self, element: Element) -> "RotaryConfig":
+        self.weight_element = Element(element)
+        return self
+
+    def with_norm(self, epsilon: float = 1e-6) -> "RotaryConfig":
+        self.epsilon = float(epsilon)
+        return self
+
+    def with_amplitude(self, amplitude: float) -> "RotaryConfig":
+        """A factor of what turns, as some scalings for long contexts have one."""
+        self.amplitude = float(amplitude)
+        return self
+
+    def with_base(self, base: float) -> "RotaryConfig":
+        self.base = float(base)
+        return self
+
+    def with_frequencies(self, frequencies: Sequence[float]) -> "RotaryConfig":
+        """Radians a position for each pair, in place of the base and its scaling."""
+        self.frequencies = [float(f) for f in frequencies]
+        return self
+
+    def with_linear_scaling(self, factor: float) -> "RotaryConfig":
+        """Contexts `factor` times as long: every pair turns that much slower."""
+        self.scaling = ("linear", float(factor))
+        return self
+
+    def with_base_scaling(self, factor: float) -> "RotaryConfig":
+        """The base times factor^(r / (r - 2)): the slowest pair turns `factor` times slower, the fastest as before."""
+        self.scaling = ("base", float(factor))
+        return self
+
+    def with_blended_scaling(self, factor: float, trained_tokens: float, fast: float = 32.0, slow: float = 1.0) -> "RotaryConfig":
+        """Pairs of `fast` turns or more in the trained context turn as before, those of `slow` or fewer `factor` times
+        slower; in between, by shares of both that go with the turns."""
+        self.scaling = ("blended", float(factor), float(trained_tokens), float(fast), float(slow))
+        return self
+
+    def turns(self) -> List[float]:
+        """Radians a position for each pair."""
+        r = self.head_dim if self.rotary_dim is None else self.rotary_dim
+        if self.frequencies is not None:
+            if len(self.frequencies) != r // 2:
+                raise VkFftError(-5, f"{r // 2} pairs need {r // 2} frequencies, got {len(self.frequencies)}")
+            return list(self.frequencies)
+        kind, factor, *rest = self.scaling or ("", 1.0)
+        numbers = [self.base, factor] + rest
+        if not all(0 < n < float("inf") for n in numbers):
+            raise VkFftError(-7, "base and scaling must be positive and finite")
+        if kind == "blended" and rest[1] <= rest[2]:
+            raise VkFftError(-7, "fast must be more turns than slow")
+        try:
+            base = self.base * factor ** (r / (r - 2)) if kind == "base" and r > 2 else self.base
+            out = [base ** (-2.0 * i / r) for i in range(r // 2)]
+        except OverflowError:
+            raise VkFftError(-7, "base and scaling must be positive and finite") from None
+        if kind == "linear" or (kind == "base" and r == 2):
+            out = [f / factor for f in out]
+        if kind == "blended":
+            trained, fast, slow = rest
+            share = [min(1.0, max(0.0, (trained * f / (2 * math.pi) - slow) / (fast - slow))) for f in out]
+            out = [f * (s + (1 - s) / factor) for f, s in zip(out, share)]
+        return out
+
+    def desc(self) -> _RotaryDesc:
+        kv = self.heads if self.kv_heads is None else self.kv_heads
+        r = self.head_dim if self.rotary_dim is None else self.rotary_dim
+        for name, n, least in (("heads", self.heads, 1), ("kv_heads", kv, 0), ("head_dim", self.head_dim, 1), ("rotary_dim", r, 0)):
+            if not least <= n < 1 << 31:
+                raise VkFftError(-7, f"{name} must be at least {least} and under 2^31")
+        if r > self.head_dim or r % 2:
+            raise VkFftError(-7, "rotary_dim must be even and at most head_dim")
+        turns = self.turns()
+        weight = self.element if self.weight_element is None else self.weight_element
+        return _RotaryDesc(self.heads, kv, self.head_dim, r, int(self.layout), int(self.element), int(weight),
+                           int(self.epsilon is not None), self.epsilon or 0.0, self.amplitude, (ctypes.c_double * len(turns))(*turns))
+
+
+class RotaryPlan(_SequencePlan):
+    """Rotary positions on device-resident torch tensors [batch][token][head][dim]
+    (any strides, the last dimension contiguous). A token's position is
+    positions[b][t], else starts[b] + t, else t (int32); `lengths`: int32 for each
+    sequence, or None for all tokens."""
+    _kind = "rotary"
+
+    def __init__(self, ctx: "HipExecutionContext", config: RotaryConfig):
+        super().__init__(ctx, config, config.desc())
+        self._dims = config.heads, config.heads if config.kv_heads is None else config.kv_heads, config.head_dim
+        self._weight_type = _torch_type(config.element if config.weight_element is None else config.weight_element)
+        self._norm = config.epsilon is not None
+        import torch
+        self._i32 = torch.int32
+
+    _NONE = (None, 0, 0, 0)
+
+    def _shape(self, name, q, k):
+        """Device, batch and tokens of a call, from its queries or else its keys."""
+        x = k if q is None else q
+        device = self._place(x)
+        if x.dim() != 4:
+            raise VkFftError(-5, f"{name} must be [batch][token][head][dim]")
+        return device, x.size(0), x.size(1)
+
+    def _pair(self, names, x, y, shape, device):
+        """Both parts of (x, its result), or neither."""
+        if x is None:
+            if y is not None:
+                raise VkFftError(-7, f"{names[1]} without {names[0]}")
+            return self._NONE, self._NONE
+        return self._sequence(names[0], x, shape, device), self._sequence(names[1], y, shape, device)
+
+    def forward_tensors(self, q, k, q_out, k_out, q_weight=None, k_weight=None, positions=None, starts=None, lengths=None,
+                        stream=None):
+        """q and k turned (q_out may be q, k_out may be k); either may be None with its result. The weights are the
+        norm's, None: 1."""
+        device, b, t = self._shape("q", q, k)
+        h, kv, d = self._dims
+        qi, qo = self._pair(("q", "q_out"), q, q_out, (b, t, h, d), device)
+        ki, ko = self._pair(("k", "k_out"), k, k_out, (b, t, kv, d), device)
+        dense, weight, i32 = self._dense, self._weight_type, self._i32
+        args = _RotaryForwardArgs(b, t, *qi, *ki, *qo, *ko, dense("q_weight", q_weight, (d,), weight, device),
+                                  dense("k_weight", k_weight, (d,), weight, device),
+                                  dense("positions", positions, (b, t), i32, device), dense("starts", starts, (b,), i32, device),
+                                  dense("lengths", lengths, (b,), i32, device))
+        _check(self._L.vkfx_rotary_forward(self.handle, ctypes.byref(args), self._stream(stream, device)), self._L)
+
+    def backward_tensors(self, dq_out, dk_out, dq, dk, q=None, k=None, q_weight=None, k_weight=None, dq_weight=None,
+                         dk_weight=None, positions=None, starts=None, lengths=None, work=None, stream=None):
+        """Gradients of q and k for dq_out and dk_out (dq may be dq_out, dk may be dk_out); with the norm, from the
+        forward call's q and k, also of its weights (None: not wanted)."""
+        device, b, t = self._shape("dq_out", dq_out, dk_out)
+        h, kv, d = self._dims
+        gq, rq = self._pair(("dq_out", "dq"), dq_out, dq, (b, t, h, d), device)
+        gk, rk = self._pair(("dk_out", "dk"), dk_out, dk, (b, t, kv, d), device)
+        qi = self._sequence("q", q, (b, t, h, d), device) if self._norm and dq_out is not None else self._NONE
+        ki = self._sequence("k", k, (b, t, kv, d), device) if self._norm and dk_out is not None else self._NONE
+        dense, weight, i32 = self._dense, self._weight_type, self._i32
+        args = _RotaryBackwardArgs(b, t, *gq, *gk, *qi, *ki, *rq, *rk, dense("q_weight", q_weight, (d,), weight, device),
+                                   dense("k_weight", k_weight, (d,), weight, device),
+                                   dense("dq_weight", dq_weight, (d,), weight, device),
+                                   dense("dk_weight", dk_weight, (d,), weight, device),
+                                   dense("positions", positions, (b, t), i32, device), dense("starts", starts, (b,), i32, device),
+                                   dense("lengths", lengths, (b,), i32, device))
+        _check(self._L.vkfx_rotary_backward(self.handle, ctypes.byref(args), self._work(work, device),
+                                            self._stream(stream, device)), self._L)
+
+
+class Gate(enum.IntEnum):
+    """How a recurrence's decay follows from its gate."""
+    Sigmoid = 0  # a = sigmoid(gate)
+    Exp = 1  # a = exp(min(gate, 0))
+
+
+@dataclass
+class GatedRecurrenceConfig:
+    """A recurrence of each channel: h[t] = a[t] h[t-1] + m[t] x[t], y[t] = h[t], where a follows from the gate and m is
+    1, or 1 - a with the complement."""
+    channels: int
+    element: Element = Element.F32
+    gate: Gate = Gate.Sigmoid
+    complement: bool = False
+
+    @staticmethod
+    def new(channels: int) -> "GatedRecurrenceConfig":
+        return GatedRecurrenceConfig(int(channels))
+
+    def with_element(self, element: Element) -> "GatedRecurrenceConfig":
+        self.element = Element(element)
+        return self
+
+    def with_gate(self, gate: Gate) -> "GatedRecurrenceConfig":
+        self.gate = Gate(gate)
+        return self
+
+    def with_complement(self, complement: bool = True) -> "GatedRecurrenceConfig":
+        self.complement = bool(complement)
+        return self
+
+    def desc(self) -> _GatedRecurrenceDesc:
+        if not 0 <= self.channels < 1 << 63:
+            raise VkFftError(-7, "channels must be 1 .. 2^30")
+        return _GatedRecurrenceDesc(self.channels, int(self.element), int(self.gate), int(self.complement), 0)
+
+
+class GatedRecurrencePlan(_SequencePlan):
+    """The gated recurrence on device-resident torch tensors [batch][token][channel]
+    (any strides, the last dimension contiguous) and states [batch][channel]
+    (float32, contiguous). `lengths`: int32 for each sequence, or None for all
+    tokens."""
+    _kind = "gated_recurrence"
+    SPAN = 16  # tokens between saved states
+
+    def __init__(self, ctx: "HipExecutionContext", config: GatedRecurrenceConfig):
+        super().__init__(ctx, config, config.desc())
+        self._channels = config.channels
+        import torch
+        self._i32 = torch.int32
+
+    def saved_shape(self, batch: int, tokens: int) -> Tuple[int, int, int]:
+        """Of the states that a forward call saves for the backward pass (float32)."""
+        return batch, -(-tokens // self.SPAN), self._channels
+
+    def _rows(self, name, x, shape, device):
+        if getattr(x, "shape", None) != shape or x.dtype is not self._type or x.get_device() != device:
+            self._refuse(name, x, shape, self._type, device)
+        b, t, c = x.stride()
+        if c != 1 and shape[2] > 1:
+            raise VkFftError(-7, f"{name}: the last dimension must be contiguous")
+        return x.data_ptr(), b, t
+
+    def _shape(self, x):
+        device = self._place(x)
+        if x.dim() != 3:
+            raise VkFftError(-5, "x must be [batch][token][channel]")
+        b, t = x.size(0), x.size(1)
+        return device, b, t, (b, t, self._channels), (b, self._channels)
+
+    def forward_tensors(self, x, gate, y, state_in=None, state_out=None, saved=None, lengths=None, work=None, stream=None):
+        """y (may be x) of a prompt, or of the next token where there is one: from state_in (None: zeros) to state_out
+        (None: not wanted; may be state_in). saved: what backward_tensors needs, of saved_shape."""
+        device, b, t, shape, state = self._shape(x)
+        rows, dense, f32 = self._rows, self._dense, self._f32
+        args = _RecurrenceForwardArgs(b, t, *rows("x", x, shape, device), *rows("gate", gate, shape, device),
+                                      *rows("y", y, shape, device), dense("lengths", lengths, (b,), self._i32, device),
+                                      dense("state_in", state_in, state, f32, device),
+                                      dense("state_out", state_out, state, f32, device),
+                                      None if saved is None else dense("saved", saved, self.saved_shape(b, t), f32, device))
+        _check(self._L.vkfx_gated_recurrence_forward(self.handle, ctypes.byref(args), self._work(work, device),
+                                                     self._stream(stream, device)), self._L)
+
+    def backward_tensors(self, x, gate, saved, dy, dx, dgate, dstate_out=None, dstate_in=None, lengths=None, work=None,
+                         stream=None):
+        """Gradients of x (dx may be dy), gate and (dstate_in, None: not wanted; may be dstate_out) of state_in, for dy
+        and dstate_out (None: zeros), with the forward call's inputs and what it saved."""
+        device, b, t, shape, state = self._shape(x)
+        rows, dense, f32 = self._rows, self._dense, self._f32
+        args = _RecurrenceBackwardArgs(b, t, *rows("x", x, shape, device), *rows("gate", gate, shape, device),
+                                       *rows("dy", dy, shape, device), *rows("dx", dx, shape, device),
+                                       *rows("dgate", dgate, shape, device), dense("lengths", lengths, (b,), self._i32, device),
+                                       dense("saved", saved, self.saved_shape(b, t), f32, device),
+                                       dense("dstate_out", dstate_out, state, f32, device),
+                                       dense("dstate_in", dstate_in, state, f32, device))
+        _check(self._L.vkfx_gated_recurrence_backward(self.handle, ctypes.byref(args), self._work(work, device),
                                                       self._stream(stream, device)), self._L)
 
 
