@@ -8,6 +8,11 @@
 //   du = the gradient turned back, g = du weight
 //   dx = rstd (g - n mean(g n)),  dweight = sum du n
 // over tokens and heads.
+//
+// Bound by memory: every row is read once, in vectors of 16 bytes. A row belongs
+// to 4 .. 32 lanes of a wave, each of which holds both elements of its pairs. A
+// lane forms its pairs' cosines and sines once for up to 4 heads of a token,
+// whose loads are on their way meanwhile.
 #include <algorithm>
 
 #include "sequence.hpp"
@@ -33,141 +38,355 @@ __device__ __forceinline__ void turn(uint64_t phase, float& c, float& s) {
     if (quarter & 2) s = -s;
 }
 
-__device__ __forceinline__ long long position(const RotaryArgs& a, long long b, long long t) {
-    return a.positions ? a.positions[b * a.tokens + t] : a.starts ? a.starts[b] + t : t;
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
+// Sum over the G lanes of a row, the same on each.
+template <int G>
+__device__ __forceinline__ float row_sum(float v) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    for (int o = 1; o < G; o <<= 1) v += __shfl_xor(v, o);
     return v;
 }
 
-// A wave a row, up to 4 elements a lane, 64 apart. The block's sums of du n go
-// to the workspace: row blockIdx.x of half blockIdx.y.
-template <typename T, typename W, bool NORM, bool BACK>
-__global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
-    const RotaryRows& h = a.rows[blockIdx.y];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long rows = a.all * h.heads, stride = (long long)gridDim.x * 4;
-    double sums[4] = {};
-    for (long long r = (long long)blockIdx.x * 4 + wave; r < rows; r += stride) {
-        const long long token = r / h.heads, b = token / a.tokens, t = token % a.tokens;
-        const int head = (int)(r % h.heads);
-        const T* x = (const T*)h.x.p + b * h.x.batch + t * h.x.token + head * h.x.head;
-        T* out = (T*)h.out.p + b * h.out.batch + t * h.out.token + head * h.out.head;
-        if (a.lengths && t >= a.lengths[b]) {
-            for (int e = lane; e < a.dim; e += 64) out[e] = (T)0.f;
-            continue;
-        }
-        const long long p = position(a, b, t);
-        float v[4], w[4], c[4], s[4], n[4], other[4];
-        float square = 0.f;
+// A lane's share of a row: two vectors of V elements that hold its V pairs
+// between them, and with TAILS two more of what does not turn.
+//   HALF: elements l V .. of the first half and of the second, then the tail's
+//   else: elements l V .. and (G + l) V .., pairs of neighbours
+template <typename T, int G, int TAILS, bool HALF>
+struct Share {
+    static constexpr int V = kVector<T>, N = 2 + TAILS;
+    typedef Some<T, V> Vectors[N];
+    int at[N], end[N], half;
+
+    __device__ __forceinline__ Share(const RotaryArgs& a, int l) {
+        half = a.turned / 2;
+        at[0] = l * V;
+        at[1] = HALF ? half + l * V : (G + l) * V;
+        end[0] = HALF ? half : a.dim;
+        end[1] = HALF ? a.turned : a.dim;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int e = lane + 64 * j, half = a.turned / 2;
-            v[j] = w[j] = c[j] = s[j] = n[j] = other[j] = 0.f;
-            if (e >= a.dim) continue;
-            v[j] = (float)x[e];
-            w[j] = 1.f;
-            if (NORM && h.weight) w[j] = (float)((const W*)h.weight)[e];
-            c[j] = 1.f;
-            if (e < a.turned) {
-                const bool second = a.layout == VKFX_ROTARY_HALF ? e >= half : e & 1;
-                const int pair = a.layout == VKFX_ROTARY_HALF ? e - second * half : e / 2;
-                const int with = a.layout == VKFX_ROTARY_HALF ? (second ? pair : e + half) : e ^ 1;
-                turn((uint64_t)p * a.turns[pair], c[j], s[j]);
-                c[j] *= a.amplitude;
-                s[j] *= second != BACK ? a.amplitude : -a.amplitude;
-                other[j] = (float)x[with];
-                if (NORM && !BACK && h.weight) other[j] *= (float)((const W*)h.weight)[with];
-            }
-            if constexpr (NORM && BACK) n[j] = (float)((const T*)h.in.p)[b * h.in.batch + t * h.in.token + head * h.in.head + e];
-            square = NORM ? BACK ? fmaf(n[j], n[j], square) : fmaf(v[j], v[j], square) : 0.f;
+        for (int j = 2; j < N; ++j) {
+            at[j] = a.turned + ((j - 2) * G + l) * V;
+            end[j] = a.dim;
         }
-        float rstd = 1.f;
-        if (NORM) {
-            square = wave_sum(square);
-            rstd = 1.f / sqrtf(square / (float)a.dim + a.epsilon);
-            if (square == INFINITY) {  // squares past 32 bits: of 2^-68 of the row, beside which epsilon is nothing
-                square = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float part = (BACK ? n[j] : v[j]) * 0x1p-68f;
-                    square = fmaf(part, part, square);
-                }
-                rstd = 0x1p-68f / sqrtf(wave_sum(square) / (float)a.dim);
-            }
-        }
-        if (!NORM || !BACK) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (lane + 64 * j < a.dim) out[lane + 64 * j] = (T)(fmaf(v[j] * w[j], c[j], other[j] * s[j]) * rstd);
-            continue;
-        }
-        float dot = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = fmaf(v[j], c[j], other[j] * s[j]);
-            n[j] *= rstd;
-            sums[j] += (double)(v[j] * n[j]);
-            v[j] *= w[j];
-            dot = fmaf(v[j], n[j], dot);
-        }
-        dot = wave_sum(dot) / (float)a.dim;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (lane + 64 * j < a.dim) out[lane + 64 * j] = (T)((v[j] - n[j] * dot) * rstd);
     }
-    if (!NORM || !BACK || !h.dweight) return;
-    __shared__ double lds[4][256];
+    __device__ __forceinline__ void load(Vectors& x, const T* row) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) lds[wave][lane + 64 * j] = sums[j];
-    __syncthreads();
-    const int e = threadIdx.x;
-    if (e < a.dim)
-        a.partial[((long long)blockIdx.y * gridDim.x + blockIdx.x) * a.dim + e] = (float)((lds[0][e] + lds[1][e]) + (lds[2][e] + lds[3][e]));
+        for (int j = 0; j < N; ++j) x[j] = load_some<T, V>(row, at[j], end[j]);
+    }
+    __device__ __forceinline__ void store(const float (&y)[N][V], T* row) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            Some<T, V> r;
+#pragma unroll
+            for (int e = 0; e < V; ++e) r[e] = (T)y[j][e];
+            store_some<T, V>(row, at[j], end[j], r);
+        }
+    }
+    // The norm's weights; 1 without.
+    __device__ __forceinline__ void weights(float (&w)[N][V], const void* p, bool f32) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[j][e] = 1.f;
+        if (!p) return;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (f32) {
+                const Some<float, V> v = load_some<float, V>((const float*)p, at[j], end[j]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) w[j][e] = v[e];
+            } else {
+                const Some<T, V> v = load_some<T, V>((const T*)p, at[j], end[j]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) w[j][e] = (float)v[e];
+            }
+        }
+    }
+    // Cosines and sines of the lane's pairs at position p, amplitude included.
+    __device__ __forceinline__ void turns(float (&c)[V], float (&s)[V], const RotaryArgs& a, long long p, float sign) const {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int pair = HALF ? at[0] + e : at[e / (V / 2)] / 2 + e % (V / 2);
+            c[e] = 1.f;
+            s[e] = 0.f;
+            if (pair >= half) continue;
+            turn((uint64_t)p * a.turns[pair], c[e], s[e]);
+            c[e] *= a.amplitude;
+            s[e] *= sign;
+        }
+    }
+    __device__ __forceinline__ static void turn_by(float (&y)[N][V], const float (&c)[V], const float (&s)[V]) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            float& u = HALF ? y[0][e] : y[e / (V / 2)][e % (V / 2) * 2];
+            float& v = HALF ? y[1][e] : y[e / (V / 2)][e % (V / 2) * 2 + 1];
+            const float first = fmaf(u, c[e], -v * s[e]);
+            v = fmaf(u, s[e], v * c[e]);
+            u = first;
+        }
+    }
+};
+
+// 1 / sqrt(mean of squares + epsilon) of a row; where the squares pass 32 bits,
+// from 2^-68 of the row, beside which epsilon is nothing.
+template <int G, int N, int V>
+__device__ __forceinline__ float deviation(const float (&x)[N][V], float over, float epsilon) {
+    float square = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) square = fmaf(x[j][e], x[j][e], square);
+    square = row_sum<G>(square);
+    if (square != INFINITY) return 1.f / sqrtf(fmaf(square, over, epsilon));
+    square = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float part = x[j][e] * 0x1p-68f;
+            square = fmaf(part, part, square);
+        }
+    return 0x1p-68f / sqrtf(row_sum<G>(square) * over);
 }
 
-template <typename W>
-__global__ __launch_bounds__(256) void k_rotary_weights(const RotaryArgs a, int parts) {
+// Which token and which heads of it a group of lanes takes: heads phase, phase +
+// phases, ... up to HB of them.
+struct Place {
+    long long b, t, position;
+    int phase;
+    bool live;  // before the sequence's length
+    __device__ __forceinline__ Place(const RotaryArgs& a, long long i, long long count, int phases) {
+        const unsigned token = count >> 32 ? (unsigned)(i / phases) : (unsigned)i / (unsigned)phases;
+        phase = (int)(i - (long long)token * phases);
+        const unsigned row = token / (unsigned)a.tokens;
+        b = row;
+        t = token - row * (unsigned)a.tokens;
+        live = !a.lengths || t < a.lengths[b];
+        position = a.positions ? a.positions[b * a.tokens + t] : a.starts ? a.starts[b] + t : t;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ T* row_of(const RotarySide& s, const Place& p, int head) {
+    return (T*)s.p + p.b * s.batch + p.t * s.token + head * s.head;
+}
+
+// Turns rows, by `sign` times their angle, behind the norm where NORM. The first
+// `split` blocks take rows[0].
+template <typename T, int G, int TAILS, int HB, bool HALF, bool NORM>
+__global__ __launch_bounds__(256) void k_turn(const RotaryArgs a, unsigned split, float sign) {
+    typedef Share<T, G, TAILS, HALF> S;
+    constexpr int V = S::V, N = S::N;
+    const bool second = blockIdx.x >= split;
+    const RotaryRows& h = a.rows[second];
+    const int phases = (h.heads + HB - 1) / HB;
+    const long long count = a.all * phases, stride = (long long)(second ? gridDim.x - split : split) * (256 / G);
+    const S share(a, threadIdx.x % G);
+    float w[N][V];
+    if constexpr (NORM) share.weights(w, h.weight, a.weight_element == VKFX_ELEMENT_F32);
+    for (long long i = (long long)(blockIdx.x - (second ? split : 0)) * (256 / G) + threadIdx.x / G; i < count; i += stride) {
+        const Place p(a, i, count, phases);
+        typename S::Vectors x[HB];
+        if (p.live)
+#pragma unroll
+            for (int k = 0; k < HB; ++k)
+                if (p.phase + k * phases < h.heads) share.load(x[k], row_of<const T>(h.x, p, p.phase + k * phases));
+        float c[V], s[V];
+        share.turns(c, s, a, p.position, sign * a.amplitude);
+#pragma unroll
+        for (int k = 0; k < HB; ++k) {
+            const int head = p.phase + k * phases;
+            if (head >= h.heads) break;
+            float y[N][V] = {};
+            if (p.live) {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) y[j][e] = (float)x[k][j][e];
+                if constexpr (NORM) {
+                    const float rstd = deviation<G>(y, 1.f / (float)a.dim, a.epsilon);
+#pragma unroll
+                    for (int j = 0; j < N; ++j)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) y[j][e] *= rstd * w[j][e];
+                }
+                S::turn_by(y, c, s);
+            }
+            share.store(y, row_of<T>(h.out, p, head));
+        }
+    }
+}
+
+// Gradients behind the norm. A lane's sums of du n are of a few heads in 32
+// bits, then in 64; the block's go to the workspace, row blockIdx.x.
+template <typename T, int G, int TAILS, int HB, bool HALF>
+__global__ __launch_bounds__(256) void k_norm_turn_back(const RotaryArgs a, unsigned split) {
+    typedef Share<T, G, TAILS, HALF> S;
+    constexpr int V = S::V, N = S::N;
+    const bool second = blockIdx.x >= split;
+    const RotaryRows& h = a.rows[second];
+    const int phases = (h.heads + HB - 1) / HB;
+    const long long count = a.all * phases, stride = (long long)(second ? gridDim.x - split : split) * (256 / G);
+    const S share(a, threadIdx.x % G);
+    const float over = 1.f / (float)a.dim;
+    float w[N][V];
+    share.weights(w, h.weight, a.weight_element == VKFX_ELEMENT_F32);
+    double sums[N][V] = {};
+    for (long long i = (long long)(blockIdx.x - (second ? split : 0)) * (256 / G) + threadIdx.x / G; i < count; i += stride) {
+        const Place p(a, i, count, phases);
+        typename S::Vectors x[HB], dy[HB];
+        if (p.live)
+#pragma unroll
+            for (int k = 0; k < HB; ++k)
+                if (p.phase + k * phases < h.heads) {
+                    share.load(dy[k], row_of<const T>(h.x, p, p.phase + k * phases));
+                    share.load(x[k], row_of<const T>(h.in, p, p.phase + k * phases));
+                }
+        float c[V], s[V], part[N][V] = {};
+        share.turns(c, s, a, p.position, -a.amplitude);
+#pragma unroll
+        for (int k = 0; k < HB; ++k) {
+            const int head = p.phase + k * phases;
+            if (head >= h.heads) break;
+            float g[N][V] = {};
+            if (p.live) {
+                float n[N][V];
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) g[j][e] = (float)dy[k][j][e], n[j][e] = (float)x[k][j][e];
+                const float rstd = deviation<G>(n, over, a.epsilon);
+                S::turn_by(g, c, s);
+                float dot = 0.f;
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        n[j][e] *= rstd;
+                        part[j][e] = fmaf(g[j][e], n[j][e], part[j][e]);
+                        g[j][e] *= w[j][e];
+                        dot = fmaf(g[j][e], n[j][e], dot);
+                    }
+                dot = row_sum<G>(dot) * over;
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) g[j][e] = fmaf(-n[j][e], dot, g[j][e]) * rstd;
+            }
+            share.store(g, row_of<T>(h.out, p, head));
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sums[j][e] += (double)part[j][e];
+    }
+    if (!h.dweight) return;
+    __shared__ double lds[4][256];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+#pragma unroll
+            for (int o = G; o < 64; o <<= 1) sums[j][e] += __shfl_xor(sums[j][e], o);
+            if ((threadIdx.x & 63) < G && share.at[j] + e < share.end[j]) lds[threadIdx.x >> 6][share.at[j] + e] = sums[j][e];
+        }
+    __syncthreads();
     const int e = threadIdx.x;
-    W* to = (W*)a.rows[blockIdx.x].dweight;
-    if (!to || e >= a.dim) return;
+    if (e < a.dim) a.partial[(long long)blockIdx.x * a.dim + e] = (float)((lds[0][e] + lds[1][e]) + (lds[2][e] + lds[3][e]));
+}
+
+// Adds the blocks' sums: 64 elements a block, its 16 waves each an equal share
+// of the blocks in their order. blockIdx.y: q's weight, k's.
+template <typename W>
+__global__ __launch_bounds__(1024) void k_norm_weights(const RotaryArgs a, int split, int blocks) {
+    __shared__ double lds[16][64];
+    W* const to = (W*)a.rows[blockIdx.y].dweight;
+    if (!to) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+    const int begin = blockIdx.y ? split : 0, parts = blockIdx.y ? blocks - split : split;
+    const int first = begin + parts * wave / 16, end = begin + parts * (wave + 1) / 16;
     double sum = 0.0;
-    for (int i = 0; i < parts; ++i) sum += (double)a.partial[((long long)blockIdx.x * parts + i) * a.dim + e];
+    if (e < a.dim)
+#pragma unroll 8
+        for (int i = first; i < end; ++i) sum += (double)a.partial[(long long)i * a.dim + e];
+    lds[wave][lane] = sum;
+    __syncthreads();
+    if (wave || e >= a.dim) return;
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += lds[i][lane];
     to[e] = (W)(float)sum;
 }
 
-template <typename T, typename W, bool BACK>
-int launch_as(const RotaryArgs& a, hipStream_t s) {
-    const long long rows = a.all * std::max(a.rows[0].heads, a.rows[1].heads);
-    const int blocks = (int)std::min((rows + 3) / 4, (long long)a.cus * 4);
-    if (blocks) {
-        if (a.norm) hipLaunchKernelGGL((k_rotary<T, W, true, BACK>), dim3(blocks, 2), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_rotary<T, W, false, BACK>), dim3(blocks, 2), dim3(256), 0, s, a);
+// Blocks of the backward pass, whose sums each are a row of the workspace.
+constexpr int kBackBlocks = 4;  // a CU
+
+template <typename T, int G, int TAILS, int HB, bool HALF>
+int launch_as(const RotaryArgs& a, hipStream_t s, bool back) {
+    const auto blocks_of = [&](const RotaryRows& r) {
+        return (a.all * ((r.heads + HB - 1) / HB) + 256 / G - 1) / (256 / G);
+    };
+    long long blocks[2] = {blocks_of(a.rows[0]), blocks_of(a.rows[1])};
+    if (!a.norm || !back) {
+        for (long long& n : blocks) n = std::min(n, 1ll << 22);
+        const unsigned all = (unsigned)(blocks[0] + blocks[1]);
+        if (!all) return (int)hipSuccess;
+        const auto kernel = a.norm ? k_turn<T, G, TAILS, HB, HALF, true> : k_turn<T, G, TAILS, HB, HALF, false>;
+        hipLaunchKernelGGL(kernel, dim3(all), dim3(256), 0, s, a, (unsigned)blocks[0], back ? -1.f : 1.f);
+        return (int)hipGetLastError();
     }
-    if (BACK && (a.rows[0].dweight || a.rows[1].dweight))
-        hipLaunchKernelGGL((k_rotary_weights<W>), dim3(2), dim3(256), 0, s, a, blocks);
+    const long long most = (long long)a.cus * kBackBlocks, all = blocks[0] + blocks[1];
+    if (all > most) {  // in the proportion of their rows, each at least one
+        const long long n = blocks[0] ? std::max(1ll, (long long)((double)blocks[0] / (double)all * (double)most)) : 0;
+        blocks[0] = blocks[1] ? std::min(n, most - 1) : most;
+        blocks[1] = most - blocks[0];
+    }
+    if (all)
+        hipLaunchKernelGGL((k_norm_turn_back<T, G, TAILS, HB, HALF>), dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0, s, a, (unsigned)blocks[0]);
+    if (a.rows[0].dweight || a.rows[1].dweight) {
+        const auto kernel = a.weight_element == VKFX_ELEMENT_F32 ? k_norm_weights<float> : k_norm_weights<T>;
+        hipLaunchKernelGGL(kernel, dim3((a.dim + 63) / 64, 2), dim3(1024), 0, s, a, (int)blocks[0], (int)(blocks[0] + blocks[1]));
+    }
     return (int)hipGetLastError();
 }
 
-template <typename T>
-int pick(const RotaryArgs& a, hipStream_t s, bool back) {
-    if (a.weight_element == VKFX_ELEMENT_F32) return back ? launch_as<T, float, true>(a, s) : launch_as<T, float, false>(a, s);
-    return back ? launch_as<T, T, true>(a, s) : launch_as<T, T, false>(a, s);
+// One head a group of lanes while there are few rows, where latency counts;
+// several from 8 waves a CU on.
+template <typename T, int G, int TAILS, bool HALF>
+int launch_heads(const RotaryArgs& a, hipStream_t s, bool back) {
+    const bool sums = a.norm && back;
+    const long long waves = a.all * ((a.rows[0].heads + a.rows[1].heads + 3) / 4) * G / 64;
+    if (waves < (long long)a.cus * 8) return launch_as<T, G, TAILS, 1, HALF>(a, s, back);
+    return sums ? launch_as<T, G, TAILS, 2, HALF>(a, s, back) : launch_as<T, G, TAILS, 4, HALF>(a, s, back);
 }
 
-int pick_element(const RotaryArgs& a, hipStream_t s, bool back) {
-    if (a.element == VKFX_ELEMENT_F32) return pick<float>(a, s, back);
-    if (a.element == VKFX_ELEMENT_F16) return pick<_Float16>(a, s, back);
-    return pick<__bf16>(a, s, back);
+template <typename T, int TAILS, bool HALF>
+int launch_lanes(const RotaryArgs& a, hipStream_t s, bool back) {
+    constexpr int V = kVector<T>;
+    const int pairs = HALF ? (a.turned / 2 + V - 1) / V : (a.dim + 2 * V - 1) / (2 * V);
+    const int lanes = std::max(pairs, TAILS ? (a.dim - a.turned + 2 * V - 1) / (2 * V) : 0);
+    if (lanes <= 4) return launch_heads<T, 4, TAILS, HALF>(a, s, back);
+    if (lanes <= 8) return launch_heads<T, 8, TAILS, HALF>(a, s, back);
+    if constexpr (sizeof(T) == 4)
+        if (lanes > 16) return launch_heads<T, 32, TAILS, HALF>(a, s, back);
+    return launch_heads<T, 16, TAILS, HALF>(a, s, back);
+}
+
+template <typename T>
+int launch_layout(const RotaryArgs& a, hipStream_t s, bool back) {
+    if (a.layout == VKFX_ROTARY_INTERLEAVED) return launch_lanes<T, 0, false>(a, s, back);
+    return a.turned == a.dim ? launch_lanes<T, 0, true>(a, s, back) : launch_lanes<T, 2, true>(a, s, back);
+}
+
+int launch_element(const RotaryArgs& a, hipStream_t s, bool back) {
+    if (a.element == VKFX_ELEMENT_F32) return launch_layout<float>(a, s, back);
+    if (a.element == VKFX_ELEMENT_F16) return launch_layout<_Float16>(a, s, back);
+    return launch_layout<__bf16>(a, s, back);
 }
 
 }  // namespace
 
-int launch_rotary_forward(const RotaryArgs& a, hipStream_t s) { return pick_element(a, s, false); }
-int launch_rotary_backward(const RotaryArgs& a, hipStream_t s) { return pick_element(a, s, true); }
-size_t rotary_workspace_bytes(int dim, int cus) { return (size_t)cus * 4 * 2 * (size_t)dim * sizeof(float); }
+int launch_rotary_forward(const RotaryArgs& a, hipStream_t s) { return launch_element(a, s, false); }
+int launch_rotary_backward(const RotaryArgs& a, hipStream_t s) { return launch_element(a, s, true); }
+size_t rotary_workspace_bytes(int dim, int cus) { return (size_t)cus * kBackBlocks * (size_t)dim * sizeof(float); }
 
 }  // namespace vkfx
