@@ -551,7 +551,7 @@ int vkfx_rotary_backward(vkfx_rotary *plan, const vkfx_rotary_backward_args *arg
  *   h[t] = a[t] h[t-1] + m[t] x[t],  y[t] = h[t]. */
 enum vkfx_gate { VKFX_GATE_SIGMOID = 0, VKFX_GATE_EXP = 1 };
 typedef struct {
-    uint64_t channels;  /* 1 .. 2^30 */
+    uint64_t channels;  /* 1 .. 2^28 */
     int32_t element;    /* vkfx_element of x, gate, y and their gradients */
     int32_t gate;       /* vkfx_gate */
     int32_t complement; /* 1: m = 1 - a */

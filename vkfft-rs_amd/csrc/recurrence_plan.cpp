@@ -69,7 +69,7 @@ int vkfx_gated_recurrence_create(vkfx_context* ctx, const vkfx_gated_recurrence_
     *out = nullptr;
     return guarded([&]() -> int {
         const vkfx_gated_recurrence_desc& d = *desc;
-        if (d.channels < 1 || d.channels > (1u << 30)) return bad("channels must be 1 .. 2^30");
+        if (d.channels < 1 || d.channels > (1u << 28)) return bad("channels must be 1 .. 2^28");
         if (!known_element(d.element)) return fail(VKFX_ERR_UNSUPPORTED_PRECISION, "element must be F32, F16 or BF16");
         if (d.gate != VKFX_GATE_SIGMOID && d.gate != VKFX_GATE_EXP) return bad("unknown gate");
         if (d.complement != 0 && d.complement != 1) return bad("complement must be 0 or 1");

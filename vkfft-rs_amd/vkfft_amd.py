@@ -1948,7 +1948,7 @@ class GatedRecurrenceConfig:
 
     def desc(self) -> _GatedRecurrenceDesc:
         if not 0 <= self.channels < 1 << 63:
-            raise VkFftError(-7, "channels must be 1 .. 2^30")
+            raise VkFftError(-7, "channels must be 1 .. 2^28")
         return _GatedRecurrenceDesc(self.channels, int(self.element), int(self.gate), int(self.complement), 0)
 
 
