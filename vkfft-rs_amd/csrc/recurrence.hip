@@ -29,8 +29,6 @@ namespace vkfx {
 namespace {
 
 constexpr int U = kSpan;  // tokens of a wave
-template <typename T>
-constexpr int kChannels = 4 / (int)sizeof(T);  // of a lane
 
 // exp(g), off by 2^-22 of it, for -87 <= g <= 0: the product with log2(e) keeps
 // its rounding.
@@ -54,18 +52,29 @@ __device__ __forceinline__ float exp_less_1(float g) {
     return fmaf(g * p, g, g);
 }
 
-// The smaller of a and 1 - a; negative (-0 too) where that is 1 - a. NEAR: no
-// |g| is past 87, from where on the hardware's exponential gives 0.
+// A gate: s is the smaller of a and 1 - a, negative (-0 too) where that is 1 - a;
+// w is 1 - a. NEAR: no |g| is past 87, from where on the hardware's exponential
+// gives 0; there it is the square of its root.
+struct Gate {
+    float s, w;
+};
+constexpr float kNear = 87.f;
+template <bool NEAR>
+__device__ __forceinline__ float exp_of(float g) {
+    if (NEAR || !(g < -kNear)) return exp_near(g);
+    const float root = exp_near(fmaxf(0.5f * g, -kNear));
+    return root * root;
+}
 template <bool SIGMOID, bool NEAR>
-__device__ __forceinline__ float gate_of(float g) {
+__device__ __forceinline__ Gate gate_of(float g) {
     if constexpr (SIGMOID) {
-        const float e = NEAR ? exp_near(-fabsf(g)) : expf(-fabsf(g));
-        const float small = e * __builtin_amdgcn_rcpf(1.f + e);
-        return g > 0.f ? -small : small;
+        const float e = exp_of<NEAR>(-fabsf(g));
+        const float large = __builtin_amdgcn_rcpf(1.f + e), small = e * large;
+        return g > 0.f ? Gate{-small, small} : Gate{small, large};
     } else {
         g = g > 0.f ? 0.f : g;  // a NaN stays one
-        if (NEAR) return g > -0.6931472f ? __int_as_float(__float_as_int(exp_less_1(g)) | (int)0x80000000) : exp_near(g);
-        return g > -0.6931472f ? g == 0.f ? -0.f : expm1f(g) : expf(g);
+        const float less = exp_less_1(g), e = exp_of<NEAR>(g);
+        return g > -0.6931472f ? Gate{__int_as_float(__float_as_int(less) | (int)0x80000000), -less} : Gate{e, 1.f - e};
     }
 }
 // v where a >= 1/2, else 0.
@@ -73,419 +82,390 @@ __device__ __forceinline__ float if_slow(float s, float v) { return __int_as_flo
 __device__ __forceinline__ float decayed(float s, float v) { return fmaf(s, v, if_slow(s, v)); }  // a v
 __device__ __forceinline__ float short_of(float s) { return __float_as_int(s) < 0 ? -s : 1.f - s; }  // 1 - a
 
-// What some tokens make of the state before them: a v + h, short = 1 - a.
+// What some tokens make of the state before them: a v + h, a by its smaller side
+// like a gate.
 struct Join {
-    float a, low, h;  // low: 1 - a
-    __device__ __forceinline__ float operator()(float v) const { return (low < 0.5f ? fmaf(-low, v, v) : a * v) + h; }
+    float s, h;
+    __device__ __forceinline__ float operator()(float v) const { return decayed(s, v) + h; }
 };
 
 __device__ __forceinline__ int clamped(const int* lengths, int b, long long tokens) {
     const long long n = lengths ? lengths[b] : tokens;
-    return (int)(n < 0 ? 0 : n < tokens ? n : tokens);
+    return __builtin_amdgcn_readfirstlane((int)(n < 0 ? 0 : n < tokens ? n : tokens));
 }
 
-// A wave's place: channels first .. + have of the lane, tokens of the wave.
+// The next row. Kept from the compiler, which would hold every row's place in
+// scalar registers, and these, past 100 of them, in lanes of vector registers.
 template <typename T>
+__device__ __forceinline__ T* behind(T* row, long long stride) {
+    row += stride;
+    asm volatile("" : "+s"(row));
+    return row;
+}
+
+// A lane's place among the channels: CH of them, or none. Lanes without any read
+// the block's first.
+template <typename T, int CH>
 struct Lane {
-    static constexpr int CH = kChannels<T>;
-    typedef Some<T, CH> Vec;
+    typedef T Vec __attribute__((ext_vector_type(CH)));
+    // A token's channels as they lie in memory: as elements, the compiler would
+    // take them apart, and wait for them, where they arrive.
+    typedef std::conditional_t<sizeof(Vec) == 4, unsigned, unsigned short> Raw;
     long long first;  // the block's first channel
-    int at, have;     // the lane's, and how many it has
+    int at;           // the lane's
+    bool have;
 
     __device__ __forceinline__ explicit Lane(long long channels) {
         first = (long long)blockIdx.x * (64 * CH);
-        at = (threadIdx.x & 63) * CH;
-        const long long left = channels - first - at;
-        have = left < 0 ? 0 : left < CH ? (int)left : CH;
+        have = first + (threadIdx.x & 63) * CH < channels;
+        at = have ? (threadIdx.x & 63) * CH : 0;
     }
-    // rows[0 .. m) of a tensor
-    template <bool FULL>
-    __device__ __forceinline__ void fetch(Vec (&r)[U], const RecurrenceSide& s, long long b, long long t, int m) const {
+    // Tokens t .. t + m - 1 of sequence b, the last one again behind them.
+    __device__ __forceinline__ void fetch(unsigned (&r)[U], const RecurrenceSide& s, long long b, long long t, int m) const {
+        if (m <= 0) return;
         const T* row = (const T*)s.p + b * s.batch + t * s.token + first;
-        if (have == CH) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (FULL || u < m) r[u] = *(const typename Packed<T, CH>::type*)(row + u * s.token + at);
-        } else if (have) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (FULL || u < m) r[u][0] = row[u * s.token + at];
+        for (int u = 0; u < U; ++u) {
+            r[u] = *(const Raw*)(row + at);
+            row += u + 1 < m ? s.token : 0;
         }
     }
-    __device__ __forceinline__ void fetch(Vec (&r)[U], const RecurrenceSide& s, long long b, long long t, int m) const {
-        if (m == U) fetch<true>(r, s, b, t, U);
-        else if (m > 0) fetch<false>(r, s, b, t, m);
-    }
+    __device__ __forceinline__ static float value(unsigned r, int c) { return (float)__builtin_bit_cast(Vec, (Raw)r)[c]; }
     __device__ __forceinline__ void store(T* row, const float (&y)[CH]) const {
         Vec r;
 #pragma unroll
         for (int c = 0; c < CH; ++c) r[c] = (T)y[c];
-        if (have == CH) *(typename Packed<T, CH>::type*)(row + at) = r;
-        else if (have) row[at] = r[0];
+        *(Vec*)(row + at) = r;
+    }
+    // Zeros in rows t .. of a tensor.
+    __device__ __forceinline__ void clear(const RecurrenceSide& s, long long b, long long t, int rows) const {
+        T* row = (T*)s.p + b * s.batch + t * s.token + first;
+        const float zero[CH] = {};
+        for (int u = 0; have && u < rows; ++u, row += s.token) store(row, zero);
     }
     __device__ __forceinline__ void load_state(float (&h)[CH], const float* row) const {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) h[c] = c < have && row ? row[first + at + c] : 0.f;
+        for (int c = 0; c < CH; ++c) h[c] = row ? row[first + at + c] : 0.f;
     }
     __device__ __forceinline__ void store_state(float* row, const float (&h)[CH]) const {
-        if (have == CH) {
-            Some<float, CH> r;
 #pragma unroll
-            for (int c = 0; c < CH; ++c) r[c] = h[c];
-            *(typename Packed<float, CH>::type*)(row + first + at) = r;
-        } else if (have) {
-            row[first + at] = h[0];
-        }
+        for (int c = 0; c < CH; ++c)
+            if (have) row[first + at + c] = h[c];
     }
 };
 
-// Gates of a wave's first m tokens.
-template <typename T, bool SIGMOID>
-__device__ __forceinline__ void gates(float (&s)[U][kChannels<T>], const Some<T, kChannels<T>> (&g)[U]) {
+// Goes over the wave's gates: f(u, c, gate) for each. WHOLE: all U tokens, none
+// past kNear; otherwise tokens from m on leave every state as it is.
+template <typename T, int CH, bool SIGMOID, typename F>
+__device__ __forceinline__ void each_gate(const unsigned (&g)[U], int m, F f) {
     float most = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int c = 0; c < kChannels<T>; ++c) most = fmaxf(most, fabsf((float)g[u][c]));
-    if (__builtin_expect(__any(most > 87.f), 0)) {
+        for (int c = 0; c < CH; ++c) most = fmaxf(most, fabsf(Lane<T, CH>::value(g[u], c)));
+    if (__builtin_expect(m == U && !__any(most > kNear), 1)) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int c = 0; c < kChannels<T>; ++c) {
-                const float v = (float)g[u][c];  // a gate's bits do not depend on its neighbours
-                s[u][c] = fabsf(v) <= 87.f ? gate_of<SIGMOID, true>(v) : gate_of<SIGMOID, false>(v);
-            }
+            for (int c = 0; c < CH; ++c) f(u, c, gate_of<SIGMOID, true>(Lane<T, CH>::value(g[u], c)));
     } else {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int c = 0; c < kChannels<T>; ++c) s[u][c] = gate_of<SIGMOID, true>((float)g[u][c]);
+            for (int c = 0; c < CH; ++c) f(u, c, u < m ? gate_of<SIGMOID, false>(Lane<T, CH>::value(g[u], c)) : Gate{-0.f, 0.f});
     }
 }
 
-// Calls f(u) for the wave's tokens u = 0 .. m - 1, or the other way round.
-template <bool BACK, typename F>
-__device__ __forceinline__ void each(int m, F f) {
-    if (m == U) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) f(BACK ? U - 1 - u : u);
-    } else {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if ((BACK ? U - 1 - u : u) < m) f(BACK ? U - 1 - u : u);
+// The product of decays: a, and low = 1 - a.
+struct Product {
+    float a = 1.f, low = 0.f;
+    __device__ __forceinline__ void by(float s, float w) {
+        a = decayed(s, a);
+        low = decayed(s, low) + w;
     }
-}
+    // The smaller of both, as a gate has it.
+    __device__ __forceinline__ float smaller() const { return low < 0.5f ? -low : a; }
+};
 
-// What the wave's tokens make of a state: in(u, c) is what token u adds to it
-// behind its decay (forward) or in front of it (BACK).
-template <typename T, bool BACK, typename F>
-__device__ __forceinline__ void local(Join (&j)[kChannels<T>], const float (&s)[U][kChannels<T>], int m, F in) {
+// A block's waves' Joins one after the other (BACK: from the last on): h, the
+// state before the tile, becomes that before the wave, and v that behind the
+// tile. all: the whole segment's decay, where it is wanted.
+template <int CH, int W, bool BACK, bool ALL>
+__device__ __forceinline__ void fold(float (&h)[CH], float (&v)[CH], Product (&all)[CH], const Join (&at)[W][64][CH]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int c = 0; c < kChannels<T>; ++c) j[c] = Join{1.f, 0.f, 0.f};
-    each<BACK>(m, [&](int u) {
+    for (int c = 0; c < CH; ++c) v[c] = h[c];
 #pragma unroll
-        for (int c = 0; c < kChannels<T>; ++c) {
-            j[c].a = decayed(s[u][c], j[c].a);
-            j[c].low = decayed(s[u][c], j[c].low) + short_of(s[u][c]);
-            j[c].h = BACK ? decayed(s[u][c], j[c].h + in(u, c)) : decayed(s[u][c], j[c].h) + in(u, c);
+    for (int i = 0; i < W; ++i) {
+        const int w = BACK ? W - 1 - i : i;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const Join k = at[w][lane][c];
+            h[c] = w == wave ? v[c] : h[c];
+            v[c] = k(v[c]);
+            if constexpr (ALL) all[c].by(k.s, short_of(k.s));
         }
-    });
+    }
 }
 
 // Segment z of a call: tokens z length .. + length.
 struct Cut {
     int length, segments;
 };
-// Place of a segment's Join of a channel in the workspace: [3][batch][segment][channel].
+// Place of a segment's Joins in the workspace: [2][batch][segment][channel].
 __device__ __forceinline__ float* join_at(const RecurrenceArgs& a, const Cut& cut, int part, int b, int z) {
     return a.work + (((long long)part * a.batch + b) * cut.segments + z) * a.channels;
 }
 
-// W waves a block, one behind the other in time. JOIN: the segment's Join alone,
-// nothing else written.
-template <typename T, bool SIGMOID, bool COMPLEMENT, int W, bool JOIN>
-__global__ __launch_bounds__(64 * W) void k_recurrence(const RecurrenceArgs a, const Cut cut) {
-    constexpr int CH = kChannels<T>;
-    __shared__ Join lds[W > 1 ? 2 : 1][W][CH][64];
-    const Lane<T> lane(a.channels);
-    const int b = blockIdx.y, z = blockIdx.z, l = threadIdx.x & 63;
-    const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-    const int n = clamped(a.lengths, b, a.tokens);
-    const int begin = z * cut.length, end = (int)std::min(a.tokens, (long long)begin + cut.length), live = std::min(n, end);
-    float h[CH];  // the state before the block's tokens
-    Join all[CH];
-    if constexpr (JOIN) {
+// The state that reaches segment z from those before it (BACK: behind it).
+template <typename T, int CH, bool BACK>
+__device__ __forceinline__ void arrive(float (&h)[CH], const Lane<T, CH>& lane, const RecurrenceArgs& a, const Cut& cut, int b, int z, int n) {
+    lane.load_state(h, a.state_in ? a.state_in + (long long)b * a.channels : nullptr);
+    const int live = (n + cut.length - 1) / cut.length;  // segments with tokens
+    for (int i = BACK ? live - 1 : 0; BACK ? i > z : i < z && i < live; i += BACK ? -1 : 1) {
+        float s[CH], v[CH];
+        lane.load_state(s, join_at(a, cut, 0, b, i));
+        lane.load_state(v, join_at(a, cut, 1, b, i));
 #pragma unroll
-        for (int c = 0; c < CH; ++c) all[c] = Join{1.f, 0.f, 0.f}, h[c] = 0.f;
-    } else {
-        lane.load_state(h, a.state_in ? a.state_in + (long long)b * a.channels : nullptr);
-        for (int i = 0; i < z && i * cut.length < n; ++i) {
-            float v[3][CH];
-#pragma unroll
-            for (int p = 0; p < 3; ++p) lane.load_state(v[p], join_at(a, cut, p, b, i));
-#pragma unroll
-            for (int c = 0; c < CH; ++c) h[c] = Join{v[0][c], v[1][c], v[2][c]}(h[c]);
-        }
-    }
-    const long long spans = (a.tokens + U - 1) / U;
-    typename Lane<T>::Vec x[U], g[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = g[u] = (T)0.f;
-    const auto tokens_of = [&](int t) { return std::max(0, std::min(live - t, U)); };
-    const int stop = JOIN ? live : end;
-    {
-        const int t = begin + wave * U, m = tokens_of(t);
-        lane.fetch(x, a.x, b, t, m);
-        lane.fetch(g, a.gate, b, t, m);
-    }
-    for (int t0 = begin, half = 0; t0 < stop; t0 += W * U, half ^= 1) {
-        const int t = t0 + wave * U, m = tokens_of(t);
-        float s[U][CH], in[U][CH];
-        gates<T, SIGMOID>(s, g);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int c = 0; c < CH; ++c) in[u][c] = COMPLEMENT ? short_of(s[u][c]) * (float)x[u][c] : (float)x[u][c];
-        if (t0 + W * U < stop) {
-            const int next = t + W * U, k = tokens_of(next);
-            lane.fetch(x, a.x, b, next, k);
-            lane.fetch(g, a.gate, b, next, k);
-        }
-        if constexpr (W > 1 || JOIN) {
-            Join j[CH];
-            local<T, false>(j, s, m, [&](int u, int c) { return in[u][c]; });
-            if constexpr (W > 1) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) lds[half][wave][c][l] = j[c];
-                __syncthreads();
-            }
-            const int waves = W > 1 ? std::min(W, (live - t0 + U - 1) / U) : 1;  // that have tokens
-            float v[CH];
-#pragma unroll
-            for (int c = 0; c < CH; ++c) v[c] = h[c];
-            for (int i = 0; i < waves; ++i)
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const Join k = W > 1 ? lds[half][i][c][l] : j[c];
-                    if (i == wave) h[c] = v[c];
-                    v[c] = k(v[c]);
-                    if constexpr (JOIN) {
-                        all[c].low = Join{k.a, k.low, k.low}(all[c].low);
-                        all[c].a *= k.a;
-                    }
-                }
-            if constexpr (JOIN) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) h[c] = v[c];
-                continue;
-            }
-            if (wave >= waves)
-#pragma unroll
-                for (int c = 0; c < CH; ++c) h[c] = v[c];
-            if (a.saved && t < end) lane.store_state(a.saved + ((long long)b * spans + t / U) * a.channels, h);
-            T* row = (T*)a.y.p + b * a.y.batch + t * a.y.token + lane.first;
-            each<false>(m, [&](int u) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) h[c] = decayed(s[u][c], h[c]) + in[u][c];
-                lane.store(row + u * a.y.token, h);
-            });
-            const float zero[CH] = {};
-            for (int u = m; u < U && t + u < end; ++u) lane.store(row + u * a.y.token, zero);
-#pragma unroll
-            for (int c = 0; c < CH; ++c) h[c] = v[c];
-        } else {
-            if (a.saved) lane.store_state(a.saved + ((long long)b * spans + t / U) * a.channels, h);
-            T* row = (T*)a.y.p + b * a.y.batch + t * a.y.token + lane.first;
-            each<false>(m, [&](int u) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) h[c] = decayed(s[u][c], h[c]) + in[u][c];
-                lane.store(row + u * a.y.token, h);
-            });
-            const float zero[CH] = {};
-            for (int u = m; u < U && t + u < end; ++u) lane.store(row + u * a.y.token, zero);
-        }
-    }
-    if (wave) return;
-    if constexpr (JOIN) {
-        float v[CH];
-#pragma unroll
-        for (int c = 0; c < CH; ++c) v[c] = all[c].a;
-        lane.store_state(join_at(a, cut, 0, b, z), v);
-#pragma unroll
-        for (int c = 0; c < CH; ++c) v[c] = all[c].low;
-        lane.store_state(join_at(a, cut, 1, b, z), v);
-        lane.store_state(join_at(a, cut, 2, b, z), h);
-    } else if (z == cut.segments - 1 && a.state_out) {
-        lane.store_state(a.state_out + (long long)b * a.channels, h);
+        for (int c = 0; c < CH; ++c) h[c] = Join{s[c], v[c]}(h[c]);
     }
 }
 
-// The same backwards: h is the gradient that arrives from the tokens behind.
-template <typename T, bool SIGMOID, bool COMPLEMENT, int W, bool JOIN>
-__global__ __launch_bounds__(64 * W) void k_recurrence_back(const RecurrenceArgs a, const Cut cut) {
-    constexpr int CH = kChannels<T>;
-    __shared__ Join lds[W > 1 ? 2 : 1][W][CH][64];
-    const Lane<T> lane(a.channels);
-    const int b = blockIdx.y, z = blockIdx.z, l = threadIdx.x & 63;
-    const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+// W waves a block, one behind the other in time. JOIN: the segment's Joins alone,
+// nothing else written.
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, int W, bool JOIN>
+__global__ __launch_bounds__(64 * W) void k_recurrence(const RecurrenceArgs a, const Cut cut) {
+    __shared__ Join lds[2][W][64][CH];
+    const Lane<T, CH> lane(a.channels);
+    const int b = blockIdx.y, z = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = clamped(a.lengths, b, a.tokens);
     const int begin = z * cut.length, end = (int)std::min(a.tokens, (long long)begin + cut.length), live = std::min(n, end);
-    float h[CH];
-    Join all[CH];
-    if constexpr (JOIN) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) all[c] = Join{1.f, 0.f, 0.f}, h[c] = 0.f;
-    } else {
-        lane.load_state(h, a.state_in ? a.state_in + (long long)b * a.channels : nullptr);
-        for (int i = std::min(cut.segments, (n + cut.length - 1) / cut.length) - 1; i > z; --i) {
-            float v[3][CH];
-#pragma unroll
-            for (int p = 0; p < 3; ++p) lane.load_state(v[p], join_at(a, cut, p, b, i));
-#pragma unroll
-            for (int c = 0; c < CH; ++c) h[c] = Join{v[0][c], v[1][c], v[2][c]}(h[c]);
-        }
-    }
     const long long spans = (a.tokens + U - 1) / U;
-    typename Lane<T>::Vec x[U], g[U], dy[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = g[u] = dy[u] = (T)0.f;
-    const auto tokens_of = [&](int t) { return std::max(0, std::min(live - t, U)); };
+    float h[CH] = {};  // the state before the tile
+    Product all[CH];
+    if constexpr (!JOIN) arrive<T, CH, false>(h, lane, a, cut, b, z, n);
+    unsigned x[U] = {}, g[U] = {};
     const auto fetch = [&](int t) {
-        const int m = tokens_of(t);
-        if constexpr (!JOIN) lane.fetch(x, a.x, b, t, m);
-        lane.fetch(g, a.gate, b, t, m);
-        lane.fetch(dy, a.dy, b, t, m);
+        lane.fetch(x, a.x, b, t, live - t);
+        lane.fetch(g, a.gate, b, t, live - t);
     };
-    const int stop = JOIN ? live : end, tiles = (std::max(0, stop - begin) + W * U - 1) / (W * U);
-    if (tiles) fetch(begin + (tiles - 1) * (W * U) + wave * U);
-    for (int i = tiles - 1, half = 0; i >= 0; --i, half ^= 1) {
-        const int t0 = begin + i * (W * U), t = t0 + wave * U, m = tokens_of(t);
-        float s[U][CH], p[U][CH], d[U][CH];
-        gates<T, SIGMOID>(s, g);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int c = 0; c < CH; ++c) d[u][c] = (float)dy[u][c];
-        if constexpr (!JOIN) {
-            float v[CH];  // the state before each token
-            lane.load_state(v, m ? a.saved + ((long long)b * spans + t / U) * a.channels : nullptr);
-            each<false>(m, [&](int u) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const float xv = (float)x[u][c];
-                    p[u][c] = COMPLEMENT ? v[c] - xv : v[c];
-                    if (!SIGMOID && (float)g[u][c] > 0.f) p[u][c] = 0.f;
-                    v[c] = decayed(s[u][c], v[c]) + (COMPLEMENT ? short_of(s[u][c]) * xv : xv);
-                }
-            });
-        }
-        if (i > 0) fetch(t - W * U);
-        float v[CH];
-        if constexpr (W > 1 || JOIN) {
-            Join j[CH];
-            local<T, true>(j, s, m, [&](int u, int c) { return d[u][c]; });
-            if constexpr (W > 1) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) lds[half][wave][c][l] = j[c];
-                __syncthreads();
+    fetch(begin + wave * U);
+    int t0 = begin;
+    for (int half = 0; t0 < live; t0 += W * U, half ^= 1) {
+        const int t = t0 + wave * U, m = std::min(live - t, U);
+        // what the wave's tokens make of a state: p a + l
+        float s[U][CH], in[U][CH], l[CH] = {}, after[CH];
+        Product p[CH];
+        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate q) {
+            s[u][c] = q.s;
+            in[u][c] = COMPLEMENT ? q.w * lane.value(x[u], c) : u < m ? lane.value(x[u], c) : 0.f;
+            if constexpr (W > 1 || JOIN) {
+                p[c].by(q.s, q.w);
+                l[c] = decayed(q.s, l[c]) + in[u][c];
             }
-            const int waves = W > 1 ? std::min(W, (live - t0 + U - 1) / U) : 1;
+        });
+        fetch(t + W * U);
+        if constexpr (W > 1 || JOIN) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) v[c] = h[c];
-            for (int k = waves - 1; k >= 0; --k)
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const Join q = W > 1 ? lds[half][k][c][l] : j[c];
-                    if (k == wave) h[c] = v[c];
-                    v[c] = q(v[c]);
-                    if constexpr (JOIN) {
-                        all[c].low = Join{q.a, q.low, q.low}(all[c].low);
-                        all[c].a *= q.a;
-                    }
-                }
+            for (int c = 0; c < CH; ++c) lds[half][threadIdx.x >> 6][threadIdx.x & 63][c] = Join{p[c].smaller(), l[c]};
+            __syncthreads();
+            fold<CH, W, false, JOIN>(h, after, all, lds[half]);
         }
         if constexpr (!JOIN) {
-            T* dx = (T*)a.y.p + b * a.y.batch + t * a.y.token + lane.first;
-            T* dg = (T*)a.dgate.p + b * a.dgate.batch + t * a.dgate.token + lane.first;
-            each<true>(m, [&](int u) {
-                float to_x[CH], to_g[CH];
+            if (a.saved && t < end) lane.store_state(a.saved + ((long long)b * spans + t / U) * a.channels, h);
+            T* row = (T*)a.y.p + b * a.y.batch + t * a.y.token + lane.first;
 #pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const float q = s[u][c], w = short_of(q), D = d[u][c] + h[c];
-                    to_x[c] = COMPLEMENT ? w * D : D;
-                    const float slope = SIGMOID ? fabsf(q) * (1.f - fabsf(q)) : decayed(q, 1.f);
-                    to_g[c] = D * p[u][c] * slope;
-                    h[c] = decayed(q, D);
-                }
-                lane.store(dx + u * a.y.token, to_x);
-                lane.store(dg + u * a.dgate.token, to_g);
-            });
-            const float zero[CH] = {};
-            for (int u = m; u < U && t + u < end; ++u) {
-                lane.store(dx + u * a.y.token, zero);
-                lane.store(dg + u * a.dgate.token, zero);
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) in[u][c] = h[c] = decayed(s[u][c], h[c]) + in[u][c];
+            if (m == U) {
+                if (lane.have)
+#pragma unroll
+                    for (int u = 0; u < U; ++u, row = behind(row, a.y.token)) lane.store(row, in[u]);
+            } else {
+                if (lane.have)
+#pragma unroll
+                    for (int u = 0; u < U; ++u, row = behind(row, a.y.token))
+                        if (u < m) lane.store(row, in[u]);
+                lane.clear(a.y, b, t + std::max(m, 0), std::min(end - t, U) - std::max(m, 0));
             }
         }
         if constexpr (W > 1 || JOIN)
 #pragma unroll
-            for (int c = 0; c < CH; ++c) h[c] = v[c];
+            for (int c = 0; c < CH; ++c) h[c] = after[c];
     }
-    if (wave) return;
     if constexpr (JOIN) {
-        float v[CH];
+        if (wave) return;
+        float decay[CH];
 #pragma unroll
-        for (int c = 0; c < CH; ++c) v[c] = all[c].a;
-        lane.store_state(join_at(a, cut, 0, b, z), v);
-#pragma unroll
-        for (int c = 0; c < CH; ++c) v[c] = all[c].low;
-        lane.store_state(join_at(a, cut, 1, b, z), v);
-        lane.store_state(join_at(a, cut, 2, b, z), h);
-    } else if (!z && a.state_out) {
-        lane.store_state(a.state_out + (long long)b * a.channels, h);
+        for (int c = 0; c < CH; ++c) decay[c] = all[c].smaller();
+        lane.store_state(join_at(a, cut, 0, b, z), decay);
+        lane.store_state(join_at(a, cut, 1, b, z), h);
+    } else {
+        for (int t = t0 + wave * U; t < end; t += W * U) {  // past the sequence
+            if (a.saved) lane.store_state(a.saved + ((long long)b * spans + t / U) * a.channels, h);
+            lane.clear(a.y, b, t, std::min(end - t, U));
+        }
+        if (!wave && z == cut.segments - 1 && a.state_out) lane.store_state(a.state_out + (long long)b * a.channels, h);
     }
 }
 
-constexpr int kCutBlocks = 4;  // a CU, that segments may make
+// The same backwards: h is the gradient that arrives from the tokens behind.
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, int W, bool JOIN>
+__global__ __launch_bounds__(64 * W) void k_recurrence_back(const RecurrenceArgs a, const Cut cut) {
+    __shared__ Join lds[2][W][64][CH];
+    const Lane<T, CH> lane(a.channels);
+    const int b = blockIdx.y, z = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = clamped(a.lengths, b, a.tokens);
+    const int begin = z * cut.length, end = (int)std::min(a.tokens, (long long)begin + cut.length), live = std::min(n, end);
+    const long long spans = (a.tokens + U - 1) / U;
+    float h[CH] = {};
+    Product all[CH];
+    if constexpr (!JOIN) arrive<T, CH, true>(h, lane, a, cut, b, z, n);
+    unsigned x[U] = {}, g[U] = {}, dy[U] = {};
+    const auto fetch = [&](int t) {
+        if constexpr (!JOIN) lane.fetch(x, a.x, b, t, live - t);
+        lane.fetch(g, a.gate, b, t, live - t);
+        lane.fetch(dy, a.dy, b, t, live - t);
+    };
+    const int tiles = (std::max(0, live - begin) + W * U - 1) / (W * U);
+    if (tiles) fetch(begin + (tiles - 1) * (W * U) + wave * U);
+    for (int i = tiles - 1, half = 0; i >= 0; --i, half ^= 1) {
+        const int t = begin + i * (W * U) + wave * U, m = std::min(live - t, U);
+        float s[U][CH], p[U][CH], v[CH], l[CH] = {}, after[CH];  // v: the state before each token
+        Product q[CH];
+        unsigned d[U];
+        if constexpr (!JOIN) lane.load_state(v, m > 0 ? a.saved + ((long long)b * spans + t / U) * a.channels : nullptr);
+        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate k) {
+            s[u][c] = k.s;
+            if constexpr (W > 1 || JOIN) q[c].by(k.s, k.w);
+            if constexpr (!JOIN) {
+                const float xv = lane.value(x[u], c);
+                p[u][c] = COMPLEMENT ? v[c] - xv : v[c];
+                if (!SIGMOID && lane.value(g[u], c) > 0.f) p[u][c] = 0.f;
+                v[c] = decayed(k.s, v[c]) + (COMPLEMENT ? k.w * xv : xv);
+            }
+        });
+#pragma unroll
+        for (int u = 0; u < U; ++u) d[u] = dy[u];
+        if (m < U)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (u >= m) d[u] = 0;
+        if (i > 0) fetch(t - W * U);
+        if constexpr (W > 1 || JOIN) {
+#pragma unroll
+            for (int u = U - 1; u >= 0; --u)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) l[c] = decayed(s[u][c], l[c] + lane.value(d[u], c));
+#pragma unroll
+            for (int c = 0; c < CH; ++c) lds[half][threadIdx.x >> 6][threadIdx.x & 63][c] = Join{q[c].smaller(), l[c]};
+            __syncthreads();
+            fold<CH, W, true, JOIN>(h, after, all, lds[half]);
+        }
+        if constexpr (!JOIN) {
+            T* dx = (T*)a.y.p + b * a.y.batch + (t + U - 1) * a.y.token + lane.first;
+            T* dg = (T*)a.dgate.p + b * a.dgate.batch + (t + U - 1) * a.dgate.token + lane.first;
+            const auto gradients = [&](int u, float (&to_x)[CH], float (&to_g)[CH]) {
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const float k = s[u][c], D = lane.value(d[u], c) + h[c];
+                    to_x[c] = COMPLEMENT ? short_of(k) * D : D;
+                    to_g[c] = p[u][c] * D * (SIGMOID ? fabsf(k) * (1.f - fabsf(k)) : decayed(k, 1.f));
+                    h[c] = decayed(k, D);
+                }
+            };
+            float to_x[CH], to_g[CH];
+            if (m == U) {
+                if (lane.have)
+#pragma unroll
+                    for (int u = U - 1; u >= 0; --u, dx = behind(dx, -a.y.token), dg = behind(dg, -a.dgate.token)) {
+                        gradients(u, to_x, to_g);
+                        lane.store(dx, to_x);
+                        lane.store(dg, to_g);
+                    }
+            } else if (lane.have) {
+#pragma unroll
+                for (int u = U - 1; u >= 0; --u, dx = behind(dx, -a.y.token), dg = behind(dg, -a.dgate.token))
+                    if (u < m) {
+                        gradients(u, to_x, to_g);
+                        lane.store(dx, to_x);
+                        lane.store(dg, to_g);
+                    }
+            }
+        }
+        if constexpr (W > 1 || JOIN)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) h[c] = after[c];
+    }
+    if constexpr (JOIN) {
+        if (wave) return;
+        float decay[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) decay[c] = all[c].smaller();
+        lane.store_state(join_at(a, cut, 0, b, z), decay);
+        lane.store_state(join_at(a, cut, 1, b, z), h);
+    } else {
+        for (int t = std::max(begin, live) + wave * U; t < end; t += W * U) {  // past the sequence
+            lane.clear(a.y, b, t, std::min(end - t, U));
+            lane.clear(a.dgate, b, t, std::min(end - t, U));
+        }
+        if (!wave && !z && a.state_out) lane.store_state(a.state_out + (long long)b * a.channels, h);
+    }
+}
 
-template <typename T, bool SIGMOID, bool COMPLEMENT, int W>
+// Blocks a CU that segments may make.
+constexpr int kCutBlocks = 2;
+
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, int W>
 int launch_as(const RecurrenceArgs& a, hipStream_t s, bool back) {
-    const long long columns = (a.channels + 64 * kChannels<T> - 1) / (64 * kChannels<T>);
+    const long long columns = (a.channels + 64 * CH - 1) / (64 * CH);
     const dim3 block(64 * W);
     Cut cut{(int)std::max(a.tokens, 1ll), 1};
     if constexpr (W >= 8) {
-        const long long tile = W * U, most = (long long)a.cus * (16 / W) / (columns * a.batch);
+        const long long tile = W * U, most = (long long)a.cus * kCutBlocks / (columns * a.batch);
         const long long segments = std::min(most, a.tokens / (2 * tile));
         if (segments > 1) {
             cut.length = (int)((a.tokens + segments * tile - 1) / (segments * tile) * tile);
             cut.segments = (int)((a.tokens + cut.length - 1) / cut.length);
         }
         if (cut.segments > 1) {
-            const auto kernel = back ? k_recurrence_back<T, SIGMOID, COMPLEMENT, W, true> : k_recurrence<T, SIGMOID, COMPLEMENT, W, true>;
+            const auto kernel = back ? k_recurrence_back<T, CH, SIGMOID, COMPLEMENT, W, true> : k_recurrence<T, CH, SIGMOID, COMPLEMENT, W, true>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)columns, (unsigned)a.batch, (unsigned)cut.segments), block, 0, s, a, cut);
         }
     }
-    const auto kernel = back ? k_recurrence_back<T, SIGMOID, COMPLEMENT, W, false> : k_recurrence<T, SIGMOID, COMPLEMENT, W, false>;
+    const auto kernel = back ? k_recurrence_back<T, CH, SIGMOID, COMPLEMENT, W, false> : k_recurrence<T, CH, SIGMOID, COMPLEMENT, W, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)columns, (unsigned)a.batch, (unsigned)cut.segments), block, 0, s, a, cut);
     return (int)hipGetLastError();
 }
 
-template <typename T, bool SIGMOID, bool COMPLEMENT>
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT>
 int launch_waves(const RecurrenceArgs& a, hipStream_t s, bool back) {
-    if (a.tokens <= U) return launch_as<T, SIGMOID, COMPLEMENT, 1>(a, s, back);
-    if (a.tokens <= 4 * U) return launch_as<T, SIGMOID, COMPLEMENT, 4>(a, s, back);
-    return launch_as<T, SIGMOID, COMPLEMENT, 8>(a, s, back);
+    if (a.tokens <= U) return launch_as<T, CH, SIGMOID, COMPLEMENT, 1>(a, s, back);
+    if (a.tokens <= 4 * U) return launch_as<T, CH, SIGMOID, COMPLEMENT, 4>(a, s, back);
+    return launch_as<T, CH, SIGMOID, COMPLEMENT, 8>(a, s, back);
 }
 
-template <typename T>
+template <typename T, int CH>
 int launch_gate(const RecurrenceArgs& a, hipStream_t s, bool back) {
-    if (a.gate_kind == VKFX_GATE_SIGMOID) return a.complement ? launch_waves<T, true, true>(a, s, back) : launch_waves<T, true, false>(a, s, back);
-    return a.complement ? launch_waves<T, false, true>(a, s, back) : launch_waves<T, false, false>(a, s, back);
+    if (a.gate_kind == VKFX_GATE_SIGMOID) return a.complement ? launch_waves<T, CH, true, true>(a, s, back) : launch_waves<T, CH, true, false>(a, s, back);
+    return a.complement ? launch_waves<T, CH, false, true>(a, s, back) : launch_waves<T, CH, false, false>(a, s, back);
+}
+
+// Two 16-bit channels a lane where every pair of them is a word.
+template <typename T>
+int launch_channels(const RecurrenceArgs& a, hipStream_t s, bool back) {
+    uintptr_t all = (uintptr_t)a.channels * 2;
+    for (const RecurrenceSide* x : {&a.x, &a.gate, &a.dy, &a.y, &a.dgate}) all |= (uintptr_t)x->p | (uintptr_t)(x->batch * 2) | (uintptr_t)(x->token * 2);
+    return all % 4 ? launch_gate<T, 1>(a, s, back) : launch_gate<T, 2>(a, s, back);
 }
 
 int launch_element(const RecurrenceArgs& a, hipStream_t s, bool back) {
-    if (a.element == VKFX_ELEMENT_F32) return launch_gate<float>(a, s, back);
-    if (a.element == VKFX_ELEMENT_F16) return launch_gate<_Float16>(a, s, back);
-    return launch_gate<__bf16>(a, s, back);
+    if (a.element == VKFX_ELEMENT_F32) return launch_gate<float, 1>(a, s, back);
+    if (a.element == VKFX_ELEMENT_F16) return launch_channels<_Float16>(a, s, back);
+    return launch_channels<__bf16>(a, s, back);
 }
 
 }  // namespace
@@ -493,6 +473,6 @@ int launch_element(const RecurrenceArgs& a, hipStream_t s, bool back) {
 int launch_recurrence_forward(const RecurrenceArgs& a, hipStream_t s) { return launch_element(a, s, false); }
 int launch_recurrence_backward(const RecurrenceArgs& a, hipStream_t s) { return launch_element(a, s, true); }
 // segments times columns is at most kCutBlocks a CU, of up to 128 channels each
-size_t recurrence_workspace_bytes(int, long long, int cus) { return (size_t)cus * kCutBlocks * 128 * 3 * sizeof(float); }
+size_t recurrence_workspace_bytes(int, long long, int cus) { return (size_t)cus * kCutBlocks * 128 * 2 * sizeof(float); }
 
 }  // namespace vkfx
