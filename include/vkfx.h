@@ -571,11 +571,12 @@ typedef struct {
 int vkfx_gated_recurrence_create(vkfx_context *ctx, const vkfx_gated_recurrence_desc *desc,
                                  vkfx_gated_recurrence **out);
 int vkfx_gated_recurrence_destroy(vkfx_gated_recurrence *plan);
-/* Bytes of the scratch a caller may pass, for any number of sequences and tokens. */
+/* Bytes of the scratch a caller may pass, aligned to 16 bytes, for any number of
+ * sequences and tokens. */
 int vkfx_gated_recurrence_workspace_bytes(const vkfx_gated_recurrence *plan, uint64_t *out);
 
 /* saved (NULL: not wanted), for the backward pass: the states before tokens 0, 16,
- * 32, ..., [batch][(tokens + 15) / 16][channels] floats. */
+ * 32, ... before a sequence's length, [batch][(tokens + 15) / 16][channels] floats. */
 #define VKFX_RECURRENCE_SPAN 16
 
 /* `tokens` may be 1 (the next token of each sequence), as many as a prompt has,

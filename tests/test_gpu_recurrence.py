@@ -381,7 +381,7 @@ def test_streams_workspaces_and_repeats(hip_ctx, t, lengths):
 
     def make():
         return [torch.empty_like(x) for _ in range(3)] + [torch.empty(2, 90, device="cuda") for _ in range(2)] \
-            + [torch.empty(plan.saved_shape(2, t), device="cuda")]
+            + [torch.full(plan.saved_shape(2, t), 7.0, device="cuda")]
 
     def run(o, **kw):
         plan.forward_tensors(x, gate, o[0], state_out=o[3], saved=o[5], lengths=n, **kw)
@@ -390,6 +390,8 @@ def test_streams_workspaces_and_repeats(hip_ctx, t, lengths):
     want = make()
     run(want)
     torch.cuda.synchronize()
+    for i, m in enumerate(lengths or []):  # saved states end with their sequence
+        assert (want[5][i, -(-m // plan.SPAN):] == 7).all()
     streams = [torch.cuda.Stream() for _ in range(3)]
     got = [make() for _ in streams]
     work = [torch.empty(max(1, plan.workspace_bytes), device="cuda", dtype=torch.uint8) for _ in streams]

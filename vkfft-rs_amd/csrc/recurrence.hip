@@ -6,14 +6,13 @@
 //   D[t] = dy[t] + E[t+1],  dx = m D,  da = D (h[t-1] - (m = 1 - a ? x : 0))
 // and dgate = da a (1 - a) or da a.
 //
-// Bound by memory, where the sequence is long enough to be read side by side. A
-// lane has 4 bytes of channels, a wave 16 tokens of them in its registers: it
+// A lane has 4 bytes of channels, a wave 16 tokens of them in its registers: it
 // forms what they make of any state before them (state -> A state + H), a
 // block's waves, one behind the other in time, fold these in LDS, and each goes
-// over its tokens once more from the state that it now knows. The next 16 times
-// as many tokens are on their way meanwhile. Where channels are too few to fill
-// the machine, a sequence is cut into segments whose (A, H) an earlier launch
-// forms.
+// over its tokens once more from the state that it now knows. So everything is
+// read once. Where sequences and channels fill the machine, a block goes along
+// its sequence with the next tokens on their way; where they do not, a sequence
+// is a chain of blocks that hand (A, H) on through memory.
 //
 // A decay near 1 is kept as what it is short of 1: rounded to 24 bits itself, a
 // memory of n tokens would be off by n 2^-25 of its length. So is A.
@@ -29,14 +28,12 @@ namespace vkfx {
 namespace {
 
 constexpr int U = kSpan;  // tokens of a wave
+constexpr float kNear = 87.f;
 
-// exp(g), off by 2^-22 of it, for -87 <= g <= 0: the product with log2(e) keeps
-// its rounding.
+// exp(g), off by 2^-22 of it, for -87 <= g <= 0: 2^t with what t's rounding left.
 __device__ __forceinline__ float exp_near(float g) {
-    constexpr float log2e = 1.44269502f, rest = 1.92596299e-8f;
-    const float t = g * log2e, low = fmaf(g, rest, fmaf(g, log2e, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, low * 0.693147181f, e);
+    const float t = g * 1.44269504f, e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, fmaf(t, -0.693147181f, g), e);
 }
 // exp(g) - 1 for -ln 2 < g <= 0: its series, the next term below 2^-26 of it.
 __device__ __forceinline__ float exp_less_1(float g) {
@@ -58,7 +55,6 @@ __device__ __forceinline__ float exp_less_1(float g) {
 struct Gate {
     float s, w;
 };
-constexpr float kNear = 87.f;
 template <bool NEAR>
 __device__ __forceinline__ float exp_of(float g) {
     if (NEAR || !(g < -kNear)) return exp_near(g);
@@ -94,6 +90,12 @@ __device__ __forceinline__ int clamped(const int* lengths, int b, long long toke
     return __builtin_amdgcn_readfirstlane((int)(n < 0 ? 0 : n < tokens ? n : tokens));
 }
 
+// A count of its own for the compiler, which would form what follows from it
+// once for all places, and keep that in scalar registers.
+__device__ __forceinline__ int apart(int m) {
+    asm volatile("" : "+s"(m));
+    return m;
+}
 // The next row. Kept from the compiler, which would hold every row's place in
 // scalar registers, and these, past 100 of them, in lanes of vector registers.
 template <typename T>
@@ -115,22 +117,40 @@ struct Lane {
     int at;           // the lane's
     bool have;
 
-    __device__ __forceinline__ explicit Lane(long long channels) {
-        first = (long long)blockIdx.x * (64 * CH);
+    __device__ __forceinline__ Lane(unsigned column, long long channels) {
+        first = (long long)column * (64 * CH);
         have = first + (threadIdx.x & 63) * CH < channels;
         at = have ? (threadIdx.x & 63) * CH : 0;
     }
     // Tokens t .. t + m - 1 of sequence b, the last one again behind them.
     __device__ __forceinline__ void fetch(unsigned (&r)[U], const RecurrenceSide& s, long long b, long long t, int m) const {
-        if (m <= 0) return;
         const T* row = (const T*)s.p + b * s.batch + t * s.token + first;
+        if (m >= U) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            r[u] = *(const Raw*)(row + at);
-            row += u + 1 < m ? s.token : 0;
+            for (int u = 0; u < U; ++u, row = behind(row, s.token)) r[u] = *(const Raw*)(row + at);
+        } else if (m > 0) {
+            m = apart(m);
+#pragma unroll
+            for (int u = 0; u < U; ++u, row = behind(row, u < m ? s.token : 0)) r[u] = *(const Raw*)(row + at);
         }
     }
     __device__ __forceinline__ static float value(unsigned r, int c) { return (float)__builtin_bit_cast(Vec, (Raw)r)[c]; }
+    // Whether an element is past kNear; of 16 bits by its bits, two at a time.
+    __device__ __forceinline__ static bool far(const unsigned (&r)[U]) {
+        if constexpr (sizeof(T) == 4) {
+            float most = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) most = fmaxf(most, fabsf(value(r[u], 0)));
+            return most > kNear;
+        } else {
+            typedef unsigned short Pair __attribute__((ext_vector_type(2)));
+            Pair most = {0, 0};
+#pragma unroll
+            for (int u = 0; u < U; ++u) most = __builtin_elementwise_max(most, __builtin_bit_cast(Pair, r[u] & 0x7fff7fffu));
+            constexpr unsigned short limit = __builtin_bit_cast(unsigned short, (T)kNear);
+            return most[0] > limit || most[1] > limit;
+        }
+    }
     __device__ __forceinline__ void store(T* row, const float (&y)[CH]) const {
         Vec r;
 #pragma unroll
@@ -158,17 +178,13 @@ struct Lane {
 // past kNear; otherwise tokens from m on leave every state as it is.
 template <typename T, int CH, bool SIGMOID, typename F>
 __device__ __forceinline__ void each_gate(const unsigned (&g)[U], int m, F f) {
-    float most = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int c = 0; c < CH; ++c) most = fmaxf(most, fabsf(Lane<T, CH>::value(g[u], c)));
-    if (__builtin_expect(m == U && !__any(most > kNear), 1)) {
+    if (__builtin_expect(m == U && !__any(Lane<T, CH>::far(g)), 1)) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int c = 0; c < CH; ++c) f(u, c, gate_of<SIGMOID, true>(Lane<T, CH>::value(g[u], c)));
     } else {
+        m = apart(m);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -187,11 +203,161 @@ struct Product {
     __device__ __forceinline__ float smaller() const { return low < 0.5f ? -low : a; }
 };
 
+// Which tokens a launch runs, and the states before and behind them (BACK: the
+// gradients behind and before them).
+struct Range {
+    int from, to;
+    const float* in;  // null: zeros
+    float* out;       // null: not wanted
+};
+
+// One block's tile: W waves of U tokens, the first at t0, those before `live` in
+// the sequence. Each wave's part of its work:
+//   fetch     the tokens on their way
+//   prepare   gates; what the wave makes of a state (with JOIN), in `join`
+//   finish    outputs, from h, the state before the wave's tokens
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, bool JOIN>
+struct Forward {
+    static constexpr bool BACK = false;
+    const RecurrenceArgs& a;
+    const Lane<T, CH>& lane;
+    const int b;
+    unsigned x[U] = {}, g[U] = {};
+    float s[U][CH], in[U][CH];
+    Join join[CH];
+
+    __device__ __forceinline__ Forward(const RecurrenceArgs& a, const Lane<T, CH>& lane, int b) : a(a), lane(lane), b(b) {}
+    __device__ __forceinline__ void fetch(int t, int live) {
+        lane.fetch(x, a.x, b, t, live - t);
+        lane.fetch(g, a.gate, b, t, live - t);
+    }
+    __device__ __forceinline__ void prepare(int t, int m) {
+        float l[CH] = {};
+        Product p[CH];
+        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate q) {
+            s[u][c] = q.s;
+            in[u][c] = COMPLEMENT ? q.w * lane.value(x[u], c) : u < m ? lane.value(x[u], c) : 0.f;
+            if constexpr (JOIN) {
+                p[c].by(q.s, q.w);
+                l[c] = decayed(q.s, l[c]) + in[u][c];
+            }
+        });
+#pragma unroll
+        for (int c = 0; c < CH; ++c) join[c] = Join{p[c].smaller(), l[c]};
+    }
+    __device__ __forceinline__ void finish(int t, int m, float (&h)[CH]) {
+        if (m <= 0) return;
+        const long long spans = (a.tokens + U - 1) / U;
+        if (a.saved) lane.store_state(a.saved + ((long long)b * spans + t / U) * a.channels, h);
+        T* row = (T*)a.y.p + b * a.y.batch + t * a.y.token + lane.first;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) in[u][c] = h[c] = decayed(s[u][c], h[c]) + in[u][c];
+        if (!lane.have) return;
+        if (m == U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u, row = behind(row, a.y.token)) lane.store(row, in[u]);
+        } else {
+            m = apart(m);
+#pragma unroll
+            for (int u = 0; u < U; ++u, row = behind(row, a.y.token))
+                if (u < m) lane.store(row, in[u]);
+        }
+    }
+    __device__ __forceinline__ void clear(int t, int rows) const { lane.clear(a.y, b, t, rows); }
+};
+
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, bool JOIN>
+struct Backward {
+    static constexpr bool BACK = true;
+    const RecurrenceArgs& a;
+    const Lane<T, CH>& lane;
+    const int b;
+    unsigned x[U] = {}, g[U] = {}, dy[U] = {};
+    float s[U][CH], p[U][CH];
+    unsigned d[U];
+    Join join[CH];
+
+    __device__ __forceinline__ Backward(const RecurrenceArgs& a, const Lane<T, CH>& lane, int b) : a(a), lane(lane), b(b) {}
+    __device__ __forceinline__ void fetch(int t, int live) {
+        lane.fetch(x, a.x, b, t, live - t);
+        lane.fetch(g, a.gate, b, t, live - t);
+        lane.fetch(dy, a.dy, b, t, live - t);
+    }
+    __device__ __forceinline__ void prepare(int t, int m) {
+        float v[CH], l[CH] = {};  // v: the state before each token
+        Product q[CH];
+        const long long spans = (a.tokens + U - 1) / U;
+        lane.load_state(v, m > 0 ? a.saved + ((long long)b * spans + t / U) * a.channels : nullptr);
+        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate k) {
+            s[u][c] = k.s;
+            if constexpr (JOIN) q[c].by(k.s, k.w);
+            const float xv = lane.value(x[u], c);
+            p[u][c] = COMPLEMENT ? v[c] - xv : v[c];
+            if (!SIGMOID && lane.value(g[u], c) > 0.f) p[u][c] = 0.f;
+            v[c] = decayed(k.s, v[c]) + (COMPLEMENT ? k.w * xv : xv);
+        });
+#pragma unroll
+        for (int u = 0; u < U; ++u) d[u] = dy[u];
+        if (m < U) {
+            m = apart(m);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (u >= m) d[u] = 0;
+        }
+        if constexpr (JOIN) {
+#pragma unroll
+            for (int u = U - 1; u >= 0; --u)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) l[c] = decayed(s[u][c], l[c] + lane.value(d[u], c));
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) join[c] = Join{q[c].smaller(), l[c]};
+    }
+    __device__ __forceinline__ void finish(int t, int m, float (&h)[CH]) {
+        if (m <= 0) return;
+        T* dx = (T*)a.y.p + b * a.y.batch + (t + U - 1) * a.y.token + lane.first;
+        T* dg = (T*)a.dgate.p + b * a.dgate.batch + (t + U - 1) * a.dgate.token + lane.first;
+        const auto gradients = [&](int u, float (&to_x)[CH], float (&to_g)[CH]) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const float k = s[u][c], D = lane.value(d[u], c) + h[c];
+                to_x[c] = COMPLEMENT ? short_of(k) * D : D;
+                to_g[c] = p[u][c] * D * (SIGMOID ? fabsf(k) * (1.f - fabsf(k)) : decayed(k, 1.f));
+                h[c] = decayed(k, D);
+            }
+        };
+        float to_x[CH], to_g[CH];
+        if (m == U) {
+            if (lane.have)
+#pragma unroll
+                for (int u = U - 1; u >= 0; --u, dx = behind(dx, -a.y.token), dg = behind(dg, -a.dgate.token)) {
+                    gradients(u, to_x, to_g);
+                    lane.store(dx, to_x);
+                    lane.store(dg, to_g);
+                }
+        } else if (lane.have) {
+            m = apart(m);
+#pragma unroll
+            for (int u = U - 1; u >= 0; --u, dx = behind(dx, -a.y.token), dg = behind(dg, -a.dgate.token))
+                if (u < m) {
+                    gradients(u, to_x, to_g);
+                    lane.store(dx, to_x);
+                    lane.store(dg, to_g);
+                }
+        }
+    }
+    __device__ __forceinline__ void clear(int t, int rows) const {
+        lane.clear(a.y, b, t, rows);
+        lane.clear(a.dgate, b, t, rows);
+    }
+};
+
 // A block's waves' Joins one after the other (BACK: from the last on): h, the
-// state before the tile, becomes that before the wave, and v that behind the
-// tile. all: the whole segment's decay, where it is wanted.
-template <int CH, int W, bool BACK, bool ALL>
-__device__ __forceinline__ void fold(float (&h)[CH], float (&v)[CH], Product (&all)[CH], const Join (&at)[W][64][CH]) {
+// state before the tile, becomes that before the wave, and v that behind the tile.
+template <int CH, int W, bool BACK>
+__device__ __forceinline__ void fold(float (&h)[CH], float (&v)[CH], const Join (&at)[W][64][CH]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int c = 0; c < CH; ++c) v[c] = h[c];
@@ -203,276 +369,269 @@ __device__ __forceinline__ void fold(float (&h)[CH], float (&v)[CH], Product (&a
             const Join k = at[w][lane][c];
             h[c] = w == wave ? v[c] : h[c];
             v[c] = k(v[c]);
-            if constexpr (ALL) all[c].by(k.s, short_of(k.s));
         }
     }
 }
 
-// Segment z of a call: tokens z length .. + length.
-struct Cut {
-    int length, segments;
+template <int CH>
+__device__ __forceinline__ void arrived(float (&h)[CH]) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) asm volatile("" : "+v"(h[c]));
+}
+
+// ---- a block along its sequence: blockIdx.x 64 CH channels, blockIdx.y the
+// sequence; W waves, one behind the other in time.
+
+template <typename T, int CH, int W, typename Pass>
+__device__ __forceinline__ void along(const RecurrenceArgs& a, const Range& r) {
+    __shared__ Join lds[2][W][64][CH];
+    const Lane<T, CH> lane(blockIdx.x, a.channels);
+    const int b = blockIdx.y, l = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int live = std::max(r.from, std::min(clamped(a.lengths, b, a.tokens), r.to)), tiles = (live - r.from + W * U - 1) / (W * U);
+    Pass pass(a, lane, b);
+    float h[CH];  // the state before the tile
+    lane.load_state(h, r.in ? r.in + (long long)b * a.channels : nullptr);
+    const auto first = [&](int i) { return r.from + (Pass::BACK ? tiles - 1 - i : i) * (W * U) + wave * U; };
+    if (tiles) pass.fetch(first(0), live);
+    for (int i = 0; i < tiles; ++i) {
+        const int t = first(i), m = std::min(live - t, U);
+        pass.prepare(t, m);
+        if (i + 1 < tiles) pass.fetch(first(i + 1), live);
+        if constexpr (W > 1) {
+            float after[CH];
+#pragma unroll
+            for (int c = 0; c < CH; ++c) lds[i & 1][threadIdx.x >> 6][l][c] = pass.join[c];
+            arrived(h);  // r.out may be r.in: all waves have read it before one writes
+            __syncthreads();
+            fold<CH, W, Pass::BACK>(h, after, lds[i & 1]);
+            pass.finish(t, m, h);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) h[c] = after[c];
+        } else {
+            pass.finish(t, m, h);
+        }
+    }
+    for (int t = live + wave * U; t < r.to; t += W * U) pass.clear(t, std::min(r.to - t, U));  // past the sequence
+    if (!wave && r.out) lane.store_state(r.out + (long long)b * a.channels, h);
+}
+
+// ---- a chain of blocks along a sequence, each with one tile. A block hands the
+// Join of its tile on, and the last of every kGroup blocks the state behind it,
+// as the first block does with the state that the sequence starts from (which it
+// alone reads: the last may write its successor over it). A block folds the state
+// before its group and the Joins of its group's blocks before it, always in this
+// order.
+//
+// Every word is handed on by itself, 64 bits at once: 0 until it is there, and
+// never 0 then. Blocks take their places in the order in which they start, by a
+// counter, earlier tiles first. So a block waits for such only as have started,
+// and hands its Join on before it waits: every wait ends, whatever else runs.
+
+constexpr int kGroup = 32, kChainWaves = 8;
+constexpr int kChainTokens = kChainWaves * U;
+// Times that a wait asks again before it gives up, some seconds: nothing that
+// this file launches needs it, a workspace that two calls share at once may.
+constexpr int kPatience = 1 << 20;
+
+struct Chain {
+    unsigned* counter;
+    uint64_t *joins, *states;  // [place][batch][channel]; before each group, [group][batch][channel]
+    int columns, places;
 };
-// Place of a segment's Joins in the workspace: [2][batch][segment][channel].
-__device__ __forceinline__ float* join_at(const RecurrenceArgs& a, const Cut& cut, int part, int b, int z) {
-    return a.work + (((long long)part * a.batch + b) * cut.segments + z) * a.channels;
-}
 
-// The state that reaches segment z from those before it (BACK: behind it).
-template <typename T, int CH, bool BACK>
-__device__ __forceinline__ void arrive(float (&h)[CH], const Lane<T, CH>& lane, const RecurrenceArgs& a, const Cut& cut, int b, int z, int n) {
-    lane.load_state(h, a.state_in ? a.state_in + (long long)b * a.channels : nullptr);
-    const int live = (n + cut.length - 1) / cut.length;  // segments with tokens
-    for (int i = BACK ? live - 1 : 0; BACK ? i > z : i < z && i < live; i += BACK ? -1 : 1) {
-        float s[CH], v[CH];
-        lane.load_state(s, join_at(a, cut, 0, b, i));
-        lane.load_state(v, join_at(a, cut, 1, b, i));
-#pragma unroll
-        for (int c = 0; c < CH; ++c) h[c] = Join{s[c], v[c]}(h[c]);
+__device__ __forceinline__ void hand_on(uint64_t* to, uint64_t word) { __hip_atomic_store(to, word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t wait_for(uint64_t* from) {
+    uint64_t word = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = 0; !word && i < kPatience; ++i) {
+        __builtin_amdgcn_s_sleep(1);
+        word = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    return word ? word : ~0ull;  // NaN
+}
+constexpr unsigned kNever = 0x7fffffffu;  // bits that no gate of a Join has
+__device__ __forceinline__ uint64_t word_of(const Join& j) {
+    const unsigned s = j.s == j.s ? __float_as_uint(j.s) : 0x7fc00000u;
+    return (uint64_t)__float_as_uint(j.h) << 32 | (s ^ kNever);
+}
+__device__ __forceinline__ Join join_of(uint64_t w) { return Join{__uint_as_float((unsigned)w ^ kNever), __uint_as_float((unsigned)(w >> 32))}; }
+__device__ __forceinline__ uint64_t word_of(float v) { return (uint64_t)__float_as_uint(v) << 32 | 1; }
+__device__ __forceinline__ float state_of(uint64_t w) { return __uint_as_float((unsigned)(w >> 32)); }
+
+__global__ __launch_bounds__(256) void k_chain_clear(uint64_t* words, long long count, unsigned* counter) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i < count) words[i] = 0;
+    if (!i) *counter = 0;
 }
 
-// W waves a block, one behind the other in time. JOIN: the segment's Joins alone,
-// nothing else written.
-template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, int W, bool JOIN>
-__global__ __launch_bounds__(64 * W) void k_recurrence(const RecurrenceArgs a, const Cut cut) {
-    __shared__ Join lds[2][W][64][CH];
-    const Lane<T, CH> lane(a.channels);
-    const int b = blockIdx.y, z = blockIdx.z;
+template <typename T, int CH, typename Pass>
+__device__ __forceinline__ void chained(const RecurrenceArgs& a, const Range& r, const Chain& chain) {
+    constexpr int W = kChainWaves;
+    __shared__ Join own[W][64][CH], before[kGroup][64][CH];
+    __shared__ float start[64][CH];
+    __shared__ unsigned ticket;
+    if (!threadIdx.x) ticket = __hip_atomic_fetch_add(chain.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const unsigned mine = __builtin_amdgcn_readfirstlane(ticket);
+    const unsigned row = mine / (unsigned)chain.columns;
+    const Lane<T, CH> lane(mine - row * (unsigned)chain.columns, a.channels);
+    const int b = (int)(row % (unsigned)a.batch), order = (int)(row / (unsigned)a.batch), l = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = clamped(a.lengths, b, a.tokens);
-    const int begin = z * cut.length, end = (int)std::min(a.tokens, (long long)begin + cut.length), live = std::min(n, end);
-    const long long spans = (a.tokens + U - 1) / U;
-    float h[CH] = {};  // the state before the tile
-    Product all[CH];
-    if constexpr (!JOIN) arrive<T, CH, false>(h, lane, a, cut, b, z, n);
-    unsigned x[U] = {}, g[U] = {};
-    const auto fetch = [&](int t) {
-        lane.fetch(x, a.x, b, t, live - t);
-        lane.fetch(g, a.gate, b, t, live - t);
-    };
-    fetch(begin + wave * U);
-    int t0 = begin;
-    for (int half = 0; t0 < live; t0 += W * U, half ^= 1) {
-        const int t = t0 + wave * U, m = std::min(live - t, U);
-        // what the wave's tokens make of a state: p a + l
-        float s[U][CH], in[U][CH], l[CH] = {}, after[CH];
-        Product p[CH];
-        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate q) {
-            s[u][c] = q.s;
-            in[u][c] = COMPLEMENT ? q.w * lane.value(x[u], c) : u < m ? lane.value(x[u], c) : 0.f;
-            if constexpr (W > 1 || JOIN) {
-                p[c].by(q.s, q.w);
-                l[c] = decayed(q.s, l[c]) + in[u][c];
-            }
-        });
-        fetch(t + W * U);
-        if constexpr (W > 1 || JOIN) {
+    const int live = std::max(r.from, std::min(clamped(a.lengths, b, a.tokens), r.to)), tiles = (live - r.from + W * U - 1) / (W * U);
+    const int tile = Pass::BACK ? chain.places - 1 - order : order;
+    const int place = Pass::BACK ? tiles - 1 - tile : tile;  // in the sequence's chain
+    const int t = r.from + tile * (W * U) + wave * U, m = std::min(live - t, U);
+    Pass pass(a, lane, b);
+    const long long channel = lane.first + lane.at, width = (long long)a.batch * a.channels, at = (long long)b * a.channels + channel;
+    if (tile < tiles) {
+        pass.fetch(t, live);
+        pass.prepare(t, m);
 #pragma unroll
-            for (int c = 0; c < CH; ++c) lds[half][threadIdx.x >> 6][threadIdx.x & 63][c] = Join{p[c].smaller(), l[c]};
-            __syncthreads();
-            fold<CH, W, false, JOIN>(h, after, all, lds[half]);
-        }
-        if constexpr (!JOIN) {
-            if (a.saved && t < end) lane.store_state(a.saved + ((long long)b * spans + t / U) * a.channels, h);
-            T* row = (T*)a.y.p + b * a.y.batch + t * a.y.token + lane.first;
+        for (int c = 0; c < CH; ++c) own[threadIdx.x >> 6][l][c] = pass.join[c];
+        __syncthreads();
+        const int group = place / kGroup, count = place % kGroup;
+        float h[CH];
+        Join all[CH];
+        if (!wave) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int c = 0; c < CH; ++c) {
+                Product p;
+                float v = 0.f;
 #pragma unroll
-                for (int c = 0; c < CH; ++c) in[u][c] = h[c] = decayed(s[u][c], h[c]) + in[u][c];
-            if (m == U) {
-                if (lane.have)
-#pragma unroll
-                    for (int u = 0; u < U; ++u, row = behind(row, a.y.token)) lane.store(row, in[u]);
-            } else {
-                if (lane.have)
-#pragma unroll
-                    for (int u = 0; u < U; ++u, row = behind(row, a.y.token))
-                        if (u < m) lane.store(row, in[u]);
-                lane.clear(a.y, b, t + std::max(m, 0), std::min(end - t, U) - std::max(m, 0));
-            }
-        }
-        if constexpr (W > 1 || JOIN)
-#pragma unroll
-            for (int c = 0; c < CH; ++c) h[c] = after[c];
-    }
-    if constexpr (JOIN) {
-        if (wave) return;
-        float decay[CH];
-#pragma unroll
-        for (int c = 0; c < CH; ++c) decay[c] = all[c].smaller();
-        lane.store_state(join_at(a, cut, 0, b, z), decay);
-        lane.store_state(join_at(a, cut, 1, b, z), h);
-    } else {
-        for (int t = t0 + wave * U; t < end; t += W * U) {  // past the sequence
-            if (a.saved) lane.store_state(a.saved + ((long long)b * spans + t / U) * a.channels, h);
-            lane.clear(a.y, b, t, std::min(end - t, U));
-        }
-        if (!wave && z == cut.segments - 1 && a.state_out) lane.store_state(a.state_out + (long long)b * a.channels, h);
-    }
-}
-
-// The same backwards: h is the gradient that arrives from the tokens behind.
-template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, int W, bool JOIN>
-__global__ __launch_bounds__(64 * W) void k_recurrence_back(const RecurrenceArgs a, const Cut cut) {
-    __shared__ Join lds[2][W][64][CH];
-    const Lane<T, CH> lane(a.channels);
-    const int b = blockIdx.y, z = blockIdx.z;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = clamped(a.lengths, b, a.tokens);
-    const int begin = z * cut.length, end = (int)std::min(a.tokens, (long long)begin + cut.length), live = std::min(n, end);
-    const long long spans = (a.tokens + U - 1) / U;
-    float h[CH] = {};
-    Product all[CH];
-    if constexpr (!JOIN) arrive<T, CH, true>(h, lane, a, cut, b, z, n);
-    unsigned x[U] = {}, g[U] = {}, dy[U] = {};
-    const auto fetch = [&](int t) {
-        if constexpr (!JOIN) lane.fetch(x, a.x, b, t, live - t);
-        lane.fetch(g, a.gate, b, t, live - t);
-        lane.fetch(dy, a.dy, b, t, live - t);
-    };
-    const int tiles = (std::max(0, live - begin) + W * U - 1) / (W * U);
-    if (tiles) fetch(begin + (tiles - 1) * (W * U) + wave * U);
-    for (int i = tiles - 1, half = 0; i >= 0; --i, half ^= 1) {
-        const int t = begin + i * (W * U) + wave * U, m = std::min(live - t, U);
-        float s[U][CH], p[U][CH], v[CH], l[CH] = {}, after[CH];  // v: the state before each token
-        Product q[CH];
-        unsigned d[U];
-        if constexpr (!JOIN) lane.load_state(v, m > 0 ? a.saved + ((long long)b * spans + t / U) * a.channels : nullptr);
-        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate k) {
-            s[u][c] = k.s;
-            if constexpr (W > 1 || JOIN) q[c].by(k.s, k.w);
-            if constexpr (!JOIN) {
-                const float xv = lane.value(x[u], c);
-                p[u][c] = COMPLEMENT ? v[c] - xv : v[c];
-                if (!SIGMOID && lane.value(g[u], c) > 0.f) p[u][c] = 0.f;
-                v[c] = decayed(k.s, v[c]) + (COMPLEMENT ? k.w * xv : xv);
-            }
-        });
-#pragma unroll
-        for (int u = 0; u < U; ++u) d[u] = dy[u];
-        if (m < U)
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (u >= m) d[u] = 0;
-        if (i > 0) fetch(t - W * U);
-        if constexpr (W > 1 || JOIN) {
-#pragma unroll
-            for (int u = U - 1; u >= 0; --u)
-#pragma unroll
-                for (int c = 0; c < CH; ++c) l[c] = decayed(s[u][c], l[c] + lane.value(d[u], c));
-#pragma unroll
-            for (int c = 0; c < CH; ++c) lds[half][threadIdx.x >> 6][threadIdx.x & 63][c] = Join{q[c].smaller(), l[c]};
-            __syncthreads();
-            fold<CH, W, true, JOIN>(h, after, all, lds[half]);
-        }
-        if constexpr (!JOIN) {
-            T* dx = (T*)a.y.p + b * a.y.batch + (t + U - 1) * a.y.token + lane.first;
-            T* dg = (T*)a.dgate.p + b * a.dgate.batch + (t + U - 1) * a.dgate.token + lane.first;
-            const auto gradients = [&](int u, float (&to_x)[CH], float (&to_g)[CH]) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const float k = s[u][c], D = lane.value(d[u], c) + h[c];
-                    to_x[c] = COMPLEMENT ? short_of(k) * D : D;
-                    to_g[c] = p[u][c] * D * (SIGMOID ? fabsf(k) * (1.f - fabsf(k)) : decayed(k, 1.f));
-                    h[c] = decayed(k, D);
+                for (int i = 0; i < W; ++i) {
+                    const Join k = own[Pass::BACK ? W - 1 - i : i][l][c];
+                    p.by(k.s, short_of(k.s));
+                    v = k(v);
                 }
-            };
-            float to_x[CH], to_g[CH];
-            if (m == U) {
-                if (lane.have)
+                all[c] = Join{p.smaller(), v};
+                if (lane.have && count < kGroup - 1 && place + 1 < tiles) hand_on(chain.joins + place * width + at + c, word_of(all[c]));
+            }
+            if (place) {
 #pragma unroll
-                    for (int u = U - 1; u >= 0; --u, dx = behind(dx, -a.y.token), dg = behind(dg, -a.dgate.token)) {
-                        gradients(u, to_x, to_g);
-                        lane.store(dx, to_x);
-                        lane.store(dg, to_g);
-                    }
-            } else if (lane.have) {
+                for (int c = 0; c < CH; ++c) h[c] = state_of(wait_for(chain.states + group * width + at + c));
+            } else {
+                lane.load_state(h, r.in ? r.in + (long long)b * a.channels : nullptr);
 #pragma unroll
-                for (int u = U - 1; u >= 0; --u, dx = behind(dx, -a.y.token), dg = behind(dg, -a.dgate.token))
-                    if (u < m) {
-                        gradients(u, to_x, to_g);
-                        lane.store(dx, to_x);
-                        lane.store(dg, to_g);
-                    }
+                for (int c = 0; c < CH; ++c)
+                    if (lane.have && tiles > 1) hand_on(chain.states + at + c, word_of(h[c]));
+            }
+        } else {
+            for (int i = wave - 1; i < count; i += W - 1)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) before[i][l][c] = join_of(wait_for(chain.joins + ((long long)group * kGroup + i) * width + at + c));
+        }
+        __syncthreads();
+        if (!wave) {
+            for (int i = 0; i < count; ++i)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) h[c] = before[i][l][c](h[c]);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                start[l][c] = h[c];
+                if (lane.have && count == kGroup - 1 && place + 1 < tiles) hand_on(chain.states + (group + 1) * width + at + c, word_of(all[c](h[c])));
             }
         }
-        if constexpr (W > 1 || JOIN)
+        __syncthreads();
+        float after[CH];
 #pragma unroll
-            for (int c = 0; c < CH; ++c) h[c] = after[c];
+        for (int c = 0; c < CH; ++c) h[c] = start[l][c];
+        fold<CH, W, Pass::BACK>(h, after, own);
+        pass.finish(t, m, h);
+        if (!wave && place + 1 == tiles && r.out) lane.store_state(r.out + (long long)b * a.channels, after);
+    } else if (!wave && !tiles && !order && r.out && r.out != r.in) {  // no tokens: the state goes on as it is
+        float h[CH];
+        lane.load_state(h, r.in ? r.in + (long long)b * a.channels : nullptr);
+        lane.store_state(r.out + (long long)b * a.channels, h);
     }
-    if constexpr (JOIN) {
-        if (wave) return;
-        float decay[CH];
-#pragma unroll
-        for (int c = 0; c < CH; ++c) decay[c] = all[c].smaller();
-        lane.store_state(join_at(a, cut, 0, b, z), decay);
-        lane.store_state(join_at(a, cut, 1, b, z), h);
-    } else {
-        for (int t = std::max(begin, live) + wave * U; t < end; t += W * U) {  // past the sequence
-            lane.clear(a.y, b, t, std::min(end - t, U));
-            lane.clear(a.dgate, b, t, std::min(end - t, U));
-        }
-        if (!wave && !z && a.state_out) lane.store_state(a.state_out + (long long)b * a.channels, h);
-    }
+    const int past = std::max(live, t);
+    if (past < r.to && past < t + U) pass.clear(past, std::min(r.to, t + U) - past);
 }
 
-// Blocks a CU that segments may make.
-constexpr int kCutBlocks = 2;
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, int W, bool BACK>
+__global__ __launch_bounds__(64 * W) void k_recurrence(const RecurrenceArgs a, const Range r) {
+    along<T, CH, W, std::conditional_t<BACK, Backward<T, CH, SIGMOID, COMPLEMENT, (W > 1)>, Forward<T, CH, SIGMOID, COMPLEMENT, (W > 1)>>>(a, r);
+}
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, bool BACK>
+__global__ __launch_bounds__(64 * kChainWaves) void k_recurrence_chain(const RecurrenceArgs a, const Range r, const Chain chain) {
+    chained<T, CH, std::conditional_t<BACK, Backward<T, CH, SIGMOID, COMPLEMENT, true>, Forward<T, CH, SIGMOID, COMPLEMENT, true>>>(a, r, chain);
+}
 
-template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, int W>
-int launch_as(const RecurrenceArgs& a, hipStream_t s, bool back) {
-    const long long columns = (a.channels + 64 * CH - 1) / (64 * CH);
-    const dim3 block(64 * W);
-    Cut cut{(int)std::max(a.tokens, 1ll), 1};
-    if constexpr (W >= 8) {
-        const long long tile = W * U, most = (long long)a.cus * kCutBlocks / (columns * a.batch);
-        const long long segments = std::min(most, a.tokens / (2 * tile));
-        if (segments > 1) {
-            cut.length = (int)((a.tokens + segments * tile - 1) / (segments * tile) * tile);
-            cut.segments = (int)((a.tokens + cut.length - 1) / cut.length);
-        }
-        if (cut.segments > 1) {
-            const auto kernel = back ? k_recurrence_back<T, CH, SIGMOID, COMPLEMENT, W, true> : k_recurrence<T, CH, SIGMOID, COMPLEMENT, W, true>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)columns, (unsigned)a.batch, (unsigned)cut.segments), block, 0, s, a, cut);
-        }
+// The workspace: the counter, states between launches, words of a launch's chains.
+constexpr long long kWords = 1 << 20;
+struct Workspace {
+    unsigned* counter;
+    float* states;
+    uint64_t* words;
+};
+// Sequences times channels that chains are for: fewer than fill the machine.
+__host__ long long most_chained(int cus) { return (long long)cus * 128; }
+Workspace workspace_of(const RecurrenceArgs& a) {
+    float* states = a.work + 16;  // a line of its own for the counter
+    return Workspace{(unsigned*)a.work, states, (uint64_t*)(states + most_chained(a.cus))};
+}
+
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, bool BACK>
+int launch_chains(const RecurrenceArgs& a, long long columns, hipStream_t s) {
+    const Workspace w = workspace_of(a);
+    const long long width = a.channels * a.batch;
+    // places of one launch: their words, and those of their groups
+    const long long most = (kWords / width - 1) * kGroup / (kGroup + 1), places = (a.tokens + kChainTokens - 1) / kChainTokens;
+    const long long launches = (places + most - 1) / most, each = (places + launches - 1) / launches;
+    for (long long i = 0; i < launches; ++i) {
+        const long long first = (BACK ? launches - 1 - i : i) * each, last = std::min(first + each, places);
+        const Range r{(int)(first * kChainTokens), (int)std::min(last * kChainTokens, a.tokens), i ? w.states : a.state_in,
+                      i + 1 < launches ? w.states : a.state_out};
+        const Chain chain{w.counter, w.words, w.words + (last - first) * width, (int)columns, (int)(last - first)};
+        const long long words = ((last - first) + (last - first + kGroup - 1) / kGroup) * width;
+        hipLaunchKernelGGL(k_chain_clear, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, w.words, words, w.counter);
+        const auto kernel = k_recurrence_chain<T, CH, SIGMOID, COMPLEMENT, BACK>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(columns * a.batch * (last - first))), dim3(64 * kChainWaves), 0, s, a, r, chain);
     }
-    const auto kernel = back ? k_recurrence_back<T, CH, SIGMOID, COMPLEMENT, W, false> : k_recurrence<T, CH, SIGMOID, COMPLEMENT, W, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)columns, (unsigned)a.batch, (unsigned)cut.segments), block, 0, s, a, cut);
     return (int)hipGetLastError();
 }
 
-template <typename T, int CH, bool SIGMOID, bool COMPLEMENT>
-int launch_waves(const RecurrenceArgs& a, hipStream_t s, bool back) {
-    if (a.tokens <= U) return launch_as<T, CH, SIGMOID, COMPLEMENT, 1>(a, s, back);
-    if (a.tokens <= 4 * U) return launch_as<T, CH, SIGMOID, COMPLEMENT, 4>(a, s, back);
-    return launch_as<T, CH, SIGMOID, COMPLEMENT, 8>(a, s, back);
+template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, bool BACK>
+int launch_as(const RecurrenceArgs& a, hipStream_t s) {
+    const long long columns = (a.channels + 64 * CH - 1) / (64 * CH);
+    const Range r{0, (int)a.tokens, a.state_in, a.state_out};
+    const dim3 grid((unsigned)columns, (unsigned)a.batch);
+    if (a.tokens <= U) {
+        hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 1, BACK>), grid, dim3(64), 0, s, a, r);
+    } else if (a.tokens <= 4 * U) {
+        hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 4, BACK>), grid, dim3(256), 0, s, a, r);
+    } else if (a.tokens <= kChainTokens || columns * a.batch >= a.cus) {
+        hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 8, BACK>), grid, dim3(512), 0, s, a, r);
+    } else {
+        return launch_chains<T, CH, SIGMOID, COMPLEMENT, BACK>(a, columns, s);
+    }
+    return (int)hipGetLastError();
 }
 
-template <typename T, int CH>
-int launch_gate(const RecurrenceArgs& a, hipStream_t s, bool back) {
-    if (a.gate_kind == VKFX_GATE_SIGMOID) return a.complement ? launch_waves<T, CH, true, true>(a, s, back) : launch_waves<T, CH, true, false>(a, s, back);
-    return a.complement ? launch_waves<T, CH, false, true>(a, s, back) : launch_waves<T, CH, false, false>(a, s, back);
+template <typename T, int CH, bool BACK>
+int launch_gate(const RecurrenceArgs& a, hipStream_t s) {
+    if (a.gate_kind == VKFX_GATE_SIGMOID) return a.complement ? launch_as<T, CH, true, true, BACK>(a, s) : launch_as<T, CH, true, false, BACK>(a, s);
+    return a.complement ? launch_as<T, CH, false, true, BACK>(a, s) : launch_as<T, CH, false, false, BACK>(a, s);
 }
 
 // Two 16-bit channels a lane where every pair of them is a word.
-template <typename T>
-int launch_channels(const RecurrenceArgs& a, hipStream_t s, bool back) {
+template <typename T, bool BACK>
+int launch_channels(const RecurrenceArgs& a, hipStream_t s) {
     uintptr_t all = (uintptr_t)a.channels * 2;
     for (const RecurrenceSide* x : {&a.x, &a.gate, &a.dy, &a.y, &a.dgate}) all |= (uintptr_t)x->p | (uintptr_t)(x->batch * 2) | (uintptr_t)(x->token * 2);
-    return all % 4 ? launch_gate<T, 1>(a, s, back) : launch_gate<T, 2>(a, s, back);
+    return all % 4 ? launch_gate<T, 1, BACK>(a, s) : launch_gate<T, 2, BACK>(a, s);
 }
 
-int launch_element(const RecurrenceArgs& a, hipStream_t s, bool back) {
-    if (a.element == VKFX_ELEMENT_F32) return launch_gate<float, 1>(a, s, back);
-    if (a.element == VKFX_ELEMENT_F16) return launch_channels<_Float16>(a, s, back);
-    return launch_channels<__bf16>(a, s, back);
+template <bool BACK>
+int launch_element(const RecurrenceArgs& a, hipStream_t s) {
+    if (a.element == VKFX_ELEMENT_F32) return launch_gate<float, 1, BACK>(a, s);
+    if (a.element == VKFX_ELEMENT_F16) return launch_channels<_Float16, BACK>(a, s);
+    return launch_channels<__bf16, BACK>(a, s);
 }
 
 }  // namespace
 
-int launch_recurrence_forward(const RecurrenceArgs& a, hipStream_t s) { return launch_element(a, s, false); }
-int launch_recurrence_backward(const RecurrenceArgs& a, hipStream_t s) { return launch_element(a, s, true); }
-// segments times columns is at most kCutBlocks a CU, of up to 128 channels each
-size_t recurrence_workspace_bytes(int, long long, int cus) { return (size_t)cus * kCutBlocks * 128 * 2 * sizeof(float); }
+int launch_recurrence_forward(const RecurrenceArgs& a, hipStream_t s) { return launch_element<false>(a, s); }
+int launch_recurrence_backward(const RecurrenceArgs& a, hipStream_t s) { return launch_element<true>(a, s); }
+size_t recurrence_workspace_bytes(int, long long, int cus) { return 64 + (size_t)most_chained(cus) * sizeof(float) + (size_t)kWords * sizeof(uint64_t); }
 
 }  // namespace vkfx

@@ -38,6 +38,10 @@ int check_in_place(const char* out, const vkfx_channels& o, const char* in, cons
     return VKFX_OK;
 }
 
+int check_work(const void* d_work) {
+    return (uintptr_t)d_work % 16 ? bad("work must be aligned to 16 bytes") : VKFX_OK;
+}
+
 int check_counts(uint64_t batch, uint64_t tokens) {
     if (batch > kMostSequences) return fail(VKFX_ERR_RESOURCE_LIMIT, "more than 65535 sequences");
     if (tokens > kMostTokens) return fail(VKFX_ERR_RESOURCE_LIMIT, "more than 2^31 - 65536 tokens");
@@ -101,6 +105,7 @@ int vkfx_gated_recurrence_forward(vkfx_gated_recurrence* plan, const vkfx_gated_
         const vkfx_gated_recurrence_desc& d = plan->desc;
         const uint64_t b = args->batch, t = args->tokens, c = d.channels;
         if (int rc = check_counts(b, t)) return rc;
+        if (int rc = check_work(d_work)) return rc;
         if (!b) return VKFX_OK;
         if (t) {
             if (int rc = check_channels("x", args->x, b, t, c, false)) return rc;
@@ -139,6 +144,7 @@ int vkfx_gated_recurrence_backward(vkfx_gated_recurrence* plan, const vkfx_gated
         const vkfx_gated_recurrence_desc& d = plan->desc;
         const uint64_t b = args->batch, t = args->tokens, c = d.channels;
         if (int rc = check_counts(b, t)) return rc;
+        if (int rc = check_work(d_work)) return rc;
         if (!b) return VKFX_OK;
         if (t) {
             if (!args->saved) return bad("null saved");
