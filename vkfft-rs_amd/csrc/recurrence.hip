@@ -85,6 +85,28 @@ struct Join {
     __device__ __forceinline__ float operator()(float v) const { return decayed(s, v) + h; }
 };
 
+// The product of decays: a, and low = 1 - a.
+struct Product {
+    float a = 1.f, low = 0.f;
+    __device__ __forceinline__ void by(float s, float w) {
+        a = decayed(s, a);
+        low = decayed(s, low) + w;
+    }
+    // The smaller of both, as a gate has it.
+    __device__ __forceinline__ float smaller() const { return low < 0.5f ? -low : a; }
+};
+
+// Several of them in their order.
+struct Joins {
+    Product p;
+    float h = 0.f;
+    __device__ __forceinline__ void add(const Join& j) {
+        p.by(j.s, short_of(j.s));
+        h = j(h);
+    }
+    __device__ __forceinline__ Join join() const { return Join{p.smaller(), h}; }
+};
+
 __device__ __forceinline__ int clamped(const int* lengths, int b, long long tokens) {
     const long long n = lengths ? lengths[b] : tokens;
     return __builtin_amdgcn_readfirstlane((int)(n < 0 ? 0 : n < tokens ? n : tokens));
@@ -96,10 +118,13 @@ __device__ __forceinline__ int apart(int m) {
     asm volatile("" : "+s"(m));
     return m;
 }
+// Pointers that are to global memory, which the compiler does not see behind asm.
+template <typename T>
+using Global = __attribute__((address_space(1))) T*;
 // The next row. Kept from the compiler, which would hold every row's place in
 // scalar registers, and these, past 100 of them, in lanes of vector registers.
 template <typename T>
-__device__ __forceinline__ T* behind(T* row, long long stride) {
+__device__ __forceinline__ Global<T> behind(Global<T> row, long long stride) {
     row += stride;
     asm volatile("" : "+s"(row));
     return row;
@@ -124,14 +149,14 @@ struct Lane {
     }
     // Tokens t .. t + m - 1 of sequence b, the last one again behind them.
     __device__ __forceinline__ void fetch(unsigned (&r)[U], const RecurrenceSide& s, long long b, long long t, int m) const {
-        const T* row = (const T*)s.p + b * s.batch + t * s.token + first;
+        Global<const T> row = (Global<const T>)((const T*)s.p + b * s.batch + t * s.token + first);
         if (m >= U) {
 #pragma unroll
-            for (int u = 0; u < U; ++u, row = behind(row, s.token)) r[u] = *(const Raw*)(row + at);
+            for (int u = 0; u < U; ++u, row = behind<const T>(row, s.token)) r[u] = *(Global<const Raw>)(row + at);
         } else if (m > 0) {
             m = apart(m);
 #pragma unroll
-            for (int u = 0; u < U; ++u, row = behind(row, u < m ? s.token : 0)) r[u] = *(const Raw*)(row + at);
+            for (int u = 0; u < U; ++u, row = behind<const T>(row, u < m ? s.token : 0)) r[u] = *(Global<const Raw>)(row + at);
         }
     }
     __device__ __forceinline__ static float value(unsigned r, int c) { return (float)__builtin_bit_cast(Vec, (Raw)r)[c]; }
@@ -151,26 +176,26 @@ struct Lane {
             return most[0] > limit || most[1] > limit;
         }
     }
-    __device__ __forceinline__ void store(T* row, const float (&y)[CH]) const {
+    __device__ __forceinline__ void store(Global<T> row, const float (&y)[CH]) const {
         Vec r;
 #pragma unroll
         for (int c = 0; c < CH; ++c) r[c] = (T)y[c];
-        *(Vec*)(row + at) = r;
+        *(Global<Vec>)(row + at) = r;
     }
     // Zeros in rows t .. of a tensor.
     __device__ __forceinline__ void clear(const RecurrenceSide& s, long long b, long long t, int rows) const {
-        T* row = (T*)s.p + b * s.batch + t * s.token + first;
+        Global<T> row = (Global<T>)((T*)s.p + b * s.batch + t * s.token + first);
         const float zero[CH] = {};
         for (int u = 0; have && u < rows; ++u, row += s.token) store(row, zero);
     }
     __device__ __forceinline__ void load_state(float (&h)[CH], const float* row) const {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) h[c] = row ? row[first + at + c] : 0.f;
+        for (int c = 0; c < CH; ++c) h[c] = row ? ((Global<const float>)row)[first + at + c] : 0.f;
     }
     __device__ __forceinline__ void store_state(float* row, const float (&h)[CH]) const {
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-            if (have) row[first + at + c] = h[c];
+            if (have) ((Global<float>)row)[first + at + c] = h[c];
     }
 };
 
@@ -191,17 +216,6 @@ __device__ __forceinline__ void each_gate(const unsigned (&g)[U], int m, F f) {
             for (int c = 0; c < CH; ++c) f(u, c, u < m ? gate_of<SIGMOID, false>(Lane<T, CH>::value(g[u], c)) : Gate{-0.f, 0.f});
     }
 }
-
-// The product of decays: a, and low = 1 - a.
-struct Product {
-    float a = 1.f, low = 0.f;
-    __device__ __forceinline__ void by(float s, float w) {
-        a = decayed(s, a);
-        low = decayed(s, low) + w;
-    }
-    // The smaller of both, as a gate has it.
-    __device__ __forceinline__ float smaller() const { return low < 0.5f ? -low : a; }
-};
 
 // Which tokens a launch runs, and the states before and behind them (BACK: the
 // gradients behind and before them).
@@ -231,7 +245,7 @@ struct Forward {
         lane.fetch(x, a.x, b, t, live - t);
         lane.fetch(g, a.gate, b, t, live - t);
     }
-    __device__ __forceinline__ void prepare(int t, int m) {
+    __device__ __forceinline__ void prepare(int m) {
         float l[CH] = {};
         Product p[CH];
         each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate q) {
@@ -249,7 +263,7 @@ struct Forward {
         if (m <= 0) return;
         const long long spans = (a.tokens + U - 1) / U;
         if (a.saved) lane.store_state(a.saved + ((long long)b * spans + t / U) * a.channels, h);
-        T* row = (T*)a.y.p + b * a.y.batch + t * a.y.token + lane.first;
+        Global<T> row = (Global<T>)((T*)a.y.p + b * a.y.batch + t * a.y.token + lane.first);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -257,11 +271,11 @@ struct Forward {
         if (!lane.have) return;
         if (m == U) {
 #pragma unroll
-            for (int u = 0; u < U; ++u, row = behind(row, a.y.token)) lane.store(row, in[u]);
+            for (int u = 0; u < U; ++u, row = behind<T>(row, a.y.token)) lane.store(row, in[u]);
         } else {
             m = apart(m);
 #pragma unroll
-            for (int u = 0; u < U; ++u, row = behind(row, a.y.token))
+            for (int u = 0; u < U; ++u, row = behind<T>(row, a.y.token))
                 if (u < m) lane.store(row, in[u]);
         }
     }
@@ -275,6 +289,7 @@ struct Backward {
     const Lane<T, CH>& lane;
     const int b;
     unsigned x[U] = {}, g[U] = {}, dy[U] = {};
+    float first[CH];  // the state before the first token
     float s[U][CH], p[U][CH];
     unsigned d[U];
     Join join[CH];
@@ -284,12 +299,14 @@ struct Backward {
         lane.fetch(x, a.x, b, t, live - t);
         lane.fetch(g, a.gate, b, t, live - t);
         lane.fetch(dy, a.dy, b, t, live - t);
+        const long long spans = (a.tokens + U - 1) / U;
+        lane.load_state(first, t < live ? a.saved + ((long long)b * spans + t / U) * a.channels : nullptr);
     }
-    __device__ __forceinline__ void prepare(int t, int m) {
+    __device__ __forceinline__ void prepare(int m) {
         float v[CH], l[CH] = {};  // v: the state before each token
         Product q[CH];
-        const long long spans = (a.tokens + U - 1) / U;
-        lane.load_state(v, m > 0 ? a.saved + ((long long)b * spans + t / U) * a.channels : nullptr);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) v[c] = first[c];
         each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate k) {
             s[u][c] = k.s;
             if constexpr (JOIN) q[c].by(k.s, k.w);
@@ -317,8 +334,8 @@ struct Backward {
     }
     __device__ __forceinline__ void finish(int t, int m, float (&h)[CH]) {
         if (m <= 0) return;
-        T* dx = (T*)a.y.p + b * a.y.batch + (t + U - 1) * a.y.token + lane.first;
-        T* dg = (T*)a.dgate.p + b * a.dgate.batch + (t + U - 1) * a.dgate.token + lane.first;
+        Global<T> dx = (Global<T>)((T*)a.y.p + b * a.y.batch + (t + U - 1) * a.y.token + lane.first);
+        Global<T> dg = (Global<T>)((T*)a.dgate.p + b * a.dgate.batch + (t + U - 1) * a.dgate.token + lane.first);
         const auto gradients = [&](int u, float (&to_x)[CH], float (&to_g)[CH]) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -332,7 +349,7 @@ struct Backward {
         if (m == U) {
             if (lane.have)
 #pragma unroll
-                for (int u = U - 1; u >= 0; --u, dx = behind(dx, -a.y.token), dg = behind(dg, -a.dgate.token)) {
+                for (int u = U - 1; u >= 0; --u, dx = behind<T>(dx, -a.y.token), dg = behind<T>(dg, -a.dgate.token)) {
                     gradients(u, to_x, to_g);
                     lane.store(dx, to_x);
                     lane.store(dg, to_g);
@@ -340,7 +357,7 @@ struct Backward {
         } else if (lane.have) {
             m = apart(m);
 #pragma unroll
-            for (int u = U - 1; u >= 0; --u, dx = behind(dx, -a.y.token), dg = behind(dg, -a.dgate.token))
+            for (int u = U - 1; u >= 0; --u, dx = behind<T>(dx, -a.y.token), dg = behind<T>(dg, -a.dgate.token))
                 if (u < m) {
                     gradients(u, to_x, to_g);
                     lane.store(dx, to_x);
@@ -394,15 +411,15 @@ __device__ __forceinline__ void along(const RecurrenceArgs& a, const Range& r) {
     lane.load_state(h, r.in ? r.in + (long long)b * a.channels : nullptr);
     const auto first = [&](int i) { return r.from + (Pass::BACK ? tiles - 1 - i : i) * (W * U) + wave * U; };
     if (tiles) pass.fetch(first(0), live);
+    if constexpr (W > 1) arrived(h);  // r.out may be r.in: all waves have read it before one writes
     for (int i = 0; i < tiles; ++i) {
         const int t = first(i), m = std::min(live - t, U);
-        pass.prepare(t, m);
+        pass.prepare(m);
         if (i + 1 < tiles) pass.fetch(first(i + 1), live);
         if constexpr (W > 1) {
             float after[CH];
 #pragma unroll
             for (int c = 0; c < CH; ++c) lds[i & 1][threadIdx.x >> 6][l][c] = pass.join[c];
-            arrived(h);  // r.out may be r.in: all waves have read it before one writes
             __syncthreads();
             fold<CH, W, Pass::BACK>(h, after, lds[i & 1]);
             pass.finish(t, m, h);
@@ -417,37 +434,61 @@ __device__ __forceinline__ void along(const RecurrenceArgs& a, const Range& r) {
 }
 
 // ---- a chain of blocks along a sequence, each with one tile. A block hands the
-// Join of its tile on, and the last of every kGroup blocks the state behind it,
-// as the first block does with the state that the sequence starts from (which it
-// alone reads: the last may write its successor over it). A block folds the state
-// before its group and the Joins of its group's blocks before it, always in this
-// order.
+// Join of its tile on, and the last block of a group the state behind it, as the
+// first block does with the state that the sequence starts from (which it alone
+// reads: the last may write its successor over it). A block joins the Joins of its
+// group's blocks before it, always in this order, and applies that to the state
+// before its group. So from a state to the next it takes one exchange and one
+// application.
+//
+// A lane has one channel here, so that three blocks fit a CU (their phases, loads,
+// gates, the exchange, outputs, are alike; two channels and two blocks: 1 x 65536
+// tokens of 1024 channels 131 us, 112 with one).
 //
 // Every word is handed on by itself, 64 bits at once: 0 until it is there, and
-// never 0 then. Blocks take their places in the order in which they start, by a
-// counter, earlier tiles first. So a block waits for such only as have started,
-// and hands its Join on before it waits: every wait ends, whatever else runs.
+// never 0 then. A chain's blocks take their places in the order in which they
+// start, by a counter. So a block waits for such only as have started, and hands
+// its Join on before it waits: every wait ends, whatever else runs. Each chain
+// counts by itself, in a line of its own: one counter for all gives a place in 23
+// ns, 8192 of them in 188 us.
 
-constexpr int kGroup = 32, kChainWaves = 8;
+constexpr int kLeastGroup = 4, kMostGroup = 32, kChainWaves = 8;
 constexpr int kChainTokens = kChainWaves * U;
 // Times that a wait asks again before it gives up, some seconds: nothing that
 // this file launches needs it, a workspace that two calls share at once may.
 constexpr int kPatience = 1 << 20;
 
+constexpr int kLine = 32;  // words of a counter's line
 struct Chain {
-    unsigned* counter;
-    uint64_t *joins, *states;  // [place][batch][channel]; before each group, [group][batch][channel]
-    int columns, places;
+    unsigned* counters;
+    uint64_t *joins, *states;  // [place][batch][channel]; before a group, [group][batch][channel]
+    int columns, places, group;  // blocks of a group, a power of 2
 };
 
 __device__ __forceinline__ void hand_on(uint64_t* to, uint64_t word) { __hip_atomic_store(to, word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ uint64_t wait_for(uint64_t* from) {
-    uint64_t word = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int i = 0; !word && i < kPatience; ++i) {
+// N CH words at from, from + stride, ...: the first `count` times CH. All are asked
+// for at once.
+template <int N, int CH>
+__device__ __forceinline__ void wait_for(uint64_t (&w)[N][CH], const uint64_t* from, long long stride, int count) {
+    for (int tries = 0;; ++tries) {
+        bool there = true;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+                w[i][c] = __hip_atomic_load(from + (i < count ? i : 0) * stride + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) there = there && w[i][c];
+        if (__all(there)) return;
+        if (tries == kPatience) break;
         __builtin_amdgcn_s_sleep(1);
-        word = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    return word ? word : ~0ull;  // NaN
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) w[i][c] = ~0ull;  // NaN
 }
 constexpr unsigned kNever = 0x7fffffffu;  // bits that no gate of a Join has
 __device__ __forceinline__ uint64_t word_of(const Join& j) {
@@ -458,24 +499,25 @@ __device__ __forceinline__ Join join_of(uint64_t w) { return Join{__uint_as_floa
 __device__ __forceinline__ uint64_t word_of(float v) { return (uint64_t)__float_as_uint(v) << 32 | 1; }
 __device__ __forceinline__ float state_of(uint64_t w) { return __uint_as_float((unsigned)(w >> 32)); }
 
-__global__ __launch_bounds__(256) void k_chain_clear(uint64_t* words, long long count, unsigned* counter) {
+__global__ __launch_bounds__(256) void k_chain_clear(uint64_t* words, long long count, unsigned* counters, int chains) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i < count) words[i] = 0;
-    if (!i) *counter = 0;
+    if (i < chains) counters[i * kLine] = 0;
 }
 
-template <typename T, int CH, typename Pass>
+template <typename T, typename Pass>
 __device__ __forceinline__ void chained(const RecurrenceArgs& a, const Range& r, const Chain& chain) {
-    constexpr int W = kChainWaves;
-    __shared__ Join own[W][64][CH], before[kGroup][64][CH];
+    constexpr int W = kChainWaves, CH = 1;
+    __shared__ Join own[W][64][CH], before[W - 1][64][CH];
     __shared__ float start[64][CH];
     __shared__ unsigned ticket;
-    if (!threadIdx.x) ticket = __hip_atomic_fetch_add(chain.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // neighbours in the order of launch are of different chains, those of one chain on different XCDs
+    const unsigned chains = (unsigned)(chain.columns * a.batch), mine = (blockIdx.x + blockIdx.x / chains) % chains;
+    if (!threadIdx.x) ticket = __hip_atomic_fetch_add(chain.counters + mine * kLine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    const unsigned mine = __builtin_amdgcn_readfirstlane(ticket);
-    const unsigned row = mine / (unsigned)chain.columns;
-    const Lane<T, CH> lane(mine - row * (unsigned)chain.columns, a.channels);
-    const int b = (int)(row % (unsigned)a.batch), order = (int)(row / (unsigned)a.batch), l = threadIdx.x & 63;
+    const int order = (int)__builtin_amdgcn_readfirstlane(ticket);
+    const int b = (int)(mine / (unsigned)chain.columns), l = threadIdx.x & 63;
+    const Lane<T, CH> lane(mine - (unsigned)(b * chain.columns), a.channels);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int live = std::max(r.from, std::min(clamped(a.lengths, b, a.tokens), r.to)), tiles = (live - r.from + W * U - 1) / (W * U);
     const int tile = Pass::BACK ? chain.places - 1 - order : order;
@@ -485,50 +527,69 @@ __device__ __forceinline__ void chained(const RecurrenceArgs& a, const Range& r,
     const long long channel = lane.first + lane.at, width = (long long)a.batch * a.channels, at = (long long)b * a.channels + channel;
     if (tile < tiles) {
         pass.fetch(t, live);
-        pass.prepare(t, m);
+        pass.prepare(m);
 #pragma unroll
         for (int c = 0; c < CH; ++c) own[threadIdx.x >> 6][l][c] = pass.join[c];
         __syncthreads();
-        const int group = place / kGroup, count = place % kGroup;
+        const int group = place / chain.group, count = place % chain.group;
+        const bool last = place + 1 == tiles;
+        constexpr int N = (kMostGroup + W - 3) / (W - 1);  // of kMostGroup - 1 Joins, a wave's
         float h[CH];
         Join all[CH];
         if (!wave) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                Product p;
-                float v = 0.f;
+                Joins k;
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const Join k = own[Pass::BACK ? W - 1 - i : i][l][c];
-                    p.by(k.s, short_of(k.s));
-                    v = k(v);
-                }
-                all[c] = Join{p.smaller(), v};
-                if (lane.have && count < kGroup - 1 && place + 1 < tiles) hand_on(chain.joins + place * width + at + c, word_of(all[c]));
+                for (int i = 0; i < W; ++i) k.add(own[Pass::BACK ? W - 1 - i : i][l][c]);
+                all[c] = k.join();
+                if (lane.have && count < chain.group - 1 && !last) hand_on(chain.joins + place * width + at + c, word_of(all[c]));
             }
-            if (place) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) h[c] = state_of(wait_for(chain.states + group * width + at + c));
-            } else {
+            if (!place) {
                 lane.load_state(h, r.in ? r.in + (long long)b * a.channels : nullptr);
 #pragma unroll
                 for (int c = 0; c < CH; ++c)
-                    if (lane.have && tiles > 1) hand_on(chain.states + at + c, word_of(h[c]));
+                    if (lane.have && !last) hand_on(chain.states + at + c, word_of(h[c]));
             }
         } else {
-            for (int i = wave - 1; i < count; i += W - 1)
+            const int first = (wave - 1) * N, some = std::min(count - first, N);
+            if (some > 0) {
+                uint64_t w[N][CH];
+                wait_for(w, chain.joins + ((long long)group * chain.group + first) * width + at, width, some);
 #pragma unroll
-                for (int c = 0; c < CH; ++c) before[i][l][c] = join_of(wait_for(chain.joins + ((long long)group * kGroup + i) * width + at + c));
+                for (int c = 0; c < CH; ++c) {
+                    Joins k;
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (i < some) k.add(join_of(w[i][c]));
+                    before[wave - 1][l][c] = k.join();
+                }
+            }
         }
         __syncthreads();
         if (!wave) {
-            for (int i = 0; i < count; ++i)
-#pragma unroll
-                for (int c = 0; c < CH; ++c) h[c] = before[i][l][c](h[c]);
+            const int parts = (count + N - 1) / N;
+            Join to[CH], behind[CH];  // from the state before the group to that before the tile, and behind it
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                start[l][c] = h[c];
-                if (lane.have && count == kGroup - 1 && place + 1 < tiles) hand_on(chain.states + (group + 1) * width + at + c, word_of(all[c](h[c])));
+                Joins k;
+#pragma unroll
+                for (int i = 0; i < W - 1; ++i)
+                    if (i < parts) k.add(before[i][l][c]);
+                to[c] = k.join();
+                k.add(all[c]);
+                behind[c] = k.join();
+            }
+            if (place) {
+                uint64_t w[1][CH];
+                wait_for(w, chain.states + group * width + at, 0, 1);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) h[c] = state_of(w[0][c]);
+            }
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (lane.have && count == chain.group - 1 && !last) hand_on(chain.states + (group + 1) * width + at + c, word_of(behind[c](h[c])));
+                start[l][c] = count ? to[c](h[c]) : h[c];
             }
         }
         __syncthreads();
@@ -547,45 +608,62 @@ __device__ __forceinline__ void chained(const RecurrenceArgs& a, const Range& r,
     if (past < r.to && past < t + U) pass.clear(past, std::min(r.to, t + U) - past);
 }
 
+// Forward with 128 registers, so that two blocks fit a CU (64 x 100 tokens of 4096
+// channels 39 us, 54 with 130 registers).
 template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, int W, bool BACK>
-__global__ __launch_bounds__(64 * W) void k_recurrence(const RecurrenceArgs a, const Range r) {
+__global__ __launch_bounds__(64 * W, W == 8 && !BACK ? 4 : 1) void k_recurrence(const RecurrenceArgs a, const Range r) {
     along<T, CH, W, std::conditional_t<BACK, Backward<T, CH, SIGMOID, COMPLEMENT, (W > 1)>, Forward<T, CH, SIGMOID, COMPLEMENT, (W > 1)>>>(a, r);
 }
-template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, bool BACK>
+template <typename T, bool SIGMOID, bool COMPLEMENT, bool BACK>
 __global__ __launch_bounds__(64 * kChainWaves) void k_recurrence_chain(const RecurrenceArgs a, const Range r, const Chain chain) {
-    chained<T, CH, std::conditional_t<BACK, Backward<T, CH, SIGMOID, COMPLEMENT, true>, Forward<T, CH, SIGMOID, COMPLEMENT, true>>>(a, r, chain);
+    chained<T, std::conditional_t<BACK, Backward<T, 1, SIGMOID, COMPLEMENT, true>, Forward<T, 1, SIGMOID, COMPLEMENT, true>>>(a, r, chain);
 }
 
-// The workspace: the counter, states between launches, words of a launch's chains.
-constexpr long long kWords = 1 << 20;
+// Whether a call is for chains: blocks that go along their sequences would leave
+// a quarter of the CUs' time unused (320 blocks for 256 CUs, 5 x 2048 tokens of 8192
+// channels: 134 us, 125 in chains; 256 blocks 93 and 106).
+bool for_chains(const RecurrenceArgs& a, long long blocks) {
+    if (a.tokens <= kChainTokens) return false;
+    const long long rounds = (blocks + a.cus - 1) / a.cus;
+    return blocks * 4 < rounds * a.cus * 3;
+}
+// Most channels of all sequences that chains run: those of 64 to 128 channels a
+// block, in up to 3 rounds (four rounds are three quarters full always).
+long long most_chained(int cus) { return (long long)cus * 128 * 3; }
+
+// The workspace: the chains' counters, their states between launches, the words
+// of a launch.
+long long words_of(int cus) { return (long long)cus * 4096; }
 struct Workspace {
-    unsigned* counter;
+    unsigned* counters;
     float* states;
     uint64_t* words;
 };
-// Sequences times channels that chains are for: fewer than fill the machine.
-__host__ long long most_chained(int cus) { return (long long)cus * 128; }
 Workspace workspace_of(const RecurrenceArgs& a) {
-    float* states = a.work + 16;  // a line of its own for the counter
+    float* states = a.work + most_chained(a.cus) / 64 * kLine;
     return Workspace{(unsigned*)a.work, states, (uint64_t*)(states + most_chained(a.cus))};
 }
 
-template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, bool BACK>
-int launch_chains(const RecurrenceArgs& a, long long columns, hipStream_t s) {
+template <typename T, bool SIGMOID, bool COMPLEMENT, bool BACK>
+int launch_chains(const RecurrenceArgs& a, hipStream_t s) {
     const Workspace w = workspace_of(a);
-    const long long width = a.channels * a.batch;
+    const long long width = a.channels * a.batch, columns = (a.channels + 63) / 64, chains = columns * a.batch;
+    // groups of about as many blocks as a chain has side by side
+    int group = kMostGroup;
+    while (group > kLeastGroup && group * chains > a.cus * 2) group /= 2;
     // places of one launch: their words, and those of their groups
-    const long long most = (kWords / width - 1) * kGroup / (kGroup + 1), places = (a.tokens + kChainTokens - 1) / kChainTokens;
+    const long long most = (words_of(a.cus) / width - 1) * group / (group + 1), places = (a.tokens + kChainTokens - 1) / kChainTokens;
     const long long launches = (places + most - 1) / most, each = (places + launches - 1) / launches;
     for (long long i = 0; i < launches; ++i) {
         const long long first = (BACK ? launches - 1 - i : i) * each, last = std::min(first + each, places);
         const Range r{(int)(first * kChainTokens), (int)std::min(last * kChainTokens, a.tokens), i ? w.states : a.state_in,
                       i + 1 < launches ? w.states : a.state_out};
-        const Chain chain{w.counter, w.words, w.words + (last - first) * width, (int)columns, (int)(last - first)};
-        const long long words = ((last - first) + (last - first + kGroup - 1) / kGroup) * width;
-        hipLaunchKernelGGL(k_chain_clear, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, w.words, words, w.counter);
-        const auto kernel = k_recurrence_chain<T, CH, SIGMOID, COMPLEMENT, BACK>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(columns * a.batch * (last - first))), dim3(64 * kChainWaves), 0, s, a, r, chain);
+        const Chain chain{w.counters, w.words, w.words + (last - first) * width, (int)columns, (int)(last - first), group};
+        const long long words = ((last - first) + (last - first + group - 1) / group) * width;
+        hipLaunchKernelGGL(k_chain_clear, dim3((unsigned)((std::max(words, chains) + 255) / 256)), dim3(256), 0, s, w.words, words, w.counters,
+                           (int)chains);
+        const auto kernel = k_recurrence_chain<T, SIGMOID, COMPLEMENT, BACK>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(chains * (last - first))), dim3(64 * kChainWaves), 0, s, a, r, chain);
     }
     return (int)hipGetLastError();
 }
@@ -593,17 +671,12 @@ int launch_chains(const RecurrenceArgs& a, long long columns, hipStream_t s) {
 template <typename T, int CH, bool SIGMOID, bool COMPLEMENT, bool BACK>
 int launch_as(const RecurrenceArgs& a, hipStream_t s) {
     const long long columns = (a.channels + 64 * CH - 1) / (64 * CH);
+    if (for_chains(a, columns * a.batch)) return launch_chains<T, SIGMOID, COMPLEMENT, BACK>(a, s);
     const Range r{0, (int)a.tokens, a.state_in, a.state_out};
     const dim3 grid((unsigned)columns, (unsigned)a.batch);
-    if (a.tokens <= U) {
-        hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 1, BACK>), grid, dim3(64), 0, s, a, r);
-    } else if (a.tokens <= 4 * U) {
-        hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 4, BACK>), grid, dim3(256), 0, s, a, r);
-    } else if (a.tokens <= kChainTokens || columns * a.batch >= a.cus) {
-        hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 8, BACK>), grid, dim3(512), 0, s, a, r);
-    } else {
-        return launch_chains<T, CH, SIGMOID, COMPLEMENT, BACK>(a, columns, s);
-    }
+    if (a.tokens <= U) hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 1, BACK>), grid, dim3(64), 0, s, a, r);
+    else if (a.tokens <= 4 * U) hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 4, BACK>), grid, dim3(256), 0, s, a, r);
+    else hipLaunchKernelGGL((k_recurrence<T, CH, SIGMOID, COMPLEMENT, 8, BACK>), grid, dim3(512), 0, s, a, r);
     return (int)hipGetLastError();
 }
 
@@ -632,6 +705,8 @@ int launch_element(const RecurrenceArgs& a, hipStream_t s) {
 
 int launch_recurrence_forward(const RecurrenceArgs& a, hipStream_t s) { return launch_element<false>(a, s); }
 int launch_recurrence_backward(const RecurrenceArgs& a, hipStream_t s) { return launch_element<true>(a, s); }
-size_t recurrence_workspace_bytes(int, long long, int cus) { return 64 + (size_t)most_chained(cus) * sizeof(float) + (size_t)kWords * sizeof(uint64_t); }
+size_t recurrence_workspace_bytes(int, long long, int cus) {
+    return (size_t)(most_chained(cus) / 64 * kLine + most_chained(cus)) * sizeof(float) + (size_t)words_of(cus) * sizeof(uint64_t);
+}
 
 }  // namespace vkfx
