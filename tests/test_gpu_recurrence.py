@@ -487,3 +487,32 @@ def test_plans_hold_their_context(hip_ctx):
     assert ctx._L.vkfx_context_destroy(ctx.handle) == -2
     plan.close()
     ctx.close()
+
+
+@pytest.mark.parametrize("lengths", [None, [5300]])
+def test_many_long_chains_take_several_launches(hip_ctx, lengths):
+    """More tokens of more channels than one launch's workspace holds; a part of the channels alone takes one."""
+    import torch
+    t, c, part = 5400, 20000, 640
+    plan, alone = _plan(hip_ctx, c, "bf16"), _plan(hip_ctx, part, "bf16")
+    x, gate, dy = _tensor(1, (1, t, c), "bf16"), _gate(2, (1, t, c), "bf16", "sigmoid"), _tensor(3, (1, t, c), "bf16")
+    s, ds = _state(4, 1, c), _state(5, 1, c)
+    n = None if lengths is None else torch.tensor(lengths, device="cuda", dtype=torch.int32)
+    outs = []
+    for p, at in ((plan, slice(0, c)), (alone, slice(c - part, c))):
+        v = [z[..., at] for z in (x, gate, dy)]
+        o = [torch.full(v[0].shape, 7, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
+        states = [s[:, at].clone(), ds[:, at].clone()]
+        saved = torch.empty(p.saved_shape(1, t), device="cuda")
+        p.forward_tensors(v[0], v[1], o[0], state_in=states[0], state_out=states[0], saved=saved, lengths=n)
+        p.backward_tensors(v[0], v[1], saved, v[2], o[1], o[2], dstate_out=states[1], dstate_in=states[1], lengths=n)
+        outs.append([z[..., -part:] for z in o + states])
+    for name, a, b in zip(("y", "dx", "dgate", "state", "dstate"), *outs):
+        # The same sums joined in other places, about 2^-20 of them apart; where a 16-bit rounding falls between, each is
+        # half a step, 2^-8, from it, on two sides: 2^-7 apart. Few of them are.
+        step = 2.0 ** -7 if a.dtype is torch.bfloat16 else 2.0 ** -18
+        far = (a.double() - b.double()).abs()
+        over = (far - step * b.double().abs() - 2.0 ** -18 * b.double().abs().max()).max().item()
+        assert over <= 0, (name, over)
+        if a.dtype is torch.bfloat16:
+            assert (far > 0).double().mean().item() <= 2.0 ** -6, name

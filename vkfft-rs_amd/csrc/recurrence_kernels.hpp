@@ -1,4 +1,4 @@
-// recurrence.hip -- the gated recurrence h[t] = a[t] h[t-1] + m[t] x[t] of every
+// recurrence_kernels.hpp -- the gated recurrence h[t] = a[t] h[t-1] + m[t] x[t] of every
 // channel, and its gradients.
 //
 // With D the gradient of the state after a token and E = a D that of the state
@@ -16,6 +16,8 @@
 //
 // A decay near 1 is kept as what it is short of 1: rounded to 24 bits itself, a
 // memory of n tokens would be off by n 2^-25 of its length. So is A.
+#pragma once
+
 #include <algorithm>
 #include <type_traits>
 
@@ -458,7 +460,6 @@ constexpr int kChainTokens = kChainWaves * U;
 // this file launches needs it, a workspace that two calls share at once may.
 constexpr int kPatience = 1 << 20;
 
-constexpr int kLine = 32;  // words of a counter's line
 struct Chain {
     unsigned* counters;
     uint64_t *joins, *states;  // [place][batch][channel]; before a group, [group][batch][channel]
@@ -502,7 +503,7 @@ __device__ __forceinline__ float state_of(uint64_t w) { return __uint_as_float((
 __global__ __launch_bounds__(256) void k_chain_clear(uint64_t* words, long long count, unsigned* counters, int chains) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i < count) words[i] = 0;
-    if (i < chains) counters[i * kLine] = 0;
+    if (i < chains) counters[i * kChainLine] = 0;
 }
 
 template <typename T, typename Pass>
@@ -513,7 +514,7 @@ __device__ __forceinline__ void chained(const RecurrenceArgs& a, const Range& r,
     __shared__ unsigned ticket;
     // neighbours in the order of launch are of different chains, those of one chain on different XCDs
     const unsigned chains = (unsigned)(chain.columns * a.batch), mine = (blockIdx.x + blockIdx.x / chains) % chains;
-    if (!threadIdx.x) ticket = __hip_atomic_fetch_add(chain.counters + mine * kLine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!threadIdx.x) ticket = __hip_atomic_fetch_add(chain.counters + mine * kChainLine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     const int order = (int)__builtin_amdgcn_readfirstlane(ticket);
     const int b = (int)(mine / (unsigned)chain.columns), l = threadIdx.x & 63;
@@ -627,20 +628,16 @@ bool for_chains(const RecurrenceArgs& a, long long blocks) {
     const long long rounds = (blocks + a.cus - 1) / a.cus;
     return blocks * 4 < rounds * a.cus * 3;
 }
-// Most channels of all sequences that chains run: those of 64 to 128 channels a
-// block, in up to 3 rounds (four rounds are three quarters full always).
-long long most_chained(int cus) { return (long long)cus * 128 * 3; }
 
-// The workspace: the chains' counters, their states between launches, the words
-// of a launch.
-long long words_of(int cus) { return (long long)cus * 4096; }
+// The workspace (recurrence_workspace_bytes): the chains' counters, their states
+// between launches, the words of a launch.
 struct Workspace {
     unsigned* counters;
     float* states;
     uint64_t* words;
 };
 Workspace workspace_of(const RecurrenceArgs& a) {
-    float* states = a.work + most_chained(a.cus) / 64 * kLine;
+    float* states = a.work + most_chained(a.cus) / 64 * kChainLine;
     return Workspace{(unsigned*)a.work, states, (uint64_t*)(states + most_chained(a.cus))};
 }
 
@@ -687,26 +684,16 @@ int launch_gate(const RecurrenceArgs& a, hipStream_t s) {
 }
 
 // Two 16-bit channels a lane where every pair of them is a word.
-template <typename T, bool BACK>
-int launch_channels(const RecurrenceArgs& a, hipStream_t s) {
-    uintptr_t all = (uintptr_t)a.channels * 2;
-    for (const RecurrenceSide* x : {&a.x, &a.gate, &a.dy, &a.y, &a.dgate}) all |= (uintptr_t)x->p | (uintptr_t)(x->batch * 2) | (uintptr_t)(x->token * 2);
-    return all % 4 ? launch_gate<T, 1, BACK>(a, s) : launch_gate<T, 2, BACK>(a, s);
-}
-
-template <bool BACK>
-int launch_element(const RecurrenceArgs& a, hipStream_t s) {
-    if (a.element == VKFX_ELEMENT_F32) return launch_gate<float, 1, BACK>(a, s);
-    if (a.element == VKFX_ELEMENT_F16) return launch_channels<_Float16, BACK>(a, s);
-    return launch_channels<__bf16, BACK>(a, s);
+template <typename T>
+int launch_channels(const RecurrenceArgs& a, hipStream_t s, bool back) {
+    if constexpr (sizeof(T) == 2) {
+        uintptr_t all = (uintptr_t)a.channels * 2;
+        for (const RecurrenceSide* x : {&a.x, &a.gate, &a.dy, &a.y, &a.dgate}) all |= (uintptr_t)x->p | (uintptr_t)(x->batch * 2) | (uintptr_t)(x->token * 2);
+        if (all % 4 == 0) return back ? launch_gate<T, 2, true>(a, s) : launch_gate<T, 2, false>(a, s);
+    }
+    return back ? launch_gate<T, 1, true>(a, s) : launch_gate<T, 1, false>(a, s);
 }
 
 }  // namespace
-
-int launch_recurrence_forward(const RecurrenceArgs& a, hipStream_t s) { return launch_element<false>(a, s); }
-int launch_recurrence_backward(const RecurrenceArgs& a, hipStream_t s) { return launch_element<true>(a, s); }
-size_t recurrence_workspace_bytes(int, long long, int cus) {
-    return (size_t)(most_chained(cus) / 64 * kLine + most_chained(cus)) * sizeof(float) + (size_t)words_of(cus) * sizeof(uint64_t);
-}
 
 }  // namespace vkfx

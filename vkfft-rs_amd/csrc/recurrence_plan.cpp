@@ -64,6 +64,12 @@ RecurrenceArgs common(const vkfx_gated_recurrence* plan, uint64_t batch, uint64_
     return a;
 }
 
+int launch(const RecurrenceArgs& a, hipStream_t s, bool back) {
+    if (a.element == VKFX_ELEMENT_F32) return launch_recurrence_f32(a, s, back);
+    if (a.element == VKFX_ELEMENT_F16) return launch_recurrence_f16(a, s, back);
+    return launch_recurrence_bf16(a, s, back);
+}
+
 }  // namespace
 
 extern "C" {
@@ -82,7 +88,7 @@ int vkfx_gated_recurrence_create(vkfx_context* ctx, const vkfx_gated_recurrence_
         p->ctx = ctx;
         p->desc = d;
         OnDevice on(ctx);
-        const size_t bytes = recurrence_workspace_bytes(d.element, (long long)d.channels, (int)ctx->profile.compute_units);
+        const size_t bytes = recurrence_workspace_bytes((int)ctx->profile.compute_units);
         if (int rc = allocate(p->work, bytes)) return rc;
         retain(ctx);
         *out = p.release();
@@ -132,7 +138,7 @@ int vkfx_gated_recurrence_forward(vkfx_gated_recurrence* plan, const vkfx_gated_
         a.state_out = args->state_out;
         a.saved = args->saved;
         OnDevice on(plan->ctx);
-        const int e = launch_recurrence_forward(a, stream_of(plan->ctx, stream));
+        const int e = launch(a, stream_of(plan->ctx, stream), false);
         return e == hipSuccess ? VKFX_OK : hip_fail((hipError_t)e, "launch gated recurrence");
     });
 }
@@ -179,7 +185,7 @@ int vkfx_gated_recurrence_backward(vkfx_gated_recurrence* plan, const vkfx_gated
         a.state_out = args->dstate_in;
         a.saved = (float*)args->saved;
         OnDevice on(plan->ctx);
-        const int e = launch_recurrence_backward(a, stream_of(plan->ctx, stream));
+        const int e = launch(a, stream_of(plan->ctx, stream), true);
         return e == hipSuccess ? VKFX_OK : hip_fail((hipError_t)e, "launch gated recurrence gradients");
     });
 }

@@ -1,4 +1,4 @@
-// rotary.hip -- heads turned by their positions, with a norm of each in front
+// rotary_kernels.hpp -- heads turned by their positions, with a norm of each in front
 // where it is wanted, and the gradients of both.
 //
 // A pair (u1, u2) at position p turns by p f: (u1 c - u2 s, u1 s + u2 c); its
@@ -13,6 +13,8 @@
 // to 4 .. 32 lanes of a wave, each of which holds both elements of its pairs. A
 // lane forms its pairs' cosines and sines once for up to 4 heads of a token,
 // whose loads are on their way meanwhile.
+#pragma once
+
 #include <algorithm>
 
 #include "sequence.hpp"
@@ -56,17 +58,18 @@ struct Share {
     typedef Some<T, V> Vectors[N];
     int at[N], end[N], half;
 
+    // Vector j of lane l, and the end of what it is a part of.
+    __device__ __forceinline__ static int place(const RotaryArgs& a, int j, int l) {
+        if constexpr (!HALF) return (j * G + l) * V;
+        return j < 2 ? j * (a.turned / 2) + l * V : a.turned + ((j - 2) * G + l) * V;
+    }
+    __device__ __forceinline__ static int limit(const RotaryArgs& a, int j) {
+        return HALF && j < 2 ? (j + 1) * (a.turned / 2) : a.dim;
+    }
     __device__ __forceinline__ Share(const RotaryArgs& a, int l) {
         half = a.turned / 2;
-        at[0] = l * V;
-        at[1] = HALF ? half + l * V : (G + l) * V;
-        end[0] = HALF ? half : a.dim;
-        end[1] = HALF ? a.turned : a.dim;
 #pragma unroll
-        for (int j = 2; j < N; ++j) {
-            at[j] = a.turned + ((j - 2) * G + l) * V;
-            end[j] = a.dim;
-        }
+        for (int j = 0; j < N; ++j) at[j] = place(a, j, l), end[j] = limit(a, j);
     }
     __device__ __forceinline__ void load(Vectors& x, const T* row) const {
 #pragma unroll
@@ -216,21 +219,38 @@ __global__ __launch_bounds__(256) void k_turn(const RotaryArgs a, unsigned split
     }
 }
 
-// Gradients behind the norm. A lane's sums of du n are of a few heads in 32
-// bits, then in 64; the block's go to the workspace, row blockIdx.x.
+// Gradients behind the norm. A lane's sums of du n are of kTurns turns in 32 bits
+// (equal numbers would round to one side each time), then in 64, in LDS; the
+// block's go to the workspace, row blockIdx.x.
+constexpr int kTurns = 8;
+
 template <typename T, int G, int TAILS, int HB, bool HALF>
 __global__ __launch_bounds__(256) void k_norm_turn_back(const RotaryArgs a, unsigned split) {
     typedef Share<T, G, TAILS, HALF> S;
     constexpr int V = S::V, N = S::N;
+    __shared__ double sums[N * V][256];  // a thread's own
     const bool second = blockIdx.x >= split;
     const RotaryRows& h = a.rows[second];
     const int phases = (h.heads + HB - 1) / HB;
     const long long count = a.all * phases, stride = (long long)(second ? gridDim.x - split : split) * (256 / G);
     const S share(a, threadIdx.x % G);
     const float over = 1.f / (float)a.dim;
-    float w[N][V];
+    float w[N][V], part[N][V];
     share.weights(w, h.weight, a.weight_element == VKFX_ELEMENT_F32);
-    double sums[N][V] = {};
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) part[j][e] = 0.f, sums[j * V + e][threadIdx.x] = 0.0;
+    const auto flush = [&]() {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                sums[j * V + e][threadIdx.x] += (double)part[j][e];
+                part[j][e] = 0.f;
+            }
+    };
+    int turns = 0;
     for (long long i = (long long)(blockIdx.x - (second ? split : 0)) * (256 / G) + threadIdx.x / G; i < count; i += stride) {
         const Place p(a, i, count, phases);
         typename S::Vectors x[HB], dy[HB];
@@ -241,7 +261,7 @@ __global__ __launch_bounds__(256) void k_norm_turn_back(const RotaryArgs a, unsi
                     share.load(dy[k], row_of<const T>(h.x, p, p.phase + k * phases));
                     share.load(x[k], row_of<const T>(h.in, p, p.phase + k * phases));
                 }
-        float c[V], s[V], part[N][V] = {};
+        float c[V], s[V];
         share.turns(c, s, a, p.position, -a.amplitude);
 #pragma unroll
         for (int k = 0; k < HB; ++k) {
@@ -274,51 +294,59 @@ __global__ __launch_bounds__(256) void k_norm_turn_back(const RotaryArgs a, unsi
             }
             share.store(g, row_of<T>(h.out, p, head));
         }
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) sums[j][e] += (double)part[j][e];
+        if (++turns % kTurns == 0) flush();
     }
     if (!h.dweight) return;
-    __shared__ double lds[4][256];
+    flush();
+    // the wave's groups, then the block's waves
 #pragma unroll
-    for (int j = 0; j < N; ++j)
+    for (int k = 0; k < N * V; ++k) {
+        double v = sums[k][threadIdx.x];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-#pragma unroll
-            for (int o = G; o < 64; o <<= 1) sums[j][e] += __shfl_xor(sums[j][e], o);
-            if ((threadIdx.x & 63) < G && share.at[j] + e < share.end[j]) lds[threadIdx.x >> 6][share.at[j] + e] = sums[j][e];
-        }
+        for (int o = G; o < 64; o <<= 1) v += __shfl_xor(v, o);
+        sums[k][threadIdx.x] = v;
+    }
     __syncthreads();
-    const int e = threadIdx.x;
-    if (e < a.dim) a.partial[(long long)blockIdx.x * a.dim + e] = (float)((lds[0][e] + lds[1][e]) + (lds[2][e] + lds[3][e]));
+    for (int i = threadIdx.x; i < N * V * G; i += 256) {
+        const int k = i / G, l = i % G, at = S::place(a, k / V, l) + k % V;
+        if (at < S::limit(a, k / V))
+            a.partial[(long long)blockIdx.x * a.dim + at] = (float)((sums[k][l] + sums[k][64 + l]) + (sums[k][128 + l] + sums[k][192 + l]));
+    }
 }
 
-// Adds the blocks' sums: 64 elements a block, its 16 waves each an equal share
-// of the blocks in their order. blockIdx.y: q's weight, k's.
+// Adds the blocks' sums: 16 elements a block, 64 threads for each of them, which
+// take the blocks in turn. blockIdx.y: q's weight, k's.
 template <typename W>
 __global__ __launch_bounds__(1024) void k_norm_weights(const RotaryArgs a, int split, int blocks) {
-    __shared__ double lds[16][64];
+    __shared__ double lds[64][16];
     W* const to = (W*)a.rows[blockIdx.y].dweight;
     if (!to) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
-    const int begin = blockIdx.y ? split : 0, parts = blockIdx.y ? blocks - split : split;
-    const int first = begin + parts * wave / 16, end = begin + parts * (wave + 1) / 16;
+    const int lane = threadIdx.x % 16, slice = threadIdx.x / 16, e = blockIdx.x * 16 + lane;
+    const int end = blockIdx.y ? blocks : split;
     double sum = 0.0;
     if (e < a.dim)
 #pragma unroll 8
-        for (int i = first; i < end; ++i) sum += (double)a.partial[(long long)i * a.dim + e];
-    lds[wave][lane] = sum;
-    __syncthreads();
-    if (wave || e >= a.dim) return;
-    sum = 0.0;
+        for (int i = (blockIdx.y ? split : 0) + slice; i < end; i += 64) sum += (double)a.partial[(long long)i * a.dim + e];
+    lds[slice][lane] = sum;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += lds[i][lane];
-    to[e] = (W)(float)sum;
+    for (int n = 8; n; n /= 8) {  // 64 slices to 8, then to one
+        __syncthreads();
+        if (slice < n) {
+            sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += lds[slice * (64 / n) + i * (8 / n)][lane];
+        }
+        __syncthreads();
+        if (slice < n) lds[slice * (64 / n)][lane] = sum;
+    }
+    if (!slice && e < a.dim) to[e] = (W)(float)sum;
 }
 
-// Blocks of the backward pass, whose sums each are a row of the workspace.
-constexpr int kBackBlocks = 4;  // a CU
+// Blocks of the backward pass, whose sums each are a row of the workspace: as many
+// as fit at once (4 x 4096 tokens of 16 and 4 heads of 128 bf16: 68 us with 3 a CU,
+// 85 with 4).
+template <typename T, int TAILS>
+constexpr int kBackBlocks = TAILS ? 2 : sizeof(T) == 4 ? 4 : 3;
 
 template <typename T, int G, int TAILS, int HB, bool HALF>
 int launch_as(const RotaryArgs& a, hipStream_t s, bool back) {
@@ -334,7 +362,7 @@ int launch_as(const RotaryArgs& a, hipStream_t s, bool back) {
         hipLaunchKernelGGL(kernel, dim3(all), dim3(256), 0, s, a, (unsigned)blocks[0], back ? -1.f : 1.f);
         return (int)hipGetLastError();
     }
-    const long long most = (long long)a.cus * kBackBlocks, all = blocks[0] + blocks[1];
+    const long long most = (long long)a.cus * kBackBlocks<T, TAILS>, all = blocks[0] + blocks[1];
     if (all > most) {  // in the proportion of their rows, each at least one
         const long long n = blocks[0] ? std::max(1ll, (long long)((double)blocks[0] / (double)all * (double)most)) : 0;
         blocks[0] = blocks[1] ? std::min(n, most - 1) : most;
@@ -344,7 +372,7 @@ int launch_as(const RotaryArgs& a, hipStream_t s, bool back) {
         hipLaunchKernelGGL((k_norm_turn_back<T, G, TAILS, HB, HALF>), dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0, s, a, (unsigned)blocks[0]);
     if (a.rows[0].dweight || a.rows[1].dweight) {
         const auto kernel = a.weight_element == VKFX_ELEMENT_F32 ? k_norm_weights<float> : k_norm_weights<T>;
-        hipLaunchKernelGGL(kernel, dim3((a.dim + 63) / 64, 2), dim3(1024), 0, s, a, (int)blocks[0], (int)(blocks[0] + blocks[1]));
+        hipLaunchKernelGGL(kernel, dim3((a.dim + 15) / 16, 2), dim3(1024), 0, s, a, (int)blocks[0], (int)(blocks[0] + blocks[1]));
     }
     return (int)hipGetLastError();
 }
@@ -377,16 +405,6 @@ int launch_layout(const RotaryArgs& a, hipStream_t s, bool back) {
     return a.turned == a.dim ? launch_lanes<T, 0, true>(a, s, back) : launch_lanes<T, 2, true>(a, s, back);
 }
 
-int launch_element(const RotaryArgs& a, hipStream_t s, bool back) {
-    if (a.element == VKFX_ELEMENT_F32) return launch_layout<float>(a, s, back);
-    if (a.element == VKFX_ELEMENT_F16) return launch_layout<_Float16>(a, s, back);
-    return launch_layout<__bf16>(a, s, back);
-}
-
 }  // namespace
-
-int launch_rotary_forward(const RotaryArgs& a, hipStream_t s) { return launch_element(a, s, false); }
-int launch_rotary_backward(const RotaryArgs& a, hipStream_t s) { return launch_element(a, s, true); }
-size_t rotary_workspace_bytes(int dim, int cus) { return (size_t)cus * kBackBlocks * (size_t)dim * sizeof(float); }
 
 }  // namespace vkfx

@@ -84,6 +84,12 @@ int common(const vkfx_rotary* plan, uint64_t batch, uint64_t tokens, const int32
     return VKFX_OK;
 }
 
+int launch(const RotaryArgs& a, hipStream_t s, bool back) {
+    if (a.element == VKFX_ELEMENT_F32) return launch_rotary_f32(a, s, back);
+    if (a.element == VKFX_ELEMENT_F16) return launch_rotary_f16(a, s, back);
+    return launch_rotary_bf16(a, s, back);
+}
+
 }  // namespace
 
 extern "C" {
@@ -170,7 +176,7 @@ int vkfx_rotary_forward(vkfx_rotary* plan, const vkfx_rotary_forward_args* args,
             a.rows[i].heads = (int)pairs[i]->heads;
         }
         OnDevice on(plan->ctx);
-        const int e = launch_rotary_forward(a, stream_of(plan->ctx, stream));
+        const int e = launch(a, stream_of(plan->ctx, stream), false);
         return e == hipSuccess ? VKFX_OK : hip_fail((hipError_t)e, "launch rotary positions");
     });
 }
@@ -222,7 +228,7 @@ int vkfx_rotary_backward(vkfx_rotary* plan, const vkfx_rotary_backward_args* arg
             a.rows[i].heads = (int)pairs[i]->heads;
         }
         OnDevice on(plan->ctx);
-        const int e = launch_rotary_backward(a, stream_of(plan->ctx, stream));
+        const int e = launch(a, stream_of(plan->ctx, stream), true);
         return e == hipSuccess ? VKFX_OK : hip_fail((hipError_t)e, "launch rotary gradients");
     });
 }

@@ -1,5 +1,5 @@
 // sequence.hpp -- launch interface of the sequence operators' kernels
-// (layer_norm.hip, linear_attention.hip, rotary.hip, recurrence.hip), used by
+// (layer_norm.hip, linear_*.hip, rotary_*.hip, recurrence_*.hip), used by
 // sequence.cpp, rotary_plan.cpp and recurrence_plan.cpp.
 #pragma once
 
@@ -120,9 +120,12 @@ struct RotaryArgs {
     float epsilon, amplitude;
     int cus;
 };
-int launch_rotary_forward(const RotaryArgs& a, hipStream_t s);
-int launch_rotary_backward(const RotaryArgs& a, hipStream_t s);
-size_t rotary_workspace_bytes(int dim, int cus);
+// By element (rotary_f32.hip, ...). back: the gradients.
+int launch_rotary_f32(const RotaryArgs& a, hipStream_t s, bool back);
+int launch_rotary_f16(const RotaryArgs& a, hipStream_t s, bool back);
+int launch_rotary_bf16(const RotaryArgs& a, hipStream_t s, bool back);
+// A row of sums for each block of the backward pass, up to 4 a CU.
+inline size_t rotary_workspace_bytes(int dim, int cus) { return (size_t)cus * 4 * (size_t)dim * sizeof(float); }
 
 // ------------------------------------------------------- gated recurrence
 
@@ -147,8 +150,19 @@ struct RecurrenceArgs {
     int element, gate_kind, complement;
     int cus;
 };
-int launch_recurrence_forward(const RecurrenceArgs& a, hipStream_t s);
-int launch_recurrence_backward(const RecurrenceArgs& a, hipStream_t s);
-size_t recurrence_workspace_bytes(int element, long long channels, int cus);
+// By element (recurrence_f32.hip, ...). back: the gradients.
+int launch_recurrence_f32(const RecurrenceArgs& a, hipStream_t s, bool back);
+int launch_recurrence_f16(const RecurrenceArgs& a, hipStream_t s, bool back);
+int launch_recurrence_bf16(const RecurrenceArgs& a, hipStream_t s, bool back);
+
+// Most channels of all sequences that run as chains of blocks: 64 to 128 channels a
+// block, in up to 3 rounds of the CUs' number. A chain has 64; its counter has a
+// line of kChainLine words. A launch has words_of 64-bit words for its chains.
+constexpr int kChainLine = 32;
+inline long long most_chained(int cus) { return (long long)cus * 128 * 3; }
+inline long long words_of(int cus) { return (long long)cus * 4096; }
+inline size_t recurrence_workspace_bytes(int cus) {
+    return (size_t)(most_chained(cus) / 64 * kChainLine + most_chained(cus)) * sizeof(float) + (size_t)words_of(cus) * sizeof(uint64_t);
+}
 
 }  // namespace vkfx
