@@ -26,11 +26,11 @@ def test_null_arguments_are_rejected():
 
 def test_descriptors_are_laid_out_as_the_header_has_them():
     assert ctypes.sizeof(vk._RotaryDesc) == 56
-    assert ctypes.sizeof(vk._RotaryForwardArgs) == 16 + 4 * 32 + 5 * 8
-    assert ctypes.sizeof(vk._RotaryBackwardArgs) == 16 + 6 * 32 + 7 * 8
+    assert vk._ROTARY_FORWARD.size == 16 + 4 * 32 + 5 * 8
+    assert vk._ROTARY_BACKWARD.size == 16 + 6 * 32 + 7 * 8
     assert ctypes.sizeof(vk._GatedRecurrenceDesc) == 24
-    assert ctypes.sizeof(vk._RecurrenceForwardArgs) == 16 + 3 * 24 + 4 * 8
-    assert ctypes.sizeof(vk._RecurrenceBackwardArgs) == 16 + 5 * 24 + 4 * 8
+    assert vk._RECURRENCE_FORWARD.size == 16 + 3 * 24 + 4 * 8
+    assert vk._RECURRENCE_BACKWARD.size == 16 + 5 * 24 + 4 * 8
 
 
 @pytest.mark.parametrize("config,kind", [

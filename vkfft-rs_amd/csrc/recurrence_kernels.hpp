@@ -25,6 +25,10 @@
 #include "sequence_device.hpp"
 #include "vkfx.h"
 
+// Products and sums join where it is written: a result does not depend on which of
+// two ways through a kernel its neighbours' values made its wave take.
+#pragma clang fp contract(off)
+
 namespace vkfx {
 
 namespace {
@@ -149,7 +153,10 @@ struct Lane {
         have = first + (threadIdx.x & 63) * CH < channels;
         at = have ? (threadIdx.x & 63) * CH : 0;
     }
-    // Tokens t .. t + m - 1 of sequence b, the last one again behind them.
+    // Tokens t .. t + m - 1 of sequence b. FEW: those alone, where a call may be of one
+    // token; otherwise the last one again behind them (without branches: both passes of
+    // 4 x 4096 tokens of 2048 channels 149 us, 157 with).
+    template <bool FEW>
     __device__ __forceinline__ void fetch(unsigned (&r)[U], const RecurrenceSide& s, long long b, long long t, int m) const {
         Global<const T> row = (Global<const T>)((const T*)s.p + b * s.batch + t * s.token + first);
         if (m >= U) {
@@ -158,7 +165,8 @@ struct Lane {
         } else if (m > 0) {
             m = apart(m);
 #pragma unroll
-            for (int u = 0; u < U; ++u, row = behind<const T>(row, u < m ? s.token : 0)) r[u] = *(Global<const Raw>)(row + at);
+            for (int u = 0; u < U; ++u, row = behind<const T>(row, FEW || u < m ? s.token : 0))
+                if (!FEW || u < m) r[u] = *(Global<const Raw>)(row + at);
         }
     }
     __device__ __forceinline__ static float value(unsigned r, int c) { return (float)__builtin_bit_cast(Vec, (Raw)r)[c]; }
@@ -201,21 +209,22 @@ struct Lane {
     }
 };
 
-// Goes over the wave's gates: f(u, c, gate) for each. WHOLE: all U tokens, none
-// past kNear; otherwise tokens from m on leave every state as it is.
+// Goes over the wave's gates: f(u, c, gate, m) for each, m: how many tokens there
+// are, a constant where there are all (and no gate is past kNear). Tokens from m on
+// leave every state as it is.
 template <typename T, int CH, bool SIGMOID, typename F>
 __device__ __forceinline__ void each_gate(const unsigned (&g)[U], int m, F f) {
     if (__builtin_expect(m == U && !__any(Lane<T, CH>::far(g)), 1)) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int c = 0; c < CH; ++c) f(u, c, gate_of<SIGMOID, true>(Lane<T, CH>::value(g[u], c)));
+            for (int c = 0; c < CH; ++c) f(u, c, gate_of<SIGMOID, true>(Lane<T, CH>::value(g[u], c)), U);
     } else {
         m = apart(m);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int c = 0; c < CH; ++c) f(u, c, u < m ? gate_of<SIGMOID, false>(Lane<T, CH>::value(g[u], c)) : Gate{-0.f, 0.f});
+            for (int c = 0; c < CH; ++c) f(u, c, u < m ? gate_of<SIGMOID, false>(Lane<T, CH>::value(g[u], c)) : Gate{-0.f, 0.f}, m);
     }
 }
 
@@ -244,15 +253,15 @@ struct Forward {
 
     __device__ __forceinline__ Forward(const RecurrenceArgs& a, const Lane<T, CH>& lane, int b) : a(a), lane(lane), b(b) {}
     __device__ __forceinline__ void fetch(int t, int live) {
-        lane.fetch(x, a.x, b, t, live - t);
-        lane.fetch(g, a.gate, b, t, live - t);
+        lane.template fetch<!JOIN>(x, a.x, b, t, live - t);
+        lane.template fetch<!JOIN>(g, a.gate, b, t, live - t);
     }
     __device__ __forceinline__ void prepare(int m) {
         float l[CH] = {};
         Product p[CH];
-        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate q) {
+        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate q, int m) {
             s[u][c] = q.s;
-            in[u][c] = COMPLEMENT ? q.w * lane.value(x[u], c) : u < m ? lane.value(x[u], c) : 0.f;
+            in[u][c] = u < m ? COMPLEMENT ? q.w * lane.value(x[u], c) : lane.value(x[u], c) : 0.f;
             if constexpr (JOIN) {
                 p[c].by(q.s, q.w);
                 l[c] = decayed(q.s, l[c]) + in[u][c];
@@ -298,9 +307,9 @@ struct Backward {
 
     __device__ __forceinline__ Backward(const RecurrenceArgs& a, const Lane<T, CH>& lane, int b) : a(a), lane(lane), b(b) {}
     __device__ __forceinline__ void fetch(int t, int live) {
-        lane.fetch(x, a.x, b, t, live - t);
-        lane.fetch(g, a.gate, b, t, live - t);
-        lane.fetch(dy, a.dy, b, t, live - t);
+        lane.template fetch<!JOIN>(x, a.x, b, t, live - t);
+        lane.template fetch<!JOIN>(g, a.gate, b, t, live - t);
+        lane.template fetch<!JOIN>(dy, a.dy, b, t, live - t);
         const long long spans = (a.tokens + U - 1) / U;
         lane.load_state(first, t < live ? a.saved + ((long long)b * spans + t / U) * a.channels : nullptr);
     }
@@ -309,10 +318,10 @@ struct Backward {
         Product q[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) v[c] = first[c];
-        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate k) {
+        each_gate<T, CH, SIGMOID>(g, m, [&](int u, int c, Gate k, int m) {
             s[u][c] = k.s;
             if constexpr (JOIN) q[c].by(k.s, k.w);
-            const float xv = lane.value(x[u], c);
+            const float xv = u < m ? lane.value(x[u], c) : 0.f;
             p[u][c] = COMPLEMENT ? v[c] - xv : v[c];
             if (!SIGMOID && lane.value(g[u], c) > 0.f) p[u][c] = 0.f;
             v[c] = decayed(k.s, v[c]) + (COMPLEMENT ? k.w * xv : xv);
