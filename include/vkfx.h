@@ -351,7 +351,9 @@ int vkfx_execute_chain_host(vkfx_plan *const *plans, uint32_t count, const void 
 /* No counterpart in vkfft-rs: what a layer that mixes a sequence needs next
  * to a long convolution. A convolution plan mixes with a fixed filter; linear
  * attention mixes with a filter that the data chooses and that can also run
- * token by token, and layer norm scales the rows that enter either. Plans
+ * token by token, and layer norm scales the rows that enter either; rotary
+ * positions turn its queries and keys by their places, and a gated recurrence
+ * mixes every channel by itself with a decay that the data chooses. Plans
  * belong to a context like FFT plans do: destroy them before it.
  *
  * Calls are asynchronous on `stream` (a hipStream_t; NULL = the context's

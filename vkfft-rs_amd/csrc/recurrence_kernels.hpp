@@ -510,8 +510,10 @@ __device__ __forceinline__ uint64_t word_of(float v) { return (uint64_t)__float_
 __device__ __forceinline__ float state_of(uint64_t w) { return __uint_as_float((unsigned)(w >> 32)); }
 
 __global__ __launch_bounds__(256) void k_chain_clear(uint64_t* words, long long count, unsigned* counters, int chains) {
+    typedef uint64_t Two __attribute__((ext_vector_type(2)));
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) words[i] = 0;
+    if (2 * i + 1 < count) ((Two*)words)[i] = Two{0, 0};
+    else if (2 * i < count) words[2 * i] = 0;
     if (i < chains) counters[i * kChainLine] = 0;
 }
 
@@ -666,7 +668,7 @@ int launch_chains(const RecurrenceArgs& a, hipStream_t s) {
                       i + 1 < launches ? w.states : a.state_out};
         const Chain chain{w.counters, w.words, w.words + (last - first) * width, (int)columns, (int)(last - first), group};
         const long long words = ((last - first) + (last - first + group - 1) / group) * width;
-        hipLaunchKernelGGL(k_chain_clear, dim3((unsigned)((std::max(words, chains) + 255) / 256)), dim3(256), 0, s, w.words, words, w.counters,
+        hipLaunchKernelGGL(k_chain_clear, dim3((unsigned)((std::max((words + 1) / 2, chains) + 255) / 256)), dim3(256), 0, s, w.words, words, w.counters,
                            (int)chains);
         const auto kernel = k_recurrence_chain<T, SIGMOID, COMPLEMENT, BACK>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(chains * (last - first))), dim3(64 * kChainWaves), 0, s, a, r, chain);
