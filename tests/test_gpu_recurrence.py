@@ -460,6 +460,7 @@ def test_refusals(hip_ctx):
     refused("InputLengthMismatch", f, x, g, y, saved=saved[:, :2])
     refused("InputLengthMismatch", f, x, g, y, lengths=n[:1])
     refused("InputLengthMismatch", f, x, g, y, work=torch.zeros(0, device="cuda"))
+    refused("InvalidArgument", f, x, g, y, work=torch.zeros(plan.workspace_bytes + 16, device="cuda", dtype=torch.uint8)[1:])
     refused("UnsupportedPrecision", f, x.half(), g, y)
     refused("UnsupportedPrecision", f, x, g.half(), y)
     refused("UnsupportedPrecision", f, x, g, y, lengths=n.long())
@@ -516,3 +517,27 @@ def test_many_long_chains_take_several_launches(hip_ctx, lengths):
         assert over <= 0, (name, over)
         if a.dtype is torch.bfloat16:
             assert (far > 0).double().mean().item() <= 2.0 ** -6, name
+
+
+def test_calls_side_by_side_on_streams_of_chains_and_others(hip_ctx):
+    """Chains wait for their own blocks only: several calls' chains share the machine, beside calls that fill it."""
+    import torch
+    plan, wide = _plan(hip_ctx, 100, "bf16"), _plan(hip_ctx, 8192, "bf16")
+    x, gate = _tensor(1, (1, 20000, 100), "bf16"), _gate(2, (1, 20000, 100), "bf16", "sigmoid")
+    xw, gw = _tensor(3, (8, 300, 8192), "bf16"), _gate(4, (8, 300, 8192), "bf16", "sigmoid")
+    want, want_wide = torch.empty_like(x), torch.empty_like(xw)
+    plan.forward_tensors(x, gate, want)
+    wide.forward_tensors(xw, gw, want_wide)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    got = [torch.empty_like(x) for _ in streams]
+    got_wide = [torch.empty_like(xw) for _ in streams]
+    work = [torch.empty(plan.workspace_bytes, device="cuda", dtype=torch.uint8) for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, o, ow, w in zip(streams, got, got_wide, work):
+            with torch.cuda.stream(s):
+                plan.forward_tensors(x, gate, o, work=w)
+                wide.forward_tensors(xw, gw, ow, work=w)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in got) and all(torch.equal(o, want_wide) for o in got_wide)

@@ -482,3 +482,18 @@ def test_plans_hold_their_context(hip_ctx):
     assert ctx._L.vkfx_context_destroy(ctx.handle) == -2
     plan.close()
     ctx.close()
+
+
+def test_more_rows_than_a_launch_has_groups(hip_ctx):
+    """Blocks go on to further tokens; the last ones are turned by their own positions."""
+    import torch
+    t = (1 << 28) + (1 << 18) + 5
+    plan = vk.RotaryPlan(hip_ctx, _config("f16", 1, 0, 2))
+    x = torch.empty(1, t, 1, 2, device="cuda", dtype=torch.float16)
+    x[:] = _tensor(1, (1, 1, 1, 2), "f16")
+    y = torch.empty_like(x)
+    plan.forward_tensors(x, None, y, None)
+    for at in (0, (1 << 28) - 500, t - 1000):
+        z = torch.empty(1, 1000, 1, 2, device="cuda", dtype=torch.float16)
+        plan.forward_tensors(x[:, at:at + 1000], None, z, None, starts=torch.tensor([at], device="cuda", dtype=torch.int32))
+        assert torch.equal(y[:, at:at + 1000], z)
