@@ -537,7 +537,8 @@ __device__ __forceinline__ void chained(const RecurrenceArgs& a, const Range& r,
     const int t = r.from + tile * (W * U) + wave * U, m = std::min(live - t, U);
     Pass pass(a, lane, b);
     const long long channel = lane.first + lane.at, width = (long long)a.batch * a.channels, at = (long long)b * a.channels + channel;
-    if (tile < tiles) {
+    // a place there is not: only where another call counts in the same workspace
+    if (tile < tiles && order < chain.places) {
         pass.fetch(t, live);
         pass.prepare(m);
 #pragma unroll
