@@ -252,8 +252,14 @@ __global__ __launch_bounds__(256) void k_turn(const RotaryArgs a, unsigned split
 // block's go to the workspace, row blockIdx.x.
 constexpr int kTurns = 8;
 
+// Blocks of the backward pass, whose sums each are a row of the workspace: as many
+// as fit at once (4 x 4096 tokens of 16 and 4 heads of 128 bf16: 68 us with 3 a CU,
+// 85 with 4).
+template <typename T, int TAILS>
+constexpr int kBackBlocks = TAILS ? 2 : sizeof(T) == 4 ? 4 : 3;
+
 template <typename T, int G, int TAILS, int HB, bool HALF>
-__global__ __launch_bounds__(256) void k_norm_turn_back(const RotaryArgs a, unsigned split) {
+__global__ __launch_bounds__(256, (kBackBlocks<T, TAILS>)) void k_norm_turn_back(const RotaryArgs a, unsigned split) {
     typedef Share<T, G, TAILS, HALF> S;
     constexpr int V = S::V, N = S::N;
     __shared__ double sums[N * V][256];  // a thread's own
@@ -368,26 +374,25 @@ __global__ __launch_bounds__(1024) void k_norm_weights(const RotaryArgs a, int s
     if (!slice && e < a.dim) to[e] = (W)(float)sum;
 }
 
-// Blocks of the backward pass, whose sums each are a row of the workspace: as many
-// as fit at once (4 x 4096 tokens of 16 and 4 heads of 128 bf16: 68 us with 3 a CU,
-// 85 with 4).
-template <typename T, int TAILS>
-constexpr int kBackBlocks = TAILS ? 2 : sizeof(T) == 4 ? 4 : 3;
+// Groups of `lanes` that a tensor's rows fill, in blocks.
+inline long long blocks_of(const RotaryArgs& a, const RotaryRows& r, int lanes, int heads) {
+    const int groups = 256 / lanes;
+    return (a.all * ((r.heads + heads - 1) / heads) + groups - 1) / groups;
+}
 
 template <typename T, int G, int TAILS, int HB, bool HALF>
-int launch_as(const RotaryArgs& a, hipStream_t s, bool back) {
-    const auto blocks_of = [&](const RotaryRows& r) {
-        return (a.all * ((r.heads + HB - 1) / HB) + 256 / G - 1) / (256 / G);
-    };
-    long long blocks[2] = {blocks_of(a.rows[0]), blocks_of(a.rows[1])};
-    if (!a.norm || !back) {
-        for (long long& n : blocks) n = std::min(n, 1ll << 22);
-        const unsigned all = (unsigned)(blocks[0] + blocks[1]);
-        if (!all) return (int)hipSuccess;
-        const auto kernel = a.norm ? k_turn<T, G, TAILS, HB, HALF, true> : k_turn<T, G, TAILS, HB, HALF, false>;
-        hipLaunchKernelGGL(kernel, dim3(all), dim3(256), 0, s, a, (unsigned)blocks[0], back ? -1.f : 1.f);
-        return (int)hipGetLastError();
-    }
+int launch_turn(const RotaryArgs& a, hipStream_t s, bool back) {
+    const auto blocks = [&](int i) { return (unsigned)std::min(blocks_of(a, a.rows[i], G, HB), 1ll << 22); };
+    const unsigned first = blocks(0), all = first + blocks(1);
+    if (!all) return (int)hipSuccess;
+    const auto kernel = a.norm ? k_turn<T, G, TAILS, HB, HALF, true> : k_turn<T, G, TAILS, HB, HALF, false>;
+    hipLaunchKernelGGL(kernel, dim3(all), dim3(256), 0, s, a, first, back ? -1.f : 1.f);
+    return (int)hipGetLastError();
+}
+
+template <typename T, int G, int TAILS, int HB, bool HALF>
+int launch_norm_back(const RotaryArgs& a, hipStream_t s) {
+    long long blocks[2] = {blocks_of(a, a.rows[0], G, HB), blocks_of(a, a.rows[1], G, HB)};
     const long long most = (long long)a.cus * kBackBlocks<T, TAILS>, all = blocks[0] + blocks[1];
     if (all > most) {  // in the proportion of their rows, each at least one
         const long long n = blocks[0] ? std::max(1ll, (long long)((double)blocks[0] / (double)all * (double)most)) : 0;
@@ -403,14 +408,20 @@ int launch_as(const RotaryArgs& a, hipStream_t s, bool back) {
     return (int)hipGetLastError();
 }
 
-// One head a group of lanes while there are few rows, where latency counts;
-// several from 8 waves a CU on.
+// One head a group of lanes while there are few rows, where latency counts; several,
+// as far as there are so many, from 8 waves a CU on.
 template <typename T, int G, int TAILS, bool HALF>
 int launch_heads(const RotaryArgs& a, hipStream_t s, bool back) {
-    const bool sums = a.norm && back;
     const long long waves = a.all * ((a.rows[0].heads + a.rows[1].heads + 3) / 4) * G / 64;
-    if (waves < (long long)a.cus * 8) return launch_as<T, G, TAILS, 1, HALF>(a, s, back);
-    return sums ? launch_as<T, G, TAILS, 2, HALF>(a, s, back) : launch_as<T, G, TAILS, 4, HALF>(a, s, back);
+    const int heads = waves < (long long)a.cus * 8 ? 1 : std::max(a.rows[0].heads, a.rows[1].heads);
+    if (a.norm && back) {
+        // two with tails are more than a lane's registers hold
+        if constexpr (!(TAILS && sizeof(T) == 2))
+            if (heads > 1) return launch_norm_back<T, G, TAILS, 2, HALF>(a, s);
+        return launch_norm_back<T, G, TAILS, 1, HALF>(a, s);
+    }
+    if (heads < 2) return launch_turn<T, G, TAILS, 1, HALF>(a, s, back);
+    return heads < 3 ? launch_turn<T, G, TAILS, 2, HALF>(a, s, back) : launch_turn<T, G, TAILS, 4, HALF>(a, s, back);
 }
 
 template <typename T, int TAILS, bool HALF>
