@@ -497,3 +497,50 @@ def test_more_rows_than_a_launch_has_groups(hip_ctx):
         z = torch.empty(1, 1000, 1, 2, device="cuda", dtype=torch.float16)
         plan.forward_tensors(x[:, at:at + 1000], None, z, None, starts=torch.tensor([at], device="cuda", dtype=torch.int32))
         assert torch.equal(y[:, at:at + 1000], z)
+
+
+@pytest.mark.parametrize("layout", [HALF, PAIRS])
+@pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("b,t,h,kv", [(2, 9, 3, 2), (2, 9000, 5, 3), (3, 12000, 2, 1)])
+@pytest.mark.parametrize("d,r", [(48, 32), (50, 22), (128, 2), (37, 30)])
+def test_what_does_not_turn_passes(hip_ctx, layout, element, b, t, h, kv, d, r):
+    """Elements from rotary_dim on are the row's, to the bit; what is not finite among them reaches no other."""
+    import torch
+    bits = torch.int32 if element == "f32" else torch.int16
+    plan = vk.RotaryPlan(hip_ctx, _config(element, h, kv, d, r, layout, amplitude=0.5))
+    q, k = _tensor(1, (b, t, h, d), element), _tensor(2, (b, t, kv, d), element)
+    runs = []
+    for bad in (False, True):
+        if bad:
+            for x in (q, k):
+                most = torch.finfo(x.dtype).max
+                for i, v in enumerate((float("inf"), -0.0, float("-inf"), most, float("nan"))):
+                    x[:, i::6, 1 % x.size(2), r + i % (d - r)] = v
+                x[:, 5::6, 0, r:] = float("inf")
+        o = [torch.full_like(x, 3) for x in (q, k, q, k)]
+        plan.forward_tensors(q, k, *o[:2])
+        plan.backward_tensors(q, k, *o[2:])
+        runs.append(o)
+        for x, y in zip((q, k, q, k), o):
+            x, y = x[..., r:], y[..., r:]
+            assert torch.equal(torch.isnan(x), torch.isnan(y))
+            assert torch.equal(x.nan_to_num(9.0, 8.0, 7.0).contiguous().view(bits), y.nan_to_num(9.0, 8.0, 7.0).contiguous().view(bits))
+    assert all(torch.equal(x[..., :r], y[..., :r]) for x, y in zip(*runs))
+
+
+@pytest.mark.parametrize("element", ELEMENTS)
+def test_what_does_not_turn_passes_the_norm(hip_ctx, element):
+    """Behind the norm it is what a plan that turns none of the row gives; zeros keep their signs."""
+    import torch
+    h, d, r = 3, 48, 32
+    x, w = _tensor(1, (2, 40, h, d), element), _vector(3, d, element, scale=0.05)
+    x[:, ::2, :, r + 1::2] = -0.0
+    bits = torch.int32 if element == "f32" else torch.int16
+    outs = []
+    for turned in (r, 0):
+        plan = vk.RotaryPlan(hip_ctx, _config(element, h, 0, d, turned, PAIRS, True))
+        y = torch.empty_like(x)
+        plan.forward_tensors(x, None, y, None, q_weight=w)
+        assert (w > 0).all() and torch.equal(torch.signbit(y[..., r:]), torch.signbit(x[..., r:]))
+        outs.append(y[..., r:].contiguous().view(bits))
+    assert torch.equal(*outs)

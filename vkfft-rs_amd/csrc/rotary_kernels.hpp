@@ -141,27 +141,33 @@ struct Share {
             }
         }
     }
+    // The lane's pair e, of the row's.
+    __device__ __forceinline__ int pair(int e) const { return HALF ? at[0] + e : at[e / (V / 2)] / 2 + e % (V / 2); }
     // Cosines and sines of the lane's pairs at position p, amplitude included.
     __device__ __forceinline__ void turns(float (&c)[V], float (&s)[V], const RotaryArgs& a, long long p, float sign) const {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const int pair = HALF ? at[0] + e : at[e / (V / 2)] / 2 + e % (V / 2);
             c[e] = 1.f;
             s[e] = 0.f;
-            if (pair >= half) continue;
-            turn((uint64_t)p * a.turns[pair], c[e], s[e]);
+            if (pair(e) >= half) continue;
+            turn((uint64_t)p * a.turns[pair(e)], c[e], s[e]);
             c[e] *= a.amplitude;
             s[e] *= sign;
         }
     }
-    __device__ __forceinline__ static void turn_by(float (&y)[N][V], const float (&c)[V], const float (&s)[V]) {
+    // Pairs of neighbours that do not turn stay what they are: with a cosine of 1 and a
+    // sine of 0, an infinity would make its neighbour a NaN, and -0 become 0. (Selected
+    // for rows that turn whole, too: 16 and 4 heads of 128 bf16, 8 x 2048 tokens, 39.0 us,
+    // 38.3 without, 41.7 with a branch for them.)
+    __device__ __forceinline__ void turn_by(float (&y)[N][V], const float (&c)[V], const float (&s)[V]) const {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             float& u = HALF ? y[0][e] : y[e / (V / 2)][e % (V / 2) * 2];
             float& v = HALF ? y[1][e] : y[e / (V / 2)][e % (V / 2) * 2 + 1];
-            const float first = fmaf(u, c[e], -v * s[e]);
-            v = fmaf(u, s[e], v * c[e]);
-            u = first;
+            const float first = fmaf(u, c[e], -v * s[e]), second = fmaf(u, s[e], v * c[e]);
+            const bool turns = HALF || pair(e) < half;
+            u = turns ? first : u;
+            v = turns ? second : v;
         }
     }
 };
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(256) void k_turn(const RotaryArgs a, unsigned split
 #pragma unroll
                         for (int e = 0; e < V; ++e) y[j][e] *= rstd * w[j][e];
                 }
-                S::turn_by(y, c, s);
+                share.turn_by(y, c, s);
             }
             share.store(y, row_of<T>(h.out, p, head));
         }
@@ -309,7 +315,7 @@ __global__ __launch_bounds__(256, (kBackBlocks<T, TAILS>)) void k_norm_turn_back
 #pragma unroll
                     for (int e = 0; e < V; ++e) g[j][e] = (float)dy[k][j][e], n[j][e] = (float)x[k][j][e];
                 const float rstd = deviation(share, n, over, a.epsilon);
-                S::turn_by(g, c, s);
+                share.turn_by(g, c, s);
 #pragma unroll
                 for (int j = 0; j < N; ++j)
 #pragma unroll
