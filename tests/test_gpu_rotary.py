@@ -544,3 +544,21 @@ def test_what_does_not_turn_passes_the_norm(hip_ctx, element):
         assert (w > 0).all() and torch.equal(torch.signbit(y[..., r:]), torch.signbit(x[..., r:]))
         outs.append(y[..., r:].contiguous().view(bits))
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("element", ["f32", "bf16"])
+@pytest.mark.parametrize("size,epsilon,d", [(1e19, 1e37, 64), (3e19, 1e38, 64), (2e19, 3e38, 64), (1e38, 3e38, 200), (1.2e19, 3.3e38, 2), (3e38, 1e-6, 64),
+                                            (1e18, 3e38, 64)])
+def test_large_epsilons(hip_ctx, element, size, epsilon, d):
+    """An epsilon that is no less than rows whose squares pass 32 bits, alone or with it, counts beside them."""
+    import torch
+    plan = vk.RotaryPlan(hip_ctx, vk.RotaryConfig.new(2, d).with_kv_heads(0).with_rotary_dim(0).with_element(ELEMENT[element]).with_norm(epsilon))
+    unit = torch.rand(1, 4, 2, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 0.5 + 0.5
+    x, dy = (unit * size).to(_types()[element]), _tensor(2, (1, 4, 2, d), element)
+    y, dw = torch.empty_like(x), torch.empty(d, device="cuda", dtype=x.dtype)
+    plan.forward_tensors(x, None, y, None)
+    want = ref.rms(_np(x), 1.0, epsilon)[0]
+    ref.check("y", y, want, np.abs(want), element, ref.NORM_TERM)
+    plan.backward_tensors(dy, None, torch.empty_like(x), None, q=x, dq_weight=dw)
+    _, _, want, total = ref.rms_gradients(_np(x), np.ones(d), epsilon, _np(dy), np.abs(_np(dy)), 1.0)
+    ref.check("dw", dw, want, total, element, ref.NORM_TERM)

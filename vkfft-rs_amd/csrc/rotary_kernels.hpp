@@ -172,17 +172,18 @@ struct Share {
     }
 };
 
-// 1 / sqrt(mean of squares + epsilon) of a row; where the squares pass 32 bits,
-// from 2^-68 of the row, beside which epsilon is nothing.
+// 1 / sqrt(mean of squares + epsilon) of a row; where that passes 32 bits, from 2^-68
+// of the row and 2^-136 of epsilon.
 template <typename S, int N, int V>
 __device__ __forceinline__ float deviation(const S& share, const float (&x)[N][V], float over, float epsilon) {
     const float square = share.sum([&](int j, int e, float v) { return fmaf(x[j][e], x[j][e], v); });
-    if (square != INFINITY) return 1.f / sqrtf(fmaf(square, over, epsilon));
+    const float mean = fmaf(square, over, epsilon);
+    if (mean != INFINITY) return 1.f / sqrtf(mean);
     const float small = share.sum([&](int j, int e, float v) {
         const float part = x[j][e] * 0x1p-68f;
         return fmaf(part, part, v);
     });
-    return 0x1p-68f / sqrtf(small * over);
+    return 0x1p-68f / sqrtf(fmaf(small, over, epsilon * 0x1p-68f * 0x1p-68f));
 }
 
 // Which token and which heads of it a group of lanes takes: heads phase, phase +
