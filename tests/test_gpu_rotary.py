@@ -562,3 +562,17 @@ def test_large_epsilons(hip_ctx, element, size, epsilon, d):
     plan.backward_tensors(dy, None, torch.empty_like(x), None, q=x, dq_weight=dw)
     _, _, want, total = ref.rms_gradients(_np(x), np.ones(d), epsilon, _np(dy), np.abs(_np(dy)), 1.0)
     ref.check("dw", dw, want, total, element, ref.NORM_TERM)
+
+
+@pytest.mark.parametrize("size,weight,epsilon", [(3e38, 1e-3, 1e-6), (1e30, 1e-12, 1e-6), (1e-20, 1e25, 2e-38), (1e-19, 1e-25, 2e-38)])
+def test_weights_beside_rows_at_the_ends(hip_ctx, size, weight, epsilon):
+    """The row's factor times the weight may leave 32 bits, or their normal numbers, where the result does not."""
+    import torch
+    d = 64
+    plan = vk.RotaryPlan(hip_ctx, _config("f32", 2, 0, d, 0).with_norm(epsilon))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = ((torch.rand(n, device="cuda", generator=g) * 0.5 + 0.5) * s for n, s in (((1, 4, 2, d), size), ((d,), weight)))
+    y = torch.empty_like(x)
+    plan.forward_tensors(x, None, y, None, q_weight=w)
+    want = ref.rms(_np(x), _np(w), epsilon)[1]
+    ref.check("y", y, want, np.abs(want), "f32", ref.NORM_TERM)

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(256) void k_turn(const RotaryArgs a, unsigned split
 #pragma unroll
                     for (int j = 0; j < N; ++j)
 #pragma unroll
-                        for (int e = 0; e < V; ++e) y[j][e] *= rstd * w[j][e];
+                        for (int e = 0; e < V; ++e) y[j][e] = y[j][e] * rstd * w[j][e];  // rstd w may leave 32 bits
                 }
                 share.turn_by(y, c, s);
             }
