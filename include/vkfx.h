@@ -482,7 +482,8 @@ int vkfx_linear_attention_backward(vkfx_linear_attention *plan, const vkfx_linea
  *   pair i < rotary_dim / 2 of u turns by p frequencies[i]:
  *     y1 = amplitude (u1 cos - u2 sin),  y2 = amplitude (u1 sin + u2 cos)
  *   elements from rotary_dim on are u.
- * Angles are right to 2^-31 of a turn at every 32-bit position. */
+ * Angles are right to 2^-31 of a turn at every 32-bit position; the cosine and sine of
+ * each are formed from it in 32 bits, off by up to 2^-21.6 of themselves. */
 enum vkfx_rotary_layout {
     VKFX_ROTARY_INTERLEAVED = 0, /* pair i: elements 2 i and 2 i + 1 */
     VKFX_ROTARY_HALF = 1         /* elements i and i + rotary_dim / 2 */

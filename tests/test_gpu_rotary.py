@@ -576,3 +576,24 @@ def test_weights_beside_rows_at_the_ends(hip_ctx, size, weight, epsilon):
     plan.forward_tensors(x, None, y, None, q_weight=w)
     want = ref.rms(_np(x), _np(w), epsilon)[1]
     ref.check("y", y, want, np.abs(want), "f32", ref.NORM_TERM)
+
+
+@pytest.mark.parametrize("frequency", [1.0, 0.01, -2.5, 1e-4])
+def test_cosines_and_sines(hip_ctx, frequency):
+    """(1, 0) turns to (cos, sin): what is above 2^-0.5 within 2^-21.9 of itself, the other within 2^-21.6."""
+    import torch
+    t = 1 << 21
+    plan = vk.RotaryPlan(hip_ctx, _config("f32", 1, 0, 2, frequencies=[frequency]))
+    x = torch.tensor([1.0, 0.0], device="cuda").expand(1, t, 1, 2)
+    y = torch.empty(1, t, 1, 2, device="cuda")
+    plan.forward_tensors(x, None, y, None)
+    a = np.arange(t, dtype=np.longdouble) * np.longdouble(frequency)
+    got = _np(y).reshape(t, 2)
+    # In 2^-24 of each: t's two roundings, that of r and of 2 pi 3.5 (r tan r <= 0.79 of them for the cosine), the sine's
+    # last product 1 and the sum in it 0.6; the cosine's last sum 0.7 and the squares in it 0.5: 5.1 and 4. A near quarter
+    # turn gives either from the other's series.
+    for i, want in enumerate((np.cos(a), np.sin(a))):
+        size = np.abs(want)
+        # the frequency is a multiple of 2^-64 turns, and the angle here of 64 bits: 2^-40 at these positions
+        over = np.abs(got[:, i] - want) - np.where(size > 2.0 ** -0.5, 2.0 ** -21.9, 2.0 ** -21.6) * size - 2.0 ** -40
+        assert over.max() <= 0, (i, int(np.argmax(over)), float(over.max()))

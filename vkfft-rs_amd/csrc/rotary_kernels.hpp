@@ -25,8 +25,12 @@ namespace vkfx {
 
 namespace {
 
-// Cosine and sine of 2^-64 `phase` turns, 1e-7 of each: the nearest quarter
-// turn, then the series of what is left (to pi/4, the next term below 2^-32).
+// Cosine and sine of 2^-64 `phase` turns: the nearest quarter turn, then the series of
+// what is left (to pi/4: the next terms are 2^-28.5 of the sine, 2^-32.5 of the cosine).
+// With two roundings of t, one of its product with 2 pi and those of the series the
+// sine is off by up to 2^-21.6 of itself (2^-21.9 seen), the cosine by 2^-21.9 (2^-22.7);
+// angles under 2^-32 turns by 2^-54. (t rounded once, and what r's rounding leaves in
+// the sine, make both 2^-22.5 and calls 1 to 3% longer.)
 __device__ __forceinline__ void turn(uint64_t phase, float& c, float& s) {
     const unsigned quarter = ((unsigned)(phase >> 61) + 1) >> 1;
     const long long left = (long long)(phase - ((uint64_t)quarter << 62));
