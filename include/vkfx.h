@@ -505,8 +505,8 @@ typedef struct vkfx_rotary vkfx_rotary;
 
 int vkfx_rotary_create(vkfx_context *ctx, const vkfx_rotary_desc *desc, vkfx_rotary **out);
 int vkfx_rotary_destroy(vkfx_rotary *plan);
-/* Bytes of the scratch a caller may pass to vkfx_rotary_backward, for any
- * number of tokens (0 without the norm). */
+/* Bytes of the scratch a caller may pass to vkfx_rotary_backward, aligned to 16
+ * bytes, for any number of tokens (0 without the norm, which uses none). */
 int vkfx_rotary_workspace_bytes(const vkfx_rotary *plan, uint64_t *out);
 
 /* Up to 2^31 - 1 tokens in all (batch times tokens). A token's position is

@@ -597,3 +597,18 @@ def test_cosines_and_sines(hip_ctx, frequency):
         # the frequency is a multiple of 2^-64 turns, and the angle here of 64 bits: 2^-40 at these positions
         over = np.abs(got[:, i] - want) - np.where(size > 2.0 ** -0.5, 2.0 ** -21.9, 2.0 ** -21.6) * size - 2.0 ** -40
         assert over.max() <= 0, (i, int(np.argmax(over)), float(over.max()))
+
+
+def test_a_workspace_at_an_odd_place_is_refused(hip_ctx):
+    """Its sums are floats; the plan without the norm uses none."""
+    import torch
+    plan, plain = (vk.RotaryPlan(hip_ctx, _config("f32", 2, 0, 16, norm=n)) for n in (True, False))
+    x, y = torch.ones(1, 4, 2, 16, device="cuda"), torch.empty(1, 4, 2, 16, device="cuda")
+    room = torch.zeros(plan.workspace_bytes + 16, device="cuda", dtype=torch.uint8)
+    for at in (1, 4, 8):
+        with pytest.raises(vk.VkFftError) as e:
+            plan.backward_tensors(x, None, y, None, q=x, work=room[at:])
+        assert e.value.kind == "InvalidArgument" and "aligned" in str(e.value)
+        plain.backward_tensors(x, None, y, None, work=room[at:])
+    assert not room.any()
+    plan.backward_tensors(x, None, y, None, q=x, work=room[16:])

@@ -38,10 +38,6 @@ int check_in_place(const char* out, const vkfx_channels& o, const char* in, cons
     return VKFX_OK;
 }
 
-int check_work(const void* d_work) {
-    return (uintptr_t)d_work % 16 ? bad("work must be aligned to 16 bytes") : VKFX_OK;
-}
-
 int check_counts(uint64_t batch, uint64_t tokens) {
     if (batch > kMostSequences) return fail(VKFX_ERR_RESOURCE_LIMIT, "more than 65535 sequences");
     if (tokens > kMostTokens) return fail(VKFX_ERR_RESOURCE_LIMIT, "more than 2^31 - 65536 tokens");

@@ -189,6 +189,8 @@ int vkfx_rotary_backward(vkfx_rotary* plan, const vkfx_rotary_backward_args* arg
         RotaryArgs a{};
         if (int rc = common(plan, b, t, args->positions, args->starts, args->lengths, args->q_weight, args->k_weight, &a)) return rc;
         if (!d.norm && (args->dq_weight || args->dk_weight)) return bad("the plan was made without the norm: it has no weights");
+        if (d.norm)
+            if (int rc = check_work(d_work)) return rc;
         const Pair q{"dq_out", "dq", args->dq_out, args->dq, d.heads}, k{"dk_out", "dk", args->dk_out, args->dk, d.kv_heads};
         const vkfx_sequence* inputs[2] = {&args->q, &args->k};
         const Pair* pairs[2] = {&q, &k};

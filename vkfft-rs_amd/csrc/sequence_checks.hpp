@@ -83,6 +83,10 @@ inline bool mul(uint64_t a, uint64_t b, uint64_t* out) { return !__builtin_mul_o
 
 inline uint64_t bytes_of(int32_t element) { return element == VKFX_ELEMENT_F32 ? 4 : 2; }
 
+inline int check_work(const void* d_work) {
+    return (uintptr_t)d_work % 16 ? bad("work must be aligned to 16 bytes") : VKFX_OK;
+}
+
 // A tensor of a call, for the check that outputs share no memory with inputs
 // nor with each other. No data: nothing.
 struct Tensor {
