@@ -612,3 +612,27 @@ def test_a_workspace_at_an_odd_place_is_refused(hip_ctx):
         plain.backward_tensors(x, None, y, None, work=room[at:])
     assert not room.any()
     plan.backward_tensors(x, None, y, None, q=x, work=room[16:])
+
+
+# From 8 waves a CU on, 2048 of the 256 CUs here, a lane takes several heads of its token: four, two where there are
+# no more, two in the gradients behind the norm. Tokens are as many as that takes with each width's lanes.
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("b,t,h,kv,d,r,layout", [
+    (2, 8203, 5, 3, 64, 64, HALF), (2, 4099, 5, 3, 128, 128, HALF), (3, 8200, 2, 1, 128, 128, PAIRS), (2, 4111, 7, 0, 90, 90, HALF),
+    (2, 4111, 3, 2, 90, 90, PAIRS), (2, 4111, 5, 1, 128, 32, HALF), (2, 8231, 6, 2, 100, 50, HALF), (2, 8229, 5, 3, 80, 40, PAIRS),
+    (2, 2063, 4, 1, 256, 256, HALF), (1, 4101, 5, 3, 256, 66, HALF), (1, 4101, 1, 6, 255, 254, PAIRS), (2, 33001, 2, 1, 20, 10, HALF)])
+def test_several_heads_a_lane(hip_ctx, norm, element, b, t, h, kv, d, r, layout):
+    _run(hip_ctx, element, b, t, h, kv, d, r, layout, norm)
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("element", ELEMENTS)
+@pytest.mark.parametrize("layout,d,r", [(HALF, 128, 128), (HALF, 90, 26), (PAIRS, 110, 50)])
+def test_several_heads_a_lane_in_place_and_ragged(hip_ctx, norm, element, layout, d, r):
+    """In place, with rows past their length, positions of their own and rows at odd places."""
+    import torch
+    starts = torch.tensor([5, 1 << 20, -3], device="cuda", dtype=torch.int32)
+    _run(hip_ctx, element, 3, 4011, 7, 3, d, r, layout, norm, in_place=True, lengths=[4011, 0, 1999], starts=starts, pad=3, offset=1, amplitude=1.25)
+    _run(hip_ctx, element, 3, 4011, 9, 3, d, r, layout, norm, lengths=[1, 2000, 4010], storage="bhtd",
+         positions=torch.randint(0, 1 << 20, (3, 4011), device="cuda", dtype=torch.int32), weight_element="f32" if norm else None)
