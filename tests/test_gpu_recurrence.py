@@ -541,3 +541,46 @@ def test_calls_side_by_side_on_streams_of_chains_and_others(hip_ctx):
                 wide.forward_tensors(xw, gw, ow, work=w)
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in got) and all(torch.equal(o, want_wide) for o in got_wide)
+
+
+# Blocks of 64 words of channels go along their sequences where there are enough for three quarters of the 256 CUs, 8 waves
+# of 16 tokens at a time.
+WIDE = [(6, 4096, "f16"), (6, 4098, "bf16"), (3, 4099, "f32"), (3, 4099, "bf16")]
+
+
+@pytest.mark.parametrize("b,c,element", WIDE)
+@pytest.mark.parametrize("t,kind,complement", [(129, "exp", False), (256, "sigmoid", True), (257, "exp", True), (385, "sigmoid", False)])
+def test_wide_sequences_of_several_tiles(hip_ctx, b, c, element, t, kind, complement):
+    _run(hip_ctx, element, b, t, c, kind, complement)
+
+
+@pytest.mark.parametrize("b,c,element", WIDE)
+def test_wide_sequences_of_uneven_lengths(hip_ctx, b, c, element):
+    """Lengths that end in the first, a middle and the last tile, at their ends and with none; in place, and strided."""
+    _run(hip_ctx, element, b, 270, c, in_place=True, lengths=[270, 5, 256, 0, 200, 129, 128, 17][:b])
+    _run(hip_ctx, element, b, 260, c, "exp", lengths=[140, 260, 257, 999, -1, 127, 16, 258][:b], layout="tbc", pad=2, offset=2)
+
+
+@pytest.mark.parametrize("b,c,element", WIDE)
+def test_wide_sequences_keep_their_states_in_one_buffer(hip_ctx, b, c, element):
+    """state_out that is state_in, dstate_in that is dstate_out, and a prompt in two calls."""
+    import torch
+    t, cut = 300, 140
+    plan = _plan(hip_ctx, c, element)
+    x, gate, dy = _tensor(1, (b, t, c), element), _gate(2, (b, t, c), element, "sigmoid"), _tensor(3, (b, t, c), element)
+    s0, ds0 = _state(4, b, c), _state(5, b, c)
+    outs = []
+    for shared in (False, True):
+        s, ds = s0.clone(), ds0.clone()
+        so, dso = (s, ds) if shared else (torch.empty_like(s), torch.empty_like(ds))
+        o, saved = [torch.empty_like(x) for _ in range(3)], torch.empty(plan.saved_shape(b, t), device="cuda")
+        plan.forward_tensors(x, gate, o[0], state_in=s, state_out=so, saved=saved)
+        plan.backward_tensors(x, gate, saved, dy, o[1], o[2], dstate_out=ds, dstate_in=dso)
+        outs.append(o + [so, dso])
+    assert all(torch.equal(p, q) for p, q in zip(*outs))
+    want, ye, h, e, _ = ref.recurrence(*_np(x, gate, s0), np.full(b, t), True, True)
+    y, s = torch.empty_like(x), s0.clone()
+    for p in (slice(0, cut), slice(cut, t)):
+        plan.forward_tensors(x[:, p], gate[:, p], y[:, p], state_in=s, state_out=s)
+    ref.check_bound("y", y, want, ye, element)
+    ref.check_bound("state", s, h, e, "f32")
